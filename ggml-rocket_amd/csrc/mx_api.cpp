@@ -577,6 +577,28 @@ MI355X_API int mi355x_flash_attn(const mi355x_fa_args * a, int nsplit,
     return mi355x_flash_attn_ex(a, nsplit, 0, workspace_dev, workspace_bytes, stream);
 }
 
+// The fused kernel of head dims up to 256; q_f16, dst_f16: q and dst hold fp16.
+static int fa_fused(const mi355x_fa_args * a, int nsplit, int flags, bool q_f16, bool dst_f16, void * workspace_dev,
+                    size_t workspace_bytes, void * stream) {
+    if (nsplit > 64) return MI355X_E_ARG;
+    const FaPlan plan = fa_plan(a, nsplit);
+    mx::FaArgs f = fa_lower(a, plan.nsplit);
+    f.tasks = plan.tasks;
+    f.q_f16 = q_f16;
+    f.dst_f16 = dst_f16;
+    nsplit = plan.nsplit;
+    const FaLayout L = fa_layout(f);
+    if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
+    char * ws = (char *)workspace_dev;
+    f.cls = (uint8_t *)(ws + L.cls);
+    f.kzero = (uint16_t *)(ws + L.zero);
+    if (nsplit > 1) {
+        f.part_o = (float *)(ws + L.po);
+        f.part_ml = (float *)(ws + L.pml);
+    }
+    return hip_status(mx::launch_fa(f, !(flags & MI355X_FA_CLASSES_READY), S(stream)));
+}
+
 MI355X_API int mi355x_flash_attn_ex(const mi355x_fa_args * a, int nsplit, int flags,
                                     void * workspace_dev, size_t workspace_bytes, void * stream) {
     if (flags & ~MI355X_FA_CLASSES_READY) return MI355X_E_ARG;
@@ -614,21 +636,152 @@ MI355X_API int mi355x_flash_attn_ex(const mi355x_fa_args * a, int nsplit, int fl
         w.psc = (float *)(ws + L.psc); w.o = (float *)(ws + L.o);
         return hip_status(mx::launch_fa_wide(w, S(stream)));
     }
+    return fa_fused(a, nsplit, flags, false, false, workspace_dev, workspace_bytes, stream);
+}
+
+// ---- the quantized KV cache ---------------------------------------------------------------------
+
+static bool kv_type(int t) { return t == mx::T_Q8_0 || t == mx::T_Q4_0; }
+
+static int kv_rows_lower(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n, int32_t * err_dev,
+                         mx::KvRowsArgs & a) {
+    if (!r || n_out < 1 || n_out > mx::KV_MAX_OUT || n < 0 || n > INT32_MAX) return MI355X_E_ARG;
+    if (idx_type != 26 && idx_type != 27) return MI355X_E_ARG;
+    if (!aligned(idx_dev, idx_type == 27 ? 8 : 4) || !aligned(err_dev, 4)) return MI355X_E_ARG;
+    memset(&a, 0, sizeof a);
+    int64_t wgs = 0;   // of either launch, one workgroup per row or per 64 blocks
+    for (int k = 0; k < n_out; k++) {
+        const mi355x_kv_rows & s = r[k];
+        if ((!kv_type(s.type) && s.type != mx::T_F16) || (s.x_type != mx::T_F32 && s.x_type != mx::T_F16)) return MI355X_E_ARG;
+        if (s.H <= 0 || s.D <= 0 || s.D % 32 || s.H > INT32_MAX / s.D || s.n_rows < 0) return MI355X_E_ARG;
+        if (s.nb1 < 0 || s.nb2 < 0 || s.nb1 % 32 || s.nb2 % 32 || s.x_nb1 < 0 || s.x_nb2 < 0 || s.x_nb1 % 8 || s.x_nb2 % 8)
+            return MI355X_E_ARG;
+        if (n > 0 && (!s.q_dev || !s.x_dev || !aligned(s.q_dev, 16) || !aligned(s.x_dev, 16))) return MI355X_E_ARG;
+        if (n > 0 && s.type != mx::T_F16 && (!s.d_dev || !aligned(s.d_dev, 8))) return MI355X_E_ARG;
+        if (!idx_dev && n > s.n_rows) return MI355X_E_ARG;
+        wgs += n * std::max<int64_t>(1, (s.H * (s.D / 32) + 63) / 64);
+        mx::KvRowsOut & o = a.o[k];
+        o.q = (uint8_t *)s.q_dev; o.d = s.d_dev; o.x = s.x_dev;
+        o.nb1 = s.nb1; o.nb2 = s.nb2; o.x_nb1 = s.x_nb1; o.x_nb2 = s.x_nb2; o.n_rows = s.n_rows;
+        o.type = s.type; o.H = (int)s.H; o.bph = (int)(s.D / 32); o.x_f16 = s.x_type == mx::T_F16;
+    }
+    if (wgs > INT32_MAX) return MI355X_E_ARG;
+    a.n_out = n_out; a.n = (int)n; a.idx = idx_dev; a.idx64 = idx_type == 27; a.err = err_dev;
+    return MI355X_OK;
+}
+
+MI355X_API int mi355x_set_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
+                               int32_t * err_dev, void * stream) {
+    mx::KvRowsArgs a;
+    const int st = kv_rows_lower(r, n_out, idx_dev, idx_type, n, err_dev, a);
+    return st != MI355X_OK || n == 0 ? st : hip_status(mx::launch_set_rows(a, S(stream)));
+}
+
+MI355X_API int mi355x_get_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
+                               int32_t * err_dev, void * stream) {
+    mx::KvRowsArgs a;
+    const int st = kv_rows_lower(r, n_out, idx_dev, idx_type, n, err_dev, a);
+    return st != MI355X_OK || n == 0 ? st : hip_status(mx::launch_get_rows(a, S(stream)));
+}
+
+static int fa_q_check_view(const mi355x_kv_view & w, bool empty) {
+    if (!kv_type(w.type)) return MI355X_E_UNSUPPORTED;
+    if ((!empty && (!w.q_dev || !w.d_dev)) || !aligned(w.q_dev, 16) || !aligned(w.d_dev, 8)) return MI355X_E_ARG;
+    if (w.nb1 < 0 || w.nb2 < 0 || w.nb3 < 0 || w.nb1 % 32 || w.nb2 % 32 || w.nb3 % 32) return MI355X_E_ARG;
+    return MI355X_OK;
+}
+
+static int fa_q_check(const mi355x_fa_q_args * a) {
+    if (!a) return MI355X_E_ARG;
+    const bool empty = a->T == 0 || a->S == 0;   // no query: nothing is read or written
+    if (!empty && (!a->q_dev || !a->dst_dev)) return MI355X_E_ARG;
+    if (a->D <= 0 || a->DV <= 0 || a->D % 32 || a->DV % 32 || !mx::fa_dims_supported(a->D, a->DV)) return MI355X_E_UNSUPPORTED;
+    if (a->max_bias != 0.0f) return MI355X_E_UNSUPPORTED;
+    for (const mi355x_kv_view * w : {&a->k, &a->v}) {
+        const int st = fa_q_check_view(*w, empty || a->KV == 0);
+        if (st != MI355X_OK) return st;
+    }
+    if (a->T < 0 || a->S < 0 || a->H <= 0 || a->HK <= 0 || a->KV < 0 || a->H % a->HK) return MI355X_E_ARG;
+    if ((int64_t)a->S * a->T * a->H > (1 << 30) || (size_t)a->KV > mx::fa_max_kv(a->D, a->DV)) return MI355X_E_UNSUPPORTED;
+    for (int t : {a->q_type, a->dst_type})
+        if (t != mx::T_F32 && t != mx::T_F16) return MI355X_E_ARG;
+    const int64_t qa = a->q_type == mx::T_F16 ? 8 : 4;
+    if (a->q_nb1 % qa || a->q_nb2 % qa || a->q_nb3 % qa || !aligned(a->q_dev, 16)) return MI355X_E_ARG;
+    if (a->dst_nb1 % 4 || a->dst_nb2 % 4 || a->dst_nb3 % 4 || !aligned(a->dst_dev, a->dst_type == mx::T_F16 ? 8 : 16)) return MI355X_E_ARG;
+    if (a->mask_dev && (a->mask_nb1 % 4 || a->mask_nb3 % 4 || a->mask_nb1 < a->KV || a->mask_nb3 < 0 || !aligned(a->mask_dev, 8)))
+        return MI355X_E_ARG;
+    return MI355X_OK;
+}
+
+// The view of sequence s.
+static mx::KvView fa_q_view(const mi355x_kv_view & w, int64_t s) {
+    mx::KvView v;
+    v.q = (const uint8_t *)w.q_dev + s * w.nb3 / (w.type == mx::T_Q4_0 ? 2 : 1);
+    v.d = w.d_dev + s * w.nb3 / 32;
+    v.nb1 = w.nb1; v.nb2 = w.nb2; v.nb3 = w.nb3; v.type = w.type;
+    return v;
+}
+
+// One sequence of the op over fp16 K and V at k16, v16, [HK][KV][D] each.
+static mi355x_fa_args fa_q_lower(const mi355x_fa_q_args * a, int s, const uint16_t * k16, const uint16_t * v16) {
+    mi355x_fa_args f;
+    memset(&f, 0, sizeof f);
+    const int64_t qe = a->q_type == mx::T_F16 ? 2 : 4, de = a->dst_type == mx::T_F16 ? 2 : 4;
+    f.q_dev = (const float *)((const char *)a->q_dev + s * a->q_nb3 * qe); f.q_nb1 = a->q_nb1; f.q_nb2 = a->q_nb2;
+    f.k_dev = k16; f.k_nb1 = a->D; f.k_nb2 = (int64_t)a->KV * a->D;
+    f.v_dev = v16; f.v_nb1 = a->DV; f.v_nb2 = (int64_t)a->KV * a->DV;
+    f.mask_dev = a->mask_dev ? a->mask_dev + s * a->mask_nb3 : nullptr; f.mask_nb1 = a->mask_nb1;
+    f.dst_dev = (float *)((char *)a->dst_dev + s * a->dst_nb3 * de); f.dst_nb1 = a->dst_nb1; f.dst_nb2 = a->dst_nb2;
+    f.D = a->D; f.DV = a->DV; f.T = a->T; f.H = a->H; f.KV = a->KV; f.HK = a->HK;
+    f.scale = a->scale; f.softcap = a->softcap;
+    return f;
+}
+
+// Workspace of the decode-first form: one sequence's K and V as fp16, then the fused kernel's own.
+struct FaQLayout {
+    size_t k, v, fa, total;
+};
+static FaQLayout fa_q_layout(const mi355x_fa_q_args * a, int nsplit) {
+    FaQLayout L;
+    const size_t rows = (size_t)a->HK * a->KV;
+    L.k = 0;
+    L.v = L.k + align256(rows * a->D * 2);
+    L.fa = L.v + align256(rows * a->DV * 2);
+    const mi355x_fa_args f = fa_q_lower(a, 0, nullptr, nullptr);
+    if (nsplit <= 0) nsplit = fa_plan(&f, 0).nsplit;
+    L.total = L.fa + align256(fa_layout(fa_lower(&f, nsplit)).total);
+    return L;
+}
+
+MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int nsplit) {
+    return fa_q_check(a) != MI355X_OK || nsplit > 64 ? 0 : fa_q_layout(a, nsplit).total;
+}
+
+MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
+                                   void * stream) {
+    const int st = fa_q_check(a);
+    if (st != MI355X_OK) return st;
     if (nsplit > 64) return MI355X_E_ARG;
-    const FaPlan plan = fa_plan(a, nsplit);
-    mx::FaArgs f = fa_lower(a, plan.nsplit);
-    f.tasks = plan.tasks;
-    nsplit = plan.nsplit;
-    const FaLayout L = fa_layout(f);
+    if (a->T == 0 || a->S == 0) return MI355X_OK;
+    const FaQLayout L = fa_q_layout(a, nsplit);
     if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
     char * ws = (char *)workspace_dev;
-    f.cls = (uint8_t *)(ws + L.cls);
-    f.kzero = (uint16_t *)(ws + L.zero);
-    if (nsplit > 1) {
-        f.part_o = (float *)(ws + L.po);
-        f.part_ml = (float *)(ws + L.pml);
+    for (int s = 0; s < a->S; s++) {
+        if (a->KV > 0) {
+            mx::KvDecodeArgs d;
+            d.k = fa_q_view(a->k, s);
+            d.v = fa_q_view(a->v, s);
+            d.k16 = (uint16_t *)(ws + L.k);
+            d.v16 = (uint16_t *)(ws + L.v);
+            d.HK = a->HK; d.KV = a->KV; d.D = a->D; d.DV = a->DV;
+            const int e = hip_status(mx::launch_kv_decode(d, S(stream)));
+            if (e != MI355X_OK) return e;
+        }
+        const mi355x_fa_args f = fa_q_lower(a, s, (const uint16_t *)(ws + L.k), (const uint16_t *)(ws + L.v));
+        const int e = fa_fused(&f, nsplit, 0, a->q_type == mx::T_F16, a->dst_type == mx::T_F16, ws + L.fa, workspace_bytes - L.fa, stream);
+        if (e != MI355X_OK) return e;
     }
-    return hip_status(mx::launch_fa(f, !(flags & MI355X_FA_CLASSES_READY), S(stream)));
+    return MI355X_OK;
 }
 
 // ---- MUL_MAT_ID -------------------------------------------------------------------------------

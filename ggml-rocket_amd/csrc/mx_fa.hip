@@ -282,6 +282,12 @@ __global__ void __launch_bounds__(256) fa_prep_kernel(FaArgs a) {
 // ---------------------------------------------------------------------------------------------
 // main kernel
 // ---------------------------------------------------------------------------------------------
+// Four output values at element offset `at` of dst, as F32 or rounded to fp16.
+__device__ __forceinline__ void fa_store4(const FaArgs & a, int64_t at, const float4v & v) {
+    if (a.dst_f16) *(u32x2 *)((uint16_t *)a.dst + at) = u32x2{pack2h(v[0], v[1]), pack2h(v[2], v[3])};
+    else *(float4v *)(a.dst + at) = v;
+}
+
 template <int DK, int DV, int NTASK, bool SOFTCAP>
 __global__ void __launch_bounds__((FaCfg<DK, DV, NTASK>::THREADS))
 __attribute__((amdgpu_waves_per_eu(FaCfg<DK, DV, NTASK>::PAR, FaCfg<DK, DV, NTASK>::PAR)))
@@ -340,15 +346,22 @@ fa_kernel(FaArgs a) {
 
     float4v qraw[KSTEPS][2];
     {
-        const float * q = a.q + (int64_t)h * a.q_nb2 + (int64_t)(qok ? tq : 0) * a.q_nb1;
+        const int64_t qo = (int64_t)h * a.q_nb2 + (int64_t)(qok ? tq : 0) * a.q_nb1;
+        const float * q = a.q + qo;
 #pragma unroll
         for (int s = 0; s < KSTEPS; s++) {
             const int d = 16 * s + 8 * lg;   // < DK
             qraw[s][0] = float4v{0, 0, 0, 0};
             qraw[s][1] = float4v{0, 0, 0, 0};
             if (qload && qok && d < a.dk) {
-                qraw[s][0] = *(const float4v *)(q + d);
-                qraw[s][1] = *(const float4v *)(q + d + 4);
+                if (a.q_f16) {
+                    const half8 x = *(const half8 *)((const uint16_t *)a.q + qo + d);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) qraw[s][e / 4][e % 4] = (float)x[e];
+                } else {
+                    qraw[s][0] = *(const float4v *)(q + d);
+                    qraw[s][1] = *(const float4v *)(q + d + 4);
+                }
             }
         }
     }
@@ -673,7 +686,8 @@ fa_kernel(FaArgs a) {
                                     for (int e = 0; e < 4; e++) mk[e] = (jb + e < a.KV) ? h2f_bits(mrow[jb + e]) : 0.0f;
                                 }
 #pragma unroll
-                                for (int e = 0; e < 4; e++) sacc[kk][4 * q4 + e] += mk[e];
+                                for (int e = 0; e < 4; e++)   // a hidden key's score may be NaN
+                                    sacc[kk][4 * q4 + e] = mk[e] == -INFINITY ? -INFINITY : sacc[kk][4 * q4 + e] + mk[e];
                             }
                     }
                 }
@@ -820,7 +834,7 @@ fa_kernel(FaArgs a) {
     if (a.nsplit == 1) {
         if (!qok) return;
         const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
-        float * dst = a.dst + (int64_t)tq * a.dst_nb2 + (int64_t)h * a.dst_nb1;
+        const int64_t dst = (int64_t)tq * a.dst_nb2 + (int64_t)h * a.dst_nb1;
 #pragma unroll
         for (int db = 0; db < DBLK; db++)
 #pragma unroll
@@ -829,7 +843,7 @@ fa_kernel(FaArgs a) {
                 float4v v;
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = o[db][4 * q4 + e] * inv;
-                if (d < a.dv) *(float4v *)(dst + d) = v;
+                if (d < a.dv) fa_store4(a, dst + d, v);
             }
         return;
     }
@@ -869,24 +883,22 @@ __global__ void __launch_bounds__(256) fa_combine_kernel(FaArgs a) {
     for (int s = 0; s < a.nsplit; s++) M = fmaxf(M, a.part_ml[2 * ((int64_t)s * rows + r)]);
     float4v num = {0, 0, 0, 0};
     float den = 0.0f;
-    if (M != -INFINITY) {
-        for (int s = 0; s < a.nsplit; s++) {
-            const int64_t pr = (int64_t)s * rows + r;
-            const float ms = a.part_ml[2 * pr];
-            if (ms == -INFINITY) continue;
-            const float w = __expf(ms - M);
-            den += w * a.part_ml[2 * pr + 1];
-            const float4v v = *(const float4v *)(a.part_o + pr * D + 4 * c);
+    for (int s = 0; s < a.nsplit; s++) {
+        const int64_t pr = (int64_t)s * rows + r;
+        const float ms = a.part_ml[2 * pr], ls = a.part_ml[2 * pr + 1];
+        if (ms == -INFINITY && ls == 0.0f) continue;   // no key seen; a NaN sum is kept
+        const float w = ms == -INFINITY ? 0.0f : __expf(ms - M);
+        den += w * ls;
+        const float4v v = *(const float4v *)(a.part_o + pr * D + 4 * c);
 #pragma unroll
-            for (int e = 0; e < 4; e++) num[e] += w * v[e];
-        }
+        for (int e = 0; e < 4; e++) num[e] += w * v[e];
     }
     const float inv = den > 0.0f ? 1.0f / den : 0.0f;
     const int tq = (int)(r / a.H), h = (int)(r % a.H);
     float4v out;
 #pragma unroll
     for (int e = 0; e < 4; e++) out[e] = num[e] * inv;
-    if (4 * c < a.dv) *(float4v *)(a.dst + (int64_t)tq * a.dst_nb2 + (int64_t)h * a.dst_nb1 + 4 * c) = out;
+    if (4 * c < a.dv) fa_store4(a, (int64_t)tq * a.dst_nb2 + (int64_t)h * a.dst_nb1 + 4 * c, out);
 }
 
 int fa_blocks_per_split(const FaArgs & a) {

@@ -54,7 +54,45 @@ struct FaArgs {
     int tasks;                 // wave tasks per block: 4, or 2 (DV <= 128; four waves a task)
     int dk, dv;                // the op's head dims (<= D, DV): columns past them are padding
     float scale, softcap;
+    bool q_f16, dst_f16;       // q / dst hold fp16 (same element strides)
 };
+
+// SET_ROWS / GET_ROWS of up to KV_MAX_OUT caches that share their indices: strides in elements.
+constexpr int KV_MAX_OUT = 4;
+struct KvRowsOut {
+    uint8_t * q;               // codes (T_F16: values)
+    uint16_t * d;              // block scales
+    void * x;                  // plain rows, F32 or F16
+    int64_t nb1, nb2, x_nb1, x_nb2, n_rows;
+    int type, H, bph;          // bph: 32-value blocks a head
+    bool x_f16;
+    int wg_begin;              // first workgroup of this output (set by the launcher)
+};
+struct KvRowsArgs {
+    KvRowsOut o[KV_MAX_OUT];
+    int n_out, n;              // n: rows
+    const void * idx;          // int32 or int64 [n], or null: row i
+    bool idx64;
+    int rows_wg;               // rows a workgroup (set by the launcher)
+    int32_t * err;             // set to 1 by an index out of range, or null
+};
+// A quantized K or V read by attention: strides in elements (planes of mi355x_kv_view).
+struct KvView {
+    const uint8_t * q;
+    const uint16_t * d;
+    int64_t nb1, nb2, nb3;
+    int type;
+};
+// K and V of one sequence as fp16 for the fused attention: k16 [HK][KV][D], v16 [HK][KV][DV].
+struct KvDecodeArgs {
+    KvView k, v;
+    uint16_t * k16;
+    uint16_t * v16;
+    int HK, KV, D, DV;
+};
+hipError_t launch_kv_decode(const KvDecodeArgs & a, hipStream_t st);
+hipError_t launch_set_rows(KvRowsArgs a, hipStream_t st);
+hipError_t launch_get_rows(KvRowsArgs a, hipStream_t st);
 
 // FLASH_ATTN_EXT with head dims past 256 (two GEMMs around a softmax pass): strides in
 // elements as in FaArgs; scratch pointers carved from the caller's workspace.

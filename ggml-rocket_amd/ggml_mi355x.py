@@ -16,7 +16,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libmi355x.so")
 
-F32, F16, Q8_0, Q4_K, Q6_K, I32, BF16, MXFP4 = 0, 1, 8, 12, 14, 26, 30, 39
+F32, F16, Q8_0, Q4_K, Q6_K, I32, I64, BF16, MXFP4 = 0, 1, 8, 12, 14, 26, 27, 30, 39
 Q4_0, Q4_1, Q5_0, Q2_K, Q5_K = 2, 3, 6, 10, 13
 F16_T = 0x101   # the library's tiled fp16 layout (16 x 32 tiles of 1 KB); not a ggml type
 Q4_K_X = 0x10C  # Q4_K blocks regrouped by 32 rows, for expert stacks (MUL_MAT_ID); not a ggml type
@@ -69,6 +69,30 @@ class MoeArgs(ctypes.Structure):
                 ("dst_dev", ctypes.c_void_p), ("dst_nb1", ctypes.c_int64), ("dst_nb2", ctypes.c_int64)]
 
 
+class KvRows(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int), ("q_dev", ctypes.c_void_p), ("d_dev", ctypes.c_void_p),
+                ("n_rows", ctypes.c_int64), ("nb1", ctypes.c_int64), ("nb2", ctypes.c_int64),
+                ("H", ctypes.c_int64), ("D", ctypes.c_int64),
+                ("x_type", ctypes.c_int), ("x_dev", ctypes.c_void_p),
+                ("x_nb1", ctypes.c_int64), ("x_nb2", ctypes.c_int64)]
+
+
+class KvView(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int), ("q_dev", ctypes.c_void_p), ("d_dev", ctypes.c_void_p),
+                ("nb1", ctypes.c_int64), ("nb2", ctypes.c_int64), ("nb3", ctypes.c_int64)]
+
+
+class FaQArgs(ctypes.Structure):
+    _fields_ = [("q_dev", ctypes.c_void_p), ("q_nb1", ctypes.c_int64), ("q_nb2", ctypes.c_int64), ("q_nb3", ctypes.c_int64),
+                ("k", KvView), ("v", KvView),
+                ("mask_dev", ctypes.c_void_p), ("mask_nb1", ctypes.c_int64), ("mask_nb3", ctypes.c_int64),
+                ("dst_dev", ctypes.c_void_p), ("dst_nb1", ctypes.c_int64), ("dst_nb2", ctypes.c_int64), ("dst_nb3", ctypes.c_int64),
+                ("q_type", ctypes.c_int), ("dst_type", ctypes.c_int),
+                ("D", ctypes.c_int), ("DV", ctypes.c_int), ("T", ctypes.c_int), ("H", ctypes.c_int),
+                ("KV", ctypes.c_int), ("HK", ctypes.c_int), ("S", ctypes.c_int),
+                ("scale", ctypes.c_float), ("max_bias", ctypes.c_float), ("softcap", ctypes.c_float)]
+
+
 def lib():
     """Load the built backend library. Raises if it has not been built."""
     global _lib
@@ -119,6 +143,13 @@ def _bind_optional(L):
         L.mi355x_flash_attn_workspace.argtypes = [pa, i32]
         L.mi355x_flash_attn.argtypes = [pa, i32, vp, sz, vp]
         L.mi355x_flash_attn_ex.argtypes = [pa, i32, i32, vp, sz, vp]
+    if hasattr(L, "mi355x_set_rows"):
+        pr, pq = ctypes.POINTER(KvRows), ctypes.POINTER(FaQArgs)
+        L.mi355x_set_rows.argtypes = [pr, i32, vp, i32, i64, vp, vp]
+        L.mi355x_get_rows.argtypes = [pr, i32, vp, i32, i64, vp, vp]
+        L.mi355x_flash_attn_q_workspace.restype = sz
+        L.mi355x_flash_attn_q_workspace.argtypes = [pq, i32]
+        L.mi355x_flash_attn_q.argtypes = [pq, i32, vp, sz, vp]
     if hasattr(L, "mi355x_mul_mat_noalloc"):
         L.mi355x_mul_mat_noalloc.argtypes = [i32, vp, i64, i64, vp, i64, i64, vp, i64, vp]
     if hasattr(L, "mi355x_mul_mat_id"):
@@ -294,6 +325,168 @@ def flash_attn(q, k, v, mask, scale: float, softcap: float = 0.0, nsplit: int = 
         raise MI355XError("flash_attn: classes_ready needs the workspace of the call that classified the mask")
     flags = FA_CLASSES_READY if classes_ready else 0
     check(lib().mi355x_flash_attn_ex(ctypes.byref(a), nsplit, flags, wp, need, stream_handle()), "flash_attn")
+    return out
+
+
+# ---- the quantized KV cache -----------------------------------------------------------------
+
+class KvCache:
+    """A K or V cache on the device, of any leading dims: `q` holds the codes (Q8_0: int8 [..., D];
+    Q4_0: uint8 [..., D / 2]; F16: the fp16 values, without `d`), `d` the blocks' fp16 scales
+    [..., D / 32]. Both planes have the same element strides; permute and slices of the leading dims
+    give views."""
+
+    __slots__ = ("type", "q", "d", "D", "shape", "nb")
+
+    def __init__(self, ttype: int, q, d=None):
+        torch = _torch()
+        self.type, self.q, self.d = ttype, q, d
+        want = {Q8_0: torch.int8, Q4_0: torch.uint8, F16: torch.float16}.get(ttype)
+        if want is None or q.dtype != want or q.dim() < 2 or q.stride(-1) != 1:
+            raise MI355XError(f"KvCache: type {ttype} does not hold codes of {q.dtype} {tuple(q.shape)}")
+        per = 2 if ttype == Q4_0 else 1
+        self.D = q.shape[-1] * per
+        self.shape = tuple(q.shape[:-1]) + (self.D,)
+        self.nb = tuple(s * per for s in q.stride()[:-1])
+        if ttype == F16:
+            if d is not None:
+                raise MI355XError("KvCache: an F16 cache has no scales")
+        elif (d is None or d.dtype != torch.float16 or d.device != q.device or self.D % 32
+              or tuple(d.shape) != self.shape[:-1] + (self.D // 32,) or (d.stride(-1) != 1 and d.shape[-1] > 1)
+              or any(n > 1 and a != 32 * b for n, a, b in zip(q.shape[:-1], self.nb, d.stride()))):
+            raise MI355XError("KvCache: the scales are not fp16 of the codes' shape and strides / 32")
+
+    def permute(self, *dims):
+        """A view with the leading dims in another order; the last dim stays last."""
+        return KvCache(self.type, self.q.permute(*dims), None if self.d is None else self.d.permute(*dims))
+
+    def __getitem__(self, at):
+        """A view by indices and slices of leading dims."""
+        return KvCache(self.type, self.q[at], None if self.d is None else self.d[at])
+
+
+def kv_cache(ttype: int, *shape, device="cuda") -> KvCache:
+    """A cache of zeros of the logical shape [..., D]."""
+    torch = _torch()
+    lead, D = tuple(shape[:-1]), shape[-1]
+    if ttype == F16:
+        return KvCache(F16, torch.zeros(*lead, D, dtype=torch.float16, device=device))
+    if ttype not in (Q8_0, Q4_0) or D % 32:
+        raise MI355XError(f"kv_cache: type {ttype} does not hold rows of {D}")
+    q = (torch.zeros(*lead, D, dtype=torch.int8, device=device) if ttype == Q8_0
+         else torch.full((*lead, D // 2), 0x88, dtype=torch.uint8, device=device))
+    return KvCache(ttype, q, torch.zeros(*lead, D // 32, dtype=torch.float16, device=device))
+
+
+def _plain_type(t, what):
+    torch = _torch()
+    if t.dtype == torch.float32:
+        return F32
+    if t.dtype == torch.float16:
+        return F16
+    raise MI355XError(f"{what}: {t.dtype} is neither F32 nor F16")
+
+
+def _kv_rows(pairs, what):
+    """mi355x_kv_rows of (cache [rows, H, D] or [rows, D], plain rows of the same trailing dims)."""
+    arr = (KvRows * len(pairs))()
+    for a, (c, x) in zip(arr, pairs):
+        if len(c.shape) not in (2, 3) or tuple(x.shape[1:]) != c.shape[1:] or x.stride(-1) != 1 or x.device != c.q.device:
+            raise MI355XError(f"{what}: rows {tuple(x.shape)} do not fit a cache {c.shape}")
+        two = len(c.shape) == 2
+        a.type, a.q_dev, a.d_dev, a.n_rows = c.type, c.q.data_ptr(), None if c.d is None else c.d.data_ptr(), c.shape[0]
+        a.nb1, a.nb2, a.H, a.D = c.nb[0], 0 if two else c.nb[1], 1 if two else c.shape[1], c.D
+        a.x_type, a.x_dev = _plain_type(x, what), x.data_ptr()
+        a.x_nb1, a.x_nb2 = x.stride(0), 0 if two else x.stride(1)
+    return arr
+
+
+def _kv_index(idx, n, device, what):
+    """(address, ggml type, count) of the row indices."""
+    if idx is None:
+        return None, I32, n
+    torch = _torch()
+    if idx.dtype not in (torch.int32, torch.int64) or idx.dim() != 1 or not idx.is_contiguous() or idx.device != device:
+        raise MI355XError(f"{what}: indices are int32 or int64, contiguous, on the cache's device")
+    return idx.data_ptr(), I64 if idx.dtype == torch.int64 else I32, idx.shape[0]
+
+
+def set_rows(pairs, idx=None, err=None):
+    """pairs: (cache, x) for up to four caches [rows, H, D] (or [rows, D]) and plain rows x [n, H, D]
+    (F32 or F16): x[i] is quantized into cache row idx[i] (int32 or int64 [n]; None: i). One launch.
+    err: a device int32 that an index out of range sets to 1."""
+    arr = _kv_rows(pairs, "set_rows")
+    n = pairs[0][1].shape[0]
+    ip, it, ni = _kv_index(idx, n, pairs[0][0].q.device, "set_rows")
+    if any(x.shape[0] != ni for _, x in pairs):
+        raise MI355XError("set_rows: one plain row for every index")
+    check(lib().mi355x_set_rows(arr, len(arr), ip, it, ni, err.data_ptr() if err is not None else None, stream_handle()), "set_rows")
+
+
+def get_rows(caches, idx=None, dtype=None, out=None, err=None):
+    """Rows idx[i] (None: all, in order) of each of up to four caches as plain values: a list of
+    [n, H, D] (or [n, D]) tensors of `dtype` (F32 by default), or `out`. One launch."""
+    torch = _torch()
+    ip, it, n = _kv_index(idx, caches[0].shape[0], caches[0].q.device, "get_rows")
+    if out is None:
+        out = [torch.empty((n,) + c.shape[1:], dtype=dtype or torch.float32, device=c.q.device) for c in caches]
+    if any(x.shape[0] != n for x in out) or len(out) != len(caches):
+        raise MI355XError("get_rows: one plain row for every index")
+    arr = _kv_rows(list(zip(caches, out)), "get_rows")
+    check(lib().mi355x_get_rows(arr, len(arr), ip, it, n, err.data_ptr() if err is not None else None, stream_handle()), "get_rows")
+    return out
+
+
+def _fa_q_args(q, k, v, mask, out, scale, softcap=0.0, max_bias=0.0):
+    a = FaQArgs()
+    many = q.dim() == 4
+    H, T, D = q.shape[-3:]
+    if q.dim() not in (3, 4) or len(k.shape) != q.dim() or len(v.shape) != q.dim() or out.dim() != q.dim():
+        raise MI355XError("flash_attn_q: q, k, v and out are all [H, T, D]-shaped or all [S, H, T, D]-shaped")
+    S = q.shape[0] if many else 1
+    HK, KV, DV = v.shape[-3:]
+    if k.shape != v.shape[:-1] + (D,) or (many and k.shape[0] != S) or tuple(out.shape) != ((S,) if many else ()) + (T, H, DV):
+        raise MI355XError(f"flash_attn_q: q {tuple(q.shape)}, k {k.shape}, v {v.shape} and out {tuple(out.shape)} do not fit")
+    if q.stride(-1) != 1 or out.stride(-1) != 1:
+        raise MI355XError("flash_attn_q: rows of q and out are contiguous")
+    for c, w in ((k, a.k), (v, a.v)):
+        if c.d is None:
+            raise MI355XError("flash_attn_q: an F16 cache is flash_attn's")
+        w.type, w.q_dev, w.d_dev = c.type, c.q.data_ptr(), c.d.data_ptr()
+        w.nb1, w.nb2, w.nb3 = c.nb[-1], c.nb[-2], c.nb[0] if many else 0
+    a.q_dev, a.q_nb1, a.q_nb2, a.q_nb3 = q.data_ptr(), q.stride(-2), q.stride(-3), q.stride(0) if many else 0
+    if mask is not None:
+        if (mask.dtype != _torch().float16 or mask.stride(-1) != 1 or mask.dim() not in (2, 3) or mask.shape[-2] < T
+                or mask.shape[-1] < KV or (mask.dim() == 3 and mask.shape[0] not in (1, S))):
+            raise MI355XError("flash_attn_q: the mask is fp16 [T', KV'], [1, T', KV'] or [S, T', KV'], T' >= T, KV' >= KV")
+        a.mask_dev, a.mask_nb1 = mask.data_ptr(), mask.stride(-2)
+        a.mask_nb3 = mask.stride(0) if mask.dim() == 3 and mask.shape[0] > 1 else 0
+    a.dst_dev, a.dst_nb1, a.dst_nb2, a.dst_nb3 = out.data_ptr(), out.stride(-2), out.stride(-3), out.stride(0) if many else 0
+    a.q_type, a.dst_type = _plain_type(q, "flash_attn_q"), _plain_type(out, "flash_attn_q")
+    a.D, a.DV, a.T, a.H, a.KV, a.HK, a.S = D, DV, T, H, KV, HK, S
+    a.scale, a.max_bias, a.softcap = scale, max_bias, softcap
+    return a
+
+
+def flash_attn_q_workspace(q, k, v, mask, out, nsplit: int = 0) -> int:
+    """Workspace bytes mi355x_flash_attn_q needs for these operands (0 for an unsupported op)."""
+    return int(lib().mi355x_flash_attn_q_workspace(ctypes.byref(_fa_q_args(q, k, v, mask, out, 1.0)), nsplit))
+
+
+def flash_attn_q(q, k: KvCache, v: KvCache, mask, scale: float, softcap: float = 0.0, nsplit: int = 0, out=None, workspace=None,
+                 max_bias: float = 0.0):
+    """FLASH_ATTN_EXT over a quantized cache: q [H, T, D] or [S, H, T, D] (F32 or F16), k and v KvCache
+    views [(S,) HK, KV, D] of Q8_0 or Q4_0, mask fp16 [T', KV'], [S, T', KV'] (S or 1) or None. Returns dst
+    [(S,) T, H, DV], F32 unless `out` is F16."""
+    torch = _torch()
+    if out is None:
+        H, T = q.shape[-3:-1]
+        out = torch.empty(tuple(q.shape[:-3]) + (T, H, v.shape[-1]), dtype=torch.float32, device=q.device)
+    a = _fa_q_args(q, k, v, mask, out, scale, softcap, max_bias)
+    if workspace is None:
+        need = int(lib().mi355x_flash_attn_q_workspace(ctypes.byref(a), nsplit))
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    check(lib().mi355x_flash_attn_q(ctypes.byref(a), nsplit, workspace.data_ptr(), workspace.numel(), stream_handle()), "flash_attn_q")
     return out
 
 

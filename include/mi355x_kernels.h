@@ -302,6 +302,86 @@ MI355X_API int mi355x_flash_attn(const mi355x_fa_args * a, int nsplit,
 MI355X_API int mi355x_flash_attn_ex(const mi355x_fa_args * a, int nsplit, int flags,
                                     void * workspace_dev, size_t workspace_bytes, void * stream);
 
+/* ---- the quantized KV cache: SET_ROWS, GET_ROWS, FLASH_ATTN_EXT over it ---------------------- */
+
+/* A cache of type MI355X_Q8_0 or MI355X_Q4_0 is two planes that share one set of element strides
+ * (every stride a multiple of 32, the block length): the codes (element e at byte e for Q8_0, byte
+ * e / 2 for Q4_0) and the blocks' fp16 scales (the scale of element e at index e / 32). Inside a
+ * block of 32 the bytes are ggml's: Q8_0 an int8 a value, Q4_0 16 bytes with value j in the low and
+ * value j + 16 in the high nibble of byte j; Q8_0 stands for d * code, Q4_0 for d * (code - 8). So a
+ * cache that mi355x_weight_pack made from ggml blocks is one too, its scales right behind its codes.
+ * An MI355X_F16 cache is the plain fp16 tensor, without scales. */
+
+/* The rows of one cache and plain values beside them. Strides in ELEMENTS. */
+typedef struct mi355x_kv_rows {
+    int type;                 /* MI355X_Q8_0, MI355X_Q4_0 or MI355X_F16 */
+    void * q_dev;             /* codes (F16: values) of the cache, 16-byte aligned */
+    uint16_t * d_dev;         /* block scales, 8-byte aligned (F16: not read) */
+    int64_t n_rows;           /* rows of the cache: an index lies in [0, n_rows) */
+    int64_t nb1, nb2;         /* row and head strides of the cache */
+    int64_t H, D;             /* heads a row, values a head (D % 32 == 0) */
+    int x_type;               /* the plain values: 0 F32 or 1 F16 */
+    void * x_dev;             /* [n][H][D], 16-byte aligned */
+    int64_t x_nb1, x_nb2;     /* their row and head strides (multiples of 8) */
+} mi355x_kv_rows;
+
+/* ggml's SET_ROWS into a cache: row i of the plain values of each of `n_out` (1..4) caches is
+ * quantized and written to cache row idx[i], for every i < n, in ONE launch (a layer's K and V share
+ * their indices). idx_dev: int32 (idx_type 26) or int64 (27) [n] on the device, or NULL for idx[i] = i.
+ * Where an index repeats, the row with the largest i stays, whole. An index outside [0, n_rows)
+ * writes nothing and sets *err_dev (a device int32, may be NULL) to 1. Rows that no index names keep
+ * their bytes.
+ * Bits are those of ggml's reference quantizers: Q8_0 d = max|x| / 127, Q4_0 d = (the value of largest
+ * magnitude, the first of equals) / -8, code = x * (1 / d) rounded half away from zero (Q4_0: plus 8.5,
+ * truncated, at most 15), each step rounded to f32, d stored as fp16 (infinite past 65504, as
+ * ggml's). A block that holds a NaN or an infinity, for which ggml defines nothing, is stored with
+ * a NaN scale and reads back as NaN. F16: round to nearest even.
+ * No counterpart in the reference, whose host writes its caches on the CPU. */
+MI355X_API int mi355x_set_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
+                               int32_t * err_dev, void * stream);
+
+/* ggml's GET_ROWS from a cache: cache row idx[i] as plain values in row i of x, for each of `n_out`
+ * caches, in ONE launch. F32 values are exact; F16 ones are rounded once (mi355x_weight_dequant_f16's
+ * values). Indices as in mi355x_set_rows; one outside [0, n_rows) leaves its row of x unwritten and
+ * sets *err_dev. */
+MI355X_API int mi355x_get_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
+                               int32_t * err_dev, void * stream);
+
+/* A quantized K or V: strides in ELEMENTS, multiples of 32. */
+typedef struct mi355x_kv_view {
+    int type;                          /* MI355X_Q8_0 or MI355X_Q4_0 */
+    const void * q_dev;                /* codes, 16-byte aligned */
+    const uint16_t * d_dev;            /* block scales, 8-byte aligned */
+    int64_t nb1, nb2, nb3;             /* key, KV head and sequence strides */
+} mi355x_kv_view;
+
+/* One attention op over a quantized cache, for S sequences (ggml's ne[3]). Strides in ELEMENTS. */
+typedef struct mi355x_fa_q_args {
+    const void * q_dev;       int64_t q_nb1, q_nb2, q_nb3;     /* token, head, sequence strides */
+    mi355x_kv_view k, v;
+    const uint16_t * mask_dev; int64_t mask_nb1, mask_nb3;     /* fp16; token, sequence strides (nb3 0: one mask for all); NULL = unmasked */
+    void * dst_dev;           int64_t dst_nb1, dst_nb2, dst_nb3;  /* head, token, sequence strides */
+    int q_type, dst_type;                                      /* 0 F32 or 1 F16 */
+    int D, DV, T, H, KV, HK, S;
+    float scale, max_bias, softcap;
+} mi355x_fa_q_args;
+
+/* Workspace bytes of mi355x_flash_attn_q with `nsplit` KV splits (0 = its own choice); 0 for an op it
+ * does not take. 256-byte aligned. */
+MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int nsplit);
+
+/* mi355x_flash_attn with K and V in a quantized cache, each Q8_0 or Q4_0: dst = softmax(cap(scale *
+ * q.k) + mask) . v. K and V enter the products as fp16 (their values rounded once), Q and P as fp16,
+ * sums in F32: an F32 dst holds values of that accuracy. Cache values past fp16's range count as its
+ * largest (65504). D and DV are multiples of 32 up to 256; H % HK == 0; max_bias 0. A key that the
+ * mask hides from a query (-inf) adds nothing to it, whatever the cache holds there, NaN included; a
+ * key with a scale that is not finite makes the rows of the queries that see it NaN; rows whose every
+ * key is hidden are written as zeros. q rows 16-byte, dst rows 16-byte (F16: 8), mask rows 8-byte
+ * aligned.
+ * Concurrent calls must not share a workspace. Equal inputs give equal bits. */
+MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
+                                   void * stream);
+
 /* ---- MUL_MAT_ID --------------------------------------------------------------------------- */
 
 /* One expert-GEMM op. Strides in ELEMENTS. */
