@@ -737,6 +737,44 @@ static mi355x_fa_args fa_q_lower(const mi355x_fa_q_args * a, int s, const uint16
     return f;
 }
 
+// The direct form: the kernel of mx_fa_q.h on the cache as it is stored.
+static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
+    mx::FaQArgs f;
+    memset(&f, 0, sizeof f);
+    f.q = a->q_dev; f.k = fa_q_view(a->k, 0); f.v = fa_q_view(a->v, 0); f.mask = a->mask_dev; f.dst = a->dst_dev;
+    f.q_nb1 = a->q_nb1; f.q_nb2 = a->q_nb2; f.q_nb3 = a->q_nb3; f.mask_nb1 = a->mask_nb1; f.mask_nb3 = a->mask_nb3;
+    f.dst_nb1 = a->dst_nb1; f.dst_nb2 = a->dst_nb2; f.dst_nb3 = a->dst_nb3;
+    mx::fa_pad_dims(a->D, a->DV, f.D, f.DV);
+    f.dk = a->D; f.dv = a->DV;
+    f.T = a->T; f.HK = a->HK; f.KV = a->KV; f.S = a->S; f.G = a->H / a->HK; f.R = a->T * f.G;
+    f.scale = a->scale; f.softcap = a->softcap;
+    f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
+    f.nq = 1;
+    while (f.nq < mx::fa_q_max_nq(f.DV) && 16 * f.nq < f.R) f.nq *= 2;
+    f.nrt = (f.R + 16 * f.nq - 1) / (16 * f.nq);
+    const int64_t units = (int64_t)f.S * f.HK * f.nrt, ntiles = (f.KV + 31) / 32;
+    f.nsplit = nsplit > 0 ? nsplit
+                          : (int)std::max<int64_t>(1, std::min<int64_t>({64, 2 * device_cus() / std::max<int64_t>(1, units), ntiles / 8}));
+    return f;
+}
+static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
+    if (a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
+    if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
+        if (*e) return atoi(e) != 0;
+    return a->H / a->HK * a->T <= 64;
+}
+struct FaQDirectLayout {
+    size_t po, pml, total;
+};
+static FaQDirectLayout fa_q_direct_layout(const mx::FaQArgs & f) {
+    FaQDirectLayout L;
+    const size_t parts = f.nsplit > 1 ? (size_t)f.S * f.HK * f.nrt * f.nsplit : 0;
+    L.po = 0;
+    L.pml = parts * f.nq * (f.DV / 16) * 1024;
+    L.total = L.pml + align256(parts * f.nq * 16 * 8) + 256;
+    return L;
+}
+
 // Workspace of the decode-first form: one sequence's K and V as fp16, then the fused kernel's own.
 struct FaQLayout {
     size_t k, v, fa, total;
@@ -754,7 +792,8 @@ static FaQLayout fa_q_layout(const mi355x_fa_q_args * a, int nsplit) {
 }
 
 MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int nsplit) {
-    return fa_q_check(a) != MI355X_OK || nsplit > 64 ? 0 : fa_q_layout(a, nsplit).total;
+    if (fa_q_check(a) != MI355X_OK || nsplit > 64) return 0;
+    return fa_q_is_direct(a) ? fa_q_direct_layout(fa_q_direct(a, nsplit)).total : fa_q_layout(a, nsplit).total;
 }
 
 MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
@@ -763,6 +802,14 @@ MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void 
     if (st != MI355X_OK) return st;
     if (nsplit > 64) return MI355X_E_ARG;
     if (a->T == 0 || a->S == 0) return MI355X_OK;
+    if (fa_q_is_direct(a)) {
+        mx::FaQArgs f = fa_q_direct(a, nsplit);
+        const FaQDirectLayout L = fa_q_direct_layout(f);
+        if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
+        f.part_o = (float *)((char *)workspace_dev + L.po);
+        f.part_ml = (float *)((char *)workspace_dev + L.pml);
+        return hip_status(mx::launch_fa_q(f, S(stream)));
+    }
     const FaQLayout L = fa_q_layout(a, nsplit);
     if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
     char * ws = (char *)workspace_dev;

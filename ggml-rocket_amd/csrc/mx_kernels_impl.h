@@ -83,6 +83,29 @@ struct KvView {
     int64_t nb1, nb2, nb3;
     int type;
 };
+// FLASH_ATTN_EXT of few rows over a quantized cache: strides in elements.
+struct FaQArgs {
+    const void * q;            // F32 or F16
+    KvView k, v;
+    const uint16_t * mask;     // or null
+    void * dst;                // F32 or F16
+    float * part_o;            // KV splits: [unit][nsplit][O^T tile][lane][4], unit = (s HK + hk) nrt + rt
+    float * part_ml;           // [unit][nsplit][16 nq rows][2]: (max, sum)
+    int64_t q_nb1, q_nb2, q_nb3, mask_nb1, mask_nb3, dst_nb1, dst_nb2, dst_nb3;
+    int D, DV, dk, dv;         // built and actual head dims
+    int T, HK, KV, S, G, R;    // G = H / HK; R = T G query rows share a KV head
+    int nq, nrt, nsplit;       // 16-row query tiles a wave, blocks of rows, KV splits
+    float scale, softcap;
+    bool q_f16, dst_f16;
+};
+constexpr int64_t FA_Q_MAX_NB1 = 1 << 24;   // its 32-bit offsets inside a 32-key tile
+inline int fa_q_max_nq(int DV) { return DV <= 128 ? 4 : 2; }
+hipError_t launch_fa_q(const FaQArgs & a, hipStream_t st);
+hipError_t launch_fa_q_combine(const FaQArgs & a, int vt, int DV, int NQ, hipStream_t st);
+hipError_t launch_fa_q_Q8_0_Q8_0(const FaQArgs & a, hipStream_t st);
+hipError_t launch_fa_q_Q8_0_Q4_0(const FaQArgs & a, hipStream_t st);
+hipError_t launch_fa_q_Q4_0_Q8_0(const FaQArgs & a, hipStream_t st);
+hipError_t launch_fa_q_Q4_0_Q4_0(const FaQArgs & a, hipStream_t st);
 // K and V of one sequence as fp16 for the fused attention: k16 [HK][KV][D], v16 [HK][KV][DV].
 struct KvDecodeArgs {
     KvView k, v;

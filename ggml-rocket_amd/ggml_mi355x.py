@@ -329,14 +329,16 @@ def flash_attn(q, k, v, mask, scale: float, softcap: float = 0.0, nsplit: int = 
 
 
 # ---- the quantized KV cache -----------------------------------------------------------------
+# Decoding calls these once a layer and token, so they avoid what costs microseconds: a cache keeps its
+# part of the C structs, and structs are filled in one call.
 
 class KvCache:
     """A K or V cache on the device, of any leading dims: `q` holds the codes (Q8_0: int8 [..., D];
     Q4_0: uint8 [..., D / 2]; F16: the fp16 values, without `d`), `d` the blocks' fp16 scales
-    [..., D / 32]. Both planes have the same element strides; permute and slices of the leading dims
+    [..., D / 32]. Both planes have the same element strides; permute and indexing of the leading dims
     give views."""
 
-    __slots__ = ("type", "q", "d", "D", "shape", "nb")
+    __slots__ = ("type", "q", "d", "D", "shape", "nb", "dev", "_tail", "_rows", "_view")
 
     def __init__(self, ttype: int, q, d=None):
         torch = _torch()
@@ -348,6 +350,7 @@ class KvCache:
         self.D = q.shape[-1] * per
         self.shape = tuple(q.shape[:-1]) + (self.D,)
         self.nb = tuple(s * per for s in q.stride()[:-1])
+        self.dev = q.get_device()
         if ttype == F16:
             if d is not None:
                 raise MI355XError("KvCache: an F16 cache has no scales")
@@ -355,13 +358,26 @@ class KvCache:
               or tuple(d.shape) != self.shape[:-1] + (self.D // 32,) or (d.stride(-1) != 1 and d.shape[-1] > 1)
               or any(n > 1 and a != 32 * b for n, a, b in zip(q.shape[:-1], self.nb, d.stride()))):
             raise MI355XError("KvCache: the scales are not fp16 of the codes' shape and strides / 32")
+        n, nb, qp, dp = len(self.shape), self.nb, q.data_ptr(), None if d is None else d.data_ptr()
+        # the cache's part of mi355x_kv_rows ([rows, D] or [rows, H, D]) and of mi355x_fa_q_args ([(S,) HK, KV, D])
+        self._tail = self.shape[1:]
+        self._rows = {2: (ttype, qp, dp, self.shape[0], nb[0], 0, 1, self.D),
+                      3: (ttype, qp, dp, self.shape[0], nb[0], nb[-1], self.shape[1], self.D)}.get(n)
+        self._view = KvView(ttype, qp, dp, nb[-1], nb[-2], nb[0] if n == 4 else 0) if n in (3, 4) and d is not None else None
 
     def permute(self, *dims):
         """A view with the leading dims in another order; the last dim stays last."""
+        lead = len(self.shape) - 1
+        if len(dims) == lead:
+            dims = dims + (lead,)
+        if dims[-1] not in (lead, -1):
+            raise MI355XError("KvCache.permute: the last dim stays last")
         return KvCache(self.type, self.q.permute(*dims), None if self.d is None else self.d.permute(*dims))
 
     def __getitem__(self, at):
         """A view by indices and slices of leading dims."""
+        if isinstance(at, tuple) and (len(at) >= len(self.shape) or any(i is Ellipsis or i is None for i in at)):
+            raise MI355XError("KvCache: indices of leading dims only")
         return KvCache(self.type, self.q[at], None if self.d is None else self.d[at])
 
 
@@ -378,99 +394,119 @@ def kv_cache(ttype: int, *shape, device="cuda") -> KvCache:
     return KvCache(ttype, q, torch.zeros(*lead, D // 32, dtype=torch.float16, device=device))
 
 
-def _plain_type(t, what):
-    torch = _torch()
-    if t.dtype == torch.float32:
-        return F32
-    if t.dtype == torch.float16:
-        return F16
-    raise MI355XError(f"{what}: {t.dtype} is neither F32 nor F16")
+_plain = {}
 
 
-def _kv_rows(pairs, what):
-    """mi355x_kv_rows of (cache [rows, H, D] or [rows, D], plain rows of the same trailing dims)."""
-    arr = (KvRows * len(pairs))()
-    for a, (c, x) in zip(arr, pairs):
-        if len(c.shape) not in (2, 3) or tuple(x.shape[1:]) != c.shape[1:] or x.stride(-1) != 1 or x.device != c.q.device:
-            raise MI355XError(f"{what}: rows {tuple(x.shape)} do not fit a cache {c.shape}")
-        two = len(c.shape) == 2
-        a.type, a.q_dev, a.d_dev, a.n_rows = c.type, c.q.data_ptr(), None if c.d is None else c.d.data_ptr(), c.shape[0]
-        a.nb1, a.nb2, a.H, a.D = c.nb[0], 0 if two else c.nb[1], 1 if two else c.shape[1], c.D
-        a.x_type, a.x_dev = _plain_type(x, what), x.data_ptr()
-        a.x_nb1, a.x_nb2 = x.stride(0), 0 if two else x.stride(1)
-    return arr
+def _plain_types():
+    if not _plain:
+        torch = _torch()
+        _plain.update({torch.float32: F32, torch.float16: F16, torch.int32: I32, torch.int64: I64})
+    return _plain
 
 
-def _kv_index(idx, n, device, what):
+def _launch_stream(dev: int, what: str):
+    """The current stream's handle, for tensors of the current device."""
+    C = _torch()._C
+    if dev < 0 or dev != C._cuda_getDevice():
+        raise MI355XError(f"{what}: the tensors are not on the current GPU")
+    return C._cuda_getCurrentRawStream(dev)
+
+
+_KV_ROWS = [None] + [KvRows * n for n in range(1, 5)]
+
+
+def _kv_rows(caches, plain, n, what):
+    """mi355x_kv_rows of caches [rows, H, D] or [rows, D] and their plain rows [n, H, D] or [n, D]."""
+    types, out = _plain_types(), []
+    if not 1 <= len(caches) <= 4:
+        raise MI355XError(f"{what}: one to four caches")
+    for c, x in zip(caches, plain):
+        shape, stride, t = x.shape, x.stride(), types.get(x.dtype)
+        if c._rows is None or shape[1:] != c._tail or shape[0] != n or stride[-1] != 1 or t not in (F32, F16) or x.get_device() != c.dev:
+            raise MI355XError(f"{what}: rows {x.dtype} {tuple(shape)} do not fit {n} rows of a cache {c.shape}")
+        out.append(KvRows(*c._rows, t, x.data_ptr(), stride[0], stride[1] if len(stride) == 3 else 0))
+    return _KV_ROWS[len(out)](*out)
+
+
+def _kv_index(idx, n, dev, what):
     """(address, ggml type, count) of the row indices."""
     if idx is None:
         return None, I32, n
-    torch = _torch()
-    if idx.dtype not in (torch.int32, torch.int64) or idx.dim() != 1 or not idx.is_contiguous() or idx.device != device:
+    t = _plain_types().get(idx.dtype)
+    if t not in (I32, I64) or idx.dim() != 1 or not idx.is_contiguous() or idx.get_device() != dev:
         raise MI355XError(f"{what}: indices are int32 or int64, contiguous, on the cache's device")
-    return idx.data_ptr(), I64 if idx.dtype == torch.int64 else I32, idx.shape[0]
+    return idx.data_ptr(), t, idx.shape[0]
+
+
+def _kv_err(err, dev, what):
+    if err is None:
+        return None
+    if _plain_types().get(err.dtype) != I32 or err.get_device() != dev or err.numel() < 1:
+        raise MI355XError(f"{what}: err is an int32 on the cache's device")
+    return err.data_ptr()
 
 
 def set_rows(pairs, idx=None, err=None):
     """pairs: (cache, x) for up to four caches [rows, H, D] (or [rows, D]) and plain rows x [n, H, D]
     (F32 or F16): x[i] is quantized into cache row idx[i] (int32 or int64 [n]; None: i). One launch.
     err: a device int32 that an index out of range sets to 1."""
-    arr = _kv_rows(pairs, "set_rows")
-    n = pairs[0][1].shape[0]
-    ip, it, ni = _kv_index(idx, n, pairs[0][0].q.device, "set_rows")
-    if any(x.shape[0] != ni for _, x in pairs):
-        raise MI355XError("set_rows: one plain row for every index")
-    check(lib().mi355x_set_rows(arr, len(arr), ip, it, ni, err.data_ptr() if err is not None else None, stream_handle()), "set_rows")
+    caches, plain = zip(*pairs)
+    dev = caches[0].dev
+    ip, it, n = _kv_index(idx, plain[0].shape[0], dev, "set_rows")
+    if any(c.dev != dev for c in caches):
+        raise MI355XError("set_rows: caches on one device")
+    arr = _kv_rows(caches, plain, n, "set_rows")
+    check(lib().mi355x_set_rows(arr, len(arr), ip, it, n, _kv_err(err, dev, "set_rows"), _launch_stream(dev, "set_rows")), "set_rows")
 
 
 def get_rows(caches, idx=None, dtype=None, out=None, err=None):
     """Rows idx[i] (None: all, in order) of each of up to four caches as plain values: a list of
     [n, H, D] (or [n, D]) tensors of `dtype` (F32 by default), or `out`. One launch."""
-    torch = _torch()
-    ip, it, n = _kv_index(idx, caches[0].shape[0], caches[0].q.device, "get_rows")
+    dev = caches[0].dev
+    ip, it, n = _kv_index(idx, caches[0].shape[0], dev, "get_rows")
+    if any(c.dev != dev for c in caches):
+        raise MI355XError("get_rows: caches on one device")
     if out is None:
-        out = [torch.empty((n,) + c.shape[1:], dtype=dtype or torch.float32, device=c.q.device) for c in caches]
-    if any(x.shape[0] != n for x in out) or len(out) != len(caches):
-        raise MI355XError("get_rows: one plain row for every index")
-    arr = _kv_rows(list(zip(caches, out)), "get_rows")
-    check(lib().mi355x_get_rows(arr, len(arr), ip, it, n, err.data_ptr() if err is not None else None, stream_handle()), "get_rows")
+        torch = _torch()
+        out = [torch.empty((n,) + c._tail, dtype=dtype or torch.float32, device=c.q.device) for c in caches]
+    elif len(out) != len(caches):
+        raise MI355XError("get_rows: one output for every cache")
+    arr = _kv_rows(caches, out, n, "get_rows")
+    check(lib().mi355x_get_rows(arr, len(arr), ip, it, n, _kv_err(err, dev, "get_rows"), _launch_stream(dev, "get_rows")), "get_rows")
     return out
 
 
 def _fa_q_args(q, k, v, mask, out, scale, softcap=0.0, max_bias=0.0):
-    a = FaQArgs()
-    many = q.dim() == 4
-    H, T, D = q.shape[-3:]
-    if q.dim() not in (3, 4) or len(k.shape) != q.dim() or len(v.shape) != q.dim() or out.dim() != q.dim():
+    types, qs, os, kv = _plain_types(), q.shape, out.shape, v.shape
+    nd, dev = len(qs), q.get_device()
+    if nd not in (3, 4) or len(k.shape) != nd or len(kv) != nd or len(os) != nd:
         raise MI355XError("flash_attn_q: q, k, v and out are all [H, T, D]-shaped or all [S, H, T, D]-shaped")
-    S = q.shape[0] if many else 1
-    HK, KV, DV = v.shape[-3:]
-    if k.shape != v.shape[:-1] + (D,) or (many and k.shape[0] != S) or tuple(out.shape) != ((S,) if many else ()) + (T, H, DV):
-        raise MI355XError(f"flash_attn_q: q {tuple(q.shape)}, k {k.shape}, v {v.shape} and out {tuple(out.shape)} do not fit")
-    if q.stride(-1) != 1 or out.stride(-1) != 1:
-        raise MI355XError("flash_attn_q: rows of q and out are contiguous")
-    for c, w in ((k, a.k), (v, a.v)):
-        if c.d is None:
-            raise MI355XError("flash_attn_q: an F16 cache is flash_attn's")
-        w.type, w.q_dev, w.d_dev = c.type, c.q.data_ptr(), c.d.data_ptr()
-        w.nb1, w.nb2, w.nb3 = c.nb[-1], c.nb[-2], c.nb[0] if many else 0
-    a.q_dev, a.q_nb1, a.q_nb2, a.q_nb3 = q.data_ptr(), q.stride(-2), q.stride(-3), q.stride(0) if many else 0
+    H, T, D = qs[-3], qs[-2], qs[-1]
+    HK, KV, DV = kv[-3:]
+    S = qs[0] if nd == 4 else 1
+    if k.shape != kv[:-1] + (D,) or (nd == 4 and (kv[0] != S or os[0] != S)) or os[-3] != T or os[-2] != H or os[-1] != DV:
+        raise MI355XError(f"flash_attn_q: q {tuple(qs)}, k {k.shape}, v {kv} and out {tuple(os)} do not fit")
+    if k._view is None or v._view is None:
+        raise MI355XError("flash_attn_q: an F16 cache is flash_attn's")
+    qn, on, qt, ot = q.stride(), out.stride(), types.get(q.dtype), types.get(out.dtype)
+    if qn[-1] != 1 or on[-1] != 1 or qt not in (F32, F16) or ot not in (F32, F16):
+        raise MI355XError("flash_attn_q: q and out are F32 or F16 with contiguous rows")
+    if k.dev != dev or v.dev != dev or out.get_device() != dev or (mask is not None and mask.get_device() != dev):
+        raise MI355XError("flash_attn_q: all tensors on one device")
+    mp, m1, m3 = None, 0, 0
     if mask is not None:
-        if (mask.dtype != _torch().float16 or mask.stride(-1) != 1 or mask.dim() not in (2, 3) or mask.shape[-2] < T
-                or mask.shape[-1] < KV or (mask.dim() == 3 and mask.shape[0] not in (1, S))):
+        ms, mn = mask.shape, mask.stride()
+        if (types.get(mask.dtype) != F16 or mn[-1] != 1 or len(ms) not in (2, 3) or ms[-2] < T or ms[-1] < KV
+                or (len(ms) == 3 and ms[0] not in (1, S))):
             raise MI355XError("flash_attn_q: the mask is fp16 [T', KV'], [1, T', KV'] or [S, T', KV'], T' >= T, KV' >= KV")
-        a.mask_dev, a.mask_nb1 = mask.data_ptr(), mask.stride(-2)
-        a.mask_nb3 = mask.stride(0) if mask.dim() == 3 and mask.shape[0] > 1 else 0
-    a.dst_dev, a.dst_nb1, a.dst_nb2, a.dst_nb3 = out.data_ptr(), out.stride(-2), out.stride(-3), out.stride(0) if many else 0
-    a.q_type, a.dst_type = _plain_type(q, "flash_attn_q"), _plain_type(out, "flash_attn_q")
-    a.D, a.DV, a.T, a.H, a.KV, a.HK, a.S = D, DV, T, H, KV, HK, S
-    a.scale, a.max_bias, a.softcap = scale, max_bias, softcap
-    return a
+        mp, m1, m3 = mask.data_ptr(), mn[-2], mn[0] if len(ms) == 3 and ms[0] > 1 else 0
+    return FaQArgs(q.data_ptr(), qn[-2], qn[-3], qn[0] if nd == 4 else 0, k._view, v._view, mp, m1, m3,
+                   out.data_ptr(), on[-2], on[-3], on[0] if nd == 4 else 0, qt, ot, D, DV, T, H, KV, HK, S, scale, max_bias, softcap)
 
 
 def flash_attn_q_workspace(q, k, v, mask, out, nsplit: int = 0) -> int:
     """Workspace bytes mi355x_flash_attn_q needs for these operands (0 for an unsupported op)."""
-    return int(lib().mi355x_flash_attn_q_workspace(ctypes.byref(_fa_q_args(q, k, v, mask, out, 1.0)), nsplit))
+    return int(lib().mi355x_flash_attn_q_workspace(_fa_q_args(q, k, v, mask, out, 1.0), nsplit))
 
 
 def flash_attn_q(q, k: KvCache, v: KvCache, mask, scale: float, softcap: float = 0.0, nsplit: int = 0, out=None, workspace=None,
@@ -484,9 +520,12 @@ def flash_attn_q(q, k: KvCache, v: KvCache, mask, scale: float, softcap: float =
         out = torch.empty(tuple(q.shape[:-3]) + (T, H, v.shape[-1]), dtype=torch.float32, device=q.device)
     a = _fa_q_args(q, k, v, mask, out, scale, softcap, max_bias)
     if workspace is None:
-        need = int(lib().mi355x_flash_attn_q_workspace(ctypes.byref(a), nsplit))
+        need = int(lib().mi355x_flash_attn_q_workspace(a, nsplit))
         workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
-    check(lib().mi355x_flash_attn_q(ctypes.byref(a), nsplit, workspace.data_ptr(), workspace.numel(), stream_handle()), "flash_attn_q")
+    elif workspace.get_device() != k.dev:
+        raise MI355XError("flash_attn_q: the workspace is on another device")
+    check(lib().mi355x_flash_attn_q(a, nsplit, workspace.data_ptr(), workspace.nbytes, _launch_stream(k.dev, "flash_attn_q")),
+          "flash_attn_q")
     return out
 
 

@@ -26,6 +26,13 @@ def mx(torch_cuda):
     return ggml_mi355x
 
 
+@pytest.fixture(params=["1", "0", ""], ids=["direct", "decoded", "chosen"])
+def form(request, monkeypatch):
+    """Attention tests run under both forms (the kernel that reads the cache as it is stored; the cache
+    decoded to fp16 first, which is the fp16 kernel's arithmetic) and the library's choice per call."""
+    monkeypatch.setenv("MI355X_FA_Q_DIRECT", request.param)
+
+
 def gpu(a):
     import torch
     return torch.from_numpy(np.ascontiguousarray(a)).cuda()
@@ -236,7 +243,7 @@ def check(got, q, kn, vn, mask, scale, softcap=0.0, half_out=False, what=""):
 
 @pytest.mark.parametrize("types", MIXES, ids=ids)
 @pytest.mark.parametrize("T,KV", [(1, 1), (1, 2), (1, 33), (1, 777), (3, 64), (7, 1000), (16, 129), (33, 500), (70, 389)])
-def test_attention_lengths(mx, types, T, KV):
+def test_attention_lengths(mx, form, types, T, KV):
     """From one token on one key to ragged prompts, GQA of four, causal."""
     H, HK, D = 8, 2, 128
     q, kn, vn, kc, vc = attn_case(mx, *types, 1, T, H, HK, KV, D, D)
@@ -250,7 +257,7 @@ def test_attention_lengths(mx, types, T, KV):
 @pytest.mark.parametrize("D,DV,H,HK", [(32, 32, 4, 4), (64, 64, 6, 3), (96, 96, 5, 1), (128, 64, 8, 2), (160, 96, 4, 2), (192, 128, 16, 2),
                                        (256, 256, 8, 4), (224, 160, 9, 3)])
 @pytest.mark.parametrize("T", [1, 5, 40])
-def test_attention_head_dims(mx, types, D, DV, H, HK, T):
+def test_attention_head_dims(mx, form, types, D, DV, H, HK, T):
     """Head dims that are multiples of 32, groups from 1 to 8 and odd ones, a soft-cap, no mask."""
     KV, cap = 203, 10.0
     q, kn, vn, kc, vc = attn_case(mx, *types, 1, T, H, HK, KV, D, DV, head_major=T == 5)
@@ -260,7 +267,7 @@ def test_attention_head_dims(mx, types, D, DV, H, HK, T):
 
 @pytest.mark.parametrize("types", [MIXES[0], MIXES[2]], ids=ids)
 @pytest.mark.parametrize("T,half", [(1, False), (1, True), (6, True), (40, True)])
-def test_attention_streams(mx, types, T, half):
+def test_attention_streams(mx, form, types, T, half):
     """Five sequences of different lengths (one of them empty), fp16 queries and outputs, outputs with a
     wider row stride left alone beside it."""
     import torch
@@ -280,7 +287,7 @@ def test_attention_streams(mx, types, T, half):
 
 @pytest.mark.parametrize("types", MIXES, ids=ids)
 @pytest.mark.parametrize("T", [1, 9, 64])
-def test_attention_mask_holes(mx, types, T):
+def test_attention_mask_holes(mx, form, types, T):
     """Scattered hidden keys, whole hidden tiles, rows that see nothing, masks of fp16's lowest value,
     biases; what the cache holds under a mask that hides it from every query (NaN and infinite
     scales, all codes) does not matter."""
@@ -311,7 +318,7 @@ def test_attention_mask_holes(mx, types, T):
 
 @pytest.mark.parametrize("T", [1, 9, 64])
 @pytest.mark.parametrize("plane", ["k", "v"])
-def test_attention_nan_reaches_who_sees_it(mx, T, plane):
+def test_attention_nan_reaches_who_sees_it(mx, form, T, plane):
     """A visible key whose scale is NaN makes the rows of the queries that see it NaN, and no others."""
     H, HK, D, KV = 4, 2, 64, 200
     q, kn, vn, kc, vc = attn_case(mx, Q8_0, Q4_0, 1, T, H, HK, KV, D, D, seed=8)
@@ -329,7 +336,7 @@ def test_attention_nan_reaches_who_sees_it(mx, T, plane):
 
 @pytest.mark.parametrize("types", [MIXES[0], MIXES[1]], ids=ids)
 @pytest.mark.parametrize("T", [1, 40])
-def test_attention_ranges(mx, types, T):
+def test_attention_ranges(mx, form, types, T):
     """Scores past fp16 (one key wins by far), queries whose scaled values pass fp16, caches of tiny
     and of large values, and blocks of very different scales."""
     H, HK, D, KV = 4, 2, 64, 300
@@ -348,7 +355,7 @@ def test_attention_ranges(mx, types, T):
         assert (np.abs(got[0] - want) <= tol + 2.0 ** -25).all(), (up, float((np.abs(got[0] - want) - tol).max()))
 
 
-def test_attention_no_keys(mx):
+def test_attention_no_keys(mx, form):
     """KV = 0: zeros."""
     import torch
     kc, vc = mx.kv_cache(Q8_0, 2, 8, 64)[:, :0], mx.kv_cache(Q4_0, 2, 8, 64)[:, :0]
@@ -357,7 +364,7 @@ def test_attention_no_keys(mx):
         assert (cpu(got) == 0).all()
 
 
-def test_attention_same_bits_and_same_as_a_decoded_cache(mx):
+def test_attention_same_bits_and_same_as_a_decoded_cache(mx, form):
     """Two calls give equal bits; the fp16 attention on the cache read back as fp16 agrees."""
     import torch
     H, HK, D = 8, 2, 128
@@ -374,7 +381,7 @@ def test_attention_same_bits_and_same_as_a_decoded_cache(mx):
 
 # ---- together -------------------------------------------------------------------------------
 
-def test_decode_loop_on_another_stream_and_in_a_graph(mx):
+def test_decode_loop_on_another_stream_and_in_a_graph(mx, form):
     """A sequence grown as it would be: a prompt stored and attended to, then token by token, on a
     stream of its own; the last token's step captured into a graph and replayed with new inputs and
     eager work in between, each replay equal to the eager step."""
