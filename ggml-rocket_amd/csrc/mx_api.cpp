@@ -755,10 +755,12 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
     const int64_t units = (int64_t)f.S * f.HK * f.nrt, ntiles = (f.KV + 31) / 32;
     f.nsplit = nsplit > 0 ? nsplit
                           : (int)std::max<int64_t>(1, std::min<int64_t>({64, 2 * device_cus() / std::max<int64_t>(1, units), ntiles / 8}));
+    f.div_nrt = mx::fq_div_by(f.nrt); f.div_hk = mx::fq_div_by(f.HK); f.div_split = mx::fq_div_by(f.nsplit);
+    f.div_g = mx::fq_div_by(f.G);
     return f;
 }
 static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
-    if (a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
+    if (a->KV < mx::FA_Q_MIN_KV || a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
     if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
         if (*e) return atoi(e) != 0;
     return a->H / a->HK * a->T <= 64;

@@ -5,42 +5,73 @@
 namespace mx {
 
 // Merges the splits of one O^T tile of one unit of rows: O = sum_s exp(m_s - M) O_s / sum_s exp(m_s - M) l_s.
-// Four waves take the splits in turn. Rows whose maxima are all -inf have sums of zero (or NaN, kept).
+// Every partial of the tile is requested at once, split i by wave i % 4, and the splits' weights are
+// formed while they come: one memory round trip. Rows whose maxima are all -inf have sums of zero (or
+// NaN, kept).
+constexpr int FQ_MAX_SPLIT = 64;
 __global__ void __launch_bounds__(256) fa_q_combine_kernel(FaQArgs a, int vt, int DV, int NQ) {
+    __shared__ float sm[16][17], sl[16][17], sw[FQ_MAX_SPLIT][16];
     __shared__ float4v so[4][WAVE];
-    __shared__ float sl[4][WAVE];
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, r = lane % 16, g = lane / 16;
+    const int t = threadIdx.x, lane = t % WAVE, wave = t / WAVE, r = lane % 16, g = lane / 16;
     const int TT = DV / 16, all = TT * NQ;
     const int at = blockIdx.x % all, n = at / TT, q = at % TT;
-    const int64_t unit = blockIdx.x / all;
-    const int rt = (int)(unit % a.nrt), hk = (int)(unit / a.nrt % a.HK), s = (int)(unit / a.nrt / a.HK);
-    const float * ml = a.part_ml + (unit * a.nsplit * NQ * 16 + n * 16 + r) * 2;
-    const float * po = a.part_o + ((unit * a.nsplit * all + at) * WAVE + lane) * 4;
-    const int64_t ml_st = NQ * 32, po_st = (int64_t)all * WAVE * 4;
-    float M = -INFINITY;
-    for (int i = 0; i < a.nsplit; i++) M = fmaxf(M, ml[i * ml_st]);
-    float4v v = {0, 0, 0, 0};
-    float L = 0.0f;
-    for (int i = wave; i < a.nsplit; i += 4) {
-        const float m = ml[i * ml_st], w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - M) * FQ_LOG2E);
-        const float4v p = *(const float4v *)(po + i * po_st);
-        L += w * ml[i * ml_st + 1];
+    const int unit = blockIdx.x / all;
+    const int sh = fq_div(unit, a.div_nrt), s = fq_div(sh, a.div_hk), rt = unit - sh * a.nrt, hk = sh - s * a.HK;
+    const float * po = a.part_o + (((int64_t)unit * a.nsplit * all + at) * WAVE + lane) * 4;
+    float4v p[FQ_MAX_SPLIT / 4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] += w * p[e];
+    for (int k = 0; k < FQ_MAX_SPLIT / 4; k++) {
+        p[k] = float4v{0, 0, 0, 0};
+        if (4 * k + wave < a.nsplit) p[k] = *(const float4v *)(po + (int64_t)(4 * k + wave) * all * WAVE * 4);
+    }
+    // thread (row t % 16, splits t / 16 + 16 k)
+    const int row16 = t % 16, s0 = t / 16;
+    const float * ml = a.part_ml + ((int64_t)unit * a.nsplit * NQ * 16 + n * 16 + row16) * 2;
+    float m[FQ_MAX_SPLIT / 16], l[FQ_MAX_SPLIT / 16], M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < FQ_MAX_SPLIT / 16; k++) {
+        m[k] = -INFINITY;
+        l[k] = 0.0f;
+        if (s0 + 16 * k < a.nsplit) {
+            m[k] = ml[(int64_t)(s0 + 16 * k) * NQ * 32];
+            l[k] = ml[(int64_t)(s0 + 16 * k) * NQ * 32 + 1];
+        }
+        M = fmaxf(M, m[k]);
+    }
+    sm[s0][row16] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; i++) M = fmaxf(M, sm[i][row16]);
+    float L = 0.0f;
+#pragma unroll
+    for (int k = 0; k < FQ_MAX_SPLIT / 16; k++) {
+        const float w = m[k] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[k] - M) * FQ_LOG2E);
+        L += w * l[k];
+        if (s0 + 16 * k < FQ_MAX_SPLIT) sw[s0 + 16 * k][row16] = w;
+    }
+    sl[s0][row16] = L;
+    __syncthreads();
+    float4v v = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < FQ_MAX_SPLIT / 4; k++) {
+        const float w = sw[4 * k + wave][r];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += w * p[k][e];
     }
     so[wave][lane] = v;
-    sl[wave][lane] = L;
     __syncthreads();
     if (wave) return;
-    for (int w = 1; w < 4; w++) {
-        L += sl[w][lane];
+    for (int w = 1; w < 4; w++)
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] += so[w][lane][e];
-    }
+    L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) L += sl[i][r];
     const int row = (rt * NQ + n) * 16 + r;
     if (row >= a.R) return;
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    const int64_t dst = (int64_t)s * a.dst_nb3 + (int64_t)(row / a.G) * a.dst_nb2 + (int64_t)(hk * a.G + row % a.G) * a.dst_nb1;
+    const int tk = fq_div(row, a.div_g);
+    const int64_t dst = (int64_t)s * a.dst_nb3 + (int64_t)tk * a.dst_nb2 + (int64_t)(hk * a.G + row - tk * a.G) * a.dst_nb1;
     const int vu = vt == T_Q8_0 || DV >= 128 ? 4 : 2;
 #pragma unroll
     for (int e = 0; e < 4; e++) {

@@ -83,6 +83,16 @@ struct KvView {
     int64_t nb1, nb2, nb3;
     int type;
 };
+// The largest fp16 scale with which every value of a block stays inside fp16: 515.5 * 127, 8188 * 8.
+__host__ __device__ constexpr float kv_scale_limit(int type) { return type == 8 ? 515.5f : 8188.0f; }
+
+// Division by d in [1, 2^30] of values below 2^30 (fq_div): mul = floor(2^32 / d) + 1 (d 1: not read).
+struct FqDiv {
+    uint32_t mul;
+    int d;
+};
+inline FqDiv fq_div_by(int d) { return {(uint32_t)(((uint64_t)1 << 32) / (uint32_t)d + 1), d}; }
+
 // FLASH_ATTN_EXT of few rows over a quantized cache: strides in elements.
 struct FaQArgs {
     const void * q;            // F32 or F16
@@ -94,11 +104,13 @@ struct FaQArgs {
     int64_t q_nb1, q_nb2, q_nb3, mask_nb1, mask_nb3, dst_nb1, dst_nb2, dst_nb3;
     int D, DV, dk, dv;         // built and actual head dims
     int T, HK, KV, S, G, R;    // G = H / HK; R = T G query rows share a KV head
+    FqDiv div_nrt, div_hk, div_split, div_g;
     int nq, nrt, nsplit;       // 16-row query tiles a wave, blocks of rows, KV splits
     float scale, softcap;
     bool q_f16, dst_f16;
 };
-constexpr int64_t FA_Q_MAX_NB1 = 1 << 24;   // its 32-bit offsets inside a 32-key tile
+constexpr int FA_Q_MIN_KV = 32;             // a tile
+constexpr int64_t FA_Q_MAX_NB1 = 1 << 24;   // its 32-bit offsets inside a tile
 inline int fa_q_max_nq(int DV) { return DV <= 128 ? 4 : 2; }
 hipError_t launch_fa_q(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_q_combine(const FaQArgs & a, int vt, int DV, int NQ, hipStream_t st);

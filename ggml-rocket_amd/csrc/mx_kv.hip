@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(KV_THREADS) get_rows_kernel(KvRowsArgs a) {
     kv_store_plain(o, (int64_t)r * o.x_nb1 + (int64_t)h * o.x_nb2 + 32 * b, l, v);
 }
 
-// K and V of one sequence as fp16, for the fused attention. Values past fp16's range are held at its
-// largest. The attention hides a key by its score, but multiplies P = 0 by the key's V all the same, so
+// K and V of one sequence as fp16, for the fused attention. A scale is held to the largest with which
+// every value stays inside fp16. The attention hides a key by its score, but multiplies P = 0 by the key's V all the same, so
 // V has to be finite: a V block whose scale is not stands for zeros here and makes the first value of
 // that key's K a NaN instead, which reaches exactly the queries that see the key.
 __global__ void __launch_bounds__(KV_THREADS) kv_decode_kernel(KvDecodeArgs a) {
@@ -230,10 +230,10 @@ __global__ void __launch_bounds__(KV_THREADS) kv_decode_kernel(KvDecodeArgs a) {
     float d = h2f_bits(w.d[at / 32]);
     const bool bad = !(fabsf(d) < INFINITY);
     if (bad && is_v) d = 0.0f;
+    const float lim = kv_scale_limit(w.type);
+    d = fmaxf(fminf(d, lim), -lim);
     float v[8];
     kv_values(w.type, w.q, d, at, l, v);
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_fmed3f(v[e], -65504.0f, 65504.0f);
     if (bad && !is_v) v[0] = NAN;
     if (b == 0 && l == 0) {
         const uint16_t * vd = a.v.d + (j * a.v.nb1 + h * a.v.nb2) / 32;

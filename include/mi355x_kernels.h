@@ -372,8 +372,8 @@ MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int 
 
 /* mi355x_flash_attn with K and V in a quantized cache, each Q8_0 or Q4_0: dst = softmax(cap(scale *
  * q.k) + mask) . v. K and V enter the products as fp16 (their values rounded once), Q and P as fp16,
- * sums in F32: an F32 dst holds values of that accuracy. Cache values past fp16's range count as its
- * largest (65504). D and DV are multiples of 32 up to 256; H % HK == 0; max_bias 0. A key that the
+ * sums in F32: an F32 dst holds values of that accuracy. So that the values stay inside fp16, a scale
+ * counts as at most 515.5 (Q8_0: 65468 / 127) or 8188 (Q4_0: 65504 / 8). D and DV are multiples of 32 up to 256; H % HK == 0; max_bias 0. A key that the
  * mask hides from a query (-inf) adds nothing to it, whatever the cache holds there, NaN included; a
  * key with a scale that is not finite makes the rows of the queries that see it NaN; rows whose every
  * key is hidden are written as zeros. q rows 16-byte, dst rows 16-byte (F16: 8), mask rows 8-byte

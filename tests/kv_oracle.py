@@ -45,6 +45,13 @@ def values(codes, d, t):
     return v.reshape(d.shape[:-1] + (-1,))
 
 
+def held(codes, d, t):
+    """The values attention takes: scales count as at most 515.5 (Q8_0) or 8188 (Q4_0), so that they stay
+    inside fp16."""
+    lim = np.float16(515.5 if t == Q8_0 else 8188)
+    return values(codes, np.clip(d, -lim, lim), t)
+
+
 def attention(q, k, v, mask, scale, softcap=0.0):
     """(dst, bound) of one sequence: q [H][T][D], k [HK][KV][D], v [HK][KV][DV] f64 values, mask [T][KV]
     f64 (-inf hides) or None. dst [T][H][DV] in 64 bits. bound: how far fp16 operands may take an
@@ -53,7 +60,6 @@ def attention(q, k, v, mask, scale, softcap=0.0):
     are rounded once each, and a P under fp16's normal range by at most 2^-25; f32 sums add the last
     2^-12 (64k terms at 2^-24, roots of which survive: the bound is loose here)."""
     q, k, v = (np.asarray(a, dtype=np.float64) for a in (q, k, v))
-    k, v = (np.clip(a, -65504.0, 65504.0) for a in (k, v))      # values past fp16's range count as its largest
     H, T, D = q.shape
     HK, KV, DV = v.shape
     out, tol = np.zeros((T, H, DV)), np.zeros((T, H, DV))

@@ -346,7 +346,7 @@ def test_attention_ranges(mx, form, types, T):
         spread = 10.0 ** rng.uniform(-1, 1, (1, KV, HK, 1))
         kq, kd = R.quantize(rng.standard_normal((1, KV, HK, D)) * ks, types[0])
         vq, vd = R.quantize(rng.standard_normal((1, KV, HK, D)) * vs * spread, types[1])
-        kn, vn = R.values(kq, kd, types[0]).transpose(0, 2, 1, 3), R.values(vq, vd, types[1]).transpose(0, 2, 1, 3)
+        kn, vn = R.held(kq, kd, types[0]).transpose(0, 2, 1, 3), R.held(vq, vd, types[1]).transpose(0, 2, 1, 3)
         kc, vc = (mx.KvCache(t, gpu(c), gpu(d)).permute(0, 2, 1, 3) for t, c, d in ((types[0], kq, kd), (types[1], vq, vd)))
         got = cpu(mx.flash_attn_q(gpu(q), kc, vc, None, 0.125))
         assert np.isfinite(got).all()
