@@ -753,8 +753,7 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
     while (f.nq < mx::fa_q_max_nq(f.DV) && 16 * f.nq < f.R) f.nq *= 2;
     f.nrt = (f.R + 16 * f.nq - 1) / (16 * f.nq);
     const int64_t units = (int64_t)f.S * f.HK * f.nrt, ntiles = (f.KV + 31) / 32;
-    f.nsplit = nsplit > 0 ? nsplit
-                          : (int)std::max<int64_t>(1, std::min<int64_t>({64, 2 * device_cus() / std::max<int64_t>(1, units), ntiles / 8}));
+    f.nsplit = nsplit > 0 ? nsplit : (int)std::max<int64_t>(1, std::min<int64_t>({64, device_cus() / std::max<int64_t>(1, units), ntiles / 8}));
     f.div_nrt = mx::fq_div_by(f.nrt); f.div_hk = mx::fq_div_by(f.HK); f.div_split = mx::fq_div_by(f.nsplit);
     f.div_g = mx::fq_div_by(f.G);
     return f;

@@ -6,31 +6,40 @@
 //
 // The T * G query rows of one KV head share its keys, so they are the columns of the products: a wave
 // takes 16 NQ rows and 32 keys at a time, in 16x16x32 MFMAs,
-//   S^T = K . Q^T   (A: 16 keys x 32 dims, B: 32 dims x 16 rows)
+//   S^T = K . Q^T    (A: 16 keys x one block of 32 dims, B: 32 dims x 16 rows)
 //   O^T += V^T . P^T (A: 16 dims x 32 keys, B: 32 keys x 16 rows)
 // with scores, softmax statistics and O in F32 and everything of a row in the four lanes of its
-// column. A wave is on its own until its keys are done: no LDS tiles and no barriers, each 32-key
-// tile's codes come straight into registers. The order of dims in a contraction and
-// of keys in a tile is free, and chosen so that no lane needs another's data:
-//   K   a lane holds one key and whole 16-byte pieces of its row; Q is laid out to match.
+// column. A wave is on its own until its keys are done: its tiles' codes come by LDS DMA into two buffers
+// of its own, so there are no barriers in the loop. (Loaded straight into the operands' lanes, where
+// neighbouring lanes are different keys, every load took the address unit a cycle a lane and the kernel
+// waited for it: 978 cycles of it a tile at head dim 128; by DMA neighbouring lanes are neighbouring bytes.)
+// The order of dims in a contraction and of keys in a tile is free, and chosen so that no lane needs
+// another's data:
+//   K   the lanes of group g hold bytes 8 g (Q8_0) or 4 g (Q4_0) on of every block of one key.
 //   P   the S^T accumulators of two 16-key products are the P^T operand: slot e of lane group g is key
 //       16 (e / 4) + 4 g + e % 4.
-//   V   the lane of group g loads the same few bytes of those eight keys; v_perm_b32 picks one byte of
-//       two keys into a pair of halves, which transposes V on the way to fp16.
-// Codes become fp16 by integer operations: a byte under the exponent of 1024 is 1024 + byte, less the
-// offset (exact), times the block's scale: the values of the cache rounded once. V's scales go through
-// a few bytes of LDS a wave, which turns a key's row of scales into eight keys' scales of one block.
-// The running maximum moves only when a score passes it by more than 8 in the exponent of 2 (P stays
-// below 256, well inside fp16), so most tiles exchange nothing between lanes.
+//   V   the lane of group g reads the same few bytes of those eight keys; v_perm_b32 picks one byte of
+//       two keys into a pair of halves, which transposes V.
 //
-// A tile's K is loaded again, for the next tile, as soon as its scores are done, its V after O: the loads
-// of one half of a tile are always in flight under the other half's work, and the registers hold one
-// tile, so that several waves share a SIMD.
-// The waves of a block take alternate tiles of the block's key range and merge through LDS at the end;
-// the key range is split over blocks where there are too few of them, and a second launch merges those.
-// Tiles that the mask hides from every row of a wave are not read: their mask is looked at before their
-// loads are issued, and hidden tiles' loads are sent to the tile before (the number of loads in flight
-// stays the same, which keeps the waits exact).
+// What bounds it is the work of turning codes into operands, so that is kept to a few integer
+// instructions a pair: an unsigned code u = code + 128 (Q8_0) or u = code (Q4_0, value u - 8) in the low
+// bits of a half is the subnormal u 2^-24, which the matrix unit multiplies exactly. A high nibble left
+// in place counts 16 times; its Q is divided by 16 beforehand, its O afterwards.
+//   K   one product is one block, so its scale multiplies the F32 result (S += d S_b), and the offset
+//       is the product's start value, -128 (or -8) sum_dims q, a product of q with a constant: K is exact.
+//   V   the halves are multiplied by d 2^k, k such that the largest scale seen by the wave is just below
+//       2^15 (it moves rarely, and O with it); the offset leaves through one more product a group of dims
+//       with the scales themselves. A V is rounded once, relative to u: off by at most 2^-11 of 255 d
+//       (Q8_0) or 15 d (Q4_0), a sixteenth or less of half a quantization step.
+// Scales go through a few bytes of LDS a wave, which turns a key's row of them into one block's of
+// several keys. The running maximum moves only when a score passes it by more than 8 in the exponent of 2
+// (P stays below 256, well inside fp16), so most tiles exchange nothing between lanes.
+//
+// While a tile is worked on, the next one is on its way; the one after it is requested when its buffer is
+// free. The waves of a block take alternate tiles of the block's key range and merge through LDS at the
+// end; the key range is split over blocks where there are too few of them, and a second launch merges those.
+// Tiles that the mask hides from every row of a wave are left out: a lane looks at one tile's mask, for 64
+// of the wave's tiles at a time (only where at most 8 tokens share a wave; else every tile is read).
 
 #pragma once
 
@@ -43,6 +52,9 @@
 namespace mx {
 
 constexpr int FQ_KEYS = 32;      // keys a tile
+constexpr int FQ_LDS_MAX = 160 * 1024;
+constexpr int FQ_BASE_REGS = 64;
+constexpr int FQ_SCAN_TOKENS = 8;
 constexpr float FQ_LAZY = 8.0f / 1.4426950408889634f;
 constexpr float FQ_LOG2E = 1.4426950408889634f;
 
@@ -50,26 +62,50 @@ constexpr float FQ_LOG2E = 1.4426950408889634f;
 template <int KT, int VT, int DK, int DV, int NQ>
 struct FqCfg {
     static constexpr int KRB = KT == T_Q8_0 ? DK : DK / 2, VRB = VT == T_Q8_0 ? DV : DV / 2;   // bytes a row
-    static constexpr int CB = (KRB / 16) % 4 == 0 ? 16 : 8;   // a lane's piece of a key: the four lanes of
-    static constexpr int KI = KRB / CB / 4;                   // a key take pieces g, g + 4, ...; KI each
-    static constexpr int KS = DK / 32;                        // Q.K products
-    static constexpr int SPP = KS / KI;                       // of them, per piece
+    static constexpr int KS = DK / 32;                        // blocks a K row: Q.K products
+    static constexpr int KW = KT == T_Q8_0 ? 2 : 1;           // dwords of a block a lane holds
+    // 16-byte chunks of a row in LDS (K: a power of two, 12 and 6 padded) and DMA instructions a tile
+    static constexpr int KCH = KRB / 16 <= 2 ? 2 : KRB / 16 <= 4 ? 4 : KRB / 16 <= 8 ? 8 : 16, VCH = VRB / 16;
+    static constexpr int KD = KCH / 2, VD = VCH / 2;
+    static constexpr int STAGE = FQ_KEYS * 16 * (KCH + VCH);
+    // Chunk c of K row r lies at c ^ kswz(r): the 16 rows that a read of one chunk takes then lie in 16
+    // different chunk slots of LDS's 256-byte window. V rows lie in the order 16 h + 4 i + g (key 16 h + 4 g
+    // + i), so that the four keys a read takes are neighbours, and chunk c at c ^ vswz(g).
+    __device__ static __forceinline__ int kswz(int row) { return (row * KCH / 16) & (KCH - 1); }
+    __device__ static __forceinline__ int vswz(int g) { return VCH == 16 ? 4 * g : VCH == 8 ? 4 * (g / 2) : 0; }
     static constexpr int VU = VT == T_Q8_0 || DV >= 128 ? 4 : 2;   // a lane's bytes of a V row: u, u + 16, ...
     static constexpr int VJ = VRB / (16 * VU);
     static constexpr int VH = VT == T_Q4_0 ? 2 : 1;           // nibbles a byte
     static constexpr int TT = DV / 16;                        // O^T tiles, index (j * VU + byte) * VH + nibble
-    static_assert(KRB % (4 * CB) == 0 && VJ * VU * VH == TT && SPP * KI == KS, "layout");
-    static constexpr int VB = DV / 32, VS = DV / 64;          // V scales a key, and a lane (32 keys, two lanes each)
-    // registers: a tile of codes, O, Q, scores and masks, the rest
-    static constexpr int REGS = 2 * KI * (CB / 4) + 8 * VJ + (TT + KS) * 4 * NQ + 22 * NQ + 50;
-    static constexpr int NW = REGS > 240 ? 4 : 8;             // waves a block
+    static_assert(KRB == 16 * KS * KW && VJ * VU * VH == TT, "layout");
+    static constexpr int VB = DV / 32, VS = DV / 64, KSC = DK / 64;   // scales a key, and a lane (32 keys, two lanes each)
+    static constexpr int Q_LDS = NQ * (KS * 1024 + 64);       // Q as B operands, then its rows' factors
+    static constexpr int SCALE_LDS = KS * FQ_KEYS * 4 + VB * FQ_KEYS * 2;   // a wave's scales: K's F32, V's F16
+    static constexpr int WAVE_LDS = SCALE_LDS + 2 * STAGE;
+    // registers: O, scores and masks, the rest; the waves a SIMD they leave room for, and as many in a
+    // block, one block a CU, as the buffers leave room for
+    static constexpr int REGS = (TT + VJ) * 4 * NQ + 30 * NQ + KD + VD + KSC + VS + FQ_BASE_REGS;
+    static constexpr int WPE = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;
+    static constexpr int FIT = (FQ_LDS_MAX - Q_LDS) / WAVE_LDS / 4 * 4;
+    static constexpr int NW = FIT < 4 * WPE ? FIT : 4 * WPE;
+    static_assert(NW >= 4, "LDS");
     static constexpr int CT = TT * NQ < 8 ? TT * NQ : 8;      // O^T tiles merged at a time
-    static constexpr int SCALE_LDS = VB * FQ_KEYS * 2;        // a wave's V scales
+    static constexpr int LOOP_LDS = Q_LDS + NW * WAVE_LDS;
     static constexpr int MERGE_LDS = NW * 16 * NQ * 8 + NW * CT * 1024;
-    static constexpr int LDS = MERGE_LDS > NW * SCALE_LDS ? MERGE_LDS : NW * SCALE_LDS;
+    static constexpr int LDS = MERGE_LDS > LOOP_LDS ? MERGE_LDS : LOOP_LDS;
 };
 
-typedef uint32_t u32_alias __attribute__((may_alias));
+typedef const void __attribute__((address_space(1))) * fq_gptr_t;
+typedef void __attribute__((address_space(3))) * fq_lptr_t;
+__device__ __forceinline__ void fq_dma16(const void * g, void * l) {
+    __builtin_amdgcn_global_load_lds((fq_gptr_t)g, (fq_lptr_t)l, 16, 0, 0);
+}
+// No memory access moves across it; waits until at most N vector loads are outstanding.
+template <int N>
+__device__ __forceinline__ void fq_wait_vm() {
+    static_assert(N >= 0 && N <= 63, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 // The element a lane's value i of O^T tile t is: its dim.
 __device__ __forceinline__ int fq_dim(int vt, int vu, int t, int g, int i) {
@@ -94,57 +130,57 @@ __device__ __forceinline__ float fq_col_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// The maximum over the wave, in every lane: four DPP steps inside the rows of 16, then across them.
+__device__ __forceinline__ float fq_wave_max(float x) {
+#define FQ_DPP_MAX(CTRL) x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true)))
+    FQ_DPP_MAX(0xB1);    // quad_perm [1,0,3,2]
+    FQ_DPP_MAX(0x4E);    // quad_perm [2,3,0,1]
+    FQ_DPP_MAX(0x141);   // row_half_mirror
+    FQ_DPP_MAX(0x140);   // row_mirror
+#undef FQ_DPP_MAX
+    return fq_col_max(x);
+}
+
 // n / d of a FqDiv made for d: the product is the quotient or one more.
 __device__ __forceinline__ int fq_div(int n, const FqDiv & d) {
     const uint32_t q = __umulhi((uint32_t)n, d.mul);
     return d.d == 1 ? n : (int)(q * (uint32_t)d.d > (uint32_t)n ? q - 1 : q);
 }
 
-// A block's scale as the products take it: held to the largest with which every value stays inside
-// fp16 (kv_scale_limit); infinite or NaN ones as `bad`.
+// A block's scale: held to the largest with which every value stays inside fp16 (kv_scale_limit), as
+// where the cache is decoded first; infinite or NaN ones as `bad`.
 template <int TYPE>
-__device__ __forceinline__ uint16_t fq_scale(uint16_t bits, uint16_t bad) {
-    constexpr uint16_t lim = TYPE == T_Q8_0 ? 0x6007 : 0x6FFF;
-    const uint16_t mag = bits & 0x7FFFu;
-    const uint16_t held = (uint16_t)(min(mag, lim) | (bits & 0x8000u));
-    return mag >= 0x7C00u ? bad : held;
+__device__ __forceinline__ float fq_scale(uint16_t bits, float bad) {
+    const float d = fmaxf(fminf(h2f_bits(bits), kv_scale_limit(TYPE)), -kv_scale_limit(TYPE));
+    return (bits & 0x7C00u) == 0x7C00u ? bad : d;
 }
 
-// Eight values of a key from its codes: a dword pair (Q8_0) or a dword (Q4_0: four low nibbles, four
-// high ones), times d.
+// A lane's eight unsigned codes of a K block, each the low bits of a half. Q8_0: dims 8 g + 0..7. Q4_0:
+// dims 4 g + {0, 2, 1, 3} and, 16 times as large, 16 + 4 g + {0, 2, 1, 3}.
 template <int KT>
-__device__ __forceinline__ half8 fq_key(uint32_t x0, uint32_t x1, half2v d) {
-    half2v p[4];
+__device__ __forceinline__ half8 fq_key(const uint32_t * x) {
+    u32x4 w;
     if constexpr (KT == T_Q8_0) {
-        const uint32_t a = x0 ^ 0x80808080u, b = x1 ^ 0x80808080u;
-        const half2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-        p[0] = (magic_pair(a, PERM_B01) + off) * d;
-        p[1] = (magic_pair(a, PERM_B23) + off) * d;
-        p[2] = (magic_pair(b, PERM_B01) + off) * d;
-        p[3] = (magic_pair(b, PERM_B23) + off) * d;
+        const uint32_t a = x[0] ^ 0x80808080u, b = x[1] ^ 0x80808080u;
+        w = u32x4{__builtin_amdgcn_perm(0u, a, 0x0C010C00u), __builtin_amdgcn_perm(0u, a, 0x0C030C02u),
+                  __builtin_amdgcn_perm(0u, b, 0x0C010C00u), __builtin_amdgcn_perm(0u, b, 0x0C030C02u)};
     } else {
-        const uint32_t a = x0 & 0x0F0F0F0Fu, b = (x0 >> 4) & 0x0F0F0F0Fu;
-        const half2v off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-        p[0] = (magic_pair(a, PERM_B01) + off) * d;
-        p[1] = (magic_pair(a, PERM_B23) + off) * d;
-        p[2] = (magic_pair(b, PERM_B01) + off) * d;
-        p[3] = (magic_pair(b, PERM_B23) + off) * d;
+        const uint32_t y = x[0] >> 8;
+        w = u32x4{x[0] & 0x000F000Fu, y & 0x000F000Fu, x[0] & 0x00F000F0u, y & 0x00F000F0u};
     }
-    half8 r;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        r[2 * i] = p[i][0];
-        r[2 * i + 1] = p[i][1];
-    }
-    return r;
+    return __builtin_bit_cast(half8, w);
 }
 
 template <int KT, int VT, int DK, int DV, int NQ>
 __global__ void __launch_bounds__((FqCfg<KT, VT, DK, DV, NQ>::NW * WAVE))
+__attribute__((amdgpu_waves_per_eu(FqCfg<KT, VT, DK, DV, NQ>::WPE, FqCfg<KT, VT, DK, DV, NQ>::WPE)))
 fa_q_kernel(FaQArgs a) {
     using C = FqCfg<KT, VT, DK, DV, NQ>;
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int NW = C::NW;
+    // The arguments lie in host memory, a round trip of half a microsecond and more a cache line; used
+    // here, one of each line, they all come at once instead of where each is first needed.
+    asm volatile("" ::"s"(a.q), "s"(a.k.nb3), "s"(a.v.nb2), "s"(a.dst), "s"(a.mask_nb3), "s"(a.T), "s"(a.div_split.mul), "s"(a.softcap));
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int r = lane % 16, g = lane / 16;
 
@@ -168,173 +204,192 @@ fa_q_kernel(FaQArgs a) {
     const uint16_t * const kd = a.k.d + ((int64_t)s * a.k.nb3 + (int64_t)hk * a.k.nb2) / 32;
     const uint16_t * const vd = a.v.d + ((int64_t)s * a.v.nb3 + (int64_t)hk * a.v.nb2) / 32;
     const uint32_t knb = (uint32_t)a.k.nb1, vnb = (uint32_t)a.v.nb1;
-    uint32_t ko[C::KI], kdo[C::KI];  // pieces of key r and their scales (a piece past dk: piece 0, Q is zero there)
+    // chunks and scales past dk or dv: the first ones (Q is zero there, O is not stored)
+    uint32_t kdma[C::KD], vdma[C::VD];   // this lane's chunk of each DMA instruction: byte offset from the tile
 #pragma unroll
-    for (int i = 0; i < C::KI; i++) {
-        int c = g + 4 * i;
-        const int elems = KT == T_Q8_0 ? C::CB : 2 * C::CB;
-        if (c * elems >= a.dk) c = 0;
-        ko[i] = ((r * knb) >> KSH) + (uint32_t)(c * C::CB);
-        kdo[i] = r * knb / 32 * 2 + (uint32_t)(c * elems / 32 * 2);
+    for (int q = 0; q < C::KD; q++) {
+        const int slot = q * WAVE + lane, row = slot / C::KCH, c = (slot % C::KCH) ^ C::kswz(row);
+        kdma[q] = (((uint32_t)row * knb) >> KSH) + (c * 16 < (a.dk >> KSH) ? 16 * c : 0);
     }
-    uint32_t vo[C::VJ];              // the lane's bytes of key 4 g's row of V
-    int vblk[C::VJ];
 #pragma unroll
-    for (int j = 0; j < C::VJ; j++) {
-        const int u = (r + 16 * j) * C::VU;                      // byte in the row
-        vblk[j] = VT == T_Q8_0 ? u / 32 : u / 16;
-        vo[j] = ((4 * g * vnb) >> VSH) + (32 * vblk[j] < a.dv ? (uint32_t)u : 0u);   // past dv: not stored
+    for (int q = 0; q < C::VD; q++) {
+        const int slot = q * WAVE + lane, pos = slot / C::VCH, c = (slot % C::VCH) ^ C::vswz(pos % 4);
+        const uint32_t key = pos / 16 * 16 + pos % 4 * 4 + pos % 16 / 4;
+        vdma[q] = ((key * vnb) >> VSH) + (c * 16 < (a.dv >> VSH) ? 16 * c : 0);
     }
-    uint32_t vdo[C::VS];             // the V scales this lane fetches: key lane % 32
+    uint32_t kdo[C::KSC], vdo[C::VS];    // the scales this lane fetches: key lane / 2, half of its blocks
+#pragma unroll
+    for (int i = 0; i < C::KSC; i++) {
+        const int blk = (lane % 2) * C::KSC + i;
+        kdo[i] = (uint32_t)(lane / 2) * knb / 32 * 2 + (32 * blk < a.dk ? 2 * blk : 0);
+    }
 #pragma unroll
     for (int i = 0; i < C::VS; i++) {
-        int blk = (lane / 32) * C::VS + i;
-        if (32 * blk >= a.dv) blk = 0;
-        vdo[i] = (uint32_t)(lane % 32) * vnb / 32 * 2 + 2 * blk;
+        const int blk = (lane % 2) * C::VS + i;
+        vdo[i] = (uint32_t)(lane / 2) * vnb / 32 * 2 + (32 * blk < a.dv ? 2 * blk : 0);
+    }
+    // where this lane reads: bytes 4 KW g on of a K block (block i at kra ^ kra_i), its bytes of V row g
+    uint32_t kra = r * C::KCH * 16, vra[C::VJ];
+    kra += KT == T_Q8_0 ? ((C::kswz(r) ^ (g / 2)) << 4) + 8 * (g % 2) : (C::kswz(r) << 4) + 4 * g;
+    int vblk[C::VJ];                     // the block of its V bytes
+#pragma unroll
+    for (int j = 0; j < C::VJ; j++) {
+        const int u = (r + 16 * j) * C::VU;
+        vblk[j] = VT == T_Q8_0 ? u / 32 : u / 16;
+        vra[j] = g * C::VRB + (((u / 16) ^ C::vswz(g)) << 4) + u % 16;
     }
 
-    uint32_t xk[2][C::KI][C::CB / 4], xv[8][C::VJ];   // the tile's codes
-    uint16_t xkd[2][C::KI], xvd[C::VS];               // and scales
-    auto load_k = [&](int t) {   // and V's scales, which are looked at with K's
+    uint8_t * const wl = smem + C::Q_LDS + wave * C::WAVE_LDS;   // this wave's scales and buffers
+    float * const wk = (float *)wl;                              // K scales [block][key]
+    uint16_t * const wv = (uint16_t *)(wk + C::KS * FQ_KEYS);    // V scales
+    auto dma = [&](int t, int buf) {
         const int64_t kb = min(FQ_KEYS * t, kb_last);
-        const uint8_t * vdt = (const uint8_t *)vd + kb * a.v.nb1 / 32 * 2;
+        const uint8_t * kt = kq + ((kb * a.k.nb1) >> KSH);
+        const uint8_t * vt = vq + ((kb * a.v.nb1) >> VSH);
+        uint8_t * st = wl + C::SCALE_LDS + buf * C::STAGE;
 #pragma unroll
-        for (int i = 0; i < C::VS; i++) xvd[i] = *(const uint16_t *)(vdt + vdo[i]);
+        for (int q = 0; q < C::KD; q++) fq_dma16(kt + kdma[q], st + q * 1024);
 #pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-            const int64_t at = (kb + 16 * hf) * a.k.nb1;
-            const uint8_t * q = kq + (at >> KSH);
-            const uint8_t * d = (const uint8_t *)kd + at / 32 * 2;
-#pragma unroll
-            for (int i = 0; i < C::KI; i++) {
-                xkd[hf][i] = *(const uint16_t *)(d + kdo[i]);
-                if constexpr (C::CB == 16) {
-                    const u32x4 w = *(const u32x4 *)(q + ko[i]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) xk[hf][i][e] = w[e];
-                } else {
-                    const u32x2 w = *(const u32x2 *)(q + ko[i]);
-#pragma unroll
-                    for (int e = 0; e < 2; e++) xk[hf][i][e] = w[e];
-                }
-            }
-        }
-    };
-    auto load_v = [&](int t) {
-        const int64_t kb = min(FQ_KEYS * t, kb_last);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint8_t * q = vq + (((kb + 16 * (e / 4) + e % 4) * a.v.nb1) >> VSH);
-#pragma unroll
-            for (int j = 0; j < C::VJ; j++) {
-                if constexpr (C::VU == 4) xv[e][j] = *(const uint32_t *)(q + vo[j]);
-                else xv[e][j] = *(const uint16_t *)(q + vo[j]);
-            }
-        }
+        for (int q = 0; q < C::VD; q++) fq_dma16(vt + vdma[q], st + FQ_KEYS * 16 * C::KCH + q * 1024);
     };
 
-    // this lane's rows: token and head
-    int tok[NQ], head[NQ];
+    // this lane's rows
     bool ok[NQ];
     const uint16_t * mrow[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const int row = (rt * NQ + n) * 16 + r;
         ok[n] = row < a.R;
-        tok[n] = ok[n] ? fq_div(row, a.div_g) : 0;
-        head[n] = hk * a.G + (ok[n] ? row - tok[n] * a.G : 0);
-        mrow[n] = a.mask ? a.mask + (int64_t)s * a.mask_nb3 + (int64_t)tok[n] * a.mask_nb1 + 4 * g : (const uint16_t *)kq;
+        const int tok = ok[n] ? fq_div(row, a.div_g) : 0;
+        mrow[n] = a.mask ? a.mask + (int64_t)s * a.mask_nb3 + (int64_t)tok * a.mask_nb1 + 4 * g : (const uint16_t *)kq;
     }
     // without a mask the same loads read the first key's codes, and nothing looks at them: a load that
     // is sometimes issued would make every wait behind it a wait for all loads
     const int mstep = a.mask ? 1 : 0;
-    typedef u32x2 Mask[NQ][2];   // this lane's four keys of either half tile
-    auto load_mask = [&](Mask & x, int t) {
-        const int kb = min(FQ_KEYS * t, kb_last);
+    struct Side {              // what of a tile comes into registers
+        uint16_t kd[C::KSC], vd[C::VS];
+        u32x2 m[NQ][2];        // the mask of this lane's four keys of either half tile
+    };
+    auto load_side = [&](Side & x, int t) {
+        const int64_t kb = min(FQ_KEYS * t, kb_last);
+        const uint8_t * kt = (const uint8_t *)kd + kb * a.k.nb1 / 32 * 2;
+        const uint8_t * vt = (const uint8_t *)vd + kb * a.v.nb1 / 32 * 2;
+#pragma unroll
+        for (int i = 0; i < C::KSC; i++) x.kd[i] = *(const uint16_t *)(kt + kdo[i]);
+#pragma unroll
+        for (int i = 0; i < C::VS; i++) x.vd[i] = *(const uint16_t *)(vt + vdo[i]);
 #pragma unroll
         for (int n = 0; n < NQ; n++)
 #pragma unroll
             for (int hf = 0; hf < 2; hf++)
-                __builtin_memcpy(&x[n][hf], mrow[n] + (kb + 16 * hf) * mstep, 8);   // any alignment of 2 bytes
+                __builtin_memcpy(&x.m[n][hf], mrow[n] + (kb + 16 * hf) * mstep, 8);   // any alignment of 2 bytes
     };
-    // whether some row of the wave sees some key of a tile
-    auto seen = [&](const Mask & x) {
-        if (!a.mask) return true;
-        bool v = false;
+    // The wave's tiles are tile0 + wave + NW k. next() gives the next k that some row sees (-1: none): bits
+    // of 64 of them, one lane a tile.
+    const int nk = tile1 - tile0 > wave ? (tile1 - tile0 - wave + NW - 1) / NW : 0;
+    const int tok_a = fq_div(rt * 16 * NQ, a.div_g), tok_b = fq_div(min(a.R, (rt + 1) * 16 * NQ) - 1, a.div_g);
+    const bool scan = a.mask && tok_b - tok_a < FQ_SCAN_TOKENS;
+    uint64_t todo = 0;
+    int k0 = -64;              // the 64 that todo is for
+    auto next = [&]() {
+        while (todo == 0) {
+            k0 += 64;
+            if (k0 >= nk) return -1;
+            const int k = k0 + lane;
+            bool v = k < nk;
+            if (v && scan) {
+                const int kb = min(FQ_KEYS * (tile0 + wave + NW * k), kb_last);
+                v = false;
+                for (int tk = tok_a; tk <= tok_b; tk++) {
+                    const uint16_t * p = a.mask + (int64_t)s * a.mask_nb3 + (int64_t)tk * a.mask_nb1 + kb;
+                    u32x4 w[4];
+                    __builtin_memcpy(w, p, 64);
 #pragma unroll
-        for (int n = 0; n < NQ; n++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) v |= ok[n] && (x[n][hf][0] != 0xFC00FC00u || x[n][hf][1] != 0xFC00FC00u);
-        return __builtin_amdgcn_readfirstlane((int)__any(v)) != 0;   // scalar
+                    for (int i = 0; i < 16; i++) v |= w[i / 4][i % 4] != 0xFC00FC00u;
+                }
+            }
+            todo = __ballot(v);
+        }
+        const int k = k0 + __builtin_ctzll(todo);
+        todo &= todo - 1;
+        return __builtin_amdgcn_readfirstlane(k);
     };
 
-    // the first tile is on its way while Q is converted
-    int t = tile0 + wave;
-    Mask mk0, mk1;
-    if (t < tile1) {
-        load_mask(mk0, t);
-        load_mask(mk1, min(t + NW, ntiles - 1));
-        load_k(t);
-        load_v(t);
+    // Q in the B layout of the Q.K products, scaled, fp16, in LDS: wave n makes the operands of query tile n.
+    // Its loads go out before the first tile's, which comes while Q is converted.
+    half8 * const lq = (half8 *)smem;                                       // [NQ][KS][64]
+    float * const lqf = (float *)(smem + NQ * C::KS * 1024);                // [NQ][16]: 0 where no row needs a factor
+    // a lane's dims of block st: runs of four at q_dim(st, 0) and q_dim(st, 1); past dk zeros
+    auto q_dim = [&](int st, int hlf) { return 32 * st + (KT == T_Q8_0 ? 8 * g + 4 * hlf : 4 * g + 16 * hlf); };
+    float4v qx[C::KS][2];
+    half4 qh[C::KS][2];
+    const int qrow = (rt * NQ + wave) * 16 + r;
+    const bool qok = qrow < a.R;
+    if (wave < NQ) {
+        const int qtok = qok ? fq_div(qrow, a.div_g) : 0, qhead = hk * a.G + (qok ? qrow - qtok * a.G : 0);
+        const int64_t at = (int64_t)s * a.q_nb3 + (int64_t)qhead * a.q_nb2 + (int64_t)qtok * a.q_nb1;
+#pragma unroll
+        for (int st = 0; st < C::KS; st++)
+#pragma unroll
+            for (int hlf = 0; hlf < 2; hlf++) {
+                const int64_t d = at + min(q_dim(st, hlf), a.dk - 4);
+                if (a.q_f16) qh[st][hlf] = *(const half4 *)((const uint16_t *)a.q + d);
+                else qx[st][hlf] = *(const float4v *)((const float *)a.q + d);
+            }
     }
 
-    // Q in the B layout of the Q.K products, scaled, fp16; a row past fp16's range is divided by a
-    // factor that multiplies its scores
-    half8 qf[NQ][C::KS];
-    float qfac[NQ];
-    bool q_scaled = false;
-#pragma unroll
-    for (int n = 0; n < NQ; n++) {
-        const int64_t at = (int64_t)s * a.q_nb3 + (int64_t)head[n] * a.q_nb2 + (int64_t)tok[n] * a.q_nb1;
-        // a lane's dims of a product: runs of four at q_dim(st, 0) and q_dim(st, 1); past dk zeros
-        auto q_dim = [&](int st, int hlf) {
-            const int i = st / C::SPP, w = st % C::SPP, c = g + 4 * i;
-            if constexpr (KT == T_Q8_0) return 16 * c + 8 * w + 4 * hlf;
-            return (C::CB == 16 ? 32 * c : 32 * (c / 2) + 8 * (c % 2)) + 4 * w + 16 * hlf;
-        };
+    // the first two tiles
+    const int ka = next();
+    int kn = ka >= 0 ? next() : -1, buf = 0;
+    int t = tile0 + wave + NW * max(ka, 0), tn = kn >= 0 ? tile0 + wave + NW * kn : t;
+    Side x;
+    if (ka >= 0) {
+        dma(t, 0);
+        asm volatile("" ::: "memory");
+        load_side(x, t);
+        asm volatile("" ::: "memory");
+        dma(tn, 1);
+    }
+
+    if (wave < NQ) {
         float v[C::KS][8], amax = 0.0f;
-        if (a.q_f16) {
-            half4 x[C::KS][2];
-#pragma unroll
-            for (int st = 0; st < C::KS; st++)
-#pragma unroll
-                for (int hlf = 0; hlf < 2; hlf++)
-                    x[st][hlf] = *(const half4 *)((const uint16_t *)a.q + at + min(q_dim(st, hlf), a.dk - 4));
-#pragma unroll
-            for (int st = 0; st < C::KS; st++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[st][e] = (float)x[st][e / 4][e % 4];
-        } else {
-            float4v x[C::KS][2];
-#pragma unroll
-            for (int st = 0; st < C::KS; st++)
-#pragma unroll
-                for (int hlf = 0; hlf < 2; hlf++) x[st][hlf] = *(const float4v *)((const float *)a.q + at + min(q_dim(st, hlf), a.dk - 4));
-#pragma unroll
-            for (int st = 0; st < C::KS; st++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[st][e] = x[st][e / 4][e % 4];
-        }
 #pragma unroll
         for (int st = 0; st < C::KS; st++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                v[st][e] = ok[n] && q_dim(st, e / 4) < a.dk ? v[st][e] * a.scale : 0.0f;
+                const float x = a.q_f16 ? (float)qh[st][e / 4][e % 4] : qx[st][e / 4][e % 4];
+                v[st][e] = qok && q_dim(st, e / 4) < a.dk ? x * a.scale : 0.0f;
                 amax = fmaxf(amax, fabsf(v[st][e]));
             }
         amax = fq_col_max(amax);
-        qfac[n] = amax > 65504.0f ? amax / 32768.0f : 1.0f;
-        const float inv = 1.0f / qfac[n];
+        // a row outside [2^-6, 2^15] is divided by a factor that multiplies its scores (its largest value
+        // goes to 2^4, so that the smaller ones, and 1/16 of them, keep their bits)
+        const float qfac = (amax > 32768.0f || (amax < 0.015625f && amax > 0.0f)) ? amax / 16.0f : 1.0f;
+        const float inv = 1.0f / qfac;
 #pragma unroll
-        for (int st = 0; st < C::KS; st++)
+        for (int st = 0; st < C::KS; st++) {
+            half8 qf;
 #pragma unroll
-            for (int e = 0; e < 8; e++) qf[n][st][e] = (_Float16)(qfac[n] == 1.0f ? v[st][e] : v[st][e] * inv);
-        q_scaled |= qfac[n] != 1.0f;
-        __builtin_amdgcn_sched_barrier(0);   // one tile's F32 rows at a time
+            for (int e = 0; e < 8; e++) {
+                // slot e of fq_key is value e (Q8_0), or 0, 2, 1, 3 of either half
+                const float x = v[st][KT == T_Q8_0 ? e : (e & 4) | (e & 1) << 1 | (e & 2) >> 1] * inv;
+                qf[e] = (_Float16)(KT == T_Q4_0 && e >= 4 ? x * 0.0625f : x);
+            }
+            lq[(wave * C::KS + st) * WAVE + lane] = qf;
+        }
+        if (g == 0) lqf[wave * 16 + r] = __any(qfac != 1.0f) ? qfac : 0.0f;
     }
-    q_scaled = __any(q_scaled);
+    // a barrier for LDS alone: the first tile's loads stay in flight
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 
-    float4v o[NQ][C::TT];
+    // the offsets' products: -128 2^-24 (Q8_0), -8 2^-24 and, for high nibbles, -128 2^-24 (Q4_0) in every
+    // element, as bits of halves
+    constexpr uint32_t kOffLo = KT == T_Q8_0 ? 0x80808080u : 0x80088008u, kOffHi = 0x80808080u;
+    u32x4 koff = {kOffLo, kOffLo, kOffHi, kOffHi};
+    float4v o[NQ][C::TT], oc[NQ][C::VJ];   // O^T without the offsets, and sum P d 2^k
     float m_run[NQ], l_run[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
@@ -342,73 +397,75 @@ fa_q_kernel(FaQArgs a) {
         l_run[n] = 0.0f;
 #pragma unroll
         for (int t = 0; t < C::TT; t++) o[n][t] = float4v{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < C::VJ; j++) oc[n][j] = float4v{0, 0, 0, 0};
     }
+    float vscale = 1.0f;        // 2^k
+    uint32_t vtop = 0;          // the largest scale it is for, as bits: 2^(15 - k)
     const float cap2 = a.softcap != 0.0f ? 2.0f * FQ_LOG2E / a.softcap : 0.0f;
-    uint8_t * const ws = smem + wave * C::SCALE_LDS;   // this wave's V scales [block][key]
 
-    bool vis = t < tile1 && seen(mk0);
-    while (t < tile1) {
-        const bool next = t + NW < tile1;
+    while (ka >= 0) {
+        fq_wait_vm<C::KD + C::VD>();   // everything older than the next tile's DMA has landed: this tile
+        Side xn;
+        load_side(xn, tn);
+        asm volatile("" ::: "memory");
         const int kb = min(FQ_KEYS * t, kb_last);
-        // the lane offsets stay 32-bit registers beside scalar bases (widened outside the loop they would
-        // be pairs, and every address a 64-bit addition)
-#pragma unroll
-        for (int i = 0; i < C::KI; i++) asm("" : "+v"(ko[i]), "+v"(kdo[i]));
-#pragma unroll
-        for (int i = 0; i < C::VJ; i++) asm("" : "+v"(vo[i]));
-#pragma unroll
-        for (int i = 0; i < C::VS; i++) asm("" : "+v"(vdo[i]));
+        const uint8_t * const st = wl + C::SCALE_LDS + buf * C::STAGE;
+        const uint8_t * const stv = st + FQ_KEYS * 16 * C::KCH;
+        asm("" : "+v"(koff));   // the offsets' products stay inside the loop: no room for them in registers
         float4v sc[NQ][2];
-        if (vis) {
-            // V's scales into LDS, those that are not finite as zeros; their keys get a NaN K scale
-            // instead, so that it is their scores that become NaN
-            bool bad = false;
+        {
+            // ---- S^T = K . Q^T, each block's product times its scale (and 2^24) ----
 #pragma unroll
-            for (int i = 0; i < C::VS; i++) {
-                bad |= (xvd[i] & 0x7C00u) == 0x7C00u;
-                *(uint16_t *)(ws + (((lane / 32) * C::VS + i) * FQ_KEYS + lane % 32) * 2) = fq_scale<VT>(xvd[i], 0);
-            }
-            const uint64_t bad_lanes = __ballot(bad);
-            if (bad_lanes) {
-                const uint32_t bad_keys = (uint32_t)bad_lanes | (uint32_t)(bad_lanes >> 32);
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++)
-                    if ((bad_keys >> (16 * hf + r)) & 1u) xkd[hf][0] = 0x7E00;
-            }
+            for (int i = 0; i < C::KSC; i++)
+                wk[((lane % 2) * C::KSC + i) * FQ_KEYS + lane / 2] = fq_scale<KT>(x.kd[i], NAN) * 16777216.0f;
             asm volatile("" ::: "memory");   // one wave's LDS operations complete in order
-            // ---- S^T = K . Q^T ----
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
+            for (int n = 0; n < NQ; n++) sc[n][0] = sc[n][1] = float4v{0, 0, 0, 0};
 #pragma unroll
-                for (int n = 0; n < NQ; n++) sc[n][hf] = float4v{0, 0, 0, 0};
+            for (int i = 0; i < C::KS; i++) {
+                float4v off[NQ];
+                half8 qf[NQ];
 #pragma unroll
-                for (int i = 0; i < C::KI; i++) {
-                    const half2v d = h2_of(fq_scale<KT>(xkd[hf][i], 0x7E00) * 0x10001u);
+                for (int n = 0; n < NQ; n++) qf[n] = lq[(n * C::KS + i) * WAVE + lane];
 #pragma unroll
-                    for (int w = 0; w < C::SPP; w++) {
-                        const half8 kf = KT == T_Q8_0 ? fq_key<KT>(xk[hf][i][(2 * w) % (C::CB / 4)], xk[hf][i][(2 * w + 1) % (C::CB / 4)], d)
-                                                      : fq_key<KT>(xk[hf][i][w % (C::CB / 4)], 0, d);
+                for (int n = 0; n < NQ; n++)
+                    off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), qf[n], float4v{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-                        for (int n = 0; n < NQ; n++)
-                            sc[n][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n][i * C::SPP + w], sc[n][hf], 0, 0, 0);
+                for (int hf = 0; hf < 2; hf++) {
+                    const float4v d = *(const float4v *)(wk + i * FQ_KEYS + 16 * hf + 4 * g);
+                    uint32_t kx[2];
+                    if constexpr (C::KW == 2) {
+                        const u32x2 w = *(const u32x2 *)(st + (kra ^ (uint32_t)(32 * i)) + hf * 256 * C::KCH);
+                        kx[0] = w[0];
+                        kx[1] = w[1];
+                    } else {
+                        kx[0] = *(const uint32_t *)(st + (kra ^ (uint32_t)(16 * i)) + hf * 256 * C::KCH);
+                    }
+                    const half8 kf = fq_key<KT>(kx);
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) {
+                        const float4v p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], off[n], 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sc[n][hf][e] = fmaf(p[e], d[e], sc[n][hf][e]);
                     }
                 }
+                if ((i + 1) * NQ % 2 == 0) __builtin_amdgcn_sched_barrier(0);   // not every block's operands at once
             }
         }
-        const bool vis1 = next && seen(mk1);
-        const int tn = __builtin_amdgcn_readfirstlane(vis1 ? t + NW : t);
-        load_k(tn);   // the next tile's, or this one's again
         half8 pf[NQ];
-        if (vis) {
+        float dv[C::VS];
+        {
             // ---- scale back, cap, mask, softmax ----
             const bool part = kb < FQ_KEYS * t;
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
-                if (q_scaled) {
+                const float qfac = lqf[n * 16 + r];
+                if (__any(qfac != 0.0f)) {
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) sc[n][hf][e] *= qfac[n];
+                        for (int e = 0; e < 4; e++) sc[n][hf][e] *= qfac;
                 }
                 if (a.softcap != 0.0f) {
                     // cap * tanh(s / cap) = cap - 2 cap / (1 + exp(2 s / cap)): off by some 1e-7 of cap
@@ -418,12 +475,12 @@ fa_q_kernel(FaQArgs a) {
                         for (int e = 0; e < 4; e++)
                             sc[n][hf][e] = fmaf(-2.0f * a.softcap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[n][hf][e] * cap2)), a.softcap);
                 }
-                if (a.mask) {
+                if (a.mask && __any((x.m[n][0][0] | x.m[n][0][1] | x.m[n][1][0] | x.m[n][1][1]) != 0)) {
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const float mv = h2f_bits((uint16_t)(mk0[n][hf][e / 2] >> (16 * (e % 2))));
+                            const float mv = h2f_bits((uint16_t)(x.m[n][hf][e / 2] >> (16 * (e % 2))));
                             sc[n][hf][e] = mv == -INFINITY ? -INFINITY : sc[n][hf][e] + mv;   // a hidden score may be NaN
                         }
                 }
@@ -449,6 +506,10 @@ fa_q_kernel(FaQArgs a) {
                     for (int q = 0; q < C::TT; q++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[n][q][e] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < C::VJ; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) oc[n][j][e] *= alpha;
                 }
                 const float mb = m_run[n] == -INFINITY ? 0.0f : m_run[n] * FQ_LOG2E;
                 const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
@@ -463,59 +524,140 @@ fa_q_kernel(FaQArgs a) {
                         l_run[n] = __builtin_amdgcn_fdot2(p, one2, l_run[n], false);   // the sum of what is multiplied
                     }
             }
-        }
-        // the mask moves up a tile here, where the one in flight has long come: a copy of a register that a
-        // load behind the codes' still writes would wait for all of them
+            // ---- V's scales (key lane / 2): the power of two they are held under ----
+            uint16_t top = 0;
+            bool bad = false;
 #pragma unroll
-        for (int n = 0; n < NQ; n++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                mk0[n][hf] = mk1[n][hf];
-                asm volatile("" : "+v"(mk0[n][hf]));
+            for (int i = 0; i < C::VS; i++) {
+                bad |= (x.vd[i] & 0x7C00u) == 0x7C00u;
+                dv[i] = fq_scale<VT>(x.vd[i], 0.0f);
+                top = max(top, (uint16_t)(x.vd[i] & 0x7FFFu));
             }
-        load_mask(mk1, min(t + 2 * NW, ntiles - 1));
-        if (vis) {
+            if (__any(top > vtop)) {
+                // a larger scale than any before, or one that is not finite (which stands for zero and makes
+                // the row sums of the rows that see its key NaN); keys that no row sees count as zeros
+                bool hidden = false;
+#pragma unroll
+                for (int n = 0; n < NQ; n++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) hidden |= ok[n] && sc[n][e / 4][e % 4] == -INFINITY;
+                if (__any(hidden)) {
+                    uint32_t seen_keys = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        bool any = false;
+#pragma unroll
+                        for (int n = 0; n < NQ; n++) any |= ok[n] && sc[n][e / 4][e % 4] != -INFINITY;
+                        const uint64_t rows = __ballot(any);
+#pragma unroll
+                        for (int gg = 0; gg < 4; gg++)
+                            seen_keys |= (uint32_t)(((rows >> (16 * gg)) & 0xFFFFu) != 0) << (16 * (e / 4) + 4 * gg + e % 4);
+                    }
+                    const bool mine = (seen_keys >> (lane / 2)) & 1u;
+                    bad &= mine;
+#pragma unroll
+                    for (int i = 0; i < C::VS; i++) dv[i] = mine ? dv[i] : 0.0f;
+                }
+                const uint64_t bad_lanes = __ballot(bad);
+                if (bad_lanes) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if ((bad_lanes >> (2 * (16 * (e / 4) + 4 * g + e % 4))) & 3u) {
+#pragma unroll
+                            for (int n = 0; n < NQ; n++)
+                                if (sc[n][e / 4][e % 4] != -INFINITY) l_run[n] = NAN;
+                        }
+                }
+                float dmax = 0.0f;
+#pragma unroll
+                for (int i = 0; i < C::VS; i++) dmax = fmaxf(dmax, fabsf(dv[i]));
+                dmax = fq_wave_max(dmax);
+                // a power of two at least as large, by its exponent
+                const uint32_t pow2 = (__float_as_uint(dmax) + 0x7FFFFFu) & 0x7F800000u;
+                const float next_scale = dmax > 0.0f ? __uint_as_float((269u << 23) - pow2) : INFINITY;   // 2^15 / pow2
+                if (next_scale < vscale || vtop == 0) {
+                    const float f = vtop == 0 ? 1.0f : next_scale * __builtin_amdgcn_rcpf(vscale);   // powers of two: exact
+                    if (dmax > 0.0f) {
+                        vscale = next_scale;
+                        vtop = f2h_bits(__uint_as_float(pow2));
+                    }
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) {
+#pragma unroll
+                        for (int q = 0; q < C::TT; q++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[n][q][e] *= f;
+#pragma unroll
+                        for (int j = 0; j < C::VJ; j++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) oc[n][j][e] *= f;
+                    }
+                }
+            }
+        }
+        {
+            // ---- V's scales into LDS, times 2^k ----
+#pragma unroll
+            for (int i = 0; i < C::VS; i++) wv[((lane % 2) * C::VS + i) * FQ_KEYS + lane / 2] = f2h_bits(dv[i] * vscale);
+            asm volatile("" ::: "memory");
             // ---- O^T += V^T . P^T ----
 #pragma unroll
             for (int j = 0; j < C::VJ; j++) {
                 half2v d[4];
                 {
-                    const uint8_t * p = ws + vblk[j] * FQ_KEYS * 2 + 8 * g;
-                    d[0] = h2_of(*(const u32_alias *)p);
-                    d[1] = h2_of(*(const u32_alias *)(p + 4));
-                    d[2] = h2_of(*(const u32_alias *)(p + 32));
-                    d[3] = h2_of(*(const u32_alias *)(p + 36));
+                    const u32x2 lo = *(const u32x2 *)(wv + vblk[j] * FQ_KEYS + 4 * g), hi = *(const u32x2 *)(wv + vblk[j] * FQ_KEYS + 16 + 4 * g);
+                    d[0] = h2_of(lo[0]);
+                    d[1] = h2_of(lo[1]);
+                    d[2] = h2_of(hi[0]);
+                    d[3] = h2_of(hi[1]);
+                }
+                const half8 ds = __builtin_bit_cast(half8, u32x4{u_of(d[0]), u_of(d[1]), u_of(d[2]), u_of(d[3])});
+#pragma unroll
+                for (int nq = 0; nq < NQ; nq++) oc[nq][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ds, pf[nq], oc[nq][j], 0, 0, 0);
+                uint32_t xe[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint8_t * p = stv + vra[j] + (e / 4 * 16 + e % 4 * 4) * C::VRB;
+                    if constexpr (C::VU == 4) xe[e] = *(const uint32_t *)p;
+                    else xe[e] = *(const uint16_t *)p;
+                    if constexpr (VT == T_Q8_0) xe[e] ^= 0x80808080u;
                 }
 #pragma unroll
                 for (int n = 0; n < C::VU; n++) {
                     uint32_t y[4];   // byte n of keys (2 e, 2 e + 1), zero-extended
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        y[e] = __builtin_amdgcn_perm(xv[2 * e + 1][j], xv[2 * e][j], 0x0C000C00u | ((uint32_t)(4 + n) << 16) | (uint32_t)n);
+                        y[e] = __builtin_amdgcn_perm(xe[2 * e + 1], xe[2 * e], 0x0C000C00u | ((uint32_t)(4 + n) << 16) | (uint32_t)n);
 #pragma unroll
                     for (int h = 0; h < C::VH; h++) {
-                        half8 vf;
+                        u32x4 w;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            half2v p;
-                            if constexpr (VT == T_Q8_0) p = h2_of(y[e] ^ 0x64806480u) + half2v{(_Float16)-1152.0f, (_Float16)-1152.0f};
-                            else p = h2_of(((h ? y[e] >> 4 : y[e]) & 0x000F000Fu) | 0x64006400u) + half2v{(_Float16)-1032.0f, (_Float16)-1032.0f};
-                            p = p * d[e];
-                            vf[2 * e] = p[0];
-                            vf[2 * e + 1] = p[1];
-                        }
+                        for (int e = 0; e < 4; e++)
+                            w[e] = u_of(h2_of(VT == T_Q8_0 ? y[e] : y[e] & (h ? 0x00F000F0u : 0x000F000Fu)) * d[e]);
                         const int q = (j * C::VU + n) * C::VH + h;
 #pragma unroll
-                        for (int nq = 0; nq < NQ; nq++) o[nq][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[nq], o[nq][q], 0, 0, 0);
+                        for (int nq = 0; nq < NQ; nq++)
+                            o[nq][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), pf[nq], o[nq][q], 0, 0, 0);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            asm volatile("" ::: "memory");   // the next tile's scales are written after these reads
         }
-        load_v(tn);
-        t += NW;
-        vis = vis1;
+        // this tile's buffer has been read: the one after the next may come into it (the last ones again,
+        // where there is none: the number of loads in flight stays what the wait above counts)
+        const int k2 = kn >= 0 ? next() : -1;
+        const int t2 = k2 >= 0 ? tile0 + wave + NW * k2 : tn;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        dma(t2, buf);
+        asm volatile("" ::: "memory");
+        if (kn < 0) break;
+        x = xn;
+        t = tn;
+        tn = t2;
+        kn = k2;
+        buf ^= 1;
     }
+    fq_wait_vm<0>();   // no DMA may still write what the merge reuses
 
     // ---- merge the block's waves ----
     float * const sml = (float *)smem;                     // [NW][16 NQ][2]: (max, sum)
@@ -560,9 +702,13 @@ fa_q_kernel(FaQArgs a) {
 #pragma unroll
         for (int i = 0; i < C::CT; i++) {
             const int n = (c0 + i) / C::TT, q = (c0 + i) % C::TT;
+            // values: the offset off (in units of 2^-24 d), then 2^24, 2^-k and a high nibble's 1/16
+            constexpr float kOff = VT == T_Q8_0 ? 128.0f : 8.0f;
+            const bool high = VT == T_Q4_0 && q % 2;
             float4v v = o[n][q];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] *= wgt[n];
+            for (int e = 0; e < 4; e++)
+                v[e] = fmaf(oc[n][q / (C::TT / C::VJ)][e], -kOff, v[e] * (high ? 1048576.0f : 16777216.0f)) * (wgt[n] * __builtin_amdgcn_rcpf(vscale));
             so[(wave * C::CT + i) * WAVE + lane] = v;
         }
         __syncthreads();
@@ -585,7 +731,7 @@ fa_q_kernel(FaQArgs a) {
 #pragma unroll
             for (int k = 1; k < NQ; k++)
                 if (n == k) Ln = L[k];
-            const float inv = Ln > 0.0f ? 1.0f / Ln : 0.0f;
+            const float inv = Ln == 0.0f ? 0.0f : 1.0f / Ln;   // no key seen: zeros; a NaN stays
             const int tk = fq_div(row, a.div_g);
             const int64_t dst = (int64_t)s * a.dst_nb3 + (int64_t)tk * a.dst_nb2 + (int64_t)(hk * a.G + row - tk * a.G) * a.dst_nb1;
 #pragma unroll

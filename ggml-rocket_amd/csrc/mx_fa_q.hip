@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256) fa_q_combine_kernel(FaQArgs a, int vt, in
     for (int i = 0; i < 16; i++) L += sl[i][r];
     const int row = (rt * NQ + n) * 16 + r;
     if (row >= a.R) return;
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const int tk = fq_div(row, a.div_g);
     const int64_t dst = (int64_t)s * a.dst_nb3 + (int64_t)tk * a.dst_nb2 + (int64_t)(hk * a.G + row - tk * a.G) * a.dst_nb1;
     const int vu = vt == T_Q8_0 || DV >= 128 ? 4 : 2;

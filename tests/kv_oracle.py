@@ -58,11 +58,16 @@ def attention(q, k, v, mask, scale, softcap=0.0):
     output. Q and K rounded once each move a score by at most e = scale * sum|q||k| * (2 * HALF +
     HALF^2), a soft-cap by no more; P and the row sum then move by a factor within exp(+-2 e), P and V
     are rounded once each, and a P under fp16's normal range by at most 2^-25; f32 sums add the last
-    2^-12 (64k terms at 2^-24, roots of which survive: the bound is loose here)."""
+    2^-12 (64k terms at 2^-24, roots of which survive: the bound is loose here). The kernel that reads the cache
+    as it is stored rounds V with its code's offset, d * (code + 128) or d * (code + 8), at most 255 d or
+    15 d where a block's largest value is 127 d or 7 d at least (a largest negative code is 8 d): off by
+    at most HALF * 15 / 7 of the largest magnitude in the block, instead of HALF of the value."""
     q, k, v = (np.asarray(a, dtype=np.float64) for a in (q, k, v))
     H, T, D = q.shape
     HK, KV, DV = v.shape
     out, tol = np.zeros((T, H, DV)), np.zeros((T, H, DV))
+    # the largest magnitude of each block of 32 dims, times 15 / 7
+    vmax = np.repeat(np.abs(v).reshape(HK, KV, DV // 32, 32).max(-1), 32, -1) * (15 / 7)
     for h in range(H):
         kh, vh = k[h * HK // H], v[h * HK // H]
         for t in range(T):
@@ -70,7 +75,7 @@ def attention(q, k, v, mask, scale, softcap=0.0):
             see = m != -np.inf
             if not see.any():
                 continue
-            ks, vs = kh[see], vh[see]
+            ks, vs, vb = kh[see], vh[see], vmax[h * HK // H][see]
             x = ks @ q[h, t] * scale
             if softcap:
                 x = softcap * np.tanh(x / softcap)
@@ -81,5 +86,5 @@ def attention(q, k, v, mask, scale, softcap=0.0):
             out[t, h] = p @ vs / p.sum()
             with np.errstate(over="ignore", invalid="ignore"):   # however the weights move, outputs stay among the values
                 moved = np.minimum(np.where(size > 0, size * np.expm1(2 * e), np.inf), 2 * np.abs(vs).max(0))
-            tol[t, h] = moved + size * (2 * HALF + 2.0 ** -12) + see.sum() * 2.0 ** -25 * np.abs(vs).max()
+            tol[t, h] = moved + size * (HALF + 2.0 ** -12) + (p @ vb / p.sum()) * HALF + see.sum() * 2.0 ** -25 * np.abs(vs).max()
     return out, tol
