@@ -645,11 +645,11 @@ static bool kv_type(int t) { return t == mx::T_Q8_0 || t == mx::T_Q4_0; }
 
 static int kv_rows_lower(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n, int32_t * err_dev,
                          mx::KvRowsArgs & a) {
-    if (!r || n_out < 1 || n_out > mx::KV_MAX_OUT || n < 0 || n > INT32_MAX) return MI355X_E_ARG;
+    if (!r || n_out < 1 || n_out > mx::KV_MAX_OUT || n < 0 || n > (1 << 30)) return MI355X_E_ARG;
     if (idx_type != 26 && idx_type != 27) return MI355X_E_ARG;
     if (!aligned(idx_dev, idx_type == 27 ? 8 : 4) || !aligned(err_dev, 4)) return MI355X_E_ARG;
     memset(&a, 0, sizeof a);
-    int64_t wgs = 0;   // of either launch, one workgroup per row or per 64 blocks
+    // 32-bit positions (fq_div): blocks of one output and of a workgroup's rows below 2^30
     for (int k = 0; k < n_out; k++) {
         const mi355x_kv_rows & s = r[k];
         if ((!kv_type(s.type) && s.type != mx::T_F16) || (s.x_type != mx::T_F32 && s.x_type != mx::T_F16)) return MI355X_E_ARG;
@@ -659,13 +659,13 @@ static int kv_rows_lower(const mi355x_kv_rows * r, int n_out, const void * idx_d
         if (n > 0 && (!s.q_dev || !s.x_dev || !aligned(s.q_dev, 16) || !aligned(s.x_dev, 16))) return MI355X_E_ARG;
         if (n > 0 && s.type != mx::T_F16 && (!s.d_dev || !aligned(s.d_dev, 8))) return MI355X_E_ARG;
         if (!idx_dev && n > s.n_rows) return MI355X_E_ARG;
-        wgs += n * std::max<int64_t>(1, (s.H * (s.D / 32) + 63) / 64);
+        const int64_t bpr = s.H * (s.D / 32);
+        if (bpr > (1 << 24) || n * bpr > (1 << 30)) return MI355X_E_ARG;
         mx::KvRowsOut & o = a.o[k];
         o.q = (uint8_t *)s.q_dev; o.d = s.d_dev; o.x = s.x_dev;
         o.nb1 = s.nb1; o.nb2 = s.nb2; o.x_nb1 = s.x_nb1; o.x_nb2 = s.x_nb2; o.n_rows = s.n_rows;
         o.type = s.type; o.H = (int)s.H; o.bph = (int)(s.D / 32); o.x_f16 = s.x_type == mx::T_F16;
     }
-    if (wgs > INT32_MAX) return MI355X_E_ARG;
     a.n_out = n_out; a.n = (int)n; a.idx = idx_dev; a.idx64 = idx_type == 27; a.err = err_dev;
     return MI355X_OK;
 }

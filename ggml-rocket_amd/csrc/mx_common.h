@@ -146,6 +146,18 @@ __device__ __forceinline__ void pack_row_wave(const float * x, int m, int K, uin
     if (lane == 0) scales[m] = s;
 }
 
+// Division by d in [1, 2^30] of values below 2^30: mul = floor(2^32 / d) + 1 (d 1: not read).
+struct FqDiv {
+    uint32_t mul;
+    int d;
+};
+inline FqDiv fq_div_by(int d) { return {(uint32_t)(((uint64_t)1 << 32) / (uint32_t)d + 1), d}; }
+// n / d: the product's high word is the quotient or one more.
+__device__ __forceinline__ int fq_div(int n, const FqDiv & d) {
+    const uint32_t q = __umulhi((uint32_t)n, d.mul);
+    return d.d == 1 ? n : (int)(q * (uint32_t)d.d > (uint32_t)n ? q - 1 : q);
+}
+
 // Blocks are handed to the 8 XCDs round-robin by linear id. Renumber so that each XCD gets a
 // contiguous run of logical ids (XCD x takes ids [x q + min(x, r), ...) of its q or q + 1
 // blocks, q = n / 8, r = n % 8; a bijection for any n): work items that share an operand panel

@@ -89,6 +89,8 @@ struct FqCfg {
     static constexpr int FIT = (FQ_LDS_MAX - Q_LDS) / WAVE_LDS / 4 * 4;
     static constexpr int NW = FIT < 4 * WPE ? FIT : 4 * WPE;
     static_assert(NW >= 4, "LDS");
+    // with two waves a SIMD or fewer and one query tile there is room to keep the offsets' products
+    static constexpr bool KEEP_OFF = NQ == 1 && NW <= 8;
     static constexpr int CT = TT * NQ < 8 ? TT * NQ : 8;      // O^T tiles merged at a time
     static constexpr int LOOP_LDS = Q_LDS + NW * WAVE_LDS;
     static constexpr int MERGE_LDS = NW * 16 * NQ * 8 + NW * CT * 1024;
@@ -141,12 +143,6 @@ __device__ __forceinline__ float fq_wave_max(float x) {
     return fq_col_max(x);
 }
 
-// n / d of a FqDiv made for d: the product is the quotient or one more.
-__device__ __forceinline__ int fq_div(int n, const FqDiv & d) {
-    const uint32_t q = __umulhi((uint32_t)n, d.mul);
-    return d.d == 1 ? n : (int)(q * (uint32_t)d.d > (uint32_t)n ? q - 1 : q);
-}
-
 // A block's scale: held to the largest with which every value stays inside fp16 (kv_scale_limit), as
 // where the cache is decoded first; infinite or NaN ones as `bad`.
 template <int TYPE>
@@ -173,7 +169,7 @@ __device__ __forceinline__ half8 fq_key(const uint32_t * x) {
 
 template <int KT, int VT, int DK, int DV, int NQ>
 __global__ void __launch_bounds__((FqCfg<KT, VT, DK, DV, NQ>::NW * WAVE))
-__attribute__((amdgpu_waves_per_eu(FqCfg<KT, VT, DK, DV, NQ>::WPE, FqCfg<KT, VT, DK, DV, NQ>::WPE)))
+__attribute__((amdgpu_waves_per_eu(FqCfg<KT, VT, DK, DV, NQ>::NW / 4, FqCfg<KT, VT, DK, DV, NQ>::NW / 4)))
 fa_q_kernel(FaQArgs a) {
     using C = FqCfg<KT, VT, DK, DV, NQ>;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -321,35 +317,39 @@ fa_q_kernel(FaQArgs a) {
     float * const lqf = (float *)(smem + NQ * C::KS * 1024);                // [NQ][16]: 0 where no row needs a factor
     // a lane's dims of block st: runs of four at q_dim(st, 0) and q_dim(st, 1); past dk zeros
     auto q_dim = [&](int st, int hlf) { return 32 * st + (KT == T_Q8_0 ? 8 * g + 4 * hlf : 4 * g + 16 * hlf); };
-    float4v qx[C::KS][2];
-    half4 qh[C::KS][2];
+    u32x4 qraw[C::KS][2];   // four values each: F32, or F16 in the first two words
     const int qrow = (rt * NQ + wave) * 16 + r;
     const bool qok = qrow < a.R;
     if (wave < NQ) {
         const int qtok = qok ? fq_div(qrow, a.div_g) : 0, qhead = hk * a.G + (qok ? qrow - qtok * a.G : 0);
         const int64_t at = (int64_t)s * a.q_nb3 + (int64_t)qhead * a.q_nb2 + (int64_t)qtok * a.q_nb1;
+        if (a.q_f16) {
 #pragma unroll
-        for (int st = 0; st < C::KS; st++)
+            for (int st = 0; st < C::KS; st++)
 #pragma unroll
-            for (int hlf = 0; hlf < 2; hlf++) {
-                const int64_t d = at + min(q_dim(st, hlf), a.dk - 4);
-                if (a.q_f16) qh[st][hlf] = *(const half4 *)((const uint16_t *)a.q + d);
-                else qx[st][hlf] = *(const float4v *)((const float *)a.q + d);
-            }
+                for (int hlf = 0; hlf < 2; hlf++) {
+                    const u32x2 w = *(const u32x2 *)((const uint16_t *)a.q + at + min(q_dim(st, hlf), a.dk - 4));
+                    qraw[st][hlf] = u32x4{w[0], w[1], 0, 0};
+                }
+        } else {
+#pragma unroll
+            for (int st = 0; st < C::KS; st++)
+#pragma unroll
+                for (int hlf = 0; hlf < 2; hlf++) qraw[st][hlf] = *(const u32x4 *)((const float *)a.q + at + min(q_dim(st, hlf), a.dk - 4));
+        }
     }
 
-    // the first two tiles
-    const int ka = next();
-    int kn = ka >= 0 ? next() : -1, buf = 0;
-    int t = tile0 + wave + NW * max(ka, 0), tn = kn >= 0 ? tile0 + wave + NW * kn : t;
+    // The first two tiles are requested before their masks are looked at; tiles that turn out hidden are
+    // replaced once they have landed. Waves without tiles read some tile all the same: loads that are
+    // sometimes issued would make every wait behind them a wait for all loads.
+    const int tile_end = ntiles - 1;
+    int t = min(tile0 + wave, tile_end), tn = min(tile0 + wave + NW, tile_end), buf = 0;
     Side x;
-    if (ka >= 0) {
-        dma(t, 0);
-        asm volatile("" ::: "memory");
-        load_side(x, t);
-        asm volatile("" ::: "memory");
-        dma(tn, 1);
-    }
+    dma(t, 0);
+    asm volatile("" ::: "memory");
+    load_side(x, t);
+    asm volatile("" ::: "memory");
+    dma(tn, 1);
 
     if (wave < NQ) {
         float v[C::KS][8], amax = 0.0f;
@@ -357,7 +357,8 @@ fa_q_kernel(FaQArgs a) {
         for (int st = 0; st < C::KS; st++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float x = a.q_f16 ? (float)qh[st][e / 4][e % 4] : qx[st][e / 4][e % 4];
+                const uint32_t half = qraw[st][e / 4][e % 4 / 2] >> (16 * (e % 2));
+                const float x = a.q_f16 ? h2f_bits((uint16_t)half) : __uint_as_float(qraw[st][e / 4][e % 4]);
                 v[st][e] = qok && q_dim(st, e / 4) < a.dk ? x * a.scale : 0.0f;
                 amax = fmaxf(amax, fabsf(v[st][e]));
             }
@@ -379,7 +380,19 @@ fa_q_kernel(FaQArgs a) {
         }
         if (g == 0) lqf[wave * 16 + r] = __any(qfac != 1.0f) ? qfac : 0.0f;
     }
-    // a barrier for LDS alone: the first tile's loads stay in flight
+    const int ka = next();
+    int kn = ka >= 0 ? next() : -1;
+    if (ka > 0 || kn > 1) {
+        fq_wait_vm<0>();
+        t = tile0 + wave + NW * ka;
+        tn = kn >= 0 ? tile0 + wave + NW * kn : t;
+        dma(t, 0);
+        asm volatile("" ::: "memory");
+        load_side(x, t);
+        asm volatile("" ::: "memory");
+        dma(tn, 1);
+    }
+    // a barrier for LDS alone: the first tiles' loads stay in flight
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
@@ -412,7 +425,7 @@ fa_q_kernel(FaQArgs a) {
         const int kb = min(FQ_KEYS * t, kb_last);
         const uint8_t * const st = wl + C::SCALE_LDS + buf * C::STAGE;
         const uint8_t * const stv = st + FQ_KEYS * 16 * C::KCH;
-        asm("" : "+v"(koff));   // the offsets' products stay inside the loop: no room for them in registers
+        if constexpr (!C::KEEP_OFF) asm("" : "+v"(koff));   // else the offsets' products would move out of the loop
         float4v sc[NQ][2];
         {
             // ---- S^T = K . Q^T, each block's product times its scale (and 2^24) ----
@@ -450,7 +463,7 @@ fa_q_kernel(FaQArgs a) {
                         for (int e = 0; e < 4; e++) sc[n][hf][e] = fmaf(p[e], d[e], sc[n][hf][e]);
                     }
                 }
-                if ((i + 1) * NQ % 2 == 0) __builtin_amdgcn_sched_barrier(0);   // not every block's operands at once
+                if (!C::KEEP_OFF) __builtin_amdgcn_sched_barrier(0);   // not every block's operands at once
             }
         }
         half8 pf[NQ];
@@ -639,7 +652,7 @@ fa_q_kernel(FaQArgs a) {
                         for (int nq = 0; nq < NQ; nq++)
                             o[nq][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), pf[nq], o[nq][q], 0, 0, 0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+                    if (!C::KEEP_OFF) __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }

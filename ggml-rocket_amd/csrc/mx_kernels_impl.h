@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "mx_common.h"
+
 namespace mx {
 
 constexpr int GEMM_MAX_GROUPS = 4;
@@ -66,7 +68,8 @@ struct KvRowsOut {
     int64_t nb1, nb2, x_nb1, x_nb2, n_rows;
     int type, H, bph;          // bph: 32-value blocks a head
     bool x_f16;
-    int wg_begin;              // first workgroup of this output (set by the launcher)
+    FqDiv div_bpr, div_bph;    // blocks a row, a head
+    int wg_begin;              // get_rows: the first workgroup of this output (set by the launcher)
 };
 struct KvRowsArgs {
     KvRowsOut o[KV_MAX_OUT];
@@ -85,13 +88,6 @@ struct KvView {
 };
 // The largest fp16 scale with which every value of a block stays inside fp16: 515.5 * 127, 8188 * 8.
 __host__ __device__ constexpr float kv_scale_limit(int type) { return type == 8 ? 515.5f : 8188.0f; }
-
-// Division by d in [1, 2^30] of values below 2^30 (fq_div): mul = floor(2^32 / d) + 1 (d 1: not read).
-struct FqDiv {
-    uint32_t mul;
-    int d;
-};
-inline FqDiv fq_div_by(int d) { return {(uint32_t)(((uint64_t)1 << 32) / (uint32_t)d + 1), d}; }
 
 // FLASH_ATTN_EXT of few rows over a quantized cache: strides in elements.
 struct FaQArgs {
@@ -121,6 +117,7 @@ hipError_t launch_fa_q_Q4_0_Q4_0(const FaQArgs & a, hipStream_t st);
 // K and V of one sequence as fp16 for the fused attention: k16 [HK][KV][D], v16 [HK][KV][DV].
 struct KvDecodeArgs {
     KvView k, v;
+    FqDiv div_blocks, div_hk;  // K and V blocks of a key and head; HK
     uint16_t * k16;
     uint16_t * v16;
     int HK, KV, D, DV;

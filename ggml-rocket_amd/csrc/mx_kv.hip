@@ -10,7 +10,10 @@
 // Both are streams: bound by HBM for many rows and by a launch's latency for few. A block of 32 is
 // the work of four lanes, a quad: lane l takes values 4l..4l+3 and 16+4l..16+4l+3, so it holds the
 // two halves of its four Q4_0 bytes, reads 16-byte pieces, and finds the block's maximum with two
-// DPP exchanges inside the quad.
+// DPP exchanges inside the quad. Reading back, lane l takes values 8l..8l+7, one 16-byte store of fp16
+// (its Q4_0 nibbles are the low or the high ones of eight bytes that two lanes read).
+
+#include <type_traits>
 
 #include "mx_common.h"
 #include "mx_kernels_impl.h"
@@ -71,18 +74,6 @@ __device__ __forceinline__ void kv_load_plain(const KvRowsOut & o, int64_t at, i
         }
     }
 }
-__device__ __forceinline__ void kv_store_plain(const KvRowsOut & o, int64_t at, int l, const float (&v)[8]) {
-    if (o.x_f16) {
-        uint16_t * p = (uint16_t *)o.x + at + 4 * l;
-        *(u32x2 *)p = u32x2{pack2h(v[0], v[1]), pack2h(v[2], v[3])};
-        *(u32x2 *)(p + 16) = u32x2{pack2h(v[4], v[5]), pack2h(v[6], v[7])};
-    } else {
-        float * p = (float *)o.x + at + 4 * l;
-        *(float4v *)p = float4v{v[0], v[1], v[2], v[3]};
-        *(float4v *)(p + 16) = float4v{v[4], v[5], v[6], v[7]};
-    }
-}
-
 // One block quantized by its quad and written at element offset `at` of the cache.
 __device__ __forceinline__ void kv_quantize(const KvRowsOut & o, int64_t at, int l, const float (&v)[8]) {
     if (o.type == T_F16) {
@@ -129,147 +120,209 @@ __device__ __forceinline__ void kv_quantize(const KvRowsOut & o, int64_t at, int
     if (l == 0) o.d[at / 32] = finite ? f2h_bits(d) : (uint16_t)0x7E00;
 }
 
-// A workgroup takes rows_wg consecutive rows of one output. An index that a later row names again
-// is dropped, so that the last of them stays whole whichever workgroup is first: every workgroup
-// scans the indices behind its rows (n * 8 bytes out of L2, while its first values are on their way).
+// A workgroup takes rows_wg consecutive rows of output blockIdx.y. An index that a later row names again is
+// dropped, so that the last of them stays whole whichever workgroup is first: every workgroup scans the
+// indices behind its rows (8 n bytes at most out of L2, four of them in flight a thread) while its first
+// block is on its way, against 4096 bits in LDS that its own indices set; only a hit is compared in full.
+// (4091 rows of 2 x 1024: 15.8 us with every index compared with every row of the workgroup.)
 __global__ void __launch_bounds__(KV_THREADS) set_rows_kernel(KvRowsArgs a) {
     __shared__ int64_t at_row[KV_ROWS_MAX];
     __shared__ int dead[KV_ROWS_MAX];
-    const KvRowsOut & o = a.o[kv_out_of(a, blockIdx.x)];
+    __shared__ uint32_t named[128];
+    const KvRowsOut & o = a.o[blockIdx.y];
     const int t = threadIdx.x, l = t % 4;
-    const int r0 = ((int)blockIdx.x - o.wg_begin) * a.rows_wg, rows = min(a.rows_wg, a.n - r0);
-    const int bpr = o.H * o.bph, items = rows * bpr;
+    const int r0 = (int)blockIdx.x * a.rows_wg, rows = min(a.rows_wg, a.n - r0);
+    const int bpr = o.div_bpr.d, items = rows * bpr;
+    auto load = [&](int it, float (&v)[8]) {
+        const int r = fq_div(it, o.div_bpr), hb = it - r * bpr, h = fq_div(hb, o.div_bph), b = hb - h * o.bph;
+        kv_load_plain(o, (int64_t)(r0 + r) * o.x_nb1 + (int64_t)h * o.x_nb2 + 32 * b, l, v);
+    };
+    float v[8];
+    if (t / 4 < items) load(t / 4, v);
+    if (t < 128) named[t] = 0;
+    __syncthreads();
     if (t < rows) {
         const int64_t i = kv_index(a, r0 + t);
         const bool ok = i >= 0 && i < o.n_rows;
         at_row[t] = ok ? i : -1;
         dead[t] = !ok;
         if (!ok && a.err) *a.err = 1;
+        if (ok) atomicOr(&named[(i & 4095) / 32], 1u << (i % 32));
     }
     __syncthreads();
-    if (a.idx) {
-        for (int j = r0 + 1 + t; j < a.n; j += KV_THREADS) {
-            const int64_t i = kv_index(a, j);
-            for (int r = 0; r < rows; r++)
-                if (j > r0 + r && i == at_row[r]) dead[r] = 1;
+    if (a.idx && a.n > r0 + 1) {
+        for (int j0 = r0 + 1 + t; j0 < a.n; j0 += 4 * KV_THREADS) {
+            int64_t i[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) i[u] = j0 + u * KV_THREADS < a.n ? kv_index(a, j0 + u * KV_THREADS) : -1;
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (i[u] >= 0 && (named[(i[u] & 4095) / 32] >> (i[u] % 32)) & 1u)
+                    for (int r = 0; r < rows; r++)
+                        if (i[u] == at_row[r] && j0 + u * KV_THREADS > r0 + r) dead[r] = 1;
         }
         __syncthreads();
     }
     for (int it = t / 4; it < items; it += KV_BLOCKS) {
-        const int r = it / bpr, hb = it % bpr, h = hb / o.bph, b = hb % o.bph;
-        if (dead[r]) continue;   // the same for the whole quad
-        float v[8];
-        kv_load_plain(o, (int64_t)(r0 + r) * o.x_nb1 + (int64_t)h * o.x_nb2 + 32 * b, l, v);
-        kv_quantize(o, at_row[r] * o.nb1 + (int64_t)h * o.nb2 + 32 * b, l, v);
+        float w[8];
+        if (it + KV_BLOCKS < items) load(it + KV_BLOCKS, w);
+        const int r = fq_div(it, o.div_bpr), hb = it - r * bpr, h = fq_div(hb, o.div_bph), b = hb - h * o.bph;
+        if (!dead[r]) kv_quantize(o, at_row[r] * o.nb1 + (int64_t)h * o.nb2 + 32 * b, l, v);   // the same for the quad
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = w[e];
     }
 }
 
-// A quad's share of a quantized block at element offset `at`: the codes times d, exact in f32.
-__device__ __forceinline__ void kv_values(int type, const uint8_t * q, float d, int64_t at, int l, float (&v)[8]) {
-    if (type == T_Q8_0) {
-        const uint32_t lo = *(const uint32_t *)(q + at + 4 * l), hi = *(const uint32_t *)(q + at + 16 + 4 * l);
+// Lane l's codes of a block at element offset `at`: Q8_0 eight bytes, Q4_0 the eight that hold its
+// nibbles, F16 eight values.
+__device__ __forceinline__ u32x4 kv_codes(int type, const uint8_t * q, int64_t at, int l) {
+    if (type == T_F16) return *(const u32x4 *)((const uint16_t *)q + at + 8 * l);
+    const u32x2 x = *(const u32x2 *)(type == T_Q8_0 ? q + at + 8 * l : q + at / 2 + 8 * (l % 2));
+    return u32x4{x[0], x[1], 0, 0};
+}
+// Their values: the codes times d, exact in f32.
+__device__ __forceinline__ void kv_values(int type, const u32x4 & x, float d, int l, float (&v)[8]) {
+    if (type == T_F16) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v[e] = mul_rn(d, (float)(int8_t)(lo >> (8 * e)));
-            v[4 + e] = mul_rn(d, (float)(int8_t)(hi >> (8 * e)));
-        }
+        for (int e = 0; e < 8; e++) v[e] = h2f_bits((uint16_t)(x[e / 2] >> (16 * (e % 2))));
+    } else if (type == T_Q8_0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = mul_rn(d, (float)(int8_t)(x[e / 4] >> (8 * (e % 4))));
     } else {
-        const uint32_t w = *(const uint32_t *)(q + at / 2 + 4 * l);
+        const u32x2 n = {x[0] >> (4 * (l / 2)), x[1] >> (4 * (l / 2))};
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v[e] = mul_rn(d, (float)((int)((w >> (8 * e)) & 15u) - 8));
-            v[4 + e] = mul_rn(d, (float)((int)((w >> (8 * e + 4)) & 15u) - 8));
-        }
+        for (int e = 0; e < 8; e++) v[e] = mul_rn(d, (float)((int)((n[e / 4] >> (8 * (e % 4))) & 15u) - 8));
     }
 }
+__device__ __forceinline__ u32x4 kv_pack8(const float (&v)[8]) {
+    return u32x4{pack2h(v[0], v[1]), pack2h(v[2], v[3]), pack2h(v[4], v[5]), pack2h(v[6], v[7])};
+}
 
+// A quad reads ILP blocks, KV_BLOCKS apart, all of them requested before the first is stored.
+template <int ILP>
 __global__ void __launch_bounds__(KV_THREADS) get_rows_kernel(KvRowsArgs a) {
     const KvRowsOut & o = a.o[kv_out_of(a, blockIdx.x)];
     const int t = threadIdx.x, l = t % 4;
-    const int bpr = o.H * o.bph;
-    const int64_t it = (int64_t)((int)blockIdx.x - o.wg_begin) * KV_BLOCKS + t / 4;
-    if (it >= (int64_t)a.n * bpr) return;
-    const int r = (int)(it / bpr), hb = (int)(it % bpr), h = hb / o.bph, b = hb % o.bph;
-    const int64_t i = kv_index(a, r);
-    if (i < 0 || i >= o.n_rows) {
-        if (a.err) *a.err = 1;
-        return;
-    }
-    const int64_t at = i * o.nb1 + (int64_t)h * o.nb2 + 32 * b;
-    float v[8];
-    if (o.type == T_F16) {
-        const uint16_t * p = (const uint16_t *)o.q + at + 4 * l;
-        const half4 lo = *(const half4 *)p, hi = *(const half4 *)(p + 16);
+    const int i0 = ((int)blockIdx.x - o.wg_begin) * (KV_BLOCKS * ILP) + t / 4, all = a.n * o.div_bpr.d;
+    u32x4 x[ILP];
+    uint16_t d[ILP];
+    int64_t to[ILP];
+    bool ok[ILP];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v[e] = (float)lo[e];
-            v[4 + e] = (float)hi[e];
+    for (int u = 0; u < ILP; u++) {
+        const int it = i0 + u * KV_BLOCKS, r = fq_div(min(it, all - 1), o.div_bpr), hb = min(it, all - 1) - r * o.div_bpr.d;
+        const int h = fq_div(hb, o.div_bph), b = hb - h * o.bph;
+        const int64_t i = kv_index(a, r);
+        const bool in = i >= 0 && i < o.n_rows;
+        if (!in && a.err) *a.err = 1;
+        ok[u] = in && it < all;
+        to[u] = (int64_t)r * o.x_nb1 + (int64_t)h * o.x_nb2 + 32 * b;
+        const int64_t at = (in ? i : 0) * o.nb1 + (int64_t)h * o.nb2 + 32 * b;
+        x[u] = u32x4{0, 0, 0, 0};
+        d[u] = 0;
+        if (ok[u]) {
+            x[u] = kv_codes(o.type, o.q, at, l);
+            if (o.type != T_F16) d[u] = o.d[at / 32];
         }
-    } else {
-        kv_values(o.type, o.q, h2f_bits(o.d[at / 32]), at, l, v);
     }
-    kv_store_plain(o, (int64_t)r * o.x_nb1 + (int64_t)h * o.x_nb2 + 32 * b, l, v);
+#pragma unroll
+    for (int u = 0; u < ILP; u++) {
+        float v[8];
+        kv_values(o.type, x[u], h2f_bits(d[u]), l, v);
+        if (!ok[u]) continue;
+        if (o.x_f16) {
+            *(u32x4 *)((uint16_t *)o.x + to[u] + 8 * l) = kv_pack8(v);
+        } else {
+            float4v * p = (float4v *)((float *)o.x + to[u] + 8 * l);
+            p[0] = float4v{v[0], v[1], v[2], v[3]};
+            p[1] = float4v{v[4], v[5], v[6], v[7]};
+        }
+    }
 }
 
 // K and V of one sequence as fp16, for the fused attention. A scale is held to the largest with which
-// every value stays inside fp16. The attention hides a key by its score, but multiplies P = 0 by the key's V all the same, so
-// V has to be finite: a V block whose scale is not stands for zeros here and makes the first value of
-// that key's K a NaN instead, which reaches exactly the queries that see the key.
+// every value stays inside fp16. The attention hides a key by its score, but multiplies P = 0 by the
+// key's V all the same, so V has to be finite: a V block whose scale is not stands for zeros here and
+// makes the first value of that key's K a NaN instead, which reaches exactly the queries that see the key.
 __global__ void __launch_bounds__(KV_THREADS) kv_decode_kernel(KvDecodeArgs a) {
     const int t = threadIdx.x, l = t % 4;
     const int kb = a.D / 32, vb = a.DV / 32;
-    const int64_t it = (int64_t)blockIdx.x * KV_BLOCKS + t / 4;
-    const int64_t key_head = it / (kb + vb);
-    const int b = (int)(it % (kb + vb));
-    if (key_head >= (int64_t)a.KV * a.HK) return;
-    const int64_t j = key_head / a.HK, h = key_head % a.HK;
+    const int64_t key_heads = (int64_t)a.KV * a.HK;
+    // a workgroup's blocks are those of a run of (key, head)s: 32-bit inside the run
+    const int64_t first = (int64_t)blockIdx.x * (KV_BLOCKS);
+    const int64_t kh0 = first / (kb + vb);
+    const int skip = (int)(first - kh0 * (kb + vb));
+    const int64_t j0 = kh0 / a.HK;
+    const int h0 = (int)(kh0 - j0 * a.HK);
+    const int it = skip + t / 4, kh = fq_div(it, a.div_blocks), b = it - kh * (kb + vb);
+    const int jj = fq_div(h0 + kh, a.div_hk), h = h0 + kh - jj * a.HK;
+    const int64_t j = j0 + jj;
+    if (kh0 + kh >= key_heads) return;
     const bool is_v = b >= kb;
     const KvView & w = is_v ? a.v : a.k;
     const int blk = is_v ? b - kb : b;
     const int64_t at = j * w.nb1 + h * w.nb2 + 32 * blk;
+    const u32x4 x = kv_codes(w.type, w.q, at, l);
     float d = h2f_bits(w.d[at / 32]);
     const bool bad = !(fabsf(d) < INFINITY);
-    if (bad && is_v) d = 0.0f;
-    const float lim = kv_scale_limit(w.type);
-    d = fmaxf(fminf(d, lim), -lim);
-    float v[8];
-    kv_values(w.type, w.q, d, at, l, v);
-    if (bad && !is_v) v[0] = NAN;
+    bool poison = bad && !is_v;
     if (b == 0 && l == 0) {
         const uint16_t * vd = a.v.d + (j * a.v.nb1 + h * a.v.nb2) / 32;
-        for (int i = 0; i < vb; i++)
-            if (!(fabsf(h2f_bits(vd[i])) < INFINITY)) v[0] = NAN;
+        for (int i = 0; i < vb; i++) poison |= (vd[i] & 0x7C00u) == 0x7C00u;
     }
-    uint16_t * p = (is_v ? a.v16 + (h * a.KV + j) * a.DV : a.k16 + (h * a.KV + j) * a.D) + 32 * blk + 4 * l;
-    *(u32x2 *)p = u32x2{pack2h(v[0], v[1]), pack2h(v[2], v[3])};
-    *(u32x2 *)(p + 16) = u32x2{pack2h(v[4], v[5]), pack2h(v[6], v[7])};
+    const float lim = kv_scale_limit(w.type);
+    d = bad ? 0.0f : fmaxf(fminf(d, lim), -lim);
+    float v[8];
+    kv_values(w.type, x, d, l, v);
+    if (poison) v[0] = NAN;
+    *(u32x4 *)((is_v ? a.v16 + (h * (int64_t)a.KV + j) * a.DV : a.k16 + (h * (int64_t)a.KV + j) * a.D) + 32 * blk + 8 * l) = kv_pack8(v);
 }
 
-hipError_t launch_kv_decode(const KvDecodeArgs & a, hipStream_t st) {
+// Four blocks a quad where that still makes four workgroups a CU, else one: more of them at once.
+// (Read back as fp16, 32768 rows of 2 x 1024 in Q8_0: 55.7 -> 48.6 us; 512 rows: 4.3 with one, 6.8 with four.)
+template <class F>
+static void kv_ilp(int64_t blocks, F launch) {
+    if (blocks >= (int64_t)1024 * KV_BLOCKS * 4) launch(std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, 1>{});
+}
+
+hipError_t launch_kv_decode(const KvDecodeArgs & args, hipStream_t st) {
+    KvDecodeArgs a = args;
+    a.div_blocks = fq_div_by((a.D + a.DV) / 32);
+    a.div_hk = fq_div_by(a.HK);
     const int64_t items = (int64_t)a.KV * a.HK * ((a.D + a.DV) / 32);
     hipLaunchKernelGGL(kv_decode_kernel, dim3((unsigned)((items + KV_BLOCKS - 1) / KV_BLOCKS)), dim3(KV_THREADS), 0, st, a);
     return hipGetLastError();
 }
 
-hipError_t launch_set_rows(KvRowsArgs a, hipStream_t st) {
-    // one row a workgroup until the chip is full several times over, then more: fewer index scans
-    a.rows_wg = min(KV_ROWS_MAX, max(1, (int)((int64_t)a.n * a.n_out / 2048)));
-    int wgs = 0;
+static void kv_divs(KvRowsArgs & a) {
     for (int k = 0; k < a.n_out; k++) {
-        a.o[k].wg_begin = wgs;
-        wgs += (a.n + a.rows_wg - 1) / a.rows_wg;
+        a.o[k].div_bpr = fq_div_by(a.o[k].H * a.o[k].bph);
+        a.o[k].div_bph = fq_div_by(a.o[k].bph);
     }
-    hipLaunchKernelGGL(set_rows_kernel, dim3(wgs), dim3(KV_THREADS), 0, st, a);
+}
+
+hipError_t launch_set_rows(KvRowsArgs a, hipStream_t st) {
+    kv_divs(a);
+    // one row a workgroup until the chip is full a few times over, then more: fewer index scans
+    a.rows_wg = min(KV_ROWS_MAX, max(1, a.n / 512));
+    hipLaunchKernelGGL(set_rows_kernel, dim3((a.n + a.rows_wg - 1) / a.rows_wg, a.n_out), dim3(KV_THREADS), 0, st, a);
     return hipGetLastError();
 }
 
 hipError_t launch_get_rows(KvRowsArgs a, hipStream_t st) {
-    int wgs = 0;
-    for (int k = 0; k < a.n_out; k++) {
-        a.o[k].wg_begin = wgs;
-        wgs += (int)(((int64_t)a.n * a.o[k].H * a.o[k].bph + KV_BLOCKS - 1) / KV_BLOCKS);
-    }
-    hipLaunchKernelGGL(get_rows_kernel, dim3(wgs), dim3(KV_THREADS), 0, st, a);
+    kv_divs(a);
+    int64_t blocks = 0;
+    for (int k = 0; k < a.n_out; k++) blocks += (int64_t)a.n * a.o[k].div_bpr.d;
+    kv_ilp(blocks, [&](auto ilp) {
+        constexpr int ILP = decltype(ilp)::value;
+        int wgs = 0;
+        for (int k = 0; k < a.n_out; k++) {
+            a.o[k].wg_begin = wgs;
+            wgs += (int)(((int64_t)a.n * a.o[k].div_bpr.d + KV_BLOCKS * ILP - 1) / (KV_BLOCKS * ILP));
+        }
+        hipLaunchKernelGGL(get_rows_kernel<ILP>, dim3(wgs), dim3(KV_THREADS), 0, st, a);
+    });
     return hipGetLastError();
 }
 

@@ -336,6 +336,7 @@ typedef struct mi355x_kv_rows {
  * truncated, at most 15), each step rounded to f32, d stored as fp16 (infinite past 65504, as
  * ggml's). A block that holds a NaN or an infinity, for which ggml defines nothing, is stored with
  * a NaN scale and reads back as NaN. F16: round to nearest even.
+ * n * H * D / 32 and n stay below 2^30, H * D / 32 below 2^24.
  * No counterpart in the reference, whose host writes its caches on the CPU. */
 MI355X_API int mi355x_set_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
                                int32_t * err_dev, void * stream);
