@@ -749,20 +749,41 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
     f.T = a->T; f.HK = a->HK; f.KV = a->KV; f.S = a->S; f.G = a->H / a->HK; f.R = a->T * f.G;
     f.scale = a->scale; f.softcap = a->softcap;
     f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
-    f.nq = 1;
-    while (f.nq < mx::fa_q_max_nq(f.DV) && 16 * f.nq < f.R) f.nq *= 2;
+    // Two row tiles a wave share the work of turning a tile's codes into operands, but halve the blocks and
+    // spill registers: taken when one tile a wave leaves more blocks than compute units, or each of them
+    // more than 128 key tiles (head dim 128, 8 KV heads, us with one and two: 128 rows of 8192 keys 31 / 35,
+    // of 32768 68 / 60; 512 rows of 1000 keys 20 / 32, 1024 34 / 31; 32 sequences x 64 rows x 1024 60 / 56).
+    const int64_t cus = device_cus(), ntiles = (f.KV + 31) / 32;
+    const int64_t units16 = (int64_t)f.S * f.HK * ((f.R + 15) / 16);
+    f.nq = f.R > 16 && (units16 > cus || units16 * ntiles > 128 * cus) ? mx::fa_q_max_nq(f.DV) : 1;
     f.nrt = (f.R + 16 * f.nq - 1) / (16 * f.nq);
-    const int64_t units = (int64_t)f.S * f.HK * f.nrt, ntiles = (f.KV + 31) / 32;
-    f.nsplit = nsplit > 0 ? nsplit : (int)std::max<int64_t>(1, std::min<int64_t>({64, device_cus() / std::max<int64_t>(1, units), ntiles / 8}));
+    const int64_t units = (int64_t)f.S * f.HK * f.nrt;
+    // Keys are split while compute units are idle, four tiles a block at least (one a wave), and not at all up
+    // to 16 tiles, which a block's waves take at once or twice: the second launch costs more (us whole,
+    // in splits of eight tiles and of four: 300 keys 11.2, 11.2, 13.4; 1000 16.1, 13.6, 13.3; 4000 38,
+    // 15.7, 15.1; 1000 at head dim 256 33, 20.9, 18.4).
+    f.nsplit = nsplit > 0 ? nsplit : ntiles <= 16 ? 1
+             : (int)std::max<int64_t>(1, std::min<int64_t>({64, cus / std::max<int64_t>(1, units), ntiles / 4}));
     f.div_nrt = mx::fq_div_by(f.nrt); f.div_hk = mx::fq_div_by(f.HK); f.div_split = mx::fq_div_by(f.nsplit);
     f.div_g = mx::fq_div_by(f.G);
     return f;
 }
+
+// The direct form or decoding first. Direct attention turns codes into operands once for every 16 or 32
+// rows, and with many rows that, not the memory, is its time; decoding turns them once and feeds the F16
+// kernel, one sequence after another, for four launches and 26 us at least. Direct up to R (D + DV) = 2^16
+// (us direct / decoded, 8 KV heads, head dim 128: 128 rows of 8192 keys 31 / 46, 256 47 / 48, 384 71 / 55;
+// 256 of 32768 97 / 131, 384 175 / 150; head dim 256, 16384 keys: 128 rows 106 / 161, 192 193 / 160), and up
+// to 96 key tiles of 16 rows a compute unit and sequence, which is done before those launches are (512 rows of
+// 1000 keys 20 / 29, 1024 31 / 30; head dim 64, 1531 keys: 400 rows 17 / 26, 800 24 / 29, 1600 45 / 30).
 static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (a->KV < mx::FA_Q_MIN_KV || a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
     if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
         if (*e) return atoi(e) != 0;
-    return a->H / a->HK * a->T <= 64;
+    int D, DV;
+    mx::fa_pad_dims(a->D, a->DV, D, DV);
+    const int64_t R = (int64_t)(a->H / a->HK) * a->T;
+    return R * (D + DV) <= 65536 || a->HK * ((R + 15) / 16) * ((a->KV + 31) / 32) <= 96 * (int64_t)device_cus();
 }
 struct FaQDirectLayout {
     size_t po, pml, total;

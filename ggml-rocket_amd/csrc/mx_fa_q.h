@@ -780,9 +780,8 @@ static hipError_t fq_launch(const FaQArgs & a, hipStream_t st) {
 template <int KT, int VT, int DK, int DV>
 static hipError_t fq_rows(const FaQArgs & a, hipStream_t st) {
     if (a.nq == 1) return fq_launch<KT, VT, DK, DV, 1>(a, st);
-    if (a.nq == 2) return fq_launch<KT, VT, DK, DV, 2>(a, st);
     if constexpr (DV <= 128)
-        if (a.nq == 4) return fq_launch<KT, VT, DK, DV, 4>(a, st);
+        if (a.nq == 2) return fq_launch<KT, VT, DK, DV, 2>(a, st);
     return hipErrorInvalidValue;
 }
 
