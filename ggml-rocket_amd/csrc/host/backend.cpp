@@ -397,7 +397,7 @@ struct mi355x_backend {
     bool dev_checked = false, dev_ok = false;
     hipStream_t stream = nullptr;
 
-    DevBuf act, a16, scales, out, part, wstage, wconv, fa_q, fa_k, fa_v, fa_m, fa_o, fa_ws, moe_b, moe_ids, moe_o, moe_ws;
+    DevBuf act, a16, scales, out, part, wstage, wconv, fa_q, fa_k, fa_v, fa_kp, fa_vp, fa_m, fa_o, fa_ws, moe_b, moe_ids, moe_o, moe_ws;
     DevBuf wscratch[4], moe_wscratch;   // per-call weights: unnamed, or over the cache budget
     DevBuf w16;                         // the decode-first form's tiled fp16 weights of one call
     size_t w16_peak = 0;                // its largest size (outside the cache budget)
@@ -1081,6 +1081,38 @@ int mul_mat_device(Ctx * c, const std::vector<mi355x_tensor *> & grp, bool want_
 }
 
 // ---- FLASH_ATTN_EXT ---------------------------------------------------------------------------
+// The output's way to the host, and its device copy for the next op.
+static int fa_done(Ctx * c, mi355x_tensor * dst, size_t ob) {
+    hipEvent_t done = mark_event(c);
+    if (!done) return MI355X_E_DEVICE;
+    const int op = dl_op(c, [dst] { cpu_flash_attn(dst); }, &c->brk_fa, "FLASH_ATTN_EXT");
+    dl_bytes(c, op, c->fa_o.p, dst->data, ob, c->fa_o.p, done);
+    if (c->mirror_ok) {
+        c->fa_mirror.host = dst->data;
+        c->fa_mirror.bytes = ob;
+        c->fa_mirror.dev = c->fa_o.p;
+    }
+    return dl_issue(c);
+}
+
+// A quantized cache's blocks, staged in `raw`, as the code and scale planes attention reads: the strides
+// of the tensor in whole blocks, so the planes hold what the host buffer holds, gaps included.
+static int kv_planes(Ctx * c, const mi355x_tensor * t, const DevBuf & raw, size_t bytes, DevBuf & planes, mi355x_kv_view & w) {
+    const int64_t held = row_bytes(t->type, 32);
+    if (held <= 2) return MI355X_E_ARG;
+    const size_t block = (size_t)held;
+    if (t->nb[0] != block || t->nb[1] % block || t->nb[2] % block || t->ne[0] % 32) return MI355X_E_ARG;
+    const int64_t blocks = (int64_t)(bytes / block);
+    TRY(planes.ensure(bytes, c->stream));
+    TRY(mi355x_weight_pack(t->type, raw.p, blocks, 32, planes.p, c->stream));
+    w.type = t->type;
+    w.q_dev = planes.p;
+    w.d_dev = (const uint16_t *)((const char *)planes.p + blocks * (int64_t)(block - 2));
+    w.nb1 = (int64_t)(t->nb[1] / block) * 32;
+    w.nb2 = (int64_t)(t->nb[2] / block) * 32;
+    return MI355X_OK;
+}
+
 int flash_attn_device(Ctx * c, mi355x_tensor * dst) {
     if (!ensure_device(c) || !staging_on(c)) return MI355X_E_DEVICE;
     begin_op(c);
@@ -1102,6 +1134,38 @@ int flash_attn_device(Ctx * c, mi355x_tensor * dst) {
     TRY(upload(c, c->fa_k.p, k->data, kb));
     if (!v_in_k) TRY(upload(c, c->fa_v.p, v->data, vb));
     if (m) TRY(upload(c, c->fa_m.p, m->data, mb));
+    if (type_is_quantized(k->type) || type_is_quantized(v->type)) {
+        mi355x_fa_q_args a;
+        memset(&a, 0, sizeof a);
+        a.q_dev = c->fa_q.p;
+        a.q_nb1 = (int64_t)(q->nb[1] / 4);
+        a.q_nb2 = (int64_t)(q->nb[2] / 4);
+        TRY(kv_planes(c, k, c->fa_k, kb, c->fa_kp, a.k));
+        if (v_in_k) {
+            a.v = a.k;
+        } else {
+            TRY(kv_planes(c, v, c->fa_v, vb, c->fa_vp, a.v));
+        }
+        a.mask_dev = m ? (const uint16_t *)c->fa_m.p : nullptr;
+        a.mask_nb1 = m ? (int64_t)(m->nb[1] / 2) : 0;
+        a.dst_dev = c->fa_o.p;
+        a.dst_nb1 = (int64_t)(dst->nb[1] / 4);
+        a.dst_nb2 = (int64_t)(dst->nb[2] / 4);
+        a.D = (int)q->ne[0];
+        a.DV = (int)v->ne[0];
+        a.T = (int)q->ne[1];
+        a.H = (int)q->ne[2];
+        a.KV = (int)k->ne[1];
+        a.HK = (int)k->ne[2];
+        a.S = 1;
+        memcpy(&a.scale, &dst->op_params[0], 4);
+        memcpy(&a.max_bias, &dst->op_params[1], 4);
+        memcpy(&a.softcap, &dst->op_params[2], 4);
+        const size_t ws = mi355x_flash_attn_q_workspace(&a, 0);
+        if (ws) TRY(c->fa_ws.ensure(ws, c->stream));
+        TRY(mi355x_flash_attn_q(&a, 0, ws ? c->fa_ws.p : nullptr, ws, c->stream));
+        return fa_done(c, dst, ob);
+    }
     mi355x_fa_args a;
     memset(&a, 0, sizeof a);
     a.q_dev = (const float *)c->fa_q.p;
@@ -1130,16 +1194,7 @@ int flash_attn_device(Ctx * c, mi355x_tensor * dst) {
     const size_t ws = mi355x_flash_attn_workspace(&a, 0);
     if (ws) TRY(c->fa_ws.ensure(ws, c->stream));
     TRY(mi355x_flash_attn(&a, 0, ws ? c->fa_ws.p : nullptr, ws, c->stream));
-    hipEvent_t done = mark_event(c);
-    if (!done) return MI355X_E_DEVICE;
-    const int op = dl_op(c, [dst] { cpu_flash_attn(dst); }, &c->brk_fa, "FLASH_ATTN_EXT");
-    dl_bytes(c, op, c->fa_o.p, dst->data, ob, c->fa_o.p, done);
-    if (c->mirror_ok) {
-        c->fa_mirror.host = dst->data;
-        c->fa_mirror.bytes = ob;
-        c->fa_mirror.dev = c->fa_o.p;
-    }
-    return dl_issue(c);
+    return fa_done(c, dst, ob);
 }
 
 // ---- MUL_MAT_ID -------------------------------------------------------------------------------
@@ -1369,7 +1424,7 @@ MI355X_API void mi355x_backend_free(mi355x_backend_t c) {
     report_routes(c);
     c->wcache.clear();
     for (DevBuf * b : {&c->act, &c->a16, &c->scales, &c->out, &c->part, &c->wstage, &c->wconv, &c->fa_q, &c->fa_k, &c->fa_v,
-                       &c->fa_m, &c->fa_o, &c->fa_ws, &c->moe_b, &c->moe_ids, &c->moe_o, &c->moe_ws,
+                       &c->fa_kp, &c->fa_vp, &c->fa_m, &c->fa_o, &c->fa_ws, &c->moe_b, &c->moe_ids, &c->moe_o, &c->moe_ws,
                        &c->wscratch[0], &c->wscratch[1], &c->wscratch[2], &c->wscratch[3], &c->moe_wscratch, &c->w16})
         b->release();
     if (c->stream) {

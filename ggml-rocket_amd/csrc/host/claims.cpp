@@ -424,10 +424,13 @@ static bool claim_flash_attn(const mi355x_tensor * op) {
     if (!m && !flash_attn_unmasked()) return false;
     if (op->src[4]) return false;                         // attention sinks (7703-7721)
     const float max_bias = op_param_f32(op, 1);
+    // a quantized cache: K and V each Q8_0 or Q4_0, both or neither (mi355x_flash_attn_q)
+    auto kv_quant = [](int t) { return t == MI355X_TYPE_Q8_0 || t == MI355X_TYPE_Q4_0; };
+    const bool quant = kv_quant(k->type) && kv_quant(v->type) && flash_attn_quant();
     const int64_t head_dim = q->ne[0], n_tokens = q->ne[1], n_head = q->ne[2];
     const int64_t dv = v->ne[0], n_kv = k->ne[1], n_kv_heads = k->ne[2];
     const bool ref_rules = max_bias == 0.0f
-        && q->type == MI355X_TYPE_F32 && k->type == MI355X_TYPE_F16 && v->type == MI355X_TYPE_F16
+        && q->type == MI355X_TYPE_F32 && (quant || (k->type == MI355X_TYPE_F16 && v->type == MI355X_TYPE_F16))
         && (!m || (m->type == MI355X_TYPE_F16 && is_contiguous(m)))
         && op->type == MI355X_TYPE_F32 && is_contiguous(op)
         && q->ne[3] == 1 && k->ne[3] == 1
@@ -444,12 +447,17 @@ static bool claim_flash_attn(const mi355x_tensor * op) {
     // == 0, dv % 8 == 0, both up to 1024; the absorbed MLA's 576 / 512 fused); element strides;
     // 16-byte rows
     int dk_pad = 0, dv_pad = 0;
+    const bool q_ok = q->nb[0] == 4 && q->nb[1] % 16 == 0 && q->nb[2] % 16 == 0;
+    const bool m_ok = !m || m->nb[1] % 8 == 0;
+    if (quant) {   // whole blocks between rows and heads, as the packed planes keep them
+        const size_t bk = (size_t)row_bytes(k->type, 32), bv = (size_t)row_bytes(v->type, 32);
+        return dv % 32 == 0 && head_dim <= 256 && dv <= 256 && q_ok && m_ok && k->nb[0] == bk && v->nb[0] == bv &&
+               k->nb[1] % bk == 0 && k->nb[2] % bk == 0 && v->nb[1] % bv == 0 && v->nb[2] % bv == 0;
+    }
     const bool dims = (head_dim <= 256 && dv <= 256 && mx::fa_pad_dims((int)head_dim, (int)dv, dk_pad, dv_pad)) ||
                       mx::fa_wide_dims((int)head_dim, (int)dv);
-    const bool q_ok = q->nb[0] == 4 && q->nb[1] % 16 == 0 && q->nb[2] % 16 == 0;
     const bool kv_ok = k->nb[0] == 2 && v->nb[0] == 2 && k->nb[1] % 16 == 0 && k->nb[2] % 16 == 0 &&
                        v->nb[1] % 16 == 0 && v->nb[2] % 16 == 0;
-    const bool m_ok = !m || m->nb[1] % 8 == 0;
     return dims && q_ok && kv_ok && m_ok;
 }
 

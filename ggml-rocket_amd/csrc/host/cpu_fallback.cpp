@@ -173,7 +173,7 @@ void cpu_mul_mat(const mi355x_tensor * dst) {
 }
 
 // Attention on the host in double precision, to the contract of ggml-rocket.cpp:5392-5442:
-// Q read as F32, K and V as fp16, logits = scale * q.k, soft-capped when a cap is set, plus the
+// Q read as F32, K and V as fp16 (or a quantized cache's blocks), logits = scale * q.k, soft-capped when a cap is set, plus the
 // mask; softmax in double; a query whose every key is masked gets a zero output row.
 // Work is laid out per (token, KV head): the H / HK query heads that share a KV head are scored
 // together, so each visible key and value row is widened to double once for all of them. The
@@ -191,13 +191,19 @@ void cpu_flash_attn(const mi355x_tensor * dst) {
     memcpy(&scale_f, &dst->op_params[0], 4);
     memcpy(&cap_f, &dst->op_params[2], 4);
     const double scale = scale_f, cap = cap_f;
-    auto widen = [](const char * row, int64_t n, double * out) {
-        for (int64_t c = 0; c < n; c++) out[c] = (double)h2f(rd16((const uint8_t *)row + 2 * c));
+    auto widen = [](int type, const char * row, std::vector<float> & f, std::vector<double> & out) {
+        if (type == MI355X_TYPE_F16) {
+            for (size_t c = 0; c < out.size(); c++) out[c] = (double)h2f(rd16((const uint8_t *)row + 2 * c));
+            return;
+        }
+        decode_row_f32(type, row, f.data(), (int64_t)out.size());
+        for (size_t c = 0; c < out.size(); c++) out[c] = f[c];
     };
     parallel_rows(n_tok * n_kvh, [&](int64_t w0, int64_t w1) {
         std::vector<double> queries((size_t)(group * dk)), logits((size_t)(group * n_key));
         std::vector<double> vsum((size_t)(group * dv)), top((size_t)group), total((size_t)group);
         std::vector<double> key((size_t)dk), val((size_t)dv);
+        std::vector<float> row((size_t)std::max(dk, dv));
         std::vector<int64_t> seen;   // keys the mask leaves visible, in order
         seen.reserve((size_t)n_key);
         for (int64_t w = w0; w < w1; w++) {
@@ -213,7 +219,7 @@ void cpu_flash_attn(const mi355x_tensor * dst) {
                 if (m) bias = (double)h2f(rd16((const uint8_t *)m->data + tok * m->nb[1] + j * 2));
                 if (std::isinf(bias) && bias < 0) continue;
                 seen.push_back(j);
-                widen((const char *)k->data + j * k->nb[1] + kvh * k->nb[2], dk, key.data());
+                widen(k->type, (const char *)k->data + j * k->nb[1] + kvh * k->nb[2], row, key);
                 for (int64_t i = 0; i < group; i++) {
                     const double * qi = &queries[(size_t)(i * dk)];
                     double dot = 0.0;
@@ -228,7 +234,7 @@ void cpu_flash_attn(const mi355x_tensor * dst) {
             std::fill(vsum.begin(), vsum.end(), 0.0);
             std::fill(total.begin(), total.end(), 0.0);
             for (const int64_t j : seen) {
-                widen((const char *)v->data + j * v->nb[1] + kvh * v->nb[2], dv, val.data());
+                widen(v->type, (const char *)v->data + j * v->nb[1] + kvh * v->nb[2], row, val);
                 for (int64_t i = 0; i < group; i++) {
                     const double x = logits[(size_t)(i * n_key + j)];
                     if (std::isinf(top[(size_t)i]) || std::isinf(x)) continue;

@@ -53,6 +53,7 @@ bool flash_attn_on();
 int flash_attn_min_t();
 int flash_attn_min_kv();
 bool flash_attn_unmasked();
+bool flash_attn_quant();
 bool quant_resident_on();
 bool fusion_on();
 

@@ -277,6 +277,10 @@ bool flash_attn_unmasked() {
     static const bool v = knob_int("FLASH_ATTN_UNMASKED", 0) > 0;
     return v;
 }
+bool flash_attn_quant() {
+    static const bool v = knob_int("FLASH_ATTN_QUANT", 0) > 0;
+    return v;
+}
 bool quant_resident_on() {
     static const bool v = [] {
         const char * e = knob_env("QUANT_RESIDENT");

@@ -286,6 +286,24 @@ def test_attention_streams(mx, form, types, T, half):
 
 
 @pytest.mark.parametrize("types", MIXES, ids=ids)
+@pytest.mark.parametrize("D,DV,G,T", [(64, 64, 4, 11), (96, 96, 1, 47), (128, 128, 4, 12), (192, 128, 4, 9), (224, 224, 4, 9)])
+def test_attention_many_short_sequences(mx, form, types, D, DV, G, T):
+    """More row tiles than compute units (24 sequences x 4 heads x 3 tiles of 16), an odd number of them a
+    head, each sequence at its own length, scattered hidden keys and whole hidden tiles, one empty row."""
+    S, HK, KV = 24, 4, 170
+    rng = np.random.default_rng(D)
+    q, kn, vn, kc, vc = attn_case(mx, *types, S, T, G * HK, HK, KV, D, DV)
+    m = causal(T, KV, [1 + (37 * s) % KV for s in range(S)])
+    m[rng.random(m.shape) > 0.8] = -np.inf
+    m[:, 4:, 64:96] = -np.inf
+    m[5, 2, :] = -np.inf
+    for ns in (0, 2):
+        got = cpu(mx.flash_attn_q(gpu(q), kc, vc, gpu(m), D ** -0.5, nsplit=ns))
+        check(got, q, kn, vn, m, D ** -0.5, what=ns)
+        assert (got[5, 2] == 0).all()
+
+
+@pytest.mark.parametrize("types", MIXES, ids=ids)
 @pytest.mark.parametrize("T", [1, 9, 64])
 def test_attention_mask_holes(mx, form, types, T):
     """Scattered hidden keys, whole hidden tiles, rows that see nothing, masks of fp16's lowest value,
