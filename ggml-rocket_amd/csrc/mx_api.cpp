@@ -577,26 +577,22 @@ MI355X_API int mi355x_flash_attn(const mi355x_fa_args * a, int nsplit,
     return mi355x_flash_attn_ex(a, nsplit, 0, workspace_dev, workspace_bytes, stream);
 }
 
-// The fused kernel of head dims up to 256; q_f16, dst_f16: q and dst hold fp16.
-static int fa_fused(const mi355x_fa_args * a, int nsplit, int flags, bool q_f16, bool dst_f16, void * workspace_dev,
-                    size_t workspace_bytes, void * stream) {
-    if (nsplit > 64) return MI355X_E_ARG;
+// The fused kernel of head dims up to 256 on the workspace ws; q_f16, dst_f16: q and dst hold fp16.
+static mx::FaArgs fa_fused_args(const mi355x_fa_args * a, int nsplit, bool q_f16, bool dst_f16, char * ws, size_t * need) {
     const FaPlan plan = fa_plan(a, nsplit);
     mx::FaArgs f = fa_lower(a, plan.nsplit);
     f.tasks = plan.tasks;
     f.q_f16 = q_f16;
     f.dst_f16 = dst_f16;
-    nsplit = plan.nsplit;
     const FaLayout L = fa_layout(f);
-    if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
-    char * ws = (char *)workspace_dev;
+    *need = L.total;
     f.cls = (uint8_t *)(ws + L.cls);
     f.kzero = (uint16_t *)(ws + L.zero);
-    if (nsplit > 1) {
+    if (plan.nsplit > 1) {
         f.part_o = (float *)(ws + L.po);
         f.part_ml = (float *)(ws + L.pml);
     }
-    return hip_status(mx::launch_fa(f, !(flags & MI355X_FA_CLASSES_READY), S(stream)));
+    return f;
 }
 
 MI355X_API int mi355x_flash_attn_ex(const mi355x_fa_args * a, int nsplit, int flags,
@@ -636,7 +632,11 @@ MI355X_API int mi355x_flash_attn_ex(const mi355x_fa_args * a, int nsplit, int fl
         w.psc = (float *)(ws + L.psc); w.o = (float *)(ws + L.o);
         return hip_status(mx::launch_fa_wide(w, S(stream)));
     }
-    return fa_fused(a, nsplit, flags, false, false, workspace_dev, workspace_bytes, stream);
+    if (nsplit > 64) return MI355X_E_ARG;
+    size_t need;
+    const mx::FaArgs f = fa_fused_args(a, nsplit, false, false, (char *)workspace_dev, &need);
+    if (!workspace_dev || workspace_bytes < need || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
+    return hip_status(mx::launch_fa(f, !(flags & MI355X_FA_CLASSES_READY), S(stream)));
 }
 
 // ---- the quantized KV cache ---------------------------------------------------------------------
@@ -702,6 +702,7 @@ static int fa_q_check(const mi355x_fa_q_args * a) {
         if (st != MI355X_OK) return st;
     }
     if (a->T < 0 || a->S < 0 || a->H <= 0 || a->HK <= 0 || a->KV < 0 || a->H % a->HK) return MI355X_E_ARG;
+    if ((int64_t)a->KV * a->HK * ((a->D + a->DV) / 32) >= 1 << 30) return MI355X_E_UNSUPPORTED;
     if ((int64_t)a->S * a->T * a->H > (1 << 30) || (size_t)a->KV > mx::fa_max_kv(a->D, a->DV)) return MI355X_E_UNSUPPORTED;
     for (int t : {a->q_type, a->dst_type})
         if (t != mx::T_F32 && t != mx::T_F16) return MI355X_E_ARG;
@@ -749,21 +750,31 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
     f.T = a->T; f.HK = a->HK; f.KV = a->KV; f.S = a->S; f.G = a->H / a->HK; f.R = a->T * f.G;
     f.scale = a->scale; f.softcap = a->softcap;
     f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
-    // Two row tiles a wave share the work of turning a tile's codes into operands, but halve the blocks and
-    // spill registers: taken when one tile a wave leaves more blocks than compute units, or each of them
-    // more than 128 key tiles (head dim 128, 8 KV heads, us with one and two: 128 rows of 8192 keys 31 / 35,
-    // of 32768 68 / 60; 512 rows of 1000 keys 20 / 32, 1024 34 / 31; 32 sequences x 64 rows x 1024 60 / 56).
-    const int64_t cus = device_cus(), ntiles = (f.KV + 31) / 32;
-    const int64_t units16 = (int64_t)f.S * f.HK * ((f.R + 15) / 16);
-    f.nq = f.R > 16 && (units16 > cus || units16 * ntiles > 128 * cus) ? mx::fa_q_max_nq(f.DV) : 1;
-    f.nrt = (f.R + 16 * f.nq - 1) / (16 * f.nq);
-    const int64_t units = (int64_t)f.S * f.HK * f.nrt;
     // Keys are split while compute units are idle, four tiles a block at least (one a wave), and not at all up
     // to 16 tiles, which a block's waves take at once or twice: the second launch costs more (us whole,
     // in splits of eight tiles and of four: 300 keys 11.2, 11.2, 13.4; 1000 16.1, 13.6, 13.3; 4000 38,
     // 15.7, 15.1; 1000 at head dim 256 33, 20.9, 18.4).
-    f.nsplit = nsplit > 0 ? nsplit : ntiles <= 16 ? 1
-             : (int)std::max<int64_t>(1, std::min<int64_t>({64, cus / std::max<int64_t>(1, units), ntiles / 4}));
+    const int64_t cus = device_cus(), ntiles = (f.KV + 31) / 32;
+    auto units = [&](int nq) { return (int64_t)f.S * f.HK * ((f.R + 16 * nq - 1) / (16 * nq)); };
+    auto splits = [&](int nq) {
+        return nsplit > 0 ? nsplit : ntiles <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>({64, cus / std::max<int64_t>(1, units(nq)), ntiles / 4}));
+    };
+    // Two row tiles a wave share the work of turning a tile's codes into operands, but spill registers: a
+    // key tile takes 1.5 times as long (1.75 at head dim 64), and a block as long as 25 key tiles more. They are
+    // taken where that is less, by the key tiles that a compute unit goes through (head dim 128, 8 KV heads, us
+    // with one and two: 128 rows of 8192 keys 30 / 30, of 32768 68 / 59; 192 of 8192 46 / 42; 512 of 1000
+    // 20 / 33; 4 sequences x 256 x 4096 83 / 66; head dim 64: 512 of 4096 28 / 31, 256 of 16384 46 / 42).
+    auto tiles = [&](int nq) {
+        const int64_t n = splits(nq);
+        return (units(nq) * n + cus - 1) / cus * ((ntiles + n - 1) / n);
+    };
+    f.nq = 1;
+    if (mx::fa_q_max_nq(f.DV) == 2 && f.R > 16) {
+        const char * e = getenv("MI355X_FA_Q_ROWS");
+        f.nq = e && *e ? (atoi(e) == 32 ? 2 : 1) : (f.DV == 64 ? 7 : 6) * tiles(2) + 100 < 4 * tiles(1) ? 2 : 1;
+    }
+    f.nrt = (f.R + 16 * f.nq - 1) / (16 * f.nq);
+    f.nsplit = (int)splits(f.nq);
     f.div_nrt = mx::fq_div_by(f.nrt); f.div_hk = mx::fq_div_by(f.HK); f.div_split = mx::fq_div_by(f.nsplit);
     f.div_g = mx::fq_div_by(f.G);
     return f;
@@ -771,11 +782,12 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
 
 // The direct form or decoding first. Direct attention turns codes into operands once for every 16 or 32
 // rows, and with many rows that, not the memory, is its time; decoding turns them once and feeds the F16
-// kernel, one sequence after another, for four launches and 26 us at least. Direct up to R (D + DV) = 2^16
-// (us direct / decoded, 8 KV heads, head dim 128: 128 rows of 8192 keys 31 / 46, 256 47 / 48, 384 71 / 55;
-// 256 of 32768 97 / 131, 384 175 / 150; head dim 256, 16384 keys: 128 rows 106 / 161, 192 193 / 160), and up
-// to 96 key tiles of 16 rows a compute unit and sequence, which is done before those launches are (512 rows of
-// 1000 keys 20 / 29, 1024 31 / 30; head dim 64, 1531 keys: 400 rows 17 / 26, 800 24 / 29, 1600 45 / 30).
+// kernel, one sequence after another, in two or three launches and 21 us at least. Direct up to R (D + DV) = 2^16
+// (us direct / decoded, 8 KV heads, head dim 128: 128 rows of 8192 keys 31 / 42, 256 47 / 44, 384 70 / 51;
+// 256 of 32768 97 / 127, 384 176 / 143; head dim 256, 16384 keys: 128 rows 106 / 149, 192 193 / 147), and up
+// to 64 key tiles of 16 rows a compute unit and sequence, which are done before those launches are (512 rows of
+// 1000 keys 20 / 25, 768 31 / 26; head dim 64, 1531 keys: 400 rows 16 / 22, 800 25 / 24; head dim 256, 1000
+// keys, 512 rows 40 / 72; 32 sequences x 256 rows x 1024 185 / 657).
 static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (a->KV < mx::FA_Q_MIN_KV || a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
     if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
@@ -783,7 +795,7 @@ static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     int D, DV;
     mx::fa_pad_dims(a->D, a->DV, D, DV);
     const int64_t R = (int64_t)(a->H / a->HK) * a->T;
-    return R * (D + DV) <= 65536 || a->HK * ((R + 15) / 16) * ((a->KV + 31) / 32) <= 96 * (int64_t)device_cus();
+    return R * (D + DV) <= 65536 || a->HK * ((R + 15) / 16) * ((a->KV + 31) / 32) <= 64 * (int64_t)device_cus();
 }
 struct FaQDirectLayout {
     size_t po, pml, total;
@@ -836,6 +848,10 @@ MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void 
     if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
     char * ws = (char *)workspace_dev;
     for (int s = 0; s < a->S; s++) {
+        const mi355x_fa_args one = fa_q_lower(a, s, (const uint16_t *)(ws + L.k), (const uint16_t *)(ws + L.v));
+        size_t need;
+        const mx::FaArgs f = fa_fused_args(&one, nsplit, a->q_type == mx::T_F16, a->dst_type == mx::T_F16, ws + L.fa, &need);
+        if (need > workspace_bytes - L.fa) return MI355X_E_NOMEM;
         if (a->KV > 0) {
             mx::KvDecodeArgs d;
             d.k = fa_q_view(a->k, s);
@@ -843,11 +859,10 @@ MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void 
             d.k16 = (uint16_t *)(ws + L.k);
             d.v16 = (uint16_t *)(ws + L.v);
             d.HK = a->HK; d.KV = a->KV; d.D = a->D; d.DV = a->DV;
-            const int e = hip_status(mx::launch_kv_decode(d, S(stream)));
+            const int e = hip_status(mx::launch_kv_decode(d, f, S(stream)));
             if (e != MI355X_OK) return e;
         }
-        const mi355x_fa_args f = fa_q_lower(a, s, (const uint16_t *)(ws + L.k), (const uint16_t *)(ws + L.v));
-        const int e = fa_fused(&f, nsplit, 0, a->q_type == mx::T_F16, a->dst_type == mx::T_F16, ws + L.fa, workspace_bytes - L.fa, stream);
+        const int e = hip_status(mx::launch_fa(f, a->KV == 0, S(stream)));
         if (e != MI355X_OK) return e;
     }
     return MI355X_OK;

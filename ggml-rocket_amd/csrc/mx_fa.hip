@@ -35,12 +35,11 @@
 
 #include "mx_common.h"
 #include "mx_fa_dims.h"
+#include "mx_fa_prep.h"
 #include "mx_kernels_impl.h"
 
 namespace mx {
 
-constexpr int FA_BKV = 64;      // keys per tile
-constexpr int FA_QW = 32;       // query rows per wave task
 // Wave tasks (head, 32-query tile) per block, FaArgs::tasks (fa_tasks_ok): 4 (two waves a task, taking
 // alternate key tiles; one wave a task for DV 256) or, for DV <= 128, 2 (four waves a task: each
 // of the two tile parities split again into the tile's two 32-key halves). Two tasks make twice
@@ -214,8 +213,6 @@ template <> __device__ __forceinline__ void fa_tr_read<8, 512>(const uint32_t (&
 // ---------------------------------------------------------------------------------------------
 // prep: the mask classes
 // ---------------------------------------------------------------------------------------------
-enum : uint8_t { FA_TILE_SKIP = 0, FA_TILE_FULL = 1, FA_TILE_MIXED = 2 };
-
 // The value of lane i ^ 32 (the lane holding the same query's other 16 scores): gfx950's
 // v_permlane32_swap exchanges lanes 32-63 of its first operand with lanes 0-31 of its second, so
 // with both operands = x, lanes 0-31 find the partner in the second result and lanes 32-63 in the
@@ -225,59 +222,7 @@ __device__ __forceinline__ float fa_partner(float x) {
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-__global__ void __launch_bounds__(256) fa_prep_kernel(FaArgs a) {
-    const int t = threadIdx.x;
-    const int nkt = a.kvp / FA_BKV;
-    const int b = blockIdx.x;
-    if (b == 0 && t < 8) a.kzero[t] = 0;   // the K and V source of the padded columns
-    const int nqt = (a.T + FA_QW - 1) / FA_QW;
-    const int nct = nqt * a.cls_stride;   // rows padded to cls_stride entries (padding: skip)
-    const int cb = b;
-    if (cb * 4 < nct) {
-        // one wave per (query tile, key tile): lane l scans row l/2, keys 32*(l%2) .. +31
-        const int wave = t / WAVE, lane = t % WAVE;
-        const int ct = cb * 4 + wave;
-        if (ct >= nct) return;
-        const int qt = ct / a.cls_stride, kt = ct % a.cls_stride;
-        bool vis = false, nz = false;
-        if (kt >= nkt) {
-            vis = false;                              // padding entry
-        } else if (a.mask) {
-            const int tq = qt * FA_QW + lane / 2;
-            const int jb = kt * FA_BKV + 32 * (lane % 2);
-            if (tq < a.T) {
-                const uint16_t * mr = a.mask + (int64_t)tq * a.mask_nb1 + jb;
-                if (jb + 32 <= a.KV) {
-                    // 8 independent 8-byte loads (rows are 8-byte aligned)
-                    u32x2 w[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) w[i] = *(const u32x2 *)(mr + 4 * i);
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float m = h2f_bits((uint16_t)((w[i][e / 2] >> (16 * (e % 2))) & 0xFFFFu));
-                            vis |= (m != -INFINITY);
-                            nz |= (m != 0.0f);
-                        }
-                } else {
-                    for (int j = 0; j < 32; j++) {
-                        if (jb + j < a.KV) {
-                            const float m = h2f_bits(mr[j]);
-                            vis |= (m != -INFINITY);
-                            nz |= (m != 0.0f);
-                        }
-                    }
-                }
-            }
-        } else {
-            vis = true;
-        }
-        const bool any_vis = __any(vis), any_nz = __any(nz);
-        if (lane == 0) a.cls[ct] = !any_vis ? FA_TILE_SKIP : (any_nz ? FA_TILE_MIXED : FA_TILE_FULL);
-        return;
-    }
-}
+__global__ void __launch_bounds__(256) fa_prep_kernel(FaArgs a) { fa_prep_block(a, blockIdx.x); }
 
 // ---------------------------------------------------------------------------------------------
 // main kernel

@@ -121,8 +121,8 @@ struct KvDecodeArgs {
     uint16_t * k16;
     uint16_t * v16;
     int HK, KV, D, DV;
+    int n_prep;                // workgroups of the mask classes, before those of the cache
 };
-hipError_t launch_kv_decode(const KvDecodeArgs & a, hipStream_t st);
 hipError_t launch_set_rows(KvRowsArgs a, hipStream_t st);
 hipError_t launch_get_rows(KvRowsArgs a, hipStream_t st);
 
@@ -184,6 +184,7 @@ bool fa_dims_supported(int dk, int dv);   // fa_pad_dims: dk, dv <= 256, multipl
 size_t fa_max_kv(int dk, int dv);          // the longest KV range one launch takes
 hipError_t launch_fa(const FaArgs & a, bool prep, hipStream_t st);
 hipError_t launch_fa_prep(const FaArgs & a, hipStream_t st);      // the mask classes (every fused kernel)
+hipError_t launch_kv_decode(const KvDecodeArgs & a, const FaArgs & f, hipStream_t st);   // and f's mask classes
 hipError_t launch_fa_combine(const FaArgs & a, hipStream_t st);   // merges KV splits at DV 512
 
 // the fused absorbed MLA (dk 576, dv 512, V the first 512 dims of K)

@@ -374,11 +374,15 @@ MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int 
 /* mi355x_flash_attn with K and V in a quantized cache, each Q8_0 or Q4_0: dst = softmax(cap(scale *
  * q.k) + mask) . v. K and V enter the products as fp16 (their values rounded once), Q and P as fp16,
  * sums in F32: an F32 dst holds values of that accuracy. So that the values stay inside fp16, a scale
- * counts as at most 515.5 (Q8_0: 65468 / 127) or 8188 (Q4_0: 65504 / 8). D and DV are multiples of 32 up to 256; H % HK == 0; max_bias 0. A key that the
- * mask hides from a query (-inf) adds nothing to it, whatever the cache holds there, NaN included; a
- * key with a scale that is not finite makes the rows of the queries that see it NaN; rows whose every
- * key is hidden are written as zeros. q rows 16-byte, dst rows 16-byte (F16: 8), mask rows 8-byte
- * aligned.
+ * counts as at most 515.5 (Q8_0: 65468 / 127) or 8188 (Q4_0: 65504 / 8). D and DV are multiples of 32
+ * up to 256; H % HK == 0; max_bias 0; KV * HK * (D + DV) / 32 < 2^30. A key that the mask hides from a
+ * query (-inf) adds nothing to it, whatever the cache holds there, NaN included; a key with a scale
+ * that is not finite makes the rows of the queries that see it NaN; rows whose every key is hidden are
+ * written as zeros. q rows 16-byte, dst rows 16-byte (F16: 8), mask rows 8-byte aligned.
+ * Few rows are taken by a kernel that reads the cache as it is stored, in any number of sequences; many by
+ * decoding it to fp16 in the workspace, a sequence at a time, for the kernel of mi355x_flash_attn. The
+ * choice follows measured costs; MI355X_FA_Q_DIRECT=1|0 pins it and MI355X_FA_Q_ROWS=16|32 the rows a
+ * wave of the first takes, for measurements and tests.
  * Concurrent calls must not share a workspace. Equal inputs give equal bits. */
 MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
                                    void * stream);

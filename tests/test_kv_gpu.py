@@ -26,11 +26,14 @@ def mx(torch_cuda):
     return ggml_mi355x
 
 
-@pytest.fixture(params=["1", "0", ""], ids=["direct", "decoded", "chosen"])
+@pytest.fixture(params=["1 16", "1 32", "0 ", " "], ids=["direct", "direct32", "decoded", "chosen"])
 def form(request, monkeypatch):
-    """Attention tests run under both forms (the kernel that reads the cache as it is stored; the cache
-    decoded to fp16 first, which is the fp16 kernel's arithmetic) and the library's choice per call."""
-    monkeypatch.setenv("MI355X_FA_Q_DIRECT", request.param)
+    """Attention tests run under every form (the kernel that reads the cache as it is stored, with 16 and with 32
+    rows a wave; the cache decoded to fp16 first, which is the fp16 kernel's arithmetic) and the library's
+    choice per call."""
+    direct, rows = request.param.split(" ")
+    monkeypatch.setenv("MI355X_FA_Q_DIRECT", direct)
+    monkeypatch.setenv("MI355X_FA_Q_ROWS", rows)
 
 
 def gpu(a):
