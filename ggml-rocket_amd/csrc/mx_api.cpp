@@ -750,28 +750,29 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
     f.T = a->T; f.HK = a->HK; f.KV = a->KV; f.S = a->S; f.G = a->H / a->HK; f.R = a->T * f.G;
     f.scale = a->scale; f.softcap = a->softcap;
     f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
-    // Keys are split while compute units are idle, four tiles a block at least (one a wave), and not at all up
-    // to 16 tiles, which a block's waves take at once or twice: the second launch costs more (us whole,
-    // in splits of eight tiles and of four: 300 keys 11.2, 11.2, 13.4; 1000 16.1, 13.6, 13.3; 4000 38,
-    // 15.7, 15.1; 1000 at head dim 256 33, 20.9, 18.4).
+    // Keys are split while compute units are idle, four tiles a block at least, and not at all up to 16 tiles,
+    // which a block's waves take at once or twice: the second launch costs more (us whole, in splits of eight
+    // tiles and of four: 300 keys 11.2, 11.2, 13.4; 1000 16.1, 13.6, 13.3; 4000 38, 15.7, 15.1; 1000 at
+    // head dim 256 33, 20.9, 18.4). Never past one block a compute unit (32 sequences of 4096 keys, 256 blocks:
+    // 70 whole, 82 in two splits; of different lengths 53 and 67).
     const int64_t cus = device_cus(), ntiles = (f.KV + 31) / 32;
     auto units = [&](int nq) { return (int64_t)f.S * f.HK * ((f.R + 16 * nq - 1) / (16 * nq)); };
     auto splits = [&](int nq) {
         return nsplit > 0 ? nsplit : ntiles <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>({64, cus / std::max<int64_t>(1, units(nq)), ntiles / 4}));
     };
-    // Two row tiles a wave share the work of turning a tile's codes into operands, but spill registers: a
-    // key tile takes 1.5 times as long (1.75 at head dim 64), and a block as long as 25 key tiles more. They are
-    // taken where that is less, by the key tiles that a compute unit goes through (head dim 128, 8 KV heads, us
-    // with one and two: 128 rows of 8192 keys 30 / 30, of 32768 68 / 59; 192 of 8192 46 / 42; 512 of 1000
-    // 20 / 33; 4 sequences x 256 x 4096 83 / 66; head dim 64: 512 of 4096 28 / 31, 256 of 16384 46 / 42).
-    auto tiles = [&](int nq) {
-        const int64_t n = splits(nq);
-        return (units(nq) * n + cus - 1) / cus * ((ntiles + n - 1) / n);
+    // Two row tiles a wave (head dim 64) share the work of turning codes into operands: a key tile takes 1.75 times
+    // as long as with one, and a block's start and end, which take as long as 60 key tiles, 85. They are taken
+    // where a compute unit is done sooner (4-bit, 8 KV heads, us with one and two: 256 rows of 16384
+    // keys 44 / 40, 512 69 / 64; 512 of 4096 26 / 29; 400 of 1531 16 / 20, 800 29 / 21). At head dim 128 their
+    // registers leave one wave a SIMD, which is never less time (128 rows of 32768 keys 66 / 86).
+    auto cost = [&](int nq) {
+        const int64_t n = splits(nq), tiles = (ntiles + n - 1) / n;
+        return (units(nq) * n + cus - 1) / cus * (nq == 2 ? 7 * tiles + 340 : 4 * tiles + 240);
     };
     f.nq = 1;
-    if (mx::fa_q_max_nq(f.DV) == 2 && f.R > 16) {
+    if (mx::fa_q_max_nq(f.D) == 2 && f.R > 16) {
         const char * e = getenv("MI355X_FA_Q_ROWS");
-        f.nq = e && *e ? (atoi(e) == 32 ? 2 : 1) : (f.DV == 64 ? 7 : 6) * tiles(2) + 100 < 4 * tiles(1) ? 2 : 1;
+        f.nq = e && *e ? (atoi(e) == 32 ? 2 : 1) : cost(2) < cost(1) ? 2 : 1;
     }
     f.nrt = (f.R + 16 * f.nq - 1) / (16 * f.nq);
     f.nsplit = (int)splits(f.nq);
@@ -783,17 +784,18 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
 // The direct form or decoding first. Direct attention turns codes into operands once for every 16 or 32
 // rows, and with many rows that, not the memory, is its time; decoding turns them once and feeds the F16
 // kernel, one sequence after another, in two or three launches and 21 us at least. Direct up to R (D + DV) = 2^16
-// (us direct / decoded, 8 KV heads, head dim 128: 128 rows of 8192 keys 31 / 42, 256 47 / 44, 384 70 / 51;
-// 256 of 32768 97 / 127, 384 176 / 143; head dim 256, 16384 keys: 128 rows 106 / 149, 192 193 / 147), and up
+// (us direct / decoded, 8 KV heads, head dim 128: 128 rows of 8192 keys 30 / 42, 256 45 / 44, 384 68 / 51;
+// 256 of 32768 115 / 127, 384 210 / 144; head dim 256, 16384 keys: 128 rows 94 / 149, 192 171 / 147), and up
 // to 64 key tiles of 16 rows a compute unit and sequence, which are done before those launches are (512 rows of
-// 1000 keys 20 / 25, 768 31 / 26; head dim 64, 1531 keys: 400 rows 16 / 22, 800 25 / 24; head dim 256, 1000
-// keys, 512 rows 40 / 72; 32 sequences x 256 rows x 1024 185 / 657).
+// 1000 keys 19 / 25, 768 33 / 25; head dim 64, 1531 keys: 400 rows 16 / 22, 800 21 / 24; head dim 256, 1000
+// keys, 512 rows 35 / 72; 32 sequences x 256 rows x 1024 213 / 639).
 static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (a->KV < mx::FA_Q_MIN_KV || a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
-    if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
-        if (*e) return atoi(e) != 0;
     int D, DV;
     mx::fa_pad_dims(a->D, a->DV, D, DV);
+    if (2 * a->D < D || 2 * a->DV < DV) return false;   // its loads of scales
+    if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
+        if (*e) return atoi(e) != 0;
     const int64_t R = (int64_t)(a->H / a->HK) * a->T;
     return R * (D + DV) <= 65536 || a->HK * ((R + 15) / 16) * ((a->KV + 31) / 32) <= 64 * (int64_t)device_cus();
 }

@@ -17,7 +17,7 @@
 // another's data:
 //   K   the lanes of group g hold bytes 8 g (Q8_0) or 4 g (Q4_0) on of every block of one key.
 //   P   the S^T accumulators of two 16-key products are the P^T operand: slot e of lane group g is key
-//       16 (e / 4) + 4 g + e % 4.
+//       8 g + e, which product e / 4 has as its row 4 g + e % 4.
 //   V   the lane of group g reads the same few bytes of those eight keys; v_perm_b32 picks one byte of
 //       two keys into a pair of halves, which transposes V.
 //
@@ -35,11 +35,18 @@
 // several keys. The running maximum moves only when a score passes it by more than 8 in the exponent of 2
 // (P stays below 256, well inside fp16), so most tiles exchange nothing between lanes.
 //
-// While a tile is worked on, the next one is on its way; the one after it is requested when its buffer is
-// free. The waves of a block take alternate tiles of the block's key range and merge through LDS at the
-// end; the key range is split over blocks where there are too few of them, and a second launch merges those.
-// Tiles that the mask hides from every row of a wave are left out: a lane looks at one tile's mask, for 64
-// of the wave's tiles at a time (only where at most 8 tokens share a wave; else every tile is read).
+// Each part of a tile is requested two tiles ahead. The waves of a block take alternate tiles of the block's
+// key range and merge through LDS at the end; the key range is split over blocks where there are too
+// few of them, and a second launch merges those. Tiles that the mask hides from every row of a wave are left
+// out: a lane looks at one tile's mask, for 64 of the wave's tiles at a time (only where at most 8 tokens
+// share a wave; else every tile is read).
+//
+// Measured (this kernel; its merge is 4.2 us more where keys are split), 32 heads on 8 of head dim 128: one token
+// on 1000 Q8_0 keys 9.4 us, on 32768 Q4_0 keys 16.1 us (38 MB, 2.3 TB/s); 32 sequences of 4096 Q8_0 keys 67 us
+// (286 MB, 4.3 TB/s, the rate of a plain read), of 1 to 4096 keys 55 us (143 MB: the longest's 16 tiles a
+// wave at 2.1 to 2.7 us each). A block's start until its first data is 3 to 5 us, its end 2.5 us. A tile at head dim
+// 128 in Q8_0, two waves a SIMD: 0.1 us waiting, 0.4 scores, 0.5 softmax and scales, 0.5 V, 0.6 requesting
+// the tile after the next: the latency of its own chain, not a unit at its limit.
 
 #pragma once
 
@@ -53,7 +60,7 @@ namespace mx {
 
 constexpr int FQ_KEYS = 32;      // keys a tile
 constexpr int FQ_LDS_MAX = 160 * 1024;
-constexpr int FQ_BASE_REGS = 64;
+constexpr int FQ_BASE_REGS = 96;  // with 64 there are more waves and spills: 32768 Q4_0 keys 19.6 us, not 16.5
 constexpr int FQ_SCAN_TOKENS = 8;
 constexpr float FQ_LAZY = 8.0f / 1.4426950408889634f;
 constexpr float FQ_LOG2E = 1.4426950408889634f;
@@ -69,8 +76,9 @@ struct FqCfg {
     static constexpr int KD = KCH / 2, VD = VCH / 2;
     static constexpr int STAGE = FQ_KEYS * 16 * (KCH + VCH);
     // Chunk c of K row r lies at c ^ kswz(r): the 16 rows that a read of one chunk takes then lie in 16
-    // different chunk slots of LDS's 256-byte window. V rows lie in the order 16 h + 4 i + g (key 16 h + 4 g
-    // + i), so that the four keys a read takes are neighbours, and chunk c at c ^ vswz(g).
+    // different chunk slots of LDS's 256-byte window. K rows lie in the order 16 h + 4 g + e and V rows in the
+    // order 16 h + 4 e + g (key 8 g + 4 h + e), so that the four V rows a read takes are neighbours, and V's
+    // chunk c at c ^ vswz(g).
     __device__ static __forceinline__ int kswz(int row) { return (row * KCH / 16) & (KCH - 1); }
     __device__ static __forceinline__ int vswz(int g) { return VCH == 16 ? 4 * g : VCH == 8 ? 4 * (g / 2) : 0; }
     static constexpr int VU = VT == T_Q8_0 || DV >= 128 ? 4 : 2;   // a lane's bytes of a V row: u, u + 16, ...
@@ -79,6 +87,7 @@ struct FqCfg {
     static constexpr int TT = DV / 16;                        // O^T tiles, index (j * VU + byte) * VH + nibble
     static_assert(KRB == 16 * KS * KW && VJ * VU * VH == TT, "layout");
     static constexpr int VB = DV / 32, VS = DV / 64, KSC = DK / 64;   // scales a key, and a lane (32 keys, two lanes each)
+    static constexpr int KSL = KSC == 3 ? 4 : KSC, VSL = VS;  // and of a lane's load
     static constexpr int Q_LDS = NQ * (KS * 1024 + 64);       // Q as B operands, then its rows' factors
     static constexpr int SCALE_LDS = KS * FQ_KEYS * 4 + VB * FQ_KEYS * 2;   // a wave's scales: K's F32, V's F16
     static constexpr int WAVE_LDS = SCALE_LDS + 2 * STAGE;
@@ -97,10 +106,15 @@ struct FqCfg {
     static constexpr int LDS = MERGE_LDS > LOOP_LDS ? MERGE_LDS : LOOP_LDS;
 };
 
-typedef const void __attribute__((address_space(1))) * fq_gptr_t;
 typedef void __attribute__((address_space(3))) * fq_lptr_t;
-__device__ __forceinline__ void fq_dma16(const void * g, void * l) {
-    __builtin_amdgcn_global_load_lds((fq_gptr_t)g, (fq_lptr_t)l, 16, 0, 0);
+// 16 bytes a lane into LDS, lane after lane, from byte `off` (below 2^31) of a wave-uniform address. As
+// buffer loads: while a global load to LDS is pending, the compiler makes every wait for a register load
+// one for all loads.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t fq_rsrc(const void * p) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, 0x7FFFFFFF, 0x00020000);
+}
+__device__ __forceinline__ void fq_dma16(__amdgpu_buffer_rsrc_t p, uint32_t off, void * l) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(p, (fq_lptr_t)l, 16, off, 0, 0, 0);
 }
 // No memory access moves across it; waits until at most N vector loads are outstanding.
 template <int N>
@@ -149,6 +163,16 @@ template <int TYPE>
 __device__ __forceinline__ float fq_scale(uint16_t bits, float bad) {
     const float d = fmaxf(fminf(h2f_bits(bits), kv_scale_limit(TYPE)), -kv_scale_limit(TYPE));
     return (bits & 0x7C00u) == 0x7C00u ? bad : d;
+}
+
+// N fp16 scales, of any alignment.
+template <int N>
+__device__ __forceinline__ uint64_t fq_load_scales(const uint8_t * p) {
+    if constexpr (N == 1) return *(const uint16_t *)p;
+    uint32_t lo, hi = 0;
+    __builtin_memcpy(&lo, p, 4);
+    if constexpr (N == 4) __builtin_memcpy(&hi, p + 4, 4);
+    return (uint64_t)hi << 32 | lo;
 }
 
 // A lane's eight unsigned codes of a K block, each the low bits of a half. Q8_0: dims 8 g + 0..7. Q4_0:
@@ -205,25 +229,21 @@ fa_q_kernel(FaQArgs a) {
 #pragma unroll
     for (int q = 0; q < C::KD; q++) {
         const int slot = q * WAVE + lane, row = slot / C::KCH, c = (slot % C::KCH) ^ C::kswz(row);
-        kdma[q] = (((uint32_t)row * knb) >> KSH) + (c * 16 < (a.dk >> KSH) ? 16 * c : 0);
+        const uint32_t key = row % 16 / 4 * 8 + row / 16 * 4 + row % 4;
+        kdma[q] = ((key * knb) >> KSH) + (c * 16 < (a.dk >> KSH) ? 16 * c : 0);
     }
 #pragma unroll
     for (int q = 0; q < C::VD; q++) {
         const int slot = q * WAVE + lane, pos = slot / C::VCH, c = (slot % C::VCH) ^ C::vswz(pos % 4);
-        const uint32_t key = pos / 16 * 16 + pos % 4 * 4 + pos % 16 / 4;
+        const uint32_t key = pos % 4 * 8 + pos / 16 * 4 + pos % 16 / 4;
         vdma[q] = ((key * vnb) >> VSH) + (c * 16 < (a.dv >> VSH) ? 16 * c : 0);
     }
-    uint32_t kdo[C::KSC], vdo[C::VS];    // the scales this lane fetches: key lane / 2, half of its blocks
-#pragma unroll
-    for (int i = 0; i < C::KSC; i++) {
-        const int blk = (lane % 2) * C::KSC + i;
-        kdo[i] = (uint32_t)(lane / 2) * knb / 32 * 2 + (32 * blk < a.dk ? 2 * blk : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < C::VS; i++) {
-        const int blk = (lane % 2) * C::VS + i;
-        vdo[i] = (uint32_t)(lane / 2) * vnb / 32 * 2 + (32 * blk < a.dv ? 2 * blk : 0);
-    }
+    // The scales this lane fetches: key lane / 2, half of its blocks, in one load that stays inside the row
+    // (dk and dv are at least half of the built dims): shifted down to the first of them, zeros behind the last.
+    const int kn32 = a.dk / 32, vn32 = a.dv / 32, half = lane % 2;
+    const int kfirst = min(half * C::KSC, kn32 - C::KSL), vfirst = min(half * C::VS, vn32 - C::VSL);
+    const uint32_t kdo = (uint32_t)(lane / 2) * (knb / 32 * 2) + 2 * kfirst, vdo = (uint32_t)(lane / 2) * (vnb / 32 * 2) + 2 * vfirst;
+    const int ksh = min(16 * (half * C::KSC - kfirst), 63), vsh = min(16 * (half * C::VS - vfirst), 63);
     // where this lane reads: bytes 4 KW g on of a K block (block i at kra ^ kra_i), its bytes of V row g
     uint32_t kra = r * C::KCH * 16, vra[C::VJ];
     kra += KT == T_Q8_0 ? ((C::kswz(r) ^ (g / 2)) << 4) + 8 * (g % 2) : (C::kswz(r) << 4) + 4 * g;
@@ -238,15 +258,21 @@ fa_q_kernel(FaQArgs a) {
     uint8_t * const wl = smem + C::Q_LDS + wave * C::WAVE_LDS;   // this wave's scales and buffers
     float * const wk = (float *)wl;                              // K scales [block][key]
     uint16_t * const wv = (uint16_t *)(wk + C::KS * FQ_KEYS);    // V scales
-    auto dma = [&](int t, int buf) {
-        const int64_t kb = min(FQ_KEYS * t, kb_last);
-        const uint8_t * kt = kq + ((kb * a.k.nb1) >> KSH);
-        const uint8_t * vt = vq + ((kb * a.v.nb1) >> VSH);
+    auto dma_k = [&](int t, int buf) {
+        const __amdgpu_buffer_rsrc_t kt = fq_rsrc(kq + ((min(FQ_KEYS * t, kb_last) * a.k.nb1) >> KSH));
         uint8_t * st = wl + C::SCALE_LDS + buf * C::STAGE;
+        asm volatile("" ::: "memory");
 #pragma unroll
-        for (int q = 0; q < C::KD; q++) fq_dma16(kt + kdma[q], st + q * 1024);
+        for (int q = 0; q < C::KD; q++) fq_dma16(kt, kdma[q], st + q * 1024);
+        asm volatile("" ::: "memory");
+    };
+    auto dma_v = [&](int t, int buf) {
+        const __amdgpu_buffer_rsrc_t vt = fq_rsrc(vq + ((min(FQ_KEYS * t, kb_last) * a.v.nb1) >> VSH));
+        uint8_t * st = wl + C::SCALE_LDS + buf * C::STAGE + FQ_KEYS * 16 * C::KCH;
+        asm volatile("" ::: "memory");
 #pragma unroll
-        for (int q = 0; q < C::VD; q++) fq_dma16(vt + vdma[q], st + FQ_KEYS * 16 * C::KCH + q * 1024);
+        for (int q = 0; q < C::VD; q++) fq_dma16(vt, vdma[q], st + q * 1024);
+        asm volatile("" ::: "memory");
     };
 
     // this lane's rows
@@ -257,28 +283,21 @@ fa_q_kernel(FaQArgs a) {
         const int row = (rt * NQ + n) * 16 + r;
         ok[n] = row < a.R;
         const int tok = ok[n] ? fq_div(row, a.div_g) : 0;
-        mrow[n] = a.mask ? a.mask + (int64_t)s * a.mask_nb3 + (int64_t)tok * a.mask_nb1 + 4 * g : (const uint16_t *)kq;
+        mrow[n] = a.mask ? a.mask + (int64_t)s * a.mask_nb3 + (int64_t)tok * a.mask_nb1 + 8 * g : (const uint16_t *)kq;
     }
     // without a mask the same loads read the first key's codes, and nothing looks at them: a load that
     // is sometimes issued would make every wait behind it a wait for all loads
     const int mstep = a.mask ? 1 : 0;
     struct Side {              // what of a tile comes into registers
-        uint16_t kd[C::KSC], vd[C::VS];
-        u32x2 m[NQ][2];        // the mask of this lane's four keys of either half tile
+        uint64_t kd, vd;
+        u32x4 m[NQ];           // the mask of this lane's eight keys
     };
     auto load_side = [&](Side & x, int t) {
         const int64_t kb = min(FQ_KEYS * t, kb_last);
-        const uint8_t * kt = (const uint8_t *)kd + kb * a.k.nb1 / 32 * 2;
-        const uint8_t * vt = (const uint8_t *)vd + kb * a.v.nb1 / 32 * 2;
+        x.kd = fq_load_scales<C::KSL>((const uint8_t *)kd + kb * a.k.nb1 / 32 * 2 + kdo);
+        x.vd = fq_load_scales<C::VSL>((const uint8_t *)vd + kb * a.v.nb1 / 32 * 2 + vdo);
 #pragma unroll
-        for (int i = 0; i < C::KSC; i++) x.kd[i] = *(const uint16_t *)(kt + kdo[i]);
-#pragma unroll
-        for (int i = 0; i < C::VS; i++) x.vd[i] = *(const uint16_t *)(vt + vdo[i]);
-#pragma unroll
-        for (int n = 0; n < NQ; n++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++)
-                __builtin_memcpy(&x.m[n][hf], mrow[n] + (kb + 16 * hf) * mstep, 8);   // any alignment of 2 bytes
+        for (int n = 0; n < NQ; n++) __builtin_memcpy(&x.m[n], mrow[n] + kb * mstep, 16);   // any alignment of 2 bytes
     };
     // The wave's tiles are tile0 + wave + NW k. next() gives the next k that some row sees (-1: none): bits
     // of 64 of them, one lane a tile.
@@ -343,13 +362,17 @@ fa_q_kernel(FaQArgs a) {
     // replaced once they have landed. Waves without tiles read some tile all the same: loads that are
     // sometimes issued would make every wait behind them a wait for all loads.
     const int tile_end = ntiles - 1;
-    int t = min(tile0 + wave, tile_end), tn = min(tile0 + wave + NW, tile_end), buf = 0;
-    Side x;
-    dma(t, 0);
-    asm volatile("" ::: "memory");
-    load_side(x, t);
-    asm volatile("" ::: "memory");
-    dma(tn, 1);
+    int t = min(tile0 + wave, tile_end), tn = min(tile0 + wave + NW, tile_end);
+    Side x0, x1;
+    auto request = [&]() {   // a tile's K, its scales and masks, its V, then the next tile's
+        dma_k(t, 0);
+        load_side(x0, t);
+        dma_v(t, 0);
+        dma_k(tn, 1);
+        load_side(x1, tn);
+        dma_v(tn, 1);
+    };
+    request();
 
     if (wave < NQ) {
         float v[C::KS][8], amax = 0.0f;
@@ -386,11 +409,7 @@ fa_q_kernel(FaQArgs a) {
         fq_wait_vm<0>();
         t = tile0 + wave + NW * ka;
         tn = kn >= 0 ? tile0 + wave + NW * kn : t;
-        dma(t, 0);
-        asm volatile("" ::: "memory");
-        load_side(x, t);
-        asm volatile("" ::: "memory");
-        dma(tn, 1);
+        request();
     }
     // a barrier for LDS alone: the first tiles' loads stay in flight
     asm volatile("" ::: "memory");
@@ -417,13 +436,17 @@ fa_q_kernel(FaQArgs a) {
     uint32_t vtop = 0;          // the largest scale it is for, as bits: 2^(15 - k)
     const float cap2 = a.softcap != 0.0f ? 2.0f * FQ_LOG2E / a.softcap : 0.0f;
 
-    while (ka >= 0) {
-        fq_wait_vm<C::KD + C::VD>();   // everything older than the next tile's DMA has landed: this tile
-        Side xn;
-        load_side(xn, tn);
-        asm volatile("" ::: "memory");
+    // Tile t in buffer BUF, with its scales and masks in x. Everything of a tile is requested two tiles ahead, each
+    // part as soon as the one that it takes the place of has been used, and waited for apart, so nearly two
+    // tiles' time is there for it. (Requested and waited for as one, a wave waited 0.9 us of a tile's
+    // 2.6 for it: 32 sequences of up to 4096 keys, Q8_0, head dim 128.) Returns false after the last tile.
+    auto tile = [&](Side & x, auto buffer) __attribute__((always_inline)) {
+        constexpr int BUF = decltype(buffer)::value;
+        constexpr int SL = 2 + NQ;                       // loads of load_side
+        // K's codes and x have landed; behind them V, and the next tile's three
+        fq_wait_vm<C::VD + C::KD + SL + C::VD>();
         const int kb = min(FQ_KEYS * t, kb_last);
-        const uint8_t * const st = wl + C::SCALE_LDS + buf * C::STAGE;
+        const uint8_t * const st = wl + C::SCALE_LDS + BUF * C::STAGE;
         const uint8_t * const stv = st + FQ_KEYS * 16 * C::KCH;
         if constexpr (!C::KEEP_OFF) asm("" : "+v"(koff));   // else the offsets' products would move out of the loop
         float4v sc[NQ][2];
@@ -431,7 +454,7 @@ fa_q_kernel(FaQArgs a) {
             // ---- S^T = K . Q^T, each block's product times its scale (and 2^24) ----
 #pragma unroll
             for (int i = 0; i < C::KSC; i++)
-                wk[((lane % 2) * C::KSC + i) * FQ_KEYS + lane / 2] = fq_scale<KT>(x.kd[i], NAN) * 16777216.0f;
+                wk[(half * C::KSC + i) * FQ_KEYS + lane / 2] = fq_scale<KT>((uint16_t)((x.kd >> ksh) >> (16 * i)), NAN) * 16777216.0f;
             asm volatile("" ::: "memory");   // one wave's LDS operations complete in order
 #pragma unroll
             for (int n = 0; n < NQ; n++) sc[n][0] = sc[n][1] = float4v{0, 0, 0, 0};
@@ -446,7 +469,7 @@ fa_q_kernel(FaQArgs a) {
                     off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), qf[n], float4v{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
-                    const float4v d = *(const float4v *)(wk + i * FQ_KEYS + 16 * hf + 4 * g);
+                    const float4v d = *(const float4v *)(wk + i * FQ_KEYS + 8 * g + 4 * hf);
                     uint32_t kx[2];
                     if constexpr (C::KW == 2) {
                         const u32x2 w = *(const u32x2 *)(st + (kra ^ (uint32_t)(32 * i)) + hf * 256 * C::KCH);
@@ -466,6 +489,12 @@ fa_q_kernel(FaQArgs a) {
                 if (!C::KEEP_OFF) __builtin_amdgcn_sched_barrier(0);   // not every block's operands at once
             }
         }
+        // K's codes have been read: the ones of the tile after the next come in their place (the last ones
+        // again, where there is none: the number of loads in flight stays what the waits count)
+        const int k2 = kn >= 0 ? next() : -1;
+        const int t2 = k2 >= 0 ? tile0 + wave + NW * k2 : tn;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        dma_k(t2, BUF);
         half8 pf[NQ];
         float dv[C::VS];
         {
@@ -488,12 +517,12 @@ fa_q_kernel(FaQArgs a) {
                         for (int e = 0; e < 4; e++)
                             sc[n][hf][e] = fmaf(-2.0f * a.softcap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[n][hf][e] * cap2)), a.softcap);
                 }
-                if (a.mask && __any((x.m[n][0][0] | x.m[n][0][1] | x.m[n][1][0] | x.m[n][1][1]) != 0)) {
+                if (a.mask && __any((x.m[n][0] | x.m[n][1] | x.m[n][2] | x.m[n][3]) != 0)) {
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const float mv = h2f_bits((uint16_t)(x.m[n][hf][e / 2] >> (16 * (e % 2))));
+                            const float mv = h2f_bits((uint16_t)(x.m[n][2 * hf + e / 2] >> (16 * (e % 2))));
                             sc[n][hf][e] = mv == -INFINITY ? -INFINITY : sc[n][hf][e] + mv;   // a hidden score may be NaN
                         }
                 }
@@ -502,7 +531,7 @@ fa_q_kernel(FaQArgs a) {
                     for (int hf = 0; hf < 2; hf++)
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (kb + 16 * hf + 4 * g + e < FQ_KEYS * t) sc[n][hf][e] = -INFINITY;
+                            if (kb + 8 * g + 4 * hf + e < FQ_KEYS * t) sc[n][hf][e] = -INFINITY;
                 }
                 float mt = -INFINITY;
 #pragma unroll
@@ -542,9 +571,10 @@ fa_q_kernel(FaQArgs a) {
             bool bad = false;
 #pragma unroll
             for (int i = 0; i < C::VS; i++) {
-                bad |= (x.vd[i] & 0x7C00u) == 0x7C00u;
-                dv[i] = fq_scale<VT>(x.vd[i], 0.0f);
-                top = max(top, (uint16_t)(x.vd[i] & 0x7FFFu));
+                const uint16_t bits = (uint16_t)((x.vd >> vsh) >> (16 * i));
+                bad |= (bits & 0x7C00u) == 0x7C00u;
+                dv[i] = fq_scale<VT>(bits, 0.0f);
+                top = max(top, (uint16_t)(bits & 0x7FFFu));
             }
             if (__any(top > vtop)) {
                 // a larger scale than any before, or one that is not finite (which stands for zero and makes
@@ -564,7 +594,7 @@ fa_q_kernel(FaQArgs a) {
                         const uint64_t rows = __ballot(any);
 #pragma unroll
                         for (int gg = 0; gg < 4; gg++)
-                            seen_keys |= (uint32_t)(((rows >> (16 * gg)) & 0xFFFFu) != 0) << (16 * (e / 4) + 4 * gg + e % 4);
+                            seen_keys |= (uint32_t)(((rows >> (16 * gg)) & 0xFFFFu) != 0) << (8 * gg + e);
                     }
                     const bool mine = (seen_keys >> (lane / 2)) & 1u;
                     bad &= mine;
@@ -575,7 +605,7 @@ fa_q_kernel(FaQArgs a) {
                 if (bad_lanes) {
 #pragma unroll
                     for (int e = 0; e < 8; e++)
-                        if ((bad_lanes >> (2 * (16 * (e / 4) + 4 * g + e % 4))) & 3u) {
+                        if ((bad_lanes >> (2 * (8 * g + e))) & 3u) {
 #pragma unroll
                             for (int n = 0; n < NQ; n++)
                                 if (sc[n][e / 4][e % 4] != -INFINITY) l_run[n] = NAN;
@@ -608,21 +638,24 @@ fa_q_kernel(FaQArgs a) {
                 }
             }
         }
+        asm volatile("" ::: "memory");
+        load_side(x, t2);
+        fq_wait_vm<C::KD + SL + C::VD + C::KD + SL>();   // this tile's V has landed
         {
             // ---- V's scales into LDS, times 2^k ----
 #pragma unroll
-            for (int i = 0; i < C::VS; i++) wv[((lane % 2) * C::VS + i) * FQ_KEYS + lane / 2] = f2h_bits(dv[i] * vscale);
+            for (int i = 0; i < C::VS; i++) wv[(half * C::VS + i) * FQ_KEYS + lane / 2] = f2h_bits(dv[i] * vscale);
             asm volatile("" ::: "memory");
             // ---- O^T += V^T . P^T ----
 #pragma unroll
             for (int j = 0; j < C::VJ; j++) {
                 half2v d[4];
                 {
-                    const u32x2 lo = *(const u32x2 *)(wv + vblk[j] * FQ_KEYS + 4 * g), hi = *(const u32x2 *)(wv + vblk[j] * FQ_KEYS + 16 + 4 * g);
-                    d[0] = h2_of(lo[0]);
-                    d[1] = h2_of(lo[1]);
-                    d[2] = h2_of(hi[0]);
-                    d[3] = h2_of(hi[1]);
+                    const u32x4 w = *(const u32x4 *)(wv + vblk[j] * FQ_KEYS + 8 * g);
+                    d[0] = h2_of(w[0]);
+                    d[1] = h2_of(w[1]);
+                    d[2] = h2_of(w[2]);
+                    d[3] = h2_of(w[3]);
                 }
                 const half8 ds = __builtin_bit_cast(half8, u32x4{u_of(d[0]), u_of(d[1]), u_of(d[2]), u_of(d[3])});
 #pragma unroll
@@ -656,20 +689,16 @@ fa_q_kernel(FaQArgs a) {
                 }
             }
         }
-        // this tile's buffer has been read: the one after the next may come into it (the last ones again,
-        // where there is none: the number of loads in flight stays what the wait above counts)
-        const int k2 = kn >= 0 ? next() : -1;
-        const int t2 = k2 >= 0 ? tile0 + wave + NW * k2 : tn;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        dma(t2, buf);
-        asm volatile("" ::: "memory");
-        if (kn < 0) break;
-        x = xn;
+        dma_v(t2, BUF);
+        if (kn < 0) return false;
         t = tn;
         tn = t2;
         kn = k2;
-        buf ^= 1;
-    }
+        return true;
+    };
+    if (ka >= 0)
+        while (tile(x0, std::integral_constant<int, 0>{}) && tile(x1, std::integral_constant<int, 1>{})) {}
     fq_wait_vm<0>();   // no DMA may still write what the merge reuses
 
     // ---- merge the block's waves ----
@@ -780,7 +809,7 @@ static hipError_t fq_launch(const FaQArgs & a, hipStream_t st) {
 template <int KT, int VT, int DK, int DV>
 static hipError_t fq_rows(const FaQArgs & a, hipStream_t st) {
     if (a.nq == 1) return fq_launch<KT, VT, DK, DV, 1>(a, st);
-    if constexpr (DV <= 128)
+    if constexpr (DK == 64)
         if (a.nq == 2) return fq_launch<KT, VT, DK, DV, 2>(a, st);
     return hipErrorInvalidValue;
 }

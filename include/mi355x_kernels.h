@@ -382,7 +382,7 @@ MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int 
  * Few rows are taken by a kernel that reads the cache as it is stored, in any number of sequences; many by
  * decoding it to fp16 in the workspace, a sequence at a time, for the kernel of mi355x_flash_attn. The
  * choice follows measured costs; MI355X_FA_Q_DIRECT=1|0 pins it and MI355X_FA_Q_ROWS=16|32 the rows a
- * wave of the first takes, for measurements and tests.
+ * wave of the first takes at head dims up to 64, for measurements and tests.
  * Concurrent calls must not share a workspace. Equal inputs give equal bits. */
 MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
                                    void * stream);
