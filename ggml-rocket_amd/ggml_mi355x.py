@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libmi355x.so")
@@ -144,9 +145,9 @@ def _bind_optional(L):
         L.mi355x_flash_attn.argtypes = [pa, i32, vp, sz, vp]
         L.mi355x_flash_attn_ex.argtypes = [pa, i32, i32, vp, sz, vp]
     if hasattr(L, "mi355x_set_rows"):
-        pr, pq = ctypes.POINTER(KvRows), ctypes.POINTER(FaQArgs)
-        L.mi355x_set_rows.argtypes = [pr, i32, vp, i32, i64, vp, vp]
-        L.mi355x_get_rows.argtypes = [pr, i32, vp, i32, i64, vp, vp]
+        pq = ctypes.POINTER(FaQArgs)
+        L.mi355x_set_rows.argtypes = [vp, i32, vp, i32, i64, vp, vp]
+        L.mi355x_get_rows.argtypes = [vp, i32, vp, i32, i64, vp, vp]
         L.mi355x_flash_attn_q_workspace.restype = sz
         L.mi355x_flash_attn_q_workspace.argtypes = [pq, i32]
         L.mi355x_flash_attn_q.argtypes = [pq, i32, vp, sz, vp]
@@ -361,8 +362,8 @@ class KvCache:
         n, nb, qp, dp = len(self.shape), self.nb, q.data_ptr(), None if d is None else d.data_ptr()
         # the cache's part of mi355x_kv_rows ([rows, D] or [rows, H, D]) and of mi355x_fa_q_args ([(S,) HK, KV, D])
         self._tail = self.shape[1:]
-        self._rows = {2: (ttype, qp, dp, self.shape[0], nb[0], 0, 1, self.D),
-                      3: (ttype, qp, dp, self.shape[0], nb[0], nb[-1], self.shape[1], self.D)}.get(n)
+        self._rows = {2: (ttype, qp, dp or 0, self.shape[0], nb[0], 0, 1, self.D),
+                      3: (ttype, qp, dp or 0, self.shape[0], nb[0], nb[-1], self.shape[1], self.D)}.get(n)
         self._view = KvView(ttype, qp, dp, nb[-1], nb[-2], nb[0] if n == 4 else 0) if n in (3, 4) and d is not None else None
 
     def permute(self, *dims):
@@ -412,20 +413,20 @@ def _launch_stream(dev: int, what: str):
     return C._cuda_getCurrentRawStream(dev)
 
 
-_KV_ROWS = [None] + [KvRows * n for n in range(1, 5)]
+_KV_ROWS = struct.Struct("@iPPqqqqqiPqq")     # mi355x_kv_rows, field by field
 
 
 def _kv_rows(caches, plain, n, what):
     """mi355x_kv_rows of caches [rows, H, D] or [rows, D] and their plain rows [n, H, D] or [n, D]."""
-    types, out = _plain_types(), []
+    types, out = _plain_types(), b""
     if not 1 <= len(caches) <= 4:
         raise MI355XError(f"{what}: one to four caches")
     for c, x in zip(caches, plain):
-        shape, stride, t = x.shape, x.stride(), types.get(x.dtype)
-        if c._rows is None or shape[1:] != c._tail or shape[0] != n or stride[-1] != 1 or t not in (F32, F16) or x.get_device() != c.dev:
-            raise MI355XError(f"{what}: rows {x.dtype} {tuple(shape)} do not fit {n} rows of a cache {c.shape}")
-        out.append(KvRows(*c._rows, t, x.data_ptr(), stride[0], stride[1] if len(stride) == 3 else 0))
-    return _KV_ROWS[len(out)](*out)
+        stride, t, rows = x.stride(), types.get(x.dtype), c._rows
+        if rows is None or x.shape != (n, *c._tail) or stride[-1] != 1 or (t != F32 and t != F16) or x.get_device() != c.dev:
+            raise MI355XError(f"{what}: rows {x.dtype} {tuple(x.shape)} do not fit {n} rows of a cache {c.shape}")
+        out += _KV_ROWS.pack(*rows, t, x.data_ptr(), stride[0], stride[1] if len(stride) == 3 else 0)
+    return out
 
 
 def _kv_index(idx, n, dev, what):
@@ -456,7 +457,7 @@ def set_rows(pairs, idx=None, err=None):
     if any(c.dev != dev for c in caches):
         raise MI355XError("set_rows: caches on one device")
     arr = _kv_rows(caches, plain, n, "set_rows")
-    check(lib().mi355x_set_rows(arr, len(arr), ip, it, n, _kv_err(err, dev, "set_rows"), _launch_stream(dev, "set_rows")), "set_rows")
+    check(lib().mi355x_set_rows(arr, len(caches), ip, it, n, _kv_err(err, dev, "set_rows"), _launch_stream(dev, "set_rows")), "set_rows")
 
 
 def get_rows(caches, idx=None, dtype=None, out=None, err=None):
@@ -467,12 +468,12 @@ def get_rows(caches, idx=None, dtype=None, out=None, err=None):
     if any(c.dev != dev for c in caches):
         raise MI355XError("get_rows: caches on one device")
     if out is None:
-        torch = _torch()
-        out = [torch.empty((n,) + c._tail, dtype=dtype or torch.float32, device=c.q.device) for c in caches]
+        dtype = dtype or _torch().float32
+        out = [c.q.new_empty((n, *c._tail), dtype=dtype) for c in caches]
     elif len(out) != len(caches):
         raise MI355XError("get_rows: one output for every cache")
     arr = _kv_rows(caches, out, n, "get_rows")
-    check(lib().mi355x_get_rows(arr, len(arr), ip, it, n, _kv_err(err, dev, "get_rows"), _launch_stream(dev, "get_rows")), "get_rows")
+    check(lib().mi355x_get_rows(arr, len(caches), ip, it, n, _kv_err(err, dev, "get_rows"), _launch_stream(dev, "get_rows")), "get_rows")
     return out
 
 
