@@ -649,7 +649,8 @@ static int kv_rows_lower(const mi355x_kv_rows * r, int n_out, const void * idx_d
     if (idx_type != 26 && idx_type != 27) return MI355X_E_ARG;
     if (!aligned(idx_dev, idx_type == 27 ? 8 : 4) || !aligned(err_dev, 4)) return MI355X_E_ARG;
     memset(&a, 0, sizeof a);
-    // 32-bit positions (fq_div): blocks of one output and of a workgroup's rows below 2^30
+    // 32-bit positions (fq_div) and threads of a launch: all outputs' blocks up to 2^30, a row's up to 2^24
+    int64_t blocks = 0;
     for (int k = 0; k < n_out; k++) {
         const mi355x_kv_rows & s = r[k];
         if ((!kv_type(s.type) && s.type != mx::T_F16) || (s.x_type != mx::T_F32 && s.x_type != mx::T_F16)) return MI355X_E_ARG;
@@ -660,7 +661,7 @@ static int kv_rows_lower(const mi355x_kv_rows * r, int n_out, const void * idx_d
         if (n > 0 && s.type != mx::T_F16 && (!s.d_dev || !aligned(s.d_dev, 8))) return MI355X_E_ARG;
         if (!idx_dev && n > s.n_rows) return MI355X_E_ARG;
         const int64_t bpr = s.H * (s.D / 32);
-        if (bpr > (1 << 24) || n * bpr > (1 << 30)) return MI355X_E_ARG;
+        if (bpr > (1 << 24) || (blocks += n * bpr) > (1 << 30)) return MI355X_E_ARG;
         mx::KvRowsOut & o = a.o[k];
         o.q = (uint8_t *)s.q_dev; o.d = s.d_dev; o.x = s.x_dev;
         o.nb1 = s.nb1; o.nb2 = s.nb2; o.x_nb1 = s.x_nb1; o.x_nb2 = s.x_nb2; o.n_rows = s.n_rows;
@@ -691,7 +692,7 @@ static int fa_q_check_view(const mi355x_kv_view & w, bool empty) {
     return MI355X_OK;
 }
 
-static int fa_q_check(const mi355x_fa_q_args * a) {
+static int fa_q_check(const mi355x_fa_q_args * a, int nsplit) {
     if (!a) return MI355X_E_ARG;
     const bool empty = a->T == 0 || a->S == 0;   // no query: nothing is read or written
     if (!empty && (!a->q_dev || !a->dst_dev)) return MI355X_E_ARG;
@@ -702,7 +703,9 @@ static int fa_q_check(const mi355x_fa_q_args * a) {
         if (st != MI355X_OK) return st;
     }
     if (a->T < 0 || a->S < 0 || a->H <= 0 || a->HK <= 0 || a->KV < 0 || a->H % a->HK) return MI355X_E_ARG;
-    if ((int64_t)a->KV * a->HK * ((a->D + a->DV) / 32) >= 1 << 30) return MI355X_E_UNSUPPORTED;
+    if ((int64_t)a->KV * a->HK * ((a->D + a->DV) / 32) >= 1 << 29) return MI355X_E_UNSUPPORTED;
+    // threads of a launch: 16 rows of a sequence and KV head, up to 1024 threads and 64 splits
+    if ((int64_t)a->S * a->HK * (((int64_t)a->T * (a->H / a->HK) + 15) / 16) > (1 << 21) / (nsplit > 1 ? nsplit : 1)) return MI355X_E_UNSUPPORTED;
     if ((int64_t)a->S * a->T * a->H > (1 << 30) || (size_t)a->KV > mx::fa_max_kv(a->D, a->DV)) return MI355X_E_UNSUPPORTED;
     for (int t : {a->q_type, a->dst_type})
         if (t != mx::T_F32 && t != mx::T_F16) return MI355X_E_ARG;
@@ -828,15 +831,15 @@ static FaQLayout fa_q_layout(const mi355x_fa_q_args * a, int nsplit) {
 }
 
 MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int nsplit) {
-    if (fa_q_check(a) != MI355X_OK || nsplit > 64) return 0;
+    if (nsplit > 64 || fa_q_check(a, nsplit) != MI355X_OK) return 0;
     return fa_q_is_direct(a) ? fa_q_direct_layout(fa_q_direct(a, nsplit)).total : fa_q_layout(a, nsplit).total;
 }
 
 MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
                                    void * stream) {
-    const int st = fa_q_check(a);
-    if (st != MI355X_OK) return st;
     if (nsplit > 64) return MI355X_E_ARG;
+    const int st = fa_q_check(a, nsplit);
+    if (st != MI355X_OK) return st;
     if (a->T == 0 || a->S == 0) return MI355X_OK;
     if (fa_q_is_direct(a)) {
         mx::FaQArgs f = fa_q_direct(a, nsplit);

@@ -24,6 +24,7 @@ namespace mx {
 constexpr int KV_THREADS = 256;
 constexpr int KV_BLOCKS = KV_THREADS / 4;   // 32-value blocks in flight in a workgroup
 constexpr int KV_ROWS_MAX = 8;              // rows a workgroup of set_rows
+constexpr int KV_ROWS_LAUNCH = 16384;       // and a launch of it
 
 template <int CTRL>
 __device__ __forceinline__ uint32_t quad_dpp(uint32_t x) {
@@ -298,12 +299,30 @@ static void kv_divs(KvRowsArgs & a) {
     }
 }
 
+// A launch takes KV_ROWS_LAUNCH rows at most, the next ones a next launch: the scans of later indices grow with the
+// square of a launch's rows, and a repeated index in a later launch comes later by itself.
 hipError_t launch_set_rows(KvRowsArgs a, hipStream_t st) {
     kv_divs(a);
-    // one row a workgroup until the chip is full a few times over, then more: fewer index scans
-    a.rows_wg = min(KV_ROWS_MAX, max(1, a.n / 512));
-    hipLaunchKernelGGL(set_rows_kernel, dim3((a.n + a.rows_wg - 1) / a.rows_wg, a.n_out), dim3(KV_THREADS), 0, st, a);
-    return hipGetLastError();
+    const int all = a.n;
+    for (int r0 = 0; r0 < all; r0 += KV_ROWS_LAUNCH) {
+        a.n = min(KV_ROWS_LAUNCH, all - r0);
+        // one row a workgroup until the chip is full a few times over, then more: fewer index scans
+        a.rows_wg = min(KV_ROWS_MAX, max(1, a.n / 512));
+        hipLaunchKernelGGL(set_rows_kernel, dim3((a.n + a.rows_wg - 1) / a.rows_wg, a.n_out), dim3(KV_THREADS), 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        if (a.idx) a.idx = (const uint8_t *)a.idx + (int64_t)KV_ROWS_LAUNCH * (a.idx64 ? 8 : 4);
+        for (int k = 0; k < a.n_out; k++) {
+            KvRowsOut & o = a.o[k];
+            o.x = (uint8_t *)o.x + KV_ROWS_LAUNCH * o.x_nb1 * (o.x_f16 ? 2 : 4);
+            if (a.idx) continue;   // else row i is cache row i
+            const int64_t e0 = KV_ROWS_LAUNCH * o.nb1;
+            o.q += o.type == T_F16 ? 2 * e0 : o.type == T_Q4_0 ? e0 / 2 : e0;
+            if (o.d) o.d += e0 / 32;
+            o.n_rows -= KV_ROWS_LAUNCH;
+        }
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_get_rows(KvRowsArgs a, hipStream_t st) {

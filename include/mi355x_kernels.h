@@ -326,8 +326,8 @@ typedef struct mi355x_kv_rows {
 } mi355x_kv_rows;
 
 /* ggml's SET_ROWS into a cache: row i of the plain values of each of `n_out` (1..4) caches is
- * quantized and written to cache row idx[i], for every i < n, in ONE launch (a layer's K and V share
- * their indices). idx_dev: int32 (idx_type 26) or int64 (27) [n] on the device, or NULL for idx[i] = i.
+ * quantized and written to cache row idx[i], for every i < n, all caches in one launch (a layer's K and V
+ * share their indices). idx_dev: int32 (idx_type 26) or int64 (27) [n] on the device, or NULL for idx[i] = i.
  * Where an index repeats, the row with the largest i stays, whole. An index outside [0, n_rows)
  * writes nothing and sets *err_dev (a device int32, may be NULL) to 1. Rows that no index names keep
  * their bytes.
@@ -336,7 +336,8 @@ typedef struct mi355x_kv_rows {
  * truncated, at most 15), each step rounded to f32, d stored as fp16 (infinite past 65504, as
  * ggml's). A block that holds a NaN or an infinity, for which ggml defines nothing, is stored with
  * a NaN scale and reads back as NaN. F16: round to nearest even.
- * n * H * D / 32 and n stay below 2^30, H * D / 32 below 2^24.
+ * n and n * H * D / 32, summed over the caches, are at most 2^30, H * D / 32 at most 2^24. One launch for
+ * every 16384 rows.
  * No counterpart in the reference, whose host writes its caches on the CPU. */
 MI355X_API int mi355x_set_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
                                int32_t * err_dev, void * stream);
@@ -375,7 +376,8 @@ MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int 
  * q.k) + mask) . v. K and V enter the products as fp16 (their values rounded once), Q and P as fp16,
  * sums in F32: an F32 dst holds values of that accuracy. So that the values stay inside fp16, a scale
  * counts as at most 515.5 (Q8_0: 65468 / 127) or 8188 (Q4_0: 65504 / 8). D and DV are multiples of 32
- * up to 256; H % HK == 0; max_bias 0; KV * HK * (D + DV) / 32 < 2^30. A key that the mask hides from a
+ * up to 256; H % HK == 0; max_bias 0; KV * HK * (D + DV) / 32 < 2^29, and
+ * S * HK row tiles of 16 (T * H / HK rows), times nsplit, at most 2^21. A key that the mask hides from a
  * query (-inf) adds nothing to it, whatever the cache holds there, NaN included; a key with a scale
  * that is not finite makes the rows of the queries that see it NaN; rows whose every key is hidden are
  * written as zeros. q rows 16-byte, dst rows 16-byte (F16: 8), mask rows 8-byte aligned.

@@ -29,6 +29,14 @@ def test_rows_refusals(fn, bad):
 
 
 @pytest.mark.parametrize("fn", ["mi355x_set_rows", "mi355x_get_rows"])
+def test_rows_of_more_blocks_than_a_launch_counts(fn):
+    two = (mx.KvRows * 2)(*[rows(H=32, D=1024, nb1=1 << 15, nb2=1024, x_nb1=1 << 15, x_nb2=1024)] * 2)
+    assert getattr(mx.lib(), fn)(two, 2, FAKE, mx.I64, (1 << 19) + 1, None, None) == mx.E_ARG
+    one = (mx.KvRows * 1)(rows(H=1 << 15, D=16416, nb1=1 << 30, nb2=16416, x_nb1=1 << 30, x_nb2=16416))
+    assert getattr(mx.lib(), fn)(one, 1, FAKE, mx.I64, 1, None, None) == mx.E_ARG
+
+
+@pytest.mark.parametrize("fn", ["mi355x_set_rows", "mi355x_get_rows"])
 def test_rows_call_refusals(fn):
     f = getattr(mx.lib(), fn)
     one = (mx.KvRows * 1)(rows())
@@ -64,6 +72,7 @@ def fa(k=None, v=None, **kw):
 U, A = "E_UNSUPPORTED", "E_ARG"
 FA_REFUSALS = [(dict(D=48), U), (dict(D=0), U), (dict(DV=-32), U), (dict(D=576, DV=512), U), (dict(max_bias=8.0), U),
                (dict(k=dict(type=mx.F16)), U), (dict(v=dict(type=mx.Q4_K)), U), (dict(KV=1 << 30), U), (dict(T=1 << 20, H=4096), U),
+               (dict(S=1 << 20, HK=8), U), (dict(KV=1 << 18, HK=1 << 9, H=1 << 9), U),
                (dict(q_dev=None), A), (dict(dst_dev=None), A), (dict(q_dev=FAKE + 8), A), (dict(dst_dev=FAKE + 8), A),
                (dict(k=dict(q_dev=None)), A), (dict(v=dict(d_dev=None)), A), (dict(k=dict(q_dev=FAKE + 8)), A),
                (dict(v=dict(d_dev=FAKE + 4)), A), (dict(k=dict(nb1=100)), A), (dict(v=dict(nb2=-128)), A), (dict(k=dict(nb3=16)), A),

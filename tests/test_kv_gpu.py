@@ -139,6 +139,25 @@ def test_set_rows_repeated_and_foreign_indices(mx, t):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=ids)
+@pytest.mark.parametrize("wide", [False, True, None], ids=["int32", "int64", "all"])
+def test_set_rows_of_a_whole_context(mx, t, wide):
+    """More rows than one launch takes, into two caches, indices repeated near and far: the last row stays."""
+    n, rows, H, D = 40000, 45000, 2, 32
+    rng = np.random.default_rng(n)
+    x, y = (rng.standard_normal((n, H, D)).astype(np.float32) for _ in range(2))
+    at = np.arange(n) if wide is None else rng.integers(0, rows, n).astype(np.int64 if wide else np.int32)
+    c, f = noisy_cache(mx, t, rows, H, D), mx.kv_cache(mx.F16, rows, H, D)
+    q0, d0 = cpu(c.q).copy(), cpu(c.d).copy()
+    mx.set_rows([(c, gpu(x)), (f, gpu(y))], None if wide is None else gpu(at))
+    codes, d = R.quantize(x, t)
+    q0[at], d0[at] = codes, d          # numpy assigns in order: the last one stays
+    want = np.zeros((rows, H, D), np.float16)
+    want[at] = y.astype(np.float16)
+    assert np.array_equal(cpu(c.q), q0) and np.array_equal(cpu(c.d).view(np.uint16), d0.view(np.uint16))
+    assert np.array_equal(cpu(f.q), want)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=ids)
 def test_set_rows_special_blocks(mx, t):
     """Zeros, ties of both signs, halves between codes, magnitudes from f32's subnormals to past the
     scale's range, infinities and NaN, one kind a block."""
