@@ -395,6 +395,22 @@ def test_attention_ranges(mx, form, types, T):
         assert (np.abs(got[0] - want) <= tol + 2.0 ** -25).all(), (up, float((np.abs(got[0] - want) - tol).max()))
 
 
+@pytest.mark.parametrize("KV,heads", [(300, 1 << 16), (150, 1 << 17)])
+def test_attention_past_32_bit_offsets(mx, form, KV, heads):
+    """A cache whose keys lie 2^23 and 2^24 elements apart, past 2^31 of them in all, two of its heads in use."""
+    H, HK, D, T = 4, 2, 128, 3
+    rng = np.random.default_rng(KV)
+    q = rng.standard_normal((1, H, T, D)).astype(np.float32)
+    x, y = (rng.standard_normal((KV, HK, D)).astype(np.float32) for _ in range(2))
+    whole = mx.kv_cache(Q4_0, KV, heads, D)
+    k, v = whole[:, heads - 3:heads - 1], whole[:, 7:9]
+    mx.set_rows([(k, gpu(x)), (v, gpu(y))])
+    m = causal(T, KV)
+    kn, vn = (R.values(*R.quantize(p, Q4_0), Q4_0).transpose(1, 0, 2)[None] for p in (x, y))
+    got = cpu(mx.flash_attn_q(gpu(q[0]), k.permute(1, 0, 2), v.permute(1, 0, 2), gpu(m[0]), D ** -0.5))
+    check(got[None], q, kn, vn, m, D ** -0.5)
+
+
 def test_attention_no_keys(mx, form):
     """KV = 0: zeros."""
     import torch
