@@ -423,8 +423,10 @@ fa_q_kernel(FaQArgs a) {
     u32x4 koff = {kOffLo, kOffLo, kOffHi, kOffHi};
     float4v o[NQ][C::TT], oc[NQ][C::VJ];   // O^T without the offsets, and sum P d 2^k
     float m_run[NQ], l_run[NQ];
+    bool scaled[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
+        scaled[n] = __any(lqf[n * 16 + r] != 0.0f);
         m_run[n] = -INFINITY;
         l_run[n] = 0.0f;
 #pragma unroll
@@ -496,14 +498,13 @@ fa_q_kernel(FaQArgs a) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         dma_k(t2, BUF);
         half8 pf[NQ];
-        float dv[C::VS];
         {
             // ---- scale back, cap, mask, softmax ----
             const bool part = kb < FQ_KEYS * t;
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
-                const float qfac = lqf[n * 16 + r];
-                if (__any(qfac != 0.0f)) {
+                if (scaled[n]) {
+                    const float qfac = lqf[n * 16 + r];
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++)
 #pragma unroll
@@ -533,40 +534,9 @@ fa_q_kernel(FaQArgs a) {
                         for (int e = 0; e < 4; e++)
                             if (kb + 8 * g + 4 * hf + e < FQ_KEYS * t) sc[n][hf][e] = -INFINITY;
                 }
-                float mt = -INFINITY;
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mt = fmaxf(mt, sc[n][hf][e]);
-                if (__any(mt > m_run[n] + FQ_LAZY)) {
-                    mt = fq_col_max(mt);
-                    const float m_new = fmaxf(m_run[n], mt);
-                    const float alpha = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m_run[n] - m_new) * FQ_LOG2E);
-                    m_run[n] = m_new;
-                    l_run[n] *= alpha;
-#pragma unroll
-                    for (int q = 0; q < C::TT; q++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[n][q][e] *= alpha;
-#pragma unroll
-                    for (int j = 0; j < C::VJ; j++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) oc[n][j][e] *= alpha;
-                }
-                const float mb = m_run[n] == -INFINITY ? 0.0f : m_run[n] * FQ_LOG2E;
-                const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const half2v p = h2_of(pack2h(__builtin_amdgcn_exp2f(fmaf(sc[n][hf][e], FQ_LOG2E, -mb)),
-                                                      __builtin_amdgcn_exp2f(fmaf(sc[n][hf][e + 1], FQ_LOG2E, -mb))));
-                        pf[n][4 * hf + e] = p[0];
-                        pf[n][4 * hf + e + 1] = p[1];
-                        l_run[n] = __builtin_amdgcn_fdot2(p, one2, l_run[n], false);   // the sum of what is multiplied
-                    }
             }
-            // ---- V's scales (key lane / 2): the power of two they are held under ----
+            // ---- V's scales (key lane / 2): the power of two they are held under; into LDS times it ----
+            float dv[C::VS];
             uint16_t top = 0;
             bool bad = false;
 #pragma unroll
@@ -637,15 +607,49 @@ fa_q_kernel(FaQArgs a) {
                     }
                 }
             }
+#pragma unroll
+            for (int i = 0; i < C::VS; i++) wv[(half * C::VS + i) * FQ_KEYS + lane / 2] = f2h_bits(dv[i] * vscale);
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+                float mt = -INFINITY;
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mt = fmaxf(mt, sc[n][hf][e]);
+                if (__any(mt > m_run[n] + FQ_LAZY)) {
+                    mt = fq_col_max(mt);
+                    const float m_new = fmaxf(m_run[n], mt);
+                    const float alpha = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m_run[n] - m_new) * FQ_LOG2E);
+                    m_run[n] = m_new;
+                    l_run[n] *= alpha;
+#pragma unroll
+                    for (int q = 0; q < C::TT; q++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[n][q][e] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < C::VJ; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) oc[n][j][e] *= alpha;
+                }
+                const float mb = m_run[n] == -INFINITY ? 0.0f : m_run[n] * FQ_LOG2E;
+                const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const half2v p = h2_of(pack2h(__builtin_amdgcn_exp2f(fmaf(sc[n][hf][e], FQ_LOG2E, -mb)),
+                                                      __builtin_amdgcn_exp2f(fmaf(sc[n][hf][e + 1], FQ_LOG2E, -mb))));
+                        pf[n][4 * hf + e] = p[0];
+                        pf[n][4 * hf + e + 1] = p[1];
+                        l_run[n] = __builtin_amdgcn_fdot2(p, one2, l_run[n], false);   // the sum of what is multiplied
+                    }
+            }
         }
         asm volatile("" ::: "memory");
         load_side(x, t2);
         fq_wait_vm<C::KD + SL + C::VD + C::KD + SL>();   // this tile's V has landed
         {
-            // ---- V's scales into LDS, times 2^k ----
-#pragma unroll
-            for (int i = 0; i < C::VS; i++) wv[(half * C::VS + i) * FQ_KEYS + lane / 2] = f2h_bits(dv[i] * vscale);
-            asm volatile("" ::: "memory");
             // ---- O^T += V^T . P^T ----
 #pragma unroll
             for (int j = 0; j < C::VJ; j++) {
