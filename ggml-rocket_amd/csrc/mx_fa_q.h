@@ -42,7 +42,7 @@
 // share a wave; else every tile is read).
 //
 // Measured (this kernel; its merge is 4.2 us more where keys are split), 32 heads on 8 of head dim 128: one token
-// on 1000 Q8_0 keys 9.4 us, on 32768 Q4_0 keys 16.1 us (38 MB, 2.3 TB/s); 32 sequences of 4096 Q8_0 keys 67 us
+// on 1000 Q8_0 keys 9.3 us, on 32768 Q4_0 keys 15.9 us (38 MB, 2.4 TB/s); 32 sequences of 4096 Q8_0 keys 67 us
 // (286 MB, 4.3 TB/s, the rate of a plain read), of 1 to 4096 keys 55 us (143 MB: the longest's 16 tiles a
 // wave at 2.1 to 2.7 us each). A block's start until its first data is 3 to 5 us, its end 2.5 us. A tile at head dim
 // 128 in Q8_0, two waves a SIMD: 0.1 us waiting, 0.4 scores, 0.5 softmax and scales, 0.5 V, 0.6 requesting
