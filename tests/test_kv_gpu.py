@@ -28,8 +28,8 @@ def mx(torch_cuda):
 
 @pytest.fixture(params=["1 16", "1 32", "0 ", " "], ids=["direct", "direct32", "decoded", "chosen"])
 def form(request, monkeypatch):
-    """Attention tests run under every form (the kernel that reads the cache as it is stored, with 16 and with 32
-    rows a wave; the cache decoded to fp16 first, which is the fp16 kernel's arithmetic) and the library's
+    """Attention tests run under every form (the kernel that reads the cache as it is stored, with 16 and, at head
+    dims up to 64, with 32 rows a wave; the cache decoded to fp16 first, which is the fp16 kernel's arithmetic) and the library's
     choice per call."""
     direct, rows = request.param.split(" ")
     monkeypatch.setenv("MI355X_FA_Q_DIRECT", direct)
@@ -436,6 +436,29 @@ def test_attention_same_bits_and_same_as_a_decoded_cache(mx, form):
 
 
 # ---- together -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T,KV", [(1, 3000), (40, 700)])
+def test_attention_on_two_streams_at_once(mx, form, T, KV):
+    """Two calls in flight with a workspace each give the bits of one after the other."""
+    import torch
+    H, HK, D = 8, 2, 64
+    cases = [attn_case(mx, Q4_0, Q8_0, 1, T, H, HK, KV - 9 * i, D, D, seed=i) for i in range(2)]
+    masks = [gpu(causal(T, KV - 9 * i)) for i in range(2)]
+    qs = [gpu(c[0]) for c in cases]
+    alone = [cpu(mx.flash_attn_q(q, c[3], c[4], m, 0.125)) for q, c, m in zip(qs, cases, masks)]
+    outs = [torch.empty(1, T, H, D, device="cuda") for _ in range(2)]
+    spaces = [torch.empty(mx.flash_attn_q_workspace(q, c[3], c[4], m, o), dtype=torch.uint8, device="cuda")
+              for q, c, m, o in zip(qs, cases, masks, outs)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for st, q, c, m, o, w in zip(streams, qs, cases, masks, outs, spaces):
+            with torch.cuda.stream(st):
+                mx.flash_attn_q(q, c[3], c[4], m, 0.125, out=o, workspace=w)
+    torch.cuda.synchronize()
+    for o, a in zip(outs, alone):
+        assert np.array_equal(cpu(o), a)
+
 
 def test_decode_loop_on_another_stream_and_in_a_graph(mx, form):
     """A sequence grown as it would be: a prompt stored and attended to, then token by token, on a
