@@ -832,6 +832,7 @@ static FaQLayout fa_q_layout(const mi355x_fa_q_args * a, int nsplit) {
 
 MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int nsplit) {
     if (nsplit > 64 || fa_q_check(a, nsplit) != MI355X_OK) return 0;
+    if (a->T == 0 || a->S == 0) return 256;   // nothing to plan for; 0 would say that the op is not taken
     return fa_q_is_direct(a) ? fa_q_direct_layout(fa_q_direct(a, nsplit)).total : fa_q_layout(a, nsplit).total;
 }
 

@@ -369,7 +369,7 @@ typedef struct mi355x_fa_q_args {
 } mi355x_fa_q_args;
 
 /* Workspace bytes of mi355x_flash_attn_q with `nsplit` KV splits (0 = its own choice); 0 for an op it
- * does not take. 256-byte aligned. */
+ * does not take (an op without query rows or sequences is taken and needs next to none). 256-byte aligned. */
 MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int nsplit);
 
 /* mi355x_flash_attn with K and V in a quantized cache, each Q8_0 or Q4_0: dst = softmax(cap(scale *
