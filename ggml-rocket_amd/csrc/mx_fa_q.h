@@ -387,8 +387,9 @@ fa_q_kernel(FaQArgs a) {
             }
         amax = fq_col_max(amax);
         // a row outside [2^-6, 2^15] is divided by a factor that multiplies its scores (its largest value
-        // goes to 2^4, so that the smaller ones, and 1/16 of them, keep their bits)
-        const float qfac = (amax > 32768.0f || (amax < 0.015625f && amax > 0.0f)) ? amax / 16.0f : 1.0f;
+        // goes to 2^4, so that the smaller ones, and 1/16 of them, keep their bits); the factor has a finite
+        // reciprocal: values below 2^-116 then come out smaller than 2^4, and their scores are zero all the same
+        const float qfac = (amax > 32768.0f || (amax < 0.015625f && amax > 0.0f)) ? fmaxf(amax / 16.0f, 0x1p-120f) : 1.0f;
         const float inv = 1.0f / qfac;
 #pragma unroll
         for (int st = 0; st < C::KS; st++) {
