@@ -7,7 +7,7 @@
 // The T * G query rows of one KV head share its keys, so they are the columns of the products: a wave
 // takes 16 NQ rows and 32 keys at a time, in 16x16x32 MFMAs,
 //   S^T = K . Q^T    (A: 16 keys x one block of 32 dims, B: 32 dims x 16 rows)
-//   O^T += V^T . P^T (A: 16 dims x 32 keys, B: 32 keys x 16 rows)
+//   O^T += V^T . (P d)^T (A: 16 dims x 32 keys, B: 32 keys x 16 rows; d: V's scales of these dims' block)
 // with scores, softmax statistics and O in F32 and everything of a row in the four lanes of its
 // column. A wave is on its own until its keys are done: its tiles' codes come by LDS DMA into two buffers
 // of its own, so there are no barriers in the loop. (Loaded straight into the operands' lanes, where
@@ -18,8 +18,8 @@
 //   K   the lanes of group g hold bytes 8 g (Q8_0) or 4 g (Q4_0) on of every block of one key.
 //   P   the S^T accumulators of two 16-key products are the P^T operand: slot e of lane group g is key
 //       8 g + e, which product e / 4 has as its row 4 g + e % 4.
-//   V   the lane of group g reads the same few bytes of those eight keys; v_perm_b32 picks one byte of
-//       two keys into a pair of halves, which transposes V.
+//   V   ds_read_b64_tr_b8 hands a lane of group g one byte of each of those eight keys, and v_perm_b32 puts
+//       two of them into a pair of halves. The 16 dims of a product are 16 bytes of a row, of one block.
 //
 // What bounds it is the work of turning codes into operands, so that is kept to a few integer
 // instructions a pair: an unsigned code u = code + 128 (Q8_0) or u = code (Q4_0, value u - 8) in the low
@@ -27,10 +27,14 @@
 // in place counts 16 times; its Q is divided by 16 beforehand, its O afterwards.
 //   K   one product is one block, so its scale multiplies the F32 result (S += d S_b), and the offset
 //       is the product's start value, -128 (or -8) sum_dims q, a product of q with a constant: K is exact.
-//   V   the halves are multiplied by d 2^k, k such that the largest scale seen by the wave is just below
-//       2^15 (it moves rarely, and O with it); the offset leaves through one more product a group of dims
-//       with the scales themselves. A V is rounded once, relative to u: off by at most 2^-11 of 255 d
-//       (Q8_0) or 15 d (Q4_0), a sixteenth or less of half a quantization step.
+//   V   its scale multiplies P, once for a block's 32 dims, and the codes are exact. P d is held times 2^k, k such
+//       that the largest d of that block of dims that the wave has seen is just below 2^7 (P goes to 2^8, see below;
+//       k moves rarely, and O with it). The offset leaves at the end, as a multiple of the sum of the same P d.
+// Roundings: Q, P and P d, once each, to fp16, the matrix unit's operands (F32 ones would take two products for each).
+// Each is off by at most 2^-11 of itself; a P below 2^-14 by 2^-25, a P d by 2^-32 of the largest d of its dims. (With V's
+// scales multiplied into V's halves, under one power of two for all dims, values 2^13 below the largest were lost, and the
+// others rounded relative to their unsigned codes: 6e-4 of an output's norm from 64 bits; now 3.7e-4.)
+//
 // Scales go through a few bytes of LDS a wave, which turns a key's row of them into one block's of
 // several keys. The running maximum moves only when a score passes it by more than 8 in the exponent of 2
 // (P stays below 256, well inside fp16), so most tiles exchange nothing between lanes.
@@ -75,25 +79,24 @@ struct FqCfg {
     static constexpr int KCH = KRB / 16 <= 2 ? 2 : KRB / 16 <= 4 ? 4 : KRB / 16 <= 8 ? 8 : 16, VCH = VRB / 16;
     static constexpr int KD = KCH / 2, VD = VCH / 2;
     static constexpr int STAGE = FQ_KEYS * 16 * (KCH + VCH);
-    // Chunk c of K row r lies at c ^ kswz(r): the 16 rows that a read of one chunk takes then lie in 16
-    // different chunk slots of LDS's 256-byte window. K rows lie in the order 16 h + 4 g + e and V rows in the
-    // order 16 h + 4 e + g (key 8 g + 4 h + e), so that the four V rows a read takes are neighbours, and V's
-    // chunk c at c ^ vswz(g).
+    // Chunk c of row r lies at c ^ swz(r): the 16 rows that a read of one chunk takes then lie in 16
+    // different chunk slots of LDS's 256-byte window. K rows lie in the order 16 h + 4 g + e (key 8 g + 4 h + e),
+    // V rows in that of the keys.
     __device__ static __forceinline__ int kswz(int row) { return (row * KCH / 16) & (KCH - 1); }
-    __device__ static __forceinline__ int vswz(int g) { return VCH == 16 ? 4 * g : VCH == 8 ? 4 * (g / 2) : 0; }
-    static constexpr int VU = VT == T_Q8_0 || DV >= 128 ? 4 : 2;   // a lane's bytes of a V row: u, u + 16, ...
-    static constexpr int VJ = VRB / (16 * VU);
+    __device__ static __forceinline__ int vswz(int row) { return (row * VCH / 16) & (VCH - 1); }
     static constexpr int VH = VT == T_Q4_0 ? 2 : 1;           // nibbles a byte
-    static constexpr int TT = DV / 16;                        // O^T tiles, index (j * VU + byte) * VH + nibble
-    static_assert(KRB == 16 * KS * KW && VJ * VU * VH == TT, "layout");
+    static constexpr int VN = 4 / VH;                         // chunks of two of V's blocks, read at a time
+    static constexpr int TT = DV / 16;                        // O^T tiles of 16 dims: chunk * VH + nibble
+    static_assert(KRB == 16 * KS * KW && VCH * VH == TT, "layout");
     static constexpr int VB = DV / 32, VS = DV / 64, KSC = DK / 64;   // scales a key, and a lane (32 keys, two lanes each)
     static constexpr int KSL = KSC == 3 ? 4 : KSC, VSL = VS;  // and of a lane's load
     static constexpr int Q_LDS = NQ * (KS * 1024 + 64);       // Q as B operands, then its rows' factors
     static constexpr int SCALE_LDS = KS * FQ_KEYS * 4 + VB * FQ_KEYS * 2;   // a wave's scales: K's F32, V's F16
     static constexpr int WAVE_LDS = SCALE_LDS + 2 * STAGE;
-    // registers: O, scores and masks, the rest; the waves a SIMD they leave room for, and as many in a
-    // block, one block a CU, as the buffers leave room for
-    static constexpr int REGS = (TT + VJ) * 4 * NQ + 30 * NQ + KD + VD + KSC + VS + FQ_BASE_REGS;
+    // registers: O, scores and masks, a block of K and the offsets' product, the rest; the waves a SIMD they
+    // leave room for, and as many in a block, one block a CU, as the buffers leave room for (5 tokens on 16384 Q4_0
+    // keys of head dim 256: one wave a SIMD 28.4 us, two, which spill, 36.8)
+    static constexpr int REGS = (TT * 4 + VB) * NQ + 30 * NQ + KD + VD + 6 * KS + KSC + VS + FQ_BASE_REGS;
     static constexpr int WPE = REGS <= 128 ? 4 : REGS <= 168 ? 3 : REGS <= 256 ? 2 : 1;
     static constexpr int FIT = (FQ_LDS_MAX - Q_LDS) / WAVE_LDS / 4 * 4;
     static constexpr int NW = FIT < 4 * WPE ? FIT : 4 * WPE;
@@ -123,11 +126,29 @@ __device__ __forceinline__ void fq_wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// The element a lane's value i of O^T tile t is: its dim.
-__device__ __forceinline__ int fq_dim(int vt, int vu, int t, int g, int i) {
-    if (vt == T_Q8_0) return 64 * (t / 4) + 16 * g + 4 * i + t % 4;
-    const int hi = t % 2, n = (t / 2) % vu, j = t / 2 / vu;
-    return vu == 4 ? 32 * (g + 4 * j) + 4 * i + n + 16 * hi : 32 * (g / 2) + 8 * (g % 2) + 2 * i + n + 16 * hi;
+// Eight bytes a lane out of LDS, transposed, from N addresses (bytes of LDS, OFF further): of the 8 x 16 bytes whose row
+// i / 2 the lanes i of a group of 16 point at (the odd ones at its second half), lane i receives column i, row 0 lowest.
+// As one statement with its wait: before a builtin of them the compiler would wait for every LDS DMA under way.
+typedef int fq_v2i __attribute__((ext_vector_type(2)));
+template <int N, int OFF>
+__device__ __forceinline__ void fq_read_tr(const uint32_t (&a)[N], fq_v2i (&w)[N]) {
+    static_assert(N == 2 || N == 4, "chunks");
+    if constexpr (N == 2)
+        asm volatile("ds_read_b64_tr_b8 %0, %2 offset:%4\n"
+                     "ds_read_b64_tr_b8 %1, %3 offset:%4\n"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(w[0]), "=&v"(w[1])
+                     : "v"(a[0]), "v"(a[1]), "n"(OFF)
+                     : "memory");
+    else
+        asm volatile("ds_read_b64_tr_b8 %0, %4 offset:%8\n"
+                     "ds_read_b64_tr_b8 %1, %5 offset:%8\n"
+                     "ds_read_b64_tr_b8 %2, %6 offset:%8\n"
+                     "ds_read_b64_tr_b8 %3, %7 offset:%8\n"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3])
+                     : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF)
+                     : "memory");
 }
 
 // Maximum and sum over the four lanes of a column (l, l ^ 16, l ^ 32, l ^ 48), the same in each of them:
@@ -146,15 +167,18 @@ __device__ __forceinline__ float fq_col_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// The maximum over the wave, in every lane: four DPP steps inside the rows of 16, then across them.
-__device__ __forceinline__ float fq_wave_max(float x) {
+// The maximum over the wave's lanes of the same parity: three rotations of the rows of 16, then across them.
+__device__ __forceinline__ float fq_parity_max(float x) {
 #define FQ_DPP_MAX(CTRL) x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true)))
-    FQ_DPP_MAX(0xB1);    // quad_perm [1,0,3,2]
-    FQ_DPP_MAX(0x4E);    // quad_perm [2,3,0,1]
-    FQ_DPP_MAX(0x141);   // row_half_mirror
-    FQ_DPP_MAX(0x140);   // row_mirror
+    FQ_DPP_MAX(0x128);   // row_ror:8
+    FQ_DPP_MAX(0x124);   // row_ror:4
+    FQ_DPP_MAX(0x122);   // row_ror:2
 #undef FQ_DPP_MAX
     return fq_col_max(x);
+}
+// Lane l's value, the same in every lane.
+__device__ __forceinline__ float fq_lane(float x, int l) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l));
 }
 
 // A block's scale: held to the largest with which every value stays inside fp16 (kv_scale_limit), as
@@ -189,6 +213,13 @@ __device__ __forceinline__ half8 fq_key(const uint32_t * x) {
         w = u32x4{x[0] & 0x000F000Fu, y & 0x000F000Fu, x[0] & 0x00F000F0u, y & 0x00F000F0u};
     }
     return __builtin_bit_cast(half8, w);
+}
+
+// A lane's four dims from d on of an output row at dst, times inv.
+__device__ __forceinline__ void fq_store4(const FaQArgs & a, int64_t dst, int d, const float4v & v, float inv) {
+    if (d >= a.dv) return;
+    if (a.dst_f16) *(u32x2 *)((uint16_t *)a.dst + dst + d) = u32x2{pack2h(v[0] * inv, v[1] * inv), pack2h(v[2] * inv, v[3] * inv)};
+    else *(float4v *)((float *)a.dst + dst + d) = v * inv;
 }
 
 template <int KT, int VT, int DK, int DV, int NQ>
@@ -234,8 +265,8 @@ fa_q_kernel(FaQArgs a) {
     }
 #pragma unroll
     for (int q = 0; q < C::VD; q++) {
-        const int slot = q * WAVE + lane, pos = slot / C::VCH, c = (slot % C::VCH) ^ C::vswz(pos % 4);
-        const uint32_t key = pos % 4 * 8 + pos / 16 * 4 + pos % 16 / 4;
+        const int slot = q * WAVE + lane, c = (slot % C::VCH) ^ C::vswz(slot / C::VCH);
+        const uint32_t key = slot / C::VCH;
         vdma[q] = ((key * vnb) >> VSH) + (c * 16 < (a.dv >> VSH) ? 16 * c : 0);
     }
     // The scales this lane fetches: key lane / 2, half of its blocks, in one load that stays inside the row
@@ -244,20 +275,16 @@ fa_q_kernel(FaQArgs a) {
     const int kfirst = min(half * C::KSC, kn32 - C::KSL), vfirst = min(half * C::VS, vn32 - C::VSL);
     const uint32_t kdo = (uint32_t)(lane / 2) * (knb / 32 * 2) + 2 * kfirst, vdo = (uint32_t)(lane / 2) * (vnb / 32 * 2) + 2 * vfirst;
     const int ksh = min(16 * (half * C::KSC - kfirst), 63), vsh = min(16 * (half * C::VS - vfirst), 63);
-    // where this lane reads: bytes 4 KW g on of a K block (block i at kra ^ kra_i), its bytes of V row g
-    uint32_t kra = r * C::KCH * 16, vra[C::VJ];
+    // where this lane reads: bytes 4 KW g on of a K block (block i at kra ^ kra_i), and half a chunk of V row 8 g + r / 2
+    // (chunk c at vra ^ 16 c)
+    uint32_t kra = r * C::KCH * 16;
     kra += KT == T_Q8_0 ? ((C::kswz(r) ^ (g / 2)) << 4) + 8 * (g % 2) : (C::kswz(r) << 4) + 4 * g;
-    int vblk[C::VJ];                     // the block of its V bytes
-#pragma unroll
-    for (int j = 0; j < C::VJ; j++) {
-        const int u = (r + 16 * j) * C::VU;
-        vblk[j] = VT == T_Q8_0 ? u / 32 : u / 16;
-        vra[j] = g * C::VRB + (((u / 16) ^ C::vswz(g)) << 4) + u % 16;
-    }
+    const uint32_t vra = (8 * g + r / 2) * C::VRB + (C::vswz(8 * g + r / 2) << 4) + 8 * (r % 2);
 
     uint8_t * const wl = smem + C::Q_LDS + wave * C::WAVE_LDS;   // this wave's scales and buffers
+    const uint32_t vlds = (uint32_t)(uintptr_t)(fq_lptr_t)wl;    // its LDS address
     float * const wk = (float *)wl;                              // K scales [block][key]
-    uint16_t * const wv = (uint16_t *)(wk + C::KS * FQ_KEYS);    // V scales
+    uint16_t * const wv = (uint16_t *)(wk + C::KS * FQ_KEYS);    // V scales [block][key]
     auto dma_k = [&](int t, int buf) {
         const __amdgpu_buffer_rsrc_t kt = fq_rsrc(kq + ((min(FQ_KEYS * t, kb_last) * a.k.nb1) >> KSH));
         uint8_t * st = wl + C::SCALE_LDS + buf * C::STAGE;
@@ -422,7 +449,8 @@ fa_q_kernel(FaQArgs a) {
     // element, as bits of halves
     constexpr uint32_t kOffLo = KT == T_Q8_0 ? 0x80808080u : 0x80088008u, kOffHi = 0x80808080u;
     u32x4 koff = {kOffLo, kOffLo, kOffHi, kOffHi};
-    float4v o[NQ][C::TT], oc[NQ][C::VJ];   // O^T without the offsets, and sum P d 2^k
+    float4v o[NQ][C::TT];      // O^T without the offsets
+    float oc[NQ][C::VB];       // sum P d 2^k of each block, this lane's keys
     float m_run[NQ], l_run[NQ];
     bool scaled[NQ];
 #pragma unroll
@@ -433,10 +461,16 @@ fa_q_kernel(FaQArgs a) {
 #pragma unroll
         for (int t = 0; t < C::TT; t++) o[n][t] = float4v{0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < C::VJ; j++) oc[n][j] = float4v{0, 0, 0, 0};
+        for (int b = 0; b < C::VB; b++) oc[n][b] = 0.0f;
     }
-    float vscale = 1.0f;        // 2^k
-    uint32_t vtop = 0;          // the largest scale it is for, as bits: 2^(15 - k)
+    float vscale[C::VS];        // 2^k of this lane's blocks, half VS + i
+    uint32_t vtop[C::VS];       // the largest scale each is for, as fp16 bits: 2^(7 - k)
+#pragma unroll
+    for (int i = 0; i < C::VS; i++) {
+        vscale[i] = 1.0f;
+        vtop[i] = 0;
+    }
+    const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
     const float cap2 = a.softcap != 0.0f ? 2.0f * FQ_LOG2E / a.softcap : 0.0f;
 
     // Tile t in buffer BUF, with its scales and masks in x. Everything of a tile is requested two tiles ahead, each
@@ -450,7 +484,6 @@ fa_q_kernel(FaQArgs a) {
         fq_wait_vm<C::VD + C::KD + SL + C::VD>();
         const int kb = min(FQ_KEYS * t, kb_last);
         const uint8_t * const st = wl + C::SCALE_LDS + BUF * C::STAGE;
-        const uint8_t * const stv = st + FQ_KEYS * 16 * C::KCH;
         if constexpr (!C::KEEP_OFF) asm("" : "+v"(koff));   // else the offsets' products would move out of the loop
         float4v sc[NQ][2];
         {
@@ -498,7 +531,7 @@ fa_q_kernel(FaQArgs a) {
         const int t2 = k2 >= 0 ? tile0 + wave + NW * k2 : tn;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         dma_k(t2, BUF);
-        half8 pf[NQ];
+        u32x4 pf[NQ];   // P, fp16
         {
             // ---- scale back, cap, mask, softmax ----
             const bool part = kb < FQ_KEYS * t;
@@ -536,18 +569,17 @@ fa_q_kernel(FaQArgs a) {
                             if (kb + 8 * g + 4 * hf + e < FQ_KEYS * t) sc[n][hf][e] = -INFINITY;
                 }
             }
-            // ---- V's scales (key lane / 2): the power of two they are held under; into LDS times it ----
+            // ---- V's scales (key lane / 2): the power of two a block's are held under; into LDS times it ----
             float dv[C::VS];
-            uint16_t top = 0;
-            bool bad = false;
+            bool bad = false, larger = false;
 #pragma unroll
             for (int i = 0; i < C::VS; i++) {
                 const uint16_t bits = (uint16_t)((x.vd >> vsh) >> (16 * i));
                 bad |= (bits & 0x7C00u) == 0x7C00u;
                 dv[i] = fq_scale<VT>(bits, 0.0f);
-                top = max(top, (uint16_t)(bits & 0x7FFFu));
+                larger |= (bits & 0x7FFFu) > vtop[i];
             }
-            if (__any(top > vtop)) {
+            if (__any(larger)) {
                 // a larger scale than any before, or one that is not finite (which stands for zero and makes
                 // the row sums of the rows that see its key NaN); keys that no row sees count as zeros
                 bool hidden = false;
@@ -582,34 +614,36 @@ fa_q_kernel(FaQArgs a) {
                                 if (sc[n][e / 4][e % 4] != -INFINITY) l_run[n] = NAN;
                         }
                 }
-                float dmax = 0.0f;
 #pragma unroll
-                for (int i = 0; i < C::VS; i++) dmax = fmaxf(dmax, fabsf(dv[i]));
-                dmax = fq_wave_max(dmax);
-                // a power of two at least as large, by its exponent
-                const uint32_t pow2 = (__float_as_uint(dmax) + 0x7FFFFFu) & 0x7F800000u;
-                const float next_scale = dmax > 0.0f ? __uint_as_float((269u << 23) - pow2) : INFINITY;   // 2^15 / pow2
-                if (next_scale < vscale || vtop == 0) {
-                    const float f = vtop == 0 ? 1.0f : next_scale * __builtin_amdgcn_rcpf(vscale);   // powers of two: exact
-                    if (dmax > 0.0f) {
-                        vscale = next_scale;
-                        vtop = f2h_bits(__uint_as_float(pow2));
+                for (int i = 0; i < C::VS; i++) {
+                    const float dmax = fq_parity_max(fabsf(dv[i]));
+                    // a power of two at least as large, by its exponent
+                    const uint32_t pow2 = (__float_as_uint(dmax) + 0x7FFFFFu) & 0x7F800000u;
+                    const float next_scale = __uint_as_float((261u << 23) - pow2);   // 2^7 / pow2
+                    float f = 1.0f;
+                    if (dmax > 0.0f && (vtop[i] == 0 || next_scale < vscale[i])) {
+                        f = next_scale * __builtin_amdgcn_rcpf(vscale[i]);   // powers of two: exact
+                        vscale[i] = next_scale;
+                        vtop[i] = f2h_bits(__uint_as_float(pow2));
                     }
 #pragma unroll
-                    for (int n = 0; n < NQ; n++) {
+                    for (int hb = 0; hb < 2; hb++) {
+                        const int b = hb * C::VS + i;
+                        const float fb = fq_lane(f, hb);
 #pragma unroll
-                        for (int q = 0; q < C::TT; q++)
+                        for (int n = 0; n < NQ; n++) {
+                            oc[n][b] *= fb;
 #pragma unroll
-                            for (int e = 0; e < 4; e++) o[n][q][e] *= f;
-#pragma unroll
-                        for (int j = 0; j < C::VJ; j++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) oc[n][j][e] *= f;
+                            for (int e = 0; e < 4; e++) {
+                                o[n][2 * b][e] *= fb;
+                                o[n][2 * b + 1][e] *= fb;
+                            }
+                        }
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < C::VS; i++) wv[(half * C::VS + i) * FQ_KEYS + lane / 2] = f2h_bits(dv[i] * vscale);
+            for (int i = 0; i < C::VS; i++) wv[(half * C::VS + i) * FQ_KEYS + lane / 2] = f2h_bits(dv[i] * vscale[i]);
             asm volatile("" ::: "memory");
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
@@ -629,66 +663,55 @@ fa_q_kernel(FaQArgs a) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[n][q][e] *= alpha;
 #pragma unroll
-                    for (int j = 0; j < C::VJ; j++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) oc[n][j][e] *= alpha;
+                    for (int b = 0; b < C::VB; b++) oc[n][b] *= alpha;
                 }
                 const float mb = m_run[n] == -INFINITY ? 0.0f : m_run[n] * FQ_LOG2E;
-                const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const half2v p = h2_of(pack2h(__builtin_amdgcn_exp2f(fmaf(sc[n][hf][e], FQ_LOG2E, -mb)),
-                                                      __builtin_amdgcn_exp2f(fmaf(sc[n][hf][e + 1], FQ_LOG2E, -mb))));
-                        pf[n][4 * hf + e] = p[0];
-                        pf[n][4 * hf + e + 1] = p[1];
-                        l_run[n] = __builtin_amdgcn_fdot2(p, one2, l_run[n], false);   // the sum of what is multiplied
-                    }
+                for (int e = 0; e < 4; e++) {
+                    const float s0 = sc[n][e / 2][2 * (e % 2)], s1 = sc[n][e / 2][2 * (e % 2) + 1];
+                    pf[n][e] = pack2h(__builtin_amdgcn_exp2f(fmaf(s0, FQ_LOG2E, -mb)), __builtin_amdgcn_exp2f(fmaf(s1, FQ_LOG2E, -mb)));
+                    l_run[n] = __builtin_amdgcn_fdot2(h2_of(pf[n][e]), one2, l_run[n], false);   // the sum of what is multiplied
+                }
             }
         }
         asm volatile("" ::: "memory");
         load_side(x, t2);
         fq_wait_vm<C::KD + SL + C::VD + C::KD + SL>();   // this tile's V has landed
         {
-            // ---- O^T += V^T . P^T ----
+            // ---- O^T += V^T . (P d 2^k)^T, two blocks of 32 dims at a time ----
 #pragma unroll
-            for (int j = 0; j < C::VJ; j++) {
-                half2v d[4];
-                {
-                    const u32x4 w = *(const u32x4 *)(wv + vblk[j] * FQ_KEYS + 8 * g);
-                    d[0] = h2_of(w[0]);
-                    d[1] = h2_of(w[1]);
-                    d[2] = h2_of(w[2]);
-                    d[3] = h2_of(w[3]);
-                }
-                const half8 ds = __builtin_bit_cast(half8, u32x4{u_of(d[0]), u_of(d[1]), u_of(d[2]), u_of(d[3])});
+            for (int c0 = 0; c0 < C::VCH; c0 += C::VN) {
+                const uint16_t * const wd = wv + c0 * C::VH / 2 * FQ_KEYS + 8 * g;
+                const u32x4 d[2] = {*(const u32x4 *)wd, *(const u32x4 *)(wd + FQ_KEYS)};
+                uint32_t va[C::VN];
+                fq_v2i w[C::VN];
 #pragma unroll
-                for (int nq = 0; nq < NQ; nq++) oc[nq][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ds, pf[nq], oc[nq][j], 0, 0, 0);
-                uint32_t xe[8];
+                for (int c = 0; c < C::VN; c++) va[c] = vlds + (vra ^ (uint32_t)(16 * (c0 + c)));
+                fq_read_tr<C::VN, C::SCALE_LDS + BUF * C::STAGE + FQ_KEYS * 16 * C::KCH>(va, w);
+                u32x4 pd[NQ];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint8_t * p = stv + vra[j] + (e / 4 * 16 + e % 4 * 4) * C::VRB;
-                    if constexpr (C::VU == 4) xe[e] = *(const uint32_t *)p;
-                    else xe[e] = *(const uint16_t *)p;
-                    if constexpr (VT == T_Q8_0) xe[e] ^= 0x80808080u;
-                }
+                for (int c = 0; c < C::VN; c++) {
+                    const int b = (c0 + c) * C::VH / 2;
+                    if ((c0 + c) * C::VH % 2 == 0) {   // a block's first chunk
 #pragma unroll
-                for (int n = 0; n < C::VU; n++) {
-                    uint32_t y[4];   // byte n of keys (2 e, 2 e + 1), zero-extended
+                        for (int n = 0; n < NQ; n++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        y[e] = __builtin_amdgcn_perm(xe[2 * e + 1], xe[2 * e], 0x0C000C00u | ((uint32_t)(4 + n) << 16) | (uint32_t)n);
+                            for (int e = 0; e < 4; e++) {
+                                pd[n][e] = u_of(h2_of(pf[n][e]) * h2_of(d[b % 2][e]));
+                                oc[n][b] = __builtin_amdgcn_fdot2(h2_of(pd[n][e]), one2, oc[n][b], false);
+                            }
+                    }
+                    const uint32_t flip = VT == T_Q8_0 ? 0x80808080u : 0u, xl = (uint32_t)w[c][0] ^ flip, xh = (uint32_t)w[c][1] ^ flip;
+                    // bytes of keys (2 e, 2 e + 1), zero-extended
+                    const u32x4 y = {__builtin_amdgcn_perm(0u, xl, 0x0C010C00u), __builtin_amdgcn_perm(0u, xl, 0x0C030C02u),
+                                     __builtin_amdgcn_perm(0u, xh, 0x0C010C00u), __builtin_amdgcn_perm(0u, xh, 0x0C030C02u)};
 #pragma unroll
                     for (int h = 0; h < C::VH; h++) {
-                        u32x4 w;
+                        const u32x4 u = VT == T_Q8_0 ? y : h ? y & 0x00F000F0u : y & 0x000F000Fu;
+                        const int q = (c0 + c) * C::VH + h;
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            w[e] = u_of(h2_of(VT == T_Q8_0 ? y[e] : y[e] & (h ? 0x00F000F0u : 0x000F000Fu)) * d[e]);
-                        const int q = (j * C::VU + n) * C::VH + h;
-#pragma unroll
-                        for (int nq = 0; nq < NQ; nq++)
-                            o[nq][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), pf[nq], o[nq][q], 0, 0, 0);
+                        for (int n = 0; n < NQ; n++)
+                            o[n][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, u), __builtin_bit_cast(half8, pd[n]), o[n][q], 0, 0, 0);
                     }
                     if (!C::KEEP_OFF) __builtin_amdgcn_sched_barrier(0);
                 }
@@ -713,6 +736,8 @@ fa_q_kernel(FaQArgs a) {
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         l_run[n] = fq_col_sum(l_run[n]);
+#pragma unroll
+        for (int b = 0; b < C::VB; b++) oc[n][b] = fq_col_sum(oc[n][b]);
         if (g == 0) {
             sml[((wave * NQ + n) * 16 + r) * 2] = m_run[n];
             sml[((wave * NQ + n) * 16 + r) * 2 + 1] = l_run[n];
@@ -755,7 +780,8 @@ fa_q_kernel(FaQArgs a) {
             float4v v = o[n][q];
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                v[e] = fmaf(oc[n][q / (C::TT / C::VJ)][e], -kOff, v[e] * (high ? 1048576.0f : 16777216.0f)) * (wgt[n] * __builtin_amdgcn_rcpf(vscale));
+                v[e] = fmaf(oc[n][q / 2], -kOff, v[e] * (high ? 1048576.0f : 16777216.0f)) *
+                       (wgt[n] * __builtin_amdgcn_rcpf(fq_lane(vscale[q / 2 % C::VS], q / 2 / C::VS)));
             so[(wave * C::CT + i) * WAVE + lane] = v;
         }
         __syncthreads();
@@ -781,14 +807,7 @@ fa_q_kernel(FaQArgs a) {
             const float inv = Ln == 0.0f ? 0.0f : 1.0f / Ln;   // no key seen: zeros; a NaN stays
             const int tk = fq_div(row, a.div_g);
             const int64_t dst = (int64_t)s * a.dst_nb3 + (int64_t)tk * a.dst_nb2 + (int64_t)(hk * a.G + row - tk * a.G) * a.dst_nb1;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int d = fq_dim(VT, C::VU, q, g, e);
-                if (d < a.dv) {
-                    if (a.dst_f16) ((uint16_t *)a.dst)[dst + d] = f2h_bits(v[e] * inv);
-                    else ((float *)a.dst)[dst + d] = v[e] * inv;
-                }
-            }
+            fq_store4(a, dst, 16 * q + 4 * g, v, inv);
         }
     }
 }
@@ -808,7 +827,7 @@ static hipError_t fq_launch(const FaQArgs & a, hipStream_t st) {
     hipLaunchKernelGGL((fa_q_kernel<KT, VT, DK, DV, NQ>), dim3((unsigned)(units * a.nsplit)), dim3(C::NW * WAVE), C::LDS, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
-    return launch_fa_q_combine(a, VT, DV, NQ, st);
+    return launch_fa_q_combine(a, DV, NQ, st);
 }
 
 template <int KT, int VT, int DK, int DV>

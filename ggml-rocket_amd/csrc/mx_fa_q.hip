@@ -9,7 +9,7 @@ namespace mx {
 // formed while they come: one memory round trip. Rows whose maxima are all -inf have sums of zero (or
 // NaN, kept).
 constexpr int FQ_MAX_SPLIT = 64;
-__global__ void __launch_bounds__(256) fa_q_combine_kernel(FaQArgs a, int vt, int DV, int NQ) {
+__global__ void __launch_bounds__(256) fa_q_combine_kernel(FaQArgs a, int DV, int NQ) {
     __shared__ float sm[16][17], sl[16][17], sw[FQ_MAX_SPLIT][16];
     __shared__ float4v so[4][WAVE];
     const int t = threadIdx.x, lane = t % WAVE, wave = t / WAVE, r = lane % 16, g = lane / 16;
@@ -72,20 +72,12 @@ __global__ void __launch_bounds__(256) fa_q_combine_kernel(FaQArgs a, int vt, in
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const int tk = fq_div(row, a.div_g);
     const int64_t dst = (int64_t)s * a.dst_nb3 + (int64_t)tk * a.dst_nb2 + (int64_t)(hk * a.G + row - tk * a.G) * a.dst_nb1;
-    const int vu = vt == T_Q8_0 || DV >= 128 ? 4 : 2;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const int d = fq_dim(vt, vu, q, g, e);
-        if (d < a.dv) {
-            if (a.dst_f16) ((uint16_t *)a.dst)[dst + d] = f2h_bits(v[e] * inv);
-            else ((float *)a.dst)[dst + d] = v[e] * inv;
-        }
-    }
+    fq_store4(a, dst, 16 * q + 4 * g, v, inv);
 }
 
-hipError_t launch_fa_q_combine(const FaQArgs & a, int vt, int DV, int NQ, hipStream_t st) {
+hipError_t launch_fa_q_combine(const FaQArgs & a, int DV, int NQ, hipStream_t st) {
     const int64_t units = (int64_t)a.S * a.HK * a.nrt;
-    hipLaunchKernelGGL(fa_q_combine_kernel, dim3((unsigned)(units * (DV / 16) * NQ)), dim3(256), 0, st, a, vt, DV, NQ);
+    hipLaunchKernelGGL(fa_q_combine_kernel, dim3((unsigned)(units * (DV / 16) * NQ)), dim3(256), 0, st, a, DV, NQ);
     return hipGetLastError();
 }
 

@@ -109,7 +109,7 @@ constexpr int FA_Q_MIN_KV = 32;             // a tile
 constexpr int64_t FA_Q_MAX_NB1 = 1 << 24;   // its 32-bit offsets inside a tile
 inline int fa_q_max_nq(int D) { return D == 64 ? 2 : 1; }
 hipError_t launch_fa_q(const FaQArgs & a, hipStream_t st);
-hipError_t launch_fa_q_combine(const FaQArgs & a, int vt, int DV, int NQ, hipStream_t st);
+hipError_t launch_fa_q_combine(const FaQArgs & a, int DV, int NQ, hipStream_t st);
 hipError_t launch_fa_q_Q8_0_Q8_0(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_q_Q8_0_Q4_0(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_q_Q4_0_Q8_0(const FaQArgs & a, hipStream_t st);

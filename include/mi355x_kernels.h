@@ -373,9 +373,11 @@ typedef struct mi355x_fa_q_args {
 MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int nsplit);
 
 /* mi355x_flash_attn with K and V in a quantized cache, each Q8_0 or Q4_0: dst = softmax(cap(scale *
- * q.k) + mask) . v. K and V enter the products as fp16 (their values rounded once), Q and P as fp16,
- * sums in F32: an F32 dst holds values of that accuracy. So that the values stay inside fp16, a scale
- * counts as at most 515.5 (Q8_0: 65468 / 127) or 8188 (Q4_0: 65504 / 8). D and DV are multiples of 32
+ * q.k) + mask) . v. The products' operands are fp16, rounded once, sums F32: Q and P in both forms below, K's and
+ * V's values where the cache is decoded first, P times the scale of V's block where it is read as stored (that product
+ * is also off by up to 2^-32 of the largest scale of its 32 dims). An F32 dst holds values of that accuracy, some 4e-4 of an
+ * output's norm. So that the values stay inside fp16, a scale counts as at most 515.5 (Q8_0: 65468 / 127) or 8188 (Q4_0:
+ * 65504 / 8). D and DV are multiples of 32
  * up to 256; H % HK == 0; max_bias 0; KV * HK * (D + DV) / 32 < 2^29, and
  * S * HK row tiles of 16 (T * H / HK rows), times nsplit, at most 2^21. A key that the mask hides from a
  * query (-inf) adds nothing to it, whatever the cache holds there, NaN included; a key with a scale
