@@ -11,6 +11,7 @@ There is no fallback: if the shared library is missing, `lib()` raises.
 from __future__ import annotations
 
 import ctypes
+import numbers
 import os
 import struct
 
@@ -376,9 +377,10 @@ class KvCache:
         return KvCache(self.type, self.q.permute(*dims), None if self.d is None else self.d.permute(*dims))
 
     def __getitem__(self, at):
-        """A view by indices and slices of leading dims."""
-        if isinstance(at, tuple) and (len(at) >= len(self.shape) or any(i is Ellipsis or i is None for i in at)):
-            raise MI355XError("KvCache: indices of leading dims only")
+        """A view by integers and slices of leading dims. Lists and tensors, which would copy, are refused."""
+        ats = at if isinstance(at, tuple) else (at,)
+        if len(ats) >= len(self.shape) or not all(isinstance(i, slice) or (isinstance(i, numbers.Integral) and not isinstance(i, bool)) for i in ats):
+            raise MI355XError("KvCache: integers and slices of leading dims only")
         return KvCache(self.type, self.q[at], None if self.d is None else self.d[at])
 
 
