@@ -643,8 +643,9 @@ MI355X_API int mi355x_flash_attn_ex(const mi355x_fa_args * a, int nsplit, int fl
 
 static bool kv_type(int t) { return t == mx::T_Q8_0 || t == mx::T_Q4_0; }
 
+// store: the caches are written, else the plain rows
 static int kv_rows_lower(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n, int32_t * err_dev,
-                         mx::KvRowsArgs & a) {
+                         bool store, mx::KvRowsArgs & a) {
     if (!r || n_out < 1 || n_out > mx::KV_MAX_OUT || n < 0 || n > (1 << 30)) return MI355X_E_ARG;
     if (idx_type != 26 && idx_type != 27) return MI355X_E_ARG;
     if (!aligned(idx_dev, idx_type == 27 ? 8 : 4) || !aligned(err_dev, 4)) return MI355X_E_ARG;
@@ -660,6 +661,8 @@ static int kv_rows_lower(const mi355x_kv_rows * r, int n_out, const void * idx_d
         if (n > 0 && (!s.q_dev || !s.x_dev || !aligned(s.q_dev, 16) || !aligned(s.x_dev, 16))) return MI355X_E_ARG;
         if (n > 0 && s.type != mx::T_F16 && (!s.d_dev || !aligned(s.d_dev, 8))) return MI355X_E_ARG;
         if (!idx_dev && n > s.n_rows) return MI355X_E_ARG;
+        for (int j = 0; j < k && n > 0; j++)   // one destination twice: written in no order
+            if (store ? r[j].q_dev == s.q_dev : r[j].x_dev == s.x_dev) return MI355X_E_ARG;
         const int64_t bpr = s.H * (s.D / 32);
         if (bpr > (1 << 24) || (blocks += n * bpr) > (1 << 30)) return MI355X_E_ARG;
         mx::KvRowsOut & o = a.o[k];
@@ -674,14 +677,14 @@ static int kv_rows_lower(const mi355x_kv_rows * r, int n_out, const void * idx_d
 MI355X_API int mi355x_set_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
                                int32_t * err_dev, void * stream) {
     mx::KvRowsArgs a;
-    const int st = kv_rows_lower(r, n_out, idx_dev, idx_type, n, err_dev, a);
+    const int st = kv_rows_lower(r, n_out, idx_dev, idx_type, n, err_dev, true, a);
     return st != MI355X_OK || n == 0 ? st : hip_status(mx::launch_set_rows(a, S(stream)));
 }
 
 MI355X_API int mi355x_get_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
                                int32_t * err_dev, void * stream) {
     mx::KvRowsArgs a;
-    const int st = kv_rows_lower(r, n_out, idx_dev, idx_type, n, err_dev, a);
+    const int st = kv_rows_lower(r, n_out, idx_dev, idx_type, n, err_dev, false, a);
     return st != MI355X_OK || n == 0 ? st : hip_status(mx::launch_get_rows(a, S(stream)));
 }
 

@@ -336,6 +336,7 @@ typedef struct mi355x_kv_rows {
  * truncated, at most 15), each step rounded to f32, d stored as fp16 (infinite past 65504, as
  * ggml's). A block that holds a NaN or an infinity, for which ggml defines nothing, is stored with
  * a NaN scale and reads back as NaN. F16: round to nearest even.
+ * Caches of one call must not overlap (two at one address are refused; mi355x_get_rows: nor their x).
  * n and n * H * D / 32, summed over the caches, are at most 2^30, H * D / 32 at most 2^24. One launch for
  * every 16384 rows.
  * No counterpart in the reference, whose host writes its caches on the CPU. */
