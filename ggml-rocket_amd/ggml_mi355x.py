@@ -453,6 +453,8 @@ def set_rows(pairs, idx=None, err=None):
     """pairs: (cache, x) for up to four caches [rows, H, D] (or [rows, D]) and plain rows x [n, H, D]
     (F32 or F16): x[i] is quantized into cache row idx[i] (int32 or int64 [n]; None: i). One launch.
     err: a device int32 that an index out of range sets to 1."""
+    if not pairs:
+        raise MI355XError("set_rows: one to four caches")
     caches, plain = zip(*pairs)
     dev = caches[0].dev
     ip, it, n = _kv_index(idx, plain[0].shape[0], dev, "set_rows")
@@ -465,6 +467,8 @@ def set_rows(pairs, idx=None, err=None):
 def get_rows(caches, idx=None, dtype=None, out=None, err=None):
     """Rows idx[i] (None: all, in order) of each of up to four caches as plain values: a list of
     [n, H, D] (or [n, D]) tensors of `dtype` (F32 by default), or `out`. One launch."""
+    if not caches:
+        raise MI355XError("get_rows: one to four caches")
     dev = caches[0].dev
     ip, it, n = _kv_index(idx, caches[0].shape[0], dev, "get_rows")
     if any(c.dev != dev for c in caches):

@@ -1,5 +1,5 @@
-"""Attention over a quantized cache with nothing to do: no query rows or no sequences (CPU; the refusals' own
-operands, never dereferenced)."""
+"""The quantized cache's calls with nothing to do: attention of no query rows or no sequences (CPU; the refusals' own
+operands, never dereferenced), rows of no cache."""
 import ctypes
 
 import pytest
@@ -36,3 +36,14 @@ def test_attention_of_nothing(torch_cuda, monkeypatch, form, lead, T):
     out = mx.flash_attn_q(q, kc, vc, None, 0.125)
     assert out.shape == (*lead, T, H, D)
     torch.cuda.synchronize()
+
+
+def test_no_caches():
+    for f in (lambda: mx.set_rows([]), lambda: mx.get_rows([])):
+        with pytest.raises(mx.MI355XError):
+            f()
+    import torch
+    c = mx.kv_cache(mx.Q8_0, 4, 2, 64, device="cpu")
+    x = torch.zeros(2, 2, 64)
+    with pytest.raises(mx.MI355XError):
+        mx.set_rows([(c, x)] * 5)
