@@ -707,8 +707,13 @@ static int fa_q_check(const mi355x_fa_q_args * a, int nsplit) {
     }
     if (a->T < 0 || a->S < 0 || a->H <= 0 || a->HK <= 0 || a->KV < 0 || a->H % a->HK) return MI355X_E_ARG;
     if ((int64_t)a->KV * a->HK * ((a->D + a->DV) / 32) >= 1 << 29) return MI355X_E_UNSUPPORTED;
-    // threads of a launch: 16 rows of a sequence and KV head, up to 1024 threads and 64 splits
-    if ((int64_t)a->S * a->HK * (((int64_t)a->T * (a->H / a->HK) + 15) / 16) > (1 << 21) / (nsplit > 1 ? nsplit : 1)) return MI355X_E_UNSUPPORTED;
+    // threads of a launch: row tiles of 16 rows of a sequence and KV head, up to 1024 threads and 64 splits; where keys
+    // are split, 256 threads a tile and 16 (built) dims merge them, and 2^32 threads are too many
+    const int64_t tiles = (int64_t)a->S * a->HK * (((int64_t)a->T * (a->H / a->HK) + 15) / 16);
+    if (tiles > (1 << 21) / (nsplit > 1 ? nsplit : 1)) return MI355X_E_UNSUPPORTED;
+    int D, DV;
+    mx::fa_pad_dims(a->D, a->DV, D, DV);
+    if (nsplit > 1 && tiles * DV >= 1 << 28) return MI355X_E_UNSUPPORTED;
     if ((int64_t)a->S * a->T * a->H > (1 << 30) || (size_t)a->KV > mx::fa_max_kv(a->D, a->DV)) return MI355X_E_UNSUPPORTED;
     for (int t : {a->q_type, a->dst_type})
         if (t != mx::T_F32 && t != mx::T_F16) return MI355X_E_ARG;

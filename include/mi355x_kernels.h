@@ -380,7 +380,8 @@ MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int 
  * output's norm. So that the values stay inside fp16, a scale counts as at most 515.5 (Q8_0: 65468 / 127) or 8188 (Q4_0:
  * 65504 / 8). D and DV are multiples of 32
  * up to 256; H % HK == 0; max_bias 0; KV * HK * (D + DV) / 32 < 2^29, and
- * S * HK row tiles of 16 (T * H / HK rows), times nsplit, at most 2^21. A key that the mask hides from a
+ * S * HK row tiles of 16 (T * H / HK rows), times nsplit, at most 2^21 (with nsplit > 1, tiles times DV also below 2^28, DV
+ * counted as 64, 128 or 256). A key that the mask hides from a
  * query (-inf) adds nothing to it, whatever the cache holds there, NaN included; a key with a scale
  * that is not finite makes the rows of the queries that see it NaN; rows whose every key is hidden are
  * written as zeros. q rows 16-byte, dst rows 16-byte (F16: 8), mask rows 8-byte aligned.
