@@ -9,8 +9,8 @@
 //
 // Both are streams: bound by HBM for many rows and by a launch's latency for few. A block of 32 is
 // the work of four lanes, a quad: lane l takes values 4l..4l+3 and 16+4l..16+4l+3, so it holds the
-// two halves of its four Q4_0 bytes, reads 16-byte pieces, and finds the block's maximum with two
-// DPP exchanges inside the quad. Reading back, lane l takes values 8l..8l+7, one 16-byte store of fp16
+// two halves of its four Q4_0 bytes, reads pieces of 16 bytes (F32) or 8 (F16), and finds the block's maximum with
+// two DPP exchanges inside the quad. Reading back, lane l takes values 8l..8l+7, one 16-byte store of fp16
 // (its Q4_0 nibbles are the low or the high ones of eight bytes that two lanes read).
 
 #include <type_traits>

@@ -451,8 +451,8 @@ def _kv_err(err, dev, what):
 
 def set_rows(pairs, idx=None, err=None):
     """pairs: (cache, x) for up to four caches [rows, H, D] (or [rows, D]) and plain rows x [n, H, D]
-    (F32 or F16): x[i] is quantized into cache row idx[i] (int32 or int64 [n]; None: i). One launch.
-    err: a device int32 that an index out of range sets to 1."""
+    (F32 or F16): x[i] is quantized into cache row idx[i] (int32 or int64 [n]; None: i), one launch
+    for every 16384 rows. err: a device int32 that an index out of range sets to 1. The caches must not overlap."""
     if not pairs:
         raise MI355XError("set_rows: one to four caches")
     caches, plain = zip(*pairs)

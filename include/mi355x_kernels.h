@@ -326,8 +326,8 @@ typedef struct mi355x_kv_rows {
 } mi355x_kv_rows;
 
 /* ggml's SET_ROWS into a cache: row i of the plain values of each of `n_out` (1..4) caches is
- * quantized and written to cache row idx[i], for every i < n, all caches in one launch (a layer's K and V
- * share their indices). idx_dev: int32 (idx_type 26) or int64 (27) [n] on the device, or NULL for idx[i] = i.
+ * quantized and written to cache row idx[i], for every i < n, all caches in the same launches (a layer's K and V
+ * share their indices), one for every 16384 rows. idx_dev: int32 (idx_type 26) or int64 (27) [n] on the device, or NULL for idx[i] = i.
  * Where an index repeats, the row with the largest i stays, whole. An index outside [0, n_rows)
  * writes nothing and sets *err_dev (a device int32, may be NULL) to 1. Rows that no index names keep
  * their bytes.
@@ -337,8 +337,7 @@ typedef struct mi355x_kv_rows {
  * ggml's). A block that holds a NaN or an infinity, for which ggml defines nothing, is stored with
  * a NaN scale and reads back as NaN. F16: round to nearest even.
  * Caches of one call must not overlap (two at one address are refused; mi355x_get_rows: nor their x).
- * n and n * H * D / 32, summed over the caches, are at most 2^30, H * D / 32 at most 2^24. One launch for
- * every 16384 rows.
+ * n and n * H * D / 32, summed over the caches, are at most 2^30, H * D / 32 at most 2^24.
  * No counterpart in the reference, whose host writes its caches on the CPU. */
 MI355X_API int mi355x_set_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
                                int32_t * err_dev, void * stream);
