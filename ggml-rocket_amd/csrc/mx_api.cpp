@@ -763,9 +763,9 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
     f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
     // Keys are split while compute units are idle, four tiles a block at least, and not at all up to 16 tiles,
     // which a block's waves take at once or twice: the second launch costs more (us whole, in splits of eight
-    // tiles and of four: 300 keys 11.2, 11.2, 13.4; 1000 16.1, 13.6, 13.3; 4000 38, 15.7, 15.1; 1000 at
-    // head dim 256 33, 20.9, 18.4). Never past one block a compute unit (32 sequences of 4096 keys, 256 blocks:
-    // 70 whole, 82 in two splits; of different lengths 53 and 67).
+    // tiles and of four, Q8_0: 300 keys 11.2, 11.3, 13.1; 1000 15.6, 13.2, 13.0; 4000 35, 15.1, 14.9; 1000 at
+    // head dim 256 33, 19.2, 16.2). Never past one block a compute unit (32 sequences of 4096 keys, 256 blocks:
+    // 69 whole, 79 in two splits; of different lengths 50 and 60).
     const int64_t cus = device_cus(), ntiles = (f.KV + 31) / 32;
     auto units = [&](int nq) { return (int64_t)f.S * f.HK * ((f.R + 16 * nq - 1) / (16 * nq)); };
     auto splits = [&](int nq) {
@@ -774,8 +774,8 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
     // Two row tiles a wave (head dim 64) share the work of turning codes into operands: a key tile takes 1.75 times
     // as long as with one, and a block's start and end, which take as long as 60 key tiles, 85. They are taken
     // where a compute unit is done sooner (4-bit, 8 KV heads, us with one and two: 256 rows of 16384
-    // keys 44 / 40, 512 69 / 64; 512 of 4096 26 / 29; 400 of 1531 16 / 20, 800 29 / 21). At head dim 128 their
-    // registers leave one wave a SIMD, which is never less time (128 rows of 32768 keys 66 / 86).
+    // keys 47 / 45, 512 73 / 70; 512 of 4096 26 / 29; 400 of 1531 16 / 20, 800 28 / 22). At head dim 128 their
+    // registers leave one wave a SIMD, which was never less time (128 rows of 32768 keys 66 / 86).
     auto cost = [&](int nq) {
         const int64_t n = splits(nq), tiles = (ntiles + n - 1) / n;
         return (units(nq) * n + cus - 1) / cus * (nq == 2 ? 7 * tiles + 340 : 4 * tiles + 240);
@@ -794,12 +794,14 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
 
 // The direct form or decoding first. Direct attention turns codes into operands once for every 16 or 32
 // rows, and with many rows that, not the memory, is its time; decoding turns them once and feeds the F16
-// kernel, one sequence after another, in two or three launches and 21 us at least. Direct up to R (D + DV) = 2^16
-// (us direct / decoded, 8 KV heads, head dim 128: 128 rows of 8192 keys 30 / 42, 256 45 / 44, 384 68 / 51;
-// 256 of 32768 115 / 127, 384 210 / 144; head dim 256, 16384 keys: 128 rows 94 / 149, 192 171 / 147), and up
+// kernel, one sequence after another, in two or three launches and 14 us at least each. Direct up to R (D + DV) = 2^16
+// (us direct / decoded, 8 KV heads, 4-bit, head dim 128: 128 rows of 8192 keys 28 / 43, 256 42 / 45, 384 61 / 52;
+// 256 of 32768 115 / 126, 384 207 / 143; head dim 256, 16384 keys: 128 rows 95 / 148, 192 171 / 147), and up
 // to 64 key tiles of 16 rows a compute unit and sequence, which are done before those launches are (512 rows of
-// 1000 keys 19 / 25, 768 33 / 25; head dim 64, 1531 keys: 400 rows 16 / 22, 800 21 / 24; head dim 256, 1000
-// keys, 512 rows 35 / 72; 32 sequences x 256 rows x 1024 213 / 639).
+// 1000 keys 17 / 25, 768 29 / 25; head dim 64, 1531 keys: 400 rows 16 / 23, 800 22 / 24; head dim 256, 1000
+// keys, 512 rows 36 / 71; 32 sequences x 256 rows x 1024 187 / 641).
+// Fewer keys than a tile's 32, whose loads the direct form does not bound a lane at a time, are always decoded first: 14 us
+// for one sequence (300 keys 10 us), but 477 us for 32 sequences of 31 keys, one after another, where 32 keys take 9.
 static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (a->KV < mx::FA_Q_MIN_KV || a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
     int D, DV;

@@ -45,12 +45,12 @@
 // out: a lane looks at one tile's mask, for 64 of the wave's tiles at a time (only where at most 8 tokens
 // share a wave; else every tile is read).
 //
-// Measured (this kernel; its merge is 4.2 us more where keys are split), 32 heads on 8 of head dim 128: one token
-// on 1000 Q8_0 keys 9.3 us, on 32768 Q4_0 keys 15.9 us (38 MB, 2.4 TB/s); 32 sequences of 4096 Q8_0 keys 67 us
-// (286 MB, 4.3 TB/s, the rate of a plain read), of 1 to 4096 keys 55 us (143 MB: the longest's 16 tiles a
-// wave at 2.1 to 2.7 us each). A block's start until its first data is 3 to 5 us, its end 2.5 us. A tile at head dim
-// 128 in Q8_0, two waves a SIMD: 0.1 us waiting, 0.4 scores, 0.5 softmax and scales, 0.5 V, 0.6 requesting
-// the tile after the next: the latency of its own chain, not a unit at its limit.
+// Measured (this kernel; its merge is 4 us more where keys are split), 32 heads on 8 of head dim 128: one token
+// on 1000 Q8_0 keys 9.4 us, on 32768 Q4_0 keys 16.7 us (38 MB, 2.3 TB/s); 32 sequences of 4096 Q8_0 keys 67 us
+// (286 MB, 4.3 TB/s, the rate of a plain read), of 1 to 4096 keys 54 us (143 MB: the longest's 16 tiles a
+// wave at some 2.5 us each). A block's start until its first data is 3 to 5 us, its end 2.5 us. A tile is the latency
+// of its wave's own chain, not a unit at its limit (32768 Q4_0 keys: VALU instructions 0.23 of a wave's time, waits
+// 0.24, matrix units 0.04 busy).
 
 #pragma once
 
@@ -64,7 +64,7 @@ namespace mx {
 
 constexpr int FQ_KEYS = 32;      // keys a tile
 constexpr int FQ_LDS_MAX = 160 * 1024;
-constexpr int FQ_BASE_REGS = 96;  // with 64 there are more waves and spills: 32768 Q4_0 keys 19.6 us, not 16.5
+constexpr int FQ_BASE_REGS = 96;  // with 64 there are more waves and spills: 32768 Q4_0 keys 30.5 us a call, not 19.8
 constexpr int FQ_SCAN_TOKENS = 8;
 constexpr float FQ_LAZY = 8.0f / 1.4426950408889634f;
 constexpr float FQ_LOG2E = 1.4426950408889634f;

@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(KV_THREADS) get_rows_kernel(KvRowsArgs a) {
     }
 }
 
-// K and V of one sequence as fp16, for the fused attention. A scale is held to the largest with which
+// K and V of one sequence as fp16, for the fused attention: each value rounded once, by at most 2^-11 of itself (2^-25
+// below 2^-14), since its products take fp16 operands and no F32 ones at their rate. A scale is held to the largest with which
 // every value stays inside fp16. The attention hides a key by its score, but multiplies P = 0 by the
 // key's V all the same, so V has to be finite: a V block whose scale is not stands for zeros here and
 // makes the first value of that key's K a NaN instead, which reaches exactly the queries that see the key.
