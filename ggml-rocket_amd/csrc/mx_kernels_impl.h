@@ -74,6 +74,7 @@ struct KvRowsOut {
 struct KvRowsArgs {
     KvRowsOut o[KV_MAX_OUT];
     int n_out, n;              // n: rows
+    int first;                 // get_rows: the launch's first row
     const void * idx;          // int32 or int64 [n], or null: row i
     bool idx64;
     int rows_wg;               // rows a workgroup (set by the launcher)

@@ -13,8 +13,6 @@
 // two DPP exchanges inside the quad. Reading back, lane l takes values 8l..8l+7, one 16-byte store of fp16
 // (its Q4_0 nibbles are the low or the high ones of eight bytes that two lanes read).
 
-#include <type_traits>
-
 #include "mx_common.h"
 #include "mx_fa_prep.h"
 #include "mx_kernels_impl.h"
@@ -25,6 +23,7 @@ constexpr int KV_THREADS = 256;
 constexpr int KV_BLOCKS = KV_THREADS / 4;   // 32-value blocks in flight in a workgroup
 constexpr int KV_ROWS_MAX = 8;              // rows a workgroup of set_rows
 constexpr int KV_ROWS_LAUNCH = 16384;       // and a launch of it
+constexpr int KV_BLOCKS_LAUNCH = 1 << 24;   // blocks a launch of get_rows
 
 template <int CTRL>
 __device__ __forceinline__ uint32_t quad_dpp(uint32_t x) {
@@ -212,8 +211,8 @@ __global__ void __launch_bounds__(KV_THREADS) get_rows_kernel(KvRowsArgs a) {
     bool ok[ILP];
 #pragma unroll
     for (int u = 0; u < ILP; u++) {
-        const int it = i0 + u * KV_BLOCKS, r = fq_div(min(it, all - 1), o.div_bpr), hb = min(it, all - 1) - r * o.div_bpr.d;
-        const int h = fq_div(hb, o.div_bph), b = hb - h * o.bph;
+        const int it = i0 + u * KV_BLOCKS, rl = fq_div(min(it, all - 1), o.div_bpr), hb = min(it, all - 1) - rl * o.div_bpr.d;
+        const int h = fq_div(hb, o.div_bph), b = hb - h * o.bph, r = a.first + rl;
         const int64_t i = kv_index(a, r);
         const bool in = i >= 0 && i < o.n_rows;
         if (!in && a.err) *a.err = 1;
@@ -275,14 +274,6 @@ __global__ void __launch_bounds__(KV_THREADS) kv_decode_kernel(KvDecodeArgs a, F
     *(u32x4 *)((is_v ? a.v16 + (h * (int64_t)a.KV + j) * a.DV : a.k16 + (h * (int64_t)a.KV + j) * a.D) + 32 * blk + 8 * l) = kv_pack8(v);
 }
 
-// Four blocks a quad where that still makes four workgroups a CU, else one: more of them at once.
-// (Read back as fp16, 32768 rows of 2 x 1024 in Q8_0: 55.7 -> 48.6 us; 512 rows: 4.3 with one, 6.8 with four.)
-template <class F>
-static void kv_ilp(int64_t blocks, F launch) {
-    if (blocks >= (int64_t)1024 * KV_BLOCKS * 4) launch(std::integral_constant<int, 4>{});
-    else launch(std::integral_constant<int, 1>{});
-}
-
 hipError_t launch_kv_decode(const KvDecodeArgs & args, const FaArgs & f, hipStream_t st) {
     KvDecodeArgs a = args;
     a.div_blocks = fq_div_by((a.D + a.DV) / 32);
@@ -327,20 +318,36 @@ hipError_t launch_set_rows(KvRowsArgs a, hipStream_t st) {
     return hipSuccess;
 }
 
+template <int ILP>
+static hipError_t get_rows_launch(KvRowsArgs a, hipStream_t st) {
+    int wgs = 0;
+    for (int k = 0; k < a.n_out; k++) {
+        a.o[k].wg_begin = wgs;
+        wgs += (int)(((int64_t)a.n * a.o[k].div_bpr.d + KV_BLOCKS * ILP - 1) / (KV_BLOCKS * ILP));
+    }
+    hipLaunchKernelGGL(get_rows_kernel<ILP>, dim3(wgs), dim3(KV_THREADS), 0, st, a);
+    return hipGetLastError();
+}
+
+// Four blocks a quad where every output is F16 and there are 2^19 blocks at least, else one: more of them at once.
+// (us with one and four, two caches of 8 x 128 in Q8_0: 512 rows as F16 3.2 / 5.2, as F32 3.8 / 5.6; 4096 8.1 / 8.8 and
+// 11.9 / 13.1; 8192 12.2 / 11.7 and 18.9 / 19.3; 16384 27.8 / 26.6 and 41.4 / 42.5; 32768 47.4 / 46.1 and 73 / 82.)
+// A launch takes KV_BLOCKS_LAUNCH blocks at most (or one row), so that its threads stay far from 2^32.
 hipError_t launch_get_rows(KvRowsArgs a, hipStream_t st) {
     kv_divs(a);
-    int64_t blocks = 0;
-    for (int k = 0; k < a.n_out; k++) blocks += (int64_t)a.n * a.o[k].div_bpr.d;
-    kv_ilp(blocks, [&](auto ilp) {
-        constexpr int ILP = decltype(ilp)::value;
-        int wgs = 0;
-        for (int k = 0; k < a.n_out; k++) {
-            a.o[k].wg_begin = wgs;
-            wgs += (int)(((int64_t)a.n * a.o[k].div_bpr.d + KV_BLOCKS * ILP - 1) / (KV_BLOCKS * ILP));
-        }
-        hipLaunchKernelGGL(get_rows_kernel<ILP>, dim3(wgs), dim3(KV_THREADS), 0, st, a);
-    });
-    return hipGetLastError();
+    int bpr = 0;
+    bool f16 = true;
+    for (int k = 0; k < a.n_out; k++) {
+        bpr += a.o[k].div_bpr.d;
+        f16 = f16 && a.o[k].x_f16;
+    }
+    const int all = a.n, most = max(1, KV_BLOCKS_LAUNCH / bpr);
+    for (a.first = 0; a.first < all; a.first += a.n) {
+        a.n = min(most, all - a.first);
+        const hipError_t e = f16 && (int64_t)a.n * bpr >= 1 << 19 ? get_rows_launch<4>(a, st) : get_rows_launch<1>(a, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace mx

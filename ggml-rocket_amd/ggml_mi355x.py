@@ -466,7 +466,7 @@ def set_rows(pairs, idx=None, err=None):
 
 def get_rows(caches, idx=None, dtype=None, out=None, err=None):
     """Rows idx[i] (None: all, in order) of each of up to four caches as plain values: a list of
-    [n, H, D] (or [n, D]) tensors of `dtype` (F32 by default), or `out`. One launch."""
+    [n, H, D] (or [n, D]) tensors of `dtype` (F32 by default), or `out`. One launch for every 2^24 blocks of 32."""
     if not caches:
         raise MI355XError("get_rows: one to four caches")
     dev = caches[0].dev

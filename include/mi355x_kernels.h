@@ -343,7 +343,7 @@ MI355X_API int mi355x_set_rows(const mi355x_kv_rows * r, int n_out, const void *
                                int32_t * err_dev, void * stream);
 
 /* ggml's GET_ROWS from a cache: cache row idx[i] as plain values in row i of x, for each of `n_out`
- * caches, in ONE launch. F32 values are exact; F16 ones are rounded once (mi355x_weight_dequant_f16's
+ * caches, in one launch for every 2^24 blocks. F32 values are exact; F16 ones are rounded once (mi355x_weight_dequant_f16's
  * values). Indices as in mi355x_set_rows; one outside [0, n_rows) leaves its row of x unwritten and
  * sets *err_dev. */
 MI355X_API int mi355x_get_rows(const mi355x_kv_rows * r, int n_out, const void * idx_dev, int idx_type, int64_t n,
