@@ -749,18 +749,8 @@ static mi355x_fa_args fa_q_lower(const mi355x_fa_q_args * a, int s, const uint16
     return f;
 }
 
-// The direct form: the kernel of mx_fa_q.h on the cache as it is stored.
-static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
-    mx::FaQArgs f;
-    memset(&f, 0, sizeof f);
-    f.q = a->q_dev; f.k = fa_q_view(a->k, 0); f.v = fa_q_view(a->v, 0); f.mask = a->mask_dev; f.dst = a->dst_dev;
-    f.q_nb1 = a->q_nb1; f.q_nb2 = a->q_nb2; f.q_nb3 = a->q_nb3; f.mask_nb1 = a->mask_nb1; f.mask_nb3 = a->mask_nb3;
-    f.dst_nb1 = a->dst_nb1; f.dst_nb2 = a->dst_nb2; f.dst_nb3 = a->dst_nb3;
-    mx::fa_pad_dims(a->D, a->DV, f.D, f.DV);
-    f.dk = a->D; f.dv = a->DV;
-    f.T = a->T; f.HK = a->HK; f.KV = a->KV; f.S = a->S; f.G = a->H / a->HK; f.R = a->T * f.G;
-    f.scale = a->scale; f.softcap = a->softcap;
-    f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
+// Rows a wave and KV splits of the kernels of mx_fa_q.h (nsplit > 0: that split).
+static void fa_q_plan(mx::FaQArgs & f, int nsplit) {
     // Keys are split while compute units are idle, four tiles a block at least, and not at all up to 16 tiles,
     // which a block's waves take at once or twice: the second launch costs more (us whole, in splits of eight
     // tiles and of four, Q8_0: 300 keys 11.2, 11.3, 13.1; 1000 15.6, 13.2, 13.0; 4000 35, 15.1, 14.9; 1000 at
@@ -789,6 +779,21 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
     f.nsplit = (int)splits(f.nq);
     f.div_nrt = mx::fq_div_by(f.nrt); f.div_hk = mx::fq_div_by(f.HK); f.div_split = mx::fq_div_by(f.nsplit);
     f.div_g = mx::fq_div_by(f.G);
+}
+
+// The direct form: the kernel of mx_fa_q.h on the cache as it is stored.
+static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
+    mx::FaQArgs f;
+    memset(&f, 0, sizeof f);
+    f.q = a->q_dev; f.k = fa_q_view(a->k, 0); f.v = fa_q_view(a->v, 0); f.mask = a->mask_dev; f.dst = a->dst_dev;
+    f.q_nb1 = a->q_nb1; f.q_nb2 = a->q_nb2; f.q_nb3 = a->q_nb3; f.mask_nb1 = a->mask_nb1; f.mask_nb3 = a->mask_nb3;
+    f.dst_nb1 = a->dst_nb1; f.dst_nb2 = a->dst_nb2; f.dst_nb3 = a->dst_nb3;
+    mx::fa_pad_dims(a->D, a->DV, f.D, f.DV);
+    f.dk = a->D; f.dv = a->DV;
+    f.T = a->T; f.HK = a->HK; f.KV = a->KV; f.S = a->S; f.G = a->H / a->HK; f.R = a->T * f.G;
+    f.scale = a->scale; f.softcap = a->softcap;
+    f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
+    fa_q_plan(f, nsplit);
     return f;
 }
 
@@ -882,6 +887,162 @@ MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void 
         if (e != MI355X_OK) return e;
     }
     return MI355X_OK;
+}
+
+// ---- a KV cache in pages ------------------------------------------------------------------------
+
+static int kv_step_lower(const mi355x_kv_step & s, int64_t n_rows, int32_t * err_dev, mx::KvStepArgs & a) {
+    if (s.S < 0 || s.T < 0 || s.page <= 0 || s.page % 32 || s.n_table < 0 || s.table_nb < 0 || s.parent_nb < 0) return MI355X_E_ARG;
+    if (!aligned(s.table_dev, 4) || !aligned(s.n_past_dev, 4) || !aligned(s.n_new_dev, 4) || !aligned(s.parent_dev, 4) || !aligned(err_dev, 4))
+        return MI355X_E_ARG;
+    if (s.n_table > (1 << 29) / s.page || (int64_t)s.S * s.T > 1 << 22 || n_rows < 0 || n_rows / s.page > INT32_MAX) return MI355X_E_ARG;
+    if (s.parent_dev && s.T > mx::KV_TREE_MAX) return MI355X_E_ARG;
+    if (s.S > 0 && s.T > 0 && (!s.table_dev || !s.n_past_dev || s.n_table < 1 || n_rows < s.page)) return MI355X_E_ARG;
+    a.table = s.table_dev; a.n_past = s.n_past_dev; a.n_new = s.n_new_dev; a.parent = s.parent_dev; a.err = err_dev;
+    a.table_nb = s.table_nb; a.parent_nb = s.parent_nb; a.n_table = (int)s.n_table; a.S = s.S; a.T = s.T; a.page = s.page;
+    a.n_pages = (int)(n_rows / s.page);
+    a.div_page = mx::fq_div_by(s.page);
+    return MI355X_OK;
+}
+
+MI355X_API int mi355x_kv_append(const mi355x_kv_append_args * p, int32_t * err_dev, void * stream) {
+    if (!p) return MI355X_E_ARG;
+    mx::KvAppendArgs a;
+    memset(&a, 0, sizeof a);
+    // the rows' own checks, as for a store of one row: a cache's rows and the sources' strides do not follow from a count here
+    mi355x_kv_rows r[2] = {p->k, p->v};
+    mx::KvRowsArgs rows;
+    const int64_t n = (int64_t)p->step.S * p->step.T;
+    if (r[0].n_rows < 0 || r[1].n_rows < 0) return MI355X_E_ARG;
+    int st = kv_step_lower(p->step, std::min(r[0].n_rows, r[1].n_rows), err_dev, a.st);
+    if (st != MI355X_OK) return st;
+    st = kv_rows_lower(r, 2, nullptr, 26, n > 0, err_dev, true, rows);
+    if (st != MI355X_OK) return st;
+    const bool queries = p->q_dev || p->qr_dev;
+    if (p->k_nb3 < 0 || p->v_nb3 < 0 || p->k_nb3 % 8 || p->v_nb3 % 8 || p->pos_nb < 0 || !aligned(p->pos_dev, 4) || !aligned(p->freq_dev, 4))
+        return MI355X_E_ARG;
+    if (p->n_rot < 0 || p->n_rot % 8 || p->n_rot > r[0].D || p->n_rot > 256 || (p->n_rot > 0 && n > 0 && !p->freq_dev)) return MI355X_E_ARG;
+    if (r[0].H != r[1].H || (queries && (p->H <= 0 || p->H > INT32_MAX / r[0].D))) return MI355X_E_ARG;
+    if (queries) {
+        for (int t : {p->q_type, p->qr_type})
+            if (t != mx::T_F32 && t != mx::T_F16) return MI355X_E_ARG;
+        for (int64_t nb : {p->q_nb1, p->q_nb2, p->q_nb3, p->qr_nb1, p->qr_nb2, p->qr_nb3})
+            if (nb < 0 || nb % 8) return MI355X_E_ARG;
+        if (n > 0 && (!p->q_dev || !p->qr_dev)) return MI355X_E_ARG;
+        if (!aligned(p->q_dev, 16) || !aligned(p->qr_dev, 16)) return MI355X_E_ARG;
+        // in place: a value that another lane still pairs with its own must not be overwritten
+        if (n > 0 && p->q_dev == p->qr_dev && (p->q_type != p->qr_type || p->q_nb1 != p->qr_nb1 || p->q_nb2 != p->qr_nb2 || p->q_nb3 != p->qr_nb3 ||
+                                              (p->neox && p->n_rot)))
+            return MI355X_E_ARG;
+    }
+    for (int k = 0; k < 2; k++) {
+        mx::KvAppendRows & o = a.r[k];
+        o.x = {r[k].x_dev, r[k].x_nb1, r[k].x_nb2, k ? p->v_nb3 : p->k_nb3, r[k].x_type == mx::T_F16};
+        o.H = (int)r[k].H; o.bph = (int)(r[k].D / 32); o.rotate = k == 0;
+        a.o[k] = rows.o[k];
+    }
+    a.r[2].x = {(void *)p->q_dev, p->q_nb1, p->q_nb2, p->q_nb3, p->q_type == mx::T_F16};
+    a.r[2].H = (int)p->H; a.r[2].bph = a.r[0].bph; a.r[2].rotate = true;
+    a.qr = {p->qr_dev, p->qr_nb1, p->qr_nb2, p->qr_nb3, p->qr_type == mx::T_F16};
+    a.n_rows = queries ? 3 : 2;
+    for (int k = 0; k < a.n_rows; k++)
+        if ((int64_t)a.r[k].H * a.r[k].bph > 1 << 16) return MI355X_E_ARG;
+    a.freq = p->freq_dev; a.pos = p->pos_dev; a.pos_nb = p->pos_nb; a.half = p->n_rot / 2; a.neox = p->neox != 0; a.mscale = p->mscale;
+    return n == 0 ? MI355X_OK : hip_status(mx::launch_kv_append(a, S(stream)));
+}
+
+MI355X_API int mi355x_kv_keep(const mi355x_kv_step * step, const mi355x_kv_rows * r, int n_out, const int32_t * path_dev,
+                              int64_t path_nb, const int32_t * n_keep_dev, int A, int32_t * err_dev, void * stream) {
+    if (!step || !r || n_out < 1 || n_out > mx::KV_MAX_OUT || A < 0 || A > mx::KV_TREE_MAX || path_nb < 0) return MI355X_E_ARG;
+    if (!aligned(path_dev, 4) || !aligned(n_keep_dev, 4)) return MI355X_E_ARG;
+    const bool some = step->S > 0 && step->T > 0 && A > 0;
+    if (some && !path_dev) return MI355X_E_ARG;
+    mx::KvKeepArgs a;
+    memset(&a, 0, sizeof a);
+    int64_t n_rows = INT64_MAX;
+    mi355x_kv_rows rows[mx::KV_MAX_OUT];
+    for (int k = 0; k < n_out; k++) {   // x is not read: anything that the check of a store takes
+        rows[k] = r[k];
+        rows[k].x_type = mx::T_F32;
+        rows[k].x_dev = rows[k].q_dev;
+        rows[k].x_nb1 = rows[k].x_nb2 = 0;
+        n_rows = std::min(n_rows, r[k].n_rows);
+    }
+    int st = kv_step_lower(*step, n_rows, err_dev, a.st);
+    if (st != MI355X_OK) return st;
+    mx::KvRowsArgs low;
+    st = kv_rows_lower(rows, n_out, nullptr, 26, some, err_dev, true, low);
+    if (st != MI355X_OK) return st;
+    for (int k = 0; k < n_out; k++) {
+        if (low.o[k].H * (int64_t)low.o[k].bph > 1 << 16) return MI355X_E_ARG;
+        a.o[k] = low.o[k];
+    }
+    a.n_out = n_out; a.A = A; a.path = path_dev; a.n_keep = n_keep_dev; a.path_nb = path_nb;
+    return some ? hip_status(mx::launch_kv_keep(a, S(stream))) : MI355X_OK;
+}
+
+static int fa_p_check(const mi355x_fa_p_args * a, int nsplit, mx::FaPArgs & f) {
+    memset(&f, 0, sizeof f);
+    if (!a) return MI355X_E_ARG;
+    const int st = kv_step_lower(a->step, a->n_rows, nullptr, f.st);
+    if (st != MI355X_OK) return st;
+    const int Sn = a->step.S, T = a->step.T;
+    const bool empty = T == 0 || Sn == 0;   // no query: nothing is read or written
+    if (!empty && (!a->q_dev || !a->dst_dev)) return MI355X_E_ARG;
+    if (a->D <= 0 || a->DV <= 0 || a->D % 32 || a->DV % 32 || !mx::fa_pad_dims(a->D, a->DV, f.D, f.DV)) return MI355X_E_UNSUPPORTED;
+    if (2 * a->D < f.D || 2 * a->DV < f.DV) return MI355X_E_UNSUPPORTED;   // the loads of scales
+    for (const mi355x_kv_view * w : {&a->k, &a->v}) {
+        if (!kv_type(w->type)) return MI355X_E_UNSUPPORTED;
+        if (w->nb1 < 0 || w->nb2 < 0 || w->nb1 % 32 || w->nb2 % 32 || w->nb1 >= mx::FA_Q_MAX_NB1) return MI355X_E_ARG;
+        if ((!empty && !w->q_dev) || !aligned(w->q_dev, 16)) return MI355X_E_ARG;
+        if ((!empty && !w->d_dev) || !aligned(w->d_dev, 8)) return MI355X_E_ARG;
+    }
+    if (a->H <= 0 || a->HK <= 0 || a->H % a->HK || a->max_kv < 0 || nsplit > 64) return MI355X_E_ARG;
+    const int64_t tiles = (int64_t)Sn * a->HK * (((int64_t)T * (a->H / a->HK) + 15) / 16);
+    if (tiles > (1 << 21) / (nsplit > 1 ? nsplit : 1) || (nsplit > 1 && tiles * f.DV >= 1 << 28)) return MI355X_E_UNSUPPORTED;
+    if ((int64_t)Sn * T * a->H > 1 << 30) return MI355X_E_UNSUPPORTED;
+    for (int t : {a->q_type, a->dst_type})
+        if (t != mx::T_F32 && t != mx::T_F16) return MI355X_E_ARG;
+    const int64_t qa = a->q_type == mx::T_F16 ? 8 : 4;
+    if (a->q_nb1 % qa || a->q_nb2 % qa || a->q_nb3 % qa || !aligned(a->q_dev, 16)) return MI355X_E_ARG;
+    if (a->dst_nb1 % 4 || a->dst_nb2 % 4 || a->dst_nb3 % 4 || !aligned(a->dst_dev, a->dst_type == mx::T_F16 ? 8 : 16)) return MI355X_E_ARG;
+    if (empty) return MI355X_OK;
+    f.q = a->q_dev; f.dst = a->dst_dev;
+    f.k = fa_q_view(a->k, 0); f.v = fa_q_view(a->v, 0);
+    f.k.nb3 = f.v.nb3 = 0;
+    f.q_nb1 = a->q_nb1; f.q_nb2 = a->q_nb2; f.q_nb3 = a->q_nb3;
+    f.dst_nb1 = a->dst_nb1; f.dst_nb2 = a->dst_nb2; f.dst_nb3 = a->dst_nb3;
+    f.dk = a->D; f.dv = a->DV;
+    const int64_t cap = a->step.n_table * a->step.page;
+    f.KV = (int)(a->max_kv ? std::min(a->max_kv, cap) : cap);
+    f.T = T; f.S = Sn; f.HK = a->HK; f.G = a->H / a->HK; f.R = T * f.G;
+    f.scale = a->scale; f.softcap = a->softcap;
+    f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
+    fa_q_plan(f, nsplit);
+    f.div_tpp = mx::fq_div_by(a->step.page / 32);
+    return MI355X_OK;
+}
+
+MI355X_API size_t mi355x_flash_attn_paged_workspace(const mi355x_fa_p_args * a, int nsplit) {
+    mx::FaPArgs f;
+    if (fa_p_check(a, nsplit, f) != MI355X_OK) return 0;
+    if (a->step.T == 0 || a->step.S == 0) return 256;
+    return fa_q_direct_layout(f).total;
+}
+
+MI355X_API int mi355x_flash_attn_paged(const mi355x_fa_p_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
+                                       int32_t * err_dev, void * stream) {
+    mx::FaPArgs f;
+    const int st = fa_p_check(a, nsplit, f);
+    if (st != MI355X_OK) return st;
+    if (!aligned(err_dev, 4)) return MI355X_E_ARG;
+    if (a->step.T == 0 || a->step.S == 0) return MI355X_OK;
+    const FaQDirectLayout L = fa_q_direct_layout(f);
+    if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
+    f.st.err = err_dev;
+    f.part_o = (float *)((char *)workspace_dev + L.po);
+    f.part_ml = (float *)((char *)workspace_dev + L.pml);
+    return hip_status(mx::launch_fa_p(f, S(stream)));
 }
 
 // ---- MUL_MAT_ID -------------------------------------------------------------------------------

@@ -54,10 +54,13 @@
 
 #pragma once
 
+#include <limits.h>
+
 #include <type_traits>
 
 #include "mx_common.h"
 #include "mx_kernels_impl.h"
+#include "mx_pages.h"
 #include "mx_weights.h"
 
 namespace mx {
@@ -222,16 +225,19 @@ __device__ __forceinline__ void fq_store4(const FaQArgs & a, int64_t dst, int d,
     else *(float4v *)((float *)a.dst + dst + d) = v * inv;
 }
 
-template <int KT, int VT, int DK, int DV, int NQ>
+// A: FaQArgs, or FaPArgs for a cache in pages.
+template <int KT, int VT, int DK, int DV, int NQ, class A>
 __global__ void __launch_bounds__((FqCfg<KT, VT, DK, DV, NQ>::NW * WAVE))
 __attribute__((amdgpu_waves_per_eu(FqCfg<KT, VT, DK, DV, NQ>::NW / 4, FqCfg<KT, VT, DK, DV, NQ>::NW / 4)))
-fa_q_kernel(FaQArgs a) {
+fa_q_kernel(A a) {
     using C = FqCfg<KT, VT, DK, DV, NQ>;
+    constexpr bool PG = std::is_same<A, FaPArgs>::value;
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int NW = C::NW;
     // The arguments lie in host memory, a round trip of half a microsecond and more a cache line; used
     // here, one of each line, they all come at once instead of where each is first needed.
     asm volatile("" ::"s"(a.q), "s"(a.k.nb3), "s"(a.v.nb2), "s"(a.dst), "s"(a.mask_nb3), "s"(a.T), "s"(a.div_split.mul), "s"(a.softcap));
+    if constexpr (PG) asm volatile("" ::"s"(a.st.table), "s"(a.st.parent_nb), "s"(a.div_tpp.mul));
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int r = lane % 16, g = lane / 16;
 
@@ -242,13 +248,40 @@ fa_q_kernel(FaQArgs a) {
     b = b1;
     b1 = fq_div(b, a.div_hk);
     const int hk = b - b1 * a.HK, s = fq_div(b1, a.div_split), split = b1 - s * a.nsplit;
-    const int ntiles = (a.KV + FQ_KEYS - 1) / FQ_KEYS, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    // pages: the first keys of the sequence, up to the last that a row of this block sees
+    int n_past = 0, n_new = 0, keys = a.KV, up = -1;
+    if constexpr (PG) {
+        const StepOf sq = step_of(a.st, s);
+        n_past = sq.past;
+        n_new = sq.fresh;
+        if (sq.bad && threadIdx.x == 0 && a.st.err) *a.st.err = 1;
+        const int tok0 = fq_div(rt * 16 * NQ, a.div_g), tok1 = fq_div(min(a.R, (rt + 1) * 16 * NQ) - 1, a.div_g);
+        const int seen = a.st.parent ? n_new : min(n_new, tok1 + 1);
+        keys = tok0 < n_new ? min(n_past + seen, a.st.n_table * a.st.page) : 0;
+        if (a.st.parent && lane < a.T) up = a.st.parent[(int64_t)s * a.st.parent_nb + lane];
+    }
+    const int ntiles = (keys + FQ_KEYS - 1) / FQ_KEYS, per = (ntiles + a.nsplit - 1) / a.nsplit;
     const int tile0 = split * per, tile1 = min(ntiles, tile0 + per);
 
     // Tile t starts at key kb(t) = min(32 t, KV - 32), KV >= 32: a last partial tile is moved back and
     // its keys before 32 t, which the tile before has, do not count. So every load stays inside the
     // cache without a bound per lane: a scalar base and the lane's fixed 32-bit offset.
-    const int kb_last = a.KV - FQ_KEYS;
+    // (In pages a tile is 32 rows of one page, all of them rows of the cache; the keys behind the last count for no row.)
+    const int kb_last = PG ? INT_MAX : a.KV - FQ_KEYS;
+    // Pages: the row where tile t begins, -1 for a tile of a page that the cache does not have
+    auto page_of = [&](int t) -> int64_t {
+        if constexpr (PG) {
+            const int p = fq_div(t, a.div_tpp);
+            const int64_t row = page_row(a.st, uniform_i32(a.st.table, (int64_t)s * a.st.table_nb + p));
+            return row < 0 ? -1 : row + FQ_KEYS * (t - p * a.div_tpp.d);
+        }
+        return 0;
+    };
+    // the row that tile t is read from
+    auto first_row = [&](int t, int64_t row) -> int64_t {
+        if constexpr (PG) return row < 0 ? 0 : row;
+        return min(FQ_KEYS * t, kb_last);
+    };
     constexpr int KSH = KT == T_Q4_0, VSH = VT == T_Q4_0;   // elements to bytes
     const uint8_t * const kq = a.k.q + (((int64_t)s * a.k.nb3 + (int64_t)hk * a.k.nb2) >> KSH);
     const uint8_t * const vq = a.v.q + (((int64_t)s * a.v.nb3 + (int64_t)hk * a.v.nb2) >> VSH);
@@ -285,16 +318,16 @@ fa_q_kernel(FaQArgs a) {
     const uint32_t vlds = (uint32_t)(uintptr_t)(fq_lptr_t)wl;    // its LDS address
     float * const wk = (float *)wl;                              // K scales [block][key]
     uint16_t * const wv = (uint16_t *)(wk + C::KS * FQ_KEYS);    // V scales [block][key]
-    auto dma_k = [&](int t, int buf) {
-        const __amdgpu_buffer_rsrc_t kt = fq_rsrc(kq + ((min(FQ_KEYS * t, kb_last) * a.k.nb1) >> KSH));
+    auto dma_k = [&](int t, int64_t row, int buf) {
+        const __amdgpu_buffer_rsrc_t kt = fq_rsrc(kq + ((first_row(t, row) * a.k.nb1) >> KSH));
         uint8_t * st = wl + C::SCALE_LDS + buf * C::STAGE;
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int q = 0; q < C::KD; q++) fq_dma16(kt, kdma[q], st + q * 1024);
         asm volatile("" ::: "memory");
     };
-    auto dma_v = [&](int t, int buf) {
-        const __amdgpu_buffer_rsrc_t vt = fq_rsrc(vq + ((min(FQ_KEYS * t, kb_last) * a.v.nb1) >> VSH));
+    auto dma_v = [&](int t, int64_t row, int buf) {
+        const __amdgpu_buffer_rsrc_t vt = fq_rsrc(vq + ((first_row(t, row) * a.v.nb1) >> VSH));
         uint8_t * st = wl + C::SCALE_LDS + buf * C::STAGE + FQ_KEYS * 16 * C::KCH;
         asm volatile("" ::: "memory");
 #pragma unroll
@@ -319,18 +352,20 @@ fa_q_kernel(FaQArgs a) {
         uint64_t kd, vd;
         u32x4 m[NQ];           // the mask of this lane's eight keys
     };
-    auto load_side = [&](Side & x, int t) {
-        const int64_t kb = min(FQ_KEYS * t, kb_last);
+    auto load_side = [&](Side & x, int t, int64_t row) {
+        const int64_t kb = first_row(t, row);
         x.kd = fq_load_scales<C::KSL>((const uint8_t *)kd + kb * a.k.nb1 / 32 * 2 + kdo);
         x.vd = fq_load_scales<C::VSL>((const uint8_t *)vd + kb * a.v.nb1 / 32 * 2 + vdo);
+        if constexpr (!PG) {
 #pragma unroll
-        for (int n = 0; n < NQ; n++) __builtin_memcpy(&x.m[n], mrow[n] + kb * mstep, 16);   // any alignment of 2 bytes
+            for (int n = 0; n < NQ; n++) __builtin_memcpy(&x.m[n], mrow[n] + kb * mstep, 16);   // any alignment of 2 bytes
+        }
     };
     // The wave's tiles are tile0 + wave + NW k. next() gives the next k that some row sees (-1: none): bits
     // of 64 of them, one lane a tile.
     const int nk = tile1 - tile0 > wave ? (tile1 - tile0 - wave + NW - 1) / NW : 0;
     const int tok_a = fq_div(rt * 16 * NQ, a.div_g), tok_b = fq_div(min(a.R, (rt + 1) * 16 * NQ) - 1, a.div_g);
-    const bool scan = a.mask && tok_b - tok_a < FQ_SCAN_TOKENS;
+    const bool scan = !PG && a.mask && tok_b - tok_a < FQ_SCAN_TOKENS;
     uint64_t todo = 0;
     int k0 = -64;              // the 64 that todo is for
     auto next = [&]() {
@@ -388,16 +423,19 @@ fa_q_kernel(FaQArgs a) {
     // The first two tiles are requested before their masks are looked at; tiles that turn out hidden are
     // replaced once they have landed. Waves without tiles read some tile all the same: loads that are
     // sometimes issued would make every wait behind them a wait for all loads.
-    const int tile_end = ntiles - 1;
+    const int tile_end = PG ? max(ntiles, 1) - 1 : ntiles - 1;
     int t = min(tile0 + wave, tile_end), tn = min(tile0 + wave + NW, tile_end);
+    // Pages: the rows of both, and of the tile that is requested next (a wave's tiles follow each other: no mask hides
+    // any): its table entry is on its way while this one's products are formed.
+    int64_t row_t = page_of(t), row_n = page_of(tn), row_p = page_of(min(tn + NW, tile_end));
     Side x0, x1;
     auto request = [&]() {   // a tile's K, its scales and masks, its V, then the next tile's
-        dma_k(t, 0);
-        load_side(x0, t);
-        dma_v(t, 0);
-        dma_k(tn, 1);
-        load_side(x1, tn);
-        dma_v(tn, 1);
+        dma_k(t, row_t, 0);
+        load_side(x0, t, row_t);
+        dma_v(t, row_t, 0);
+        dma_k(tn, row_n, 1);
+        load_side(x1, tn, row_n);
+        dma_v(tn, row_n, 1);
     };
     request();
 
@@ -433,11 +471,35 @@ fa_q_kernel(FaQArgs a) {
     }
     const int ka = next();
     int kn = ka >= 0 ? next() : -1;
-    if (ka > 0 || kn > 1) {
+    if (!PG && (ka > 0 || kn > 1)) {
         fq_wait_vm<0>();
         t = tile0 + wave + NW * ka;
         tn = kn >= 0 ? tile0 + wave + NW * kn : t;
         request();
+    }
+    // Pages: row n of this lane sees keys below lim[n] and, of the new tokens', those whose bits are set in anc[n]; every key
+    // below full_to counts for every row.
+    int lim[NQ], full_to = INT_MAX;
+    uint64_t anc[NQ];
+    if constexpr (PG) {
+        const uint64_t node = a.st.parent ? tree_ancestors(up, lane) : 0;
+        if (a.st.parent && lane < n_new && !node && a.st.err) *a.st.err = 1;
+        bool none = false;
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const int row = (rt * NQ + n) * 16 + r, tok = ok[n] ? fq_div(row, a.div_g) : 0;
+            lim[n] = tok < n_new ? n_past : 0;
+            anc[n] = 0;
+            if (a.st.parent) {
+                const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)node, tok, WAVE), hi = (uint32_t)__shfl((int)(uint32_t)(node >> 32), tok, WAVE);
+                anc[n] = tok < n_new ? (uint64_t)hi << 32 | lo : 0;
+                if (!anc[n]) lim[n] = 0;
+            } else if (tok < n_new) {
+                lim[n] = n_past + tok + 1;
+            }
+            none |= ok[n] && lim[n] < n_past + (a.st.parent ? 0 : tok_a + 1);
+        }
+        full_to = __any(none) ? 0 : min(keys, n_past + (a.st.parent ? 0 : tok_a + 1));
     }
     // a barrier for LDS alone: the first tiles' loads stay in flight
     asm volatile("" ::: "memory");
@@ -479,7 +541,7 @@ fa_q_kernel(FaQArgs a) {
     // 2.6 for it: 32 sequences of up to 4096 keys, Q8_0, head dim 128.) Returns false after the last tile.
     auto tile = [&](Side & x, auto buffer) __attribute__((always_inline)) {
         constexpr int BUF = decltype(buffer)::value;
-        constexpr int SL = 2 + NQ;                       // loads of load_side
+        constexpr int SL = PG ? 2 : 2 + NQ;              // loads of load_side
         // K's codes and x have landed; behind them V, and the next tile's three
         fq_wait_vm<C::VD + C::KD + SL + C::VD>();
         const int kb = min(FQ_KEYS * t, kb_last);
@@ -529,8 +591,10 @@ fa_q_kernel(FaQArgs a) {
         // again, where there is none: the number of loads in flight stays what the waits count)
         const int k2 = kn >= 0 ? next() : -1;
         const int t2 = k2 >= 0 ? tile0 + wave + NW * k2 : tn;
+        const int64_t row2 = k2 >= 0 ? row_p : row_n;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        dma_k(t2, BUF);
+        dma_k(t2, row2, BUF);
+        if constexpr (PG) row_p = page_of(min(t2 + NW, tile_end));
         u32x4 pf[NQ];   // P, fp16
         {
             // ---- scale back, cap, mask, softmax ----
@@ -552,7 +616,21 @@ fa_q_kernel(FaQArgs a) {
                         for (int e = 0; e < 4; e++)
                             sc[n][hf][e] = fmaf(-2.0f * a.softcap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[n][hf][e] * cap2)), a.softcap);
                 }
-                if (a.mask && __any((x.m[n][0] | x.m[n][1] | x.m[n][2] | x.m[n][3]) != 0)) {
+                if constexpr (PG) {
+                    if (FQ_KEYS * (t + 1) > full_to || row_t < 0) {
+                        if (row_t < 0 && a.st.err) *a.st.err = 1;
+                        // of keys j .. j + 7, those below lim and those whose bits are set
+                        const int j = FQ_KEYS * t + 8 * g, c = lim[n] - j, u = j - n_past;
+                        uint32_t vis = c >= 8 ? 0xFFu : c > 0 ? (1u << c) - 1 : 0u;
+                        if (u > -8 && u < 64) vis |= (uint32_t)(u >= 0 ? anc[n] >> u : anc[n] << -u);
+                        if (row_t < 0) vis = 0;
+#pragma unroll
+                        for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (!((vis >> (4 * hf + e)) & 1u)) sc[n][hf][e] = -INFINITY;   // a hidden score may be NaN
+                    }
+                } else if (a.mask && __any((x.m[n][0] | x.m[n][1] | x.m[n][2] | x.m[n][3]) != 0)) {
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++)
 #pragma unroll
@@ -561,7 +639,7 @@ fa_q_kernel(FaQArgs a) {
                             sc[n][hf][e] = mv == -INFINITY ? -INFINITY : sc[n][hf][e] + mv;   // a hidden score may be NaN
                         }
                 }
-                if (part) {
+                if (!PG && part) {
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++)
 #pragma unroll
@@ -675,7 +753,7 @@ fa_q_kernel(FaQArgs a) {
             }
         }
         asm volatile("" ::: "memory");
-        load_side(x, t2);
+        load_side(x, t2, row2);
         fq_wait_vm<C::KD + SL + C::VD + C::KD + SL>();   // this tile's V has landed
         {
             // ---- O^T += V^T . (P d 2^k)^T, two blocks of 32 dims at a time ----
@@ -718,10 +796,12 @@ fa_q_kernel(FaQArgs a) {
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        dma_v(t2, BUF);
+        dma_v(t2, row2, BUF);
         if (kn < 0) return false;
         t = tn;
         tn = t2;
+        row_t = row_n;
+        row_n = row2;
         kn = k2;
         return true;
     };
@@ -812,34 +892,34 @@ fa_q_kernel(FaQArgs a) {
     }
 }
 
-template <int KT, int VT, int DK, int DV, int NQ>
-static hipError_t fq_launch(const FaQArgs & a, hipStream_t st) {
+template <int KT, int VT, int DK, int DV, int NQ, class A>
+static hipError_t fq_launch(const A & a, hipStream_t st) {
     using C = FqCfg<KT, VT, DK, DV, NQ>;
     static_assert(C::LDS <= 160 * 1024, "LDS");
     static bool done = false;
     if (!done) {
-        const hipError_t e = hipFuncSetAttribute((const void *)fa_q_kernel<KT, VT, DK, DV, NQ>,
+        const hipError_t e = hipFuncSetAttribute((const void *)fa_q_kernel<KT, VT, DK, DV, NQ, A>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
         if (e != hipSuccess) return e;
         done = true;
     }
     const int64_t units = (int64_t)a.S * a.HK * a.nrt;
-    hipLaunchKernelGGL((fa_q_kernel<KT, VT, DK, DV, NQ>), dim3((unsigned)(units * a.nsplit)), dim3(C::NW * WAVE), C::LDS, st, a);
+    hipLaunchKernelGGL((fa_q_kernel<KT, VT, DK, DV, NQ, A>), dim3((unsigned)(units * a.nsplit)), dim3(C::NW * WAVE), C::LDS, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     return launch_fa_q_combine(a, DV, NQ, st);
 }
 
-template <int KT, int VT, int DK, int DV>
-static hipError_t fq_rows(const FaQArgs & a, hipStream_t st) {
+template <int KT, int VT, int DK, int DV, class A>
+static hipError_t fq_rows(const A & a, hipStream_t st) {
     if (a.nq == 1) return fq_launch<KT, VT, DK, DV, 1>(a, st);
     if constexpr (DK == 64)
         if (a.nq == 2) return fq_launch<KT, VT, DK, DV, 2>(a, st);
     return hipErrorInvalidValue;
 }
 
-template <int KT, int VT>
-static hipError_t fq_dims(const FaQArgs & a, hipStream_t st) {
+template <int KT, int VT, class A>
+static hipError_t fq_dims(const A & a, hipStream_t st) {
     if (a.D == 64 && a.DV == 64) return fq_rows<KT, VT, 64, 64>(a, st);
     if (a.D == 128 && a.DV == 128) return fq_rows<KT, VT, 128, 128>(a, st);
     if (a.D == 192 && a.DV == 128) return fq_rows<KT, VT, 192, 128>(a, st);
@@ -849,5 +929,7 @@ static hipError_t fq_dims(const FaQArgs & a, hipStream_t st) {
 
 #define FQ_TYPES(K, V) \
     hipError_t launch_fa_q_##K##_##V(const FaQArgs & a, hipStream_t st) { return fq_dims<T_##K, T_##V>(a, st); }
+#define FP_TYPES(K, V) \
+    hipError_t launch_fa_p_##K##_##V(const FaPArgs & a, hipStream_t st) { return fq_dims<T_##K, T_##V>(a, st); }
 
 }  // namespace mx

@@ -106,6 +106,26 @@ struct FaQArgs {
     float scale, softcap;
     bool q_f16, dst_f16;
 };
+// One step of S sequences over a cache in pages (mi355x_kv_step). Logical row j of sequence s is row
+// table[s][j / page] * page + j % page; positions below 2^30.
+constexpr int KV_TREE_MAX = 64;             // nodes of a tree: a lane each
+struct KvStepArgs {
+    const int32_t * table;     // [S][n_table], sequence stride table_nb
+    const int32_t * n_past;    // [S]
+    const int32_t * n_new;     // [S], or null: T
+    const int32_t * parent;    // [S][T], sequence stride parent_nb, or null: a chain
+    int32_t * err;             // set to 1 by what the device finds wrong, or null
+    int64_t table_nb, parent_nb;
+    int n_table, S, T, page, n_pages;   // n_pages: whole pages of the cache
+    FqDiv div_page;
+};
+// The same over a cache in pages of whole 32-key tiles: the keys of sequence s are its first n_past + n_new logical rows
+// (k and v: nb3 0, of the whole cache), the rows its T new tokens, which see what mi355x_flash_attn_paged
+// says. KV is what the launch was planned for; mask is null.
+struct FaPArgs : FaQArgs {
+    KvStepArgs st;
+    FqDiv div_tpp;             // 32-key tiles a page
+};
 constexpr int FA_Q_MIN_KV = 32;             // a tile
 constexpr int64_t FA_Q_MAX_NB1 = 1 << 24;   // its 32-bit offsets inside a tile
 inline int fa_q_max_nq(int D) { return D == 64 ? 2 : 1; }
@@ -115,6 +135,11 @@ hipError_t launch_fa_q_Q8_0_Q8_0(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_q_Q8_0_Q4_0(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_q_Q4_0_Q8_0(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_q_Q4_0_Q4_0(const FaQArgs & a, hipStream_t st);
+hipError_t launch_fa_p(const FaPArgs & a, hipStream_t st);
+hipError_t launch_fa_p_Q8_0_Q8_0(const FaPArgs & a, hipStream_t st);
+hipError_t launch_fa_p_Q8_0_Q4_0(const FaPArgs & a, hipStream_t st);
+hipError_t launch_fa_p_Q4_0_Q8_0(const FaPArgs & a, hipStream_t st);
+hipError_t launch_fa_p_Q4_0_Q4_0(const FaPArgs & a, hipStream_t st);
 // K and V of one sequence as fp16 for the fused attention: k16 [HK][KV][D], v16 [HK][KV][DV].
 struct KvDecodeArgs {
     KvView k, v;
@@ -125,6 +150,48 @@ struct KvDecodeArgs {
     int n_prep;                // workgroups of the mask classes, before those of the cache
 };
 hipError_t launch_set_rows(KvRowsArgs a, hipStream_t st);
+
+// The new tokens' keys (rotated) and values stored, the queries rotated.
+struct KvPlainRows {           // [S][T][H][32 bph], strides in elements
+    void * x;
+    int64_t nb1, nb2, nb3;     // token, head, sequence
+    bool f16;
+};
+struct KvAppendRows {          // K, V or Q
+    KvPlainRows x;
+    int H, bph;                // heads, 32-value blocks a head
+    bool rotate;
+    int items, tok_wg, parts, groups, wg_begin;   // set by the launcher
+    FqDiv div_bph, div_items, div_parts, div_groups;
+};
+struct KvAppendArgs {
+    KvStepArgs st;
+    KvAppendRows r[3];         // K, V, Q
+    KvRowsOut o[2];            // the caches of K and V
+    KvPlainRows qr;            // the rotated queries
+    int n_rows;                // 3, or 2 without queries
+    const float * freq;        // [half] radians a position
+    const int32_t * pos;       // [S][T], sequence stride pos_nb, or null
+    int64_t pos_nb;
+    int half;                  // half the rotated dims
+    bool neox;                 // pairs (i, i + half), else (2 i, 2 i + 1)
+    float mscale;
+    int span;                  // pages that a sequence's new rows may touch (set by the launcher)
+    FqDiv div_half, div_span;
+};
+hipError_t launch_kv_append(KvAppendArgs a, hipStream_t st);
+// Rows path[s][i] of the new ones moved to row i of them, for each of up to KV_MAX_OUT caches.
+struct KvKeepArgs {
+    KvStepArgs st;
+    KvRowsOut o[KV_MAX_OUT];   // div_bpr, div_bph set by the launcher
+    int n_out, A;              // A: entries of a path
+    const int32_t * path;      // [S][A], sequence stride path_nb
+    const int32_t * n_keep;    // [S], or null: A
+    int64_t path_nb;
+    int wgs;                   // workgroups a sequence (set by the launcher)
+};
+hipError_t launch_kv_keep(KvKeepArgs a, hipStream_t st);
+
 hipError_t launch_get_rows(KvRowsArgs a, hipStream_t st);
 
 // FLASH_ATTN_EXT with head dims past 256 (two GEMMs around a softmax pass): strides in

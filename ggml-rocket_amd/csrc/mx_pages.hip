@@ -1,0 +1,267 @@
+// SPDX-License-Identifier: MIT
+// A KV cache in pages: new tokens' keys and values stored at their sequences' ends, with the position rotation
+// of keys and queries, and accepted drafts moved to where the sequence goes on.
+//
+// Token t of sequence s has logical row j = n_past[s] + t, cache row table[s][j / page] * page + j % page and position
+// p = n_past[s] + depth(t) (or a given one). Its keys and queries are rotated in pairs (a, b) of dims, pair i by
+//   theta = p freq[i] in 64 bits,  c = f32(m cos theta),  s = f32(m sin theta)
+//   a' = f32(f32(a c) - f32(b s)),  b' = f32(f32(a s) + f32(b c))
+// every step rounded on its own, so the codes made of them are the definition's bits: an angle in 32 bits is off by
+// 2^-24 of itself, 0.004 rad at position 65536, half a step of 8 bits and more.
+//
+// Append reads every value once and writes rows and queries: HBM bounds many tokens, latency a few. The sines are taken once
+// a token and pair, not once a head, by the workgroup whose heads share them. Blocks of 32 are the work of a quad, as in
+// mx_kv.hip.
+
+#include <algorithm>
+
+#include "mx_common.h"
+#include "mx_kernels_impl.h"
+#include "mx_kv_rows.h"
+#include "mx_pages.h"
+
+namespace mx {
+
+constexpr int AP_THREADS = 256;
+constexpr int AP_BLOCKS = AP_THREADS / 4;   // quads
+constexpr int AP_TOK = 8;                   // tokens a workgroup
+constexpr int AP_HALF = 128;                // pairs at most (head dim 256)
+
+__device__ __forceinline__ float4v ap_load4(const KvPlainRows & x, int64_t at) {
+    if (!x.f16) return *(const float4v *)((const float *)x.x + at);
+    const half4 v = *(const half4 *)((const uint16_t *)x.x + at);
+    return float4v{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+__device__ __forceinline__ void ap_store4(const KvPlainRows & x, int64_t at, const float * v) {
+    if (x.f16) *(u32x2 *)((uint16_t *)x.x + at) = u32x2{pack2h(v[0], v[1]), pack2h(v[2], v[3])};
+    else *(float4v *)((float *)x.x + at) = float4v{v[0], v[1], v[2], v[3]};
+}
+
+// A workgroup takes tok_wg tokens of a sequence, one after the other, or one of `parts` of a token's blocks, of K, of V or of
+// Q. A row that a later token (of this sequence or the next ones) has too, because tables share a page where they
+// are written, is left to the last of them, so that it is whole: every workgroup of K and V looks at the pages that
+// the step writes behind its own.
+__global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
+    __shared__ float cs[AP_TOK][AP_HALF][2];
+    __shared__ int64_t at_row[AP_TOK];
+    __shared__ int pos[AP_TOK], entry[AP_TOK], off[AP_TOK], dead[AP_TOK];   // dead: 1 its row is not written, 2 nor its query
+    const int t = threadIdx.x, l = t % 4;
+    int what = 0;
+    while (what + 1 < a.n_rows && (int)blockIdx.x >= a.r[what + 1].wg_begin) what++;
+    const KvAppendRows & r = a.r[what];
+    const int wg = (int)blockIdx.x - r.wg_begin, grp = fq_div(wg, r.div_parts), part = wg - grp * r.parts;
+    const int s = fq_div(grp, r.div_groups), t0 = (grp - s * r.groups) * r.tok_wg;
+    const StepOf sq = step_of(a.st, s);
+    const int toks = min(r.tok_wg, sq.fresh - t0);
+    if (sq.bad && t == 0 && t0 == 0 && a.st.err) *a.st.err = 1;
+    if (toks <= 0) return;
+    const int per = (r.items + r.parts - 1) / r.parts;
+    const int begin = part * per, end = r.parts > 1 ? min(r.items, begin + per) : toks * r.items;
+    const int rotated = r.rotate ? 2 * a.half : 0;
+
+    auto load = [&](int it, float (&v)[8], float (&w)[8]) {   // a block's values and those they are paired with
+        const int tok = fq_div(it, r.div_items), hb = it - tok * r.items, h = fq_div(hb, r.div_bph), b = hb - h * r.bph;
+        const int64_t at = (int64_t)s * r.x.nb3 + (int64_t)(t0 + tok) * r.x.nb1 + (int64_t)h * r.x.nb2;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const int j = 32 * b + 16 * g + 4 * l;
+            const float4v y = ap_load4(r.x, at + j);
+            float4v z = y;
+            if (a.neox && j < rotated) z = ap_load4(r.x, at + (j < a.half ? j + a.half : j - a.half));
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[4 * g + e] = y[e];
+                w[4 * g + e] = z[e];
+            }
+        }
+    };
+    float v[8], w[8];
+    if (begin + t / 4 < end) load(begin + t / 4, v, w);
+
+    // ---- rows and positions of the tokens ----
+    if (t < WAVE) {
+        int depth = t0 + t;
+        if (a.st.parent) {
+            const uint64_t anc = tree_ancestors(t < a.st.T ? a.st.parent[(int64_t)s * a.st.parent_nb + t] : -1, t);
+            depth = __shfl(__popcll(anc) - 1, t0 + t, WAVE);
+        }
+        if (t < toks) {
+            const int j = sq.past + t0 + t, pi = fq_div(j, a.st.div_page);
+            const int e = pi < a.st.n_table ? a.st.table[(int64_t)s * a.st.table_nb + pi] : -1;
+            const int64_t row = page_row(a.st, e);
+            entry[t] = e;
+            off[t] = j - pi * a.st.page;
+            at_row[t] = row + off[t];
+            pos[t] = a.pos ? a.pos[(int64_t)s * a.pos_nb + t0 + t] : sq.past + depth;
+            dead[t] = depth < 0 ? 2 : row < 0 ? 1 : 0;
+            if (dead[t] && a.st.err) *a.st.err = 1;
+        }
+    }
+    __syncthreads();
+    // ---- the sines, and the later owners of the rows ----
+    for (int i = t; i < toks * (rotated / 2); i += AP_THREADS) {
+        const int tok = fq_div(i, a.div_half), p = i - tok * a.half;
+        double sn, c;
+        sincos((double)pos[tok] * (double)a.freq[p], &sn, &c);
+        cs[tok][p][0] = (float)(c * (double)a.mscale);
+        cs[tok][p][1] = (float)(sn * (double)a.mscale);
+    }
+    if (what < 2) {
+        for (int i = s * a.span + t; i < a.st.S * a.span; i += AP_THREADS) {
+            const int s2 = fq_div(i, a.div_span), k = i - s2 * a.span;
+            const int p0 = a.st.n_past[s2], n2 = a.st.n_new ? min(a.st.n_new[s2], a.st.T) : a.st.T;
+            if (p0 < 0 || p0 >= a.st.n_table * a.st.page) continue;
+            const int pi = fq_div(p0, a.st.div_page) + k, first = pi * a.st.page;
+            if (pi >= a.st.n_table || first - p0 >= n2) continue;
+            const int e = a.st.table[(int64_t)s2 * a.st.table_nb + pi];
+            for (int u = 0; u < toks; u++)
+                if (e == entry[u]) {
+                    const int j = first + off[u];   // the row of s2 that this one is
+                    if (j >= p0 && j - p0 < n2 && (s2 > s || j > sq.past + t0 + u)) dead[u] |= 1;
+                }
+        }
+    }
+    __syncthreads();
+    // ---- blocks ----
+    for (int it = begin + t / 4; it < end; it += AP_BLOCKS) {
+        float v2[8], w2[8];
+        if (it + AP_BLOCKS < end) load(it + AP_BLOCKS, v2, w2);
+        const int tok = fq_div(it, r.div_items), hb = it - tok * r.items, h = fq_div(hb, r.div_bph), b = hb - h * r.bph;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const int j = 32 * b + 16 * g + 4 * l;
+            if (j >= rotated) continue;
+            if (a.neox) {
+                const bool second = j >= a.half;
+                const float * c = cs[tok][second ? j - a.half : j];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p = mul_rn(v[4 * g + e], c[2 * e]), q = mul_rn(w[4 * g + e], c[2 * e + 1]);
+                    v[4 * g + e] = sub_rn(p, second ? -q : q);
+                }
+            } else {
+                const float * c = cs[tok][j / 2];
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const float x0 = v[4 * g + e], x1 = v[4 * g + e + 1];
+                    v[4 * g + e] = sub_rn(mul_rn(x0, c[e]), mul_rn(x1, c[e + 1]));
+                    v[4 * g + e + 1] = sub_rn(mul_rn(x0, c[e + 1]), -mul_rn(x1, c[e]));
+                }
+            }
+        }
+        if (what == 2) {
+            if (dead[tok] < 2) {
+                const int64_t at = (int64_t)s * a.qr.nb3 + (int64_t)(t0 + tok) * a.qr.nb1 + (int64_t)h * a.qr.nb2 + 32 * b + 4 * l;
+                ap_store4(a.qr, at, v);
+                ap_store4(a.qr, at + 16, v + 4);
+            }
+        } else if (!dead[tok]) {   // the same for the quad
+            const KvRowsOut & o = a.o[what];
+            kv_quantize(o, at_row[tok] * o.nb1 + (int64_t)h * o.nb2 + 32 * b, l, v);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[e] = v2[e];
+            w[e] = w2[e];
+        }
+    }
+}
+
+// A block a quad while that makes fewer than 2048 workgroups, then more of them: up to eight whole tokens a workgroup.
+hipError_t launch_kv_append(KvAppendArgs a, hipStream_t st) {
+    int64_t all = 0, wgs = 0;
+    for (int k = 0; k < a.n_rows; k++) all += (int64_t)a.st.S * a.st.T * a.r[k].H * a.r[k].bph;
+    const int64_t per = std::max<int64_t>(AP_BLOCKS, all / 2048);
+    for (int k = 0; k < a.n_rows; k++) {
+        KvAppendRows & r = a.r[k];
+        r.items = r.H * r.bph;
+        r.tok_wg = (int)std::min<int64_t>({std::max<int64_t>(1, per / r.items), AP_TOK, a.st.T});
+        r.parts = per >= r.items ? 1 : (int)((r.items + per - 1) / per);
+        r.groups = (a.st.T + r.tok_wg - 1) / r.tok_wg;
+        r.wg_begin = (int)wgs;
+        wgs += (int64_t)a.st.S * r.groups * r.parts;
+        r.div_bph = fq_div_by(r.bph); r.div_items = fq_div_by(r.items); r.div_parts = fq_div_by(r.parts); r.div_groups = fq_div_by(r.groups);
+    }
+    a.span = (a.st.T + a.st.page - 2) / a.st.page + 1;
+    a.div_half = fq_div_by(std::max(1, a.half));
+    a.div_span = fq_div_by(a.span);
+    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)wgs), dim3(AP_THREADS), 0, st, a);
+    return hipGetLastError();
+}
+
+// A thread moves one block of 32 values and its scale, row after row. Source path[i] lies at or behind
+// destination i and behind every earlier source, so in that order no row is read after it was written: what is read for
+// i' > i lies behind i. KEEP_ILP rows are read before the first of them is written.
+constexpr int KEEP_ILP = 4;
+__global__ void __launch_bounds__(AP_THREADS) kv_keep_kernel(KvKeepArgs a) {
+    __shared__ int64_t from[KV_TREE_MAX], to[KV_TREE_MAX];
+    __shared__ int no;
+    const int t = threadIdx.x, s = blockIdx.x / a.wgs, wg = blockIdx.x % a.wgs;
+    const KvRowsOut & o = a.o[blockIdx.y];
+    const StepOf sq = step_of(a.st, s);
+    const int n = a.n_keep ? uniform_i32(a.n_keep, s) : a.A;
+    if (t == 0) no = sq.bad || n < 0 || n > a.A;
+    __syncthreads();
+    if (t < KV_TREE_MAX && t < min(n, a.A)) {
+        const int32_t * path = a.path + (int64_t)s * a.path_nb;
+        const int p = path[t], before = t ? path[t - 1] : -1;
+        bool ok = p >= t && p > before && p < sq.fresh;
+        if (ok) {
+            const int js = sq.past + p, jd = sq.past + t, ps = fq_div(js, a.st.div_page), pd = fq_div(jd, a.st.div_page);
+            const int32_t * table = a.st.table + (int64_t)s * a.st.table_nb;
+            const int64_t rs = ps < a.st.n_table ? page_row(a.st, table[ps]) : -1, rd = pd < a.st.n_table ? page_row(a.st, table[pd]) : -1;
+            ok = rs >= 0 && rd >= 0;
+            from[t] = rs + js - ps * a.st.page;
+            to[t] = rd + jd - pd * a.st.page;
+        }
+        if (!ok) no = 1;
+    }
+    __syncthreads();
+    if (no) {
+        if (t == 0 && a.st.err) *a.st.err = 1;
+        return;
+    }
+    const int hb = wg * AP_THREADS + t;
+    if (hb >= o.div_bpr.d) return;
+    const int h = fq_div(hb, o.div_bph), b = hb - h * o.bph;
+    const int64_t at = (int64_t)h * o.nb2 + 32 * b;
+    const int shift = o.type == T_F16 ? -1 : o.type == T_Q4_0;   // elements to bytes
+    const int pieces = o.type == T_F16 ? 4 : o.type == T_Q8_0 ? 2 : 1;
+    auto bytes = [&](int64_t e) { return shift < 0 ? 2 * e : e >> shift; };
+    for (int i0 = 0; i0 < n; i0 += KEEP_ILP) {
+        u32x4 x[KEEP_ILP][4];
+        uint16_t d[KEEP_ILP];
+#pragma unroll
+        for (int u = 0; u < KEEP_ILP; u++) {
+            if (i0 + u >= n) continue;
+            const int64_t e = from[i0 + u] * o.nb1 + at;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (c < pieces) x[u][c] = *(const u32x4 *)(o.q + bytes(e) + 16 * c);
+            if (o.type != T_F16) d[u] = o.d[e / 32];
+        }
+#pragma unroll
+        for (int u = 0; u < KEEP_ILP; u++) {
+            if (i0 + u >= n || from[i0 + u] == to[i0 + u]) continue;
+            const int64_t e = to[i0 + u] * o.nb1 + at;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (c < pieces) *(u32x4 *)(o.q + bytes(e) + 16 * c) = x[u][c];
+            if (o.type != T_F16) o.d[e / 32] = d[u];
+        }
+    }
+}
+
+hipError_t launch_kv_keep(KvKeepArgs a, hipStream_t st) {
+    int bpr = 0;
+    for (int k = 0; k < a.n_out; k++) {
+        a.o[k].div_bpr = fq_div_by(a.o[k].H * a.o[k].bph);
+        a.o[k].div_bph = fq_div_by(a.o[k].bph);
+        bpr = std::max(bpr, a.o[k].div_bpr.d);
+    }
+    a.wgs = (bpr + AP_THREADS - 1) / AP_THREADS;
+    hipLaunchKernelGGL(kv_keep_kernel, dim3((unsigned)(a.st.S * a.wgs), a.n_out), dim3(AP_THREADS), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace mx

@@ -95,6 +95,29 @@ class FaQArgs(ctypes.Structure):
                 ("scale", ctypes.c_float), ("max_bias", ctypes.c_float), ("softcap", ctypes.c_float)]
 
 
+class KvStepArgs(ctypes.Structure):
+    _fields_ = [("table_dev", ctypes.c_void_p), ("table_nb", ctypes.c_int64), ("n_past_dev", ctypes.c_void_p),
+                ("n_new_dev", ctypes.c_void_p), ("parent_dev", ctypes.c_void_p), ("parent_nb", ctypes.c_int64),
+                ("n_table", ctypes.c_int64), ("S", ctypes.c_int), ("T", ctypes.c_int), ("page", ctypes.c_int)]
+
+
+class KvAppendArgs(ctypes.Structure):
+    _fields_ = [("step", KvStepArgs), ("k", KvRows), ("v", KvRows), ("k_nb3", ctypes.c_int64), ("v_nb3", ctypes.c_int64),
+                ("q_dev", ctypes.c_void_p), ("q_nb1", ctypes.c_int64), ("q_nb2", ctypes.c_int64), ("q_nb3", ctypes.c_int64),
+                ("qr_dev", ctypes.c_void_p), ("qr_nb1", ctypes.c_int64), ("qr_nb2", ctypes.c_int64), ("qr_nb3", ctypes.c_int64),
+                ("q_type", ctypes.c_int), ("qr_type", ctypes.c_int), ("H", ctypes.c_int64), ("freq_dev", ctypes.c_void_p),
+                ("pos_dev", ctypes.c_void_p), ("pos_nb", ctypes.c_int64), ("n_rot", ctypes.c_int), ("neox", ctypes.c_int),
+                ("mscale", ctypes.c_float)]
+
+
+class FaPArgs(ctypes.Structure):
+    _fields_ = [("step", KvStepArgs), ("q_dev", ctypes.c_void_p), ("q_nb1", ctypes.c_int64), ("q_nb2", ctypes.c_int64),
+                ("q_nb3", ctypes.c_int64), ("k", KvView), ("v", KvView), ("n_rows", ctypes.c_int64), ("dst_dev", ctypes.c_void_p),
+                ("dst_nb1", ctypes.c_int64), ("dst_nb2", ctypes.c_int64), ("dst_nb3", ctypes.c_int64), ("q_type", ctypes.c_int),
+                ("dst_type", ctypes.c_int), ("D", ctypes.c_int), ("DV", ctypes.c_int), ("H", ctypes.c_int), ("HK", ctypes.c_int),
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("max_kv", ctypes.c_int64)]
+
+
 def lib():
     """Load the built backend library. Raises if it has not been built."""
     global _lib
@@ -152,6 +175,13 @@ def _bind_optional(L):
         L.mi355x_flash_attn_q_workspace.restype = sz
         L.mi355x_flash_attn_q_workspace.argtypes = [pq, i32]
         L.mi355x_flash_attn_q.argtypes = [pq, i32, vp, sz, vp]
+    if hasattr(L, "mi355x_kv_append"):
+        pp, ps = ctypes.POINTER(FaPArgs), ctypes.POINTER(KvStepArgs)
+        L.mi355x_kv_append.argtypes = [ctypes.POINTER(KvAppendArgs), vp, vp]
+        L.mi355x_flash_attn_paged_workspace.restype = sz
+        L.mi355x_flash_attn_paged_workspace.argtypes = [pp, i32]
+        L.mi355x_flash_attn_paged.argtypes = [pp, i32, vp, sz, vp, vp]
+        L.mi355x_kv_keep.argtypes = [ps, vp, i32, vp, i64, vp, i32, vp, vp]
     if hasattr(L, "mi355x_mul_mat_noalloc"):
         L.mi355x_mul_mat_noalloc.argtypes = [i32, vp, i64, i64, vp, i64, i64, vp, i64, vp]
     if hasattr(L, "mi355x_mul_mat_id"):
@@ -533,6 +563,164 @@ def flash_attn_q(q, k: KvCache, v: KvCache, mask, scale: float, softcap: float =
         raise MI355XError("flash_attn_q: the workspace is on another device")
     check(lib().mi355x_flash_attn_q(a, nsplit, workspace.data_ptr(), workspace.nbytes, _launch_stream(k.dev, "flash_attn_q")),
           "flash_attn_q")
+    return out
+
+
+# ---- a KV cache in pages --------------------------------------------------------------------
+
+class KvStep:
+    """A step of S sequences over caches in pages (mi355x_kv_step): page p of a cache [rows, HK, D] is its rows
+    p * page .. p * page + page - 1; sequence s holds n_past[s] rows, found through the pages table[s] names, and
+    adds up to T tokens, n_new[s] of them real (None: all), a chain or, with parents [S, T] (the number of the token
+    before, -1: the rows held; T <= 64), a tree. All int32 on one device, read when a call runs, not when the step is
+    made: a program keeps the step and changes the tensors' values."""
+
+    __slots__ = ("table", "n_past", "n_new", "parents", "S", "T", "page", "dev", "args")
+
+    def __init__(self, table, n_past, T: int, page: int, n_new=None, parents=None):
+        self.table, self.n_past, self.n_new, self.parents = table, n_past, n_new, parents
+        self.S, self.T, self.page, self.dev = table.shape[0], int(T), int(page), table.get_device()
+        i32 = _torch().int32
+        for t, shape in ((table, (self.S, None)), (n_past, (self.S,)), (n_new, (self.S,)), (parents, (self.S, self.T))):
+            if t is None:
+                continue
+            if (t.dtype != i32 or t.get_device() != self.dev or t.dim() != len(shape) or (t.shape[-1] > 1 and t.stride(-1) != 1)
+                    or any(n is not None and n != m for n, m in zip(shape, t.shape))):
+                raise MI355XError(f"KvStep: {t.dtype} {tuple(t.shape)} where an int32 of {shape} on the table's device is wanted")
+        if self.page <= 0 or self.page % 32 or self.T < 0:
+            raise MI355XError("KvStep: pages of whole 32-row tiles")
+        if parents is not None and self.T > 64:
+            raise MI355XError("KvStep: trees of at most 64 tokens")
+        self.args = KvStepArgs(table.data_ptr(), table.stride(0), n_past.data_ptr(), None if n_new is None else n_new.data_ptr(),
+                               None if parents is None else parents.data_ptr(), 0 if parents is None else parents.stride(0),
+                               table.shape[1], self.S, self.T, self.page)
+
+
+class Rope:
+    """The position rotation of kv_append: pair i of a head's first 2 * len(freq) dims, (2 i, 2 i + 1) or with neox
+    (i, i + len(freq)), turns by position * freq[i] (F32 on the device, radians a position); cosine and sine are
+    multiplied by mscale. positions [S, T] int32, or None: n_past[s] plus a token's depth."""
+
+    __slots__ = ("freq", "neox", "mscale", "positions")
+
+    def __init__(self, freq, neox: bool = False, mscale: float = 1.0, positions=None):
+        torch = _torch()
+        if freq.dtype != torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or freq.shape[0] % 4:
+            raise MI355XError("Rope: freq is a contiguous F32 tensor of a multiple of 4 values")
+        if positions is not None and (positions.dtype != torch.int32 or positions.dim() != 2 or positions.get_device() != freq.get_device()
+                                      or (positions.shape[-1] > 1 and positions.stride(-1) != 1)):
+            raise MI355XError("Rope: positions are int32 [S, T] on freq's device")
+        self.freq, self.neox, self.mscale, self.positions = freq, bool(neox), float(mscale), positions
+
+
+def rope_freqs(n_rot: int, base: float = 10000.0, factors=None, device="cuda"):
+    """base^(-2 i / n_rot), divided by factors[i] where given, formed in 64 bits: Rope's freq."""
+    torch = _torch()
+    f = base ** (-torch.arange(0, n_rot, 2, dtype=torch.float64) / n_rot)
+    if factors is not None:
+        f = f / torch.as_tensor(factors, dtype=torch.float64).cpu()
+    return f.float().to(device)
+
+
+def _step_rows(c, x, step, what):
+    """mi355x_kv_rows of cache [rows, H, D] and the step's plain rows x [S, T, H, D], with their sequence stride."""
+    t, n = _plain_types().get(x.dtype), x.stride()
+    if c._rows is None or len(c.shape) != 3 or x.shape != (step.S, step.T, *c._tail) or n[-1] != 1 or (t != F32 and t != F16) or x.get_device() != c.dev:
+        raise MI355XError(f"{what}: rows {x.dtype} {tuple(x.shape)} do not fit {step.S} x {step.T} rows of a cache {c.shape}")
+    return KvRows(*c._rows, t, x.data_ptr(), n[1], n[2]), n[0]
+
+
+def kv_append(step: KvStep, k_cache: KvCache, v_cache: KvCache, k, v, rope: Rope = None, q=None, q_out=None, err=None):
+    """The step's new keys k [S, T, HK, D], rotated, and values v [S, T, HK, DV] (F32 or F16) into the rows of their
+    tokens in the caches [rows, HK, D] and [rows, HK, DV], and the queries q [S, T, H, D], rotated, into q_out (a new tensor
+    like q by default), which is returned. One launch. Rows of padding are left as they were. err: a device int32 that
+    numbers out of range set to 1 (mi355x_kv_step)."""
+    dev = step.dev
+    if k_cache.dev != dev or v_cache.dev != dev:
+        raise MI355XError("kv_append: the caches are on another device than the step")
+    kr, k3 = _step_rows(k_cache, k, step, "kv_append")
+    vr, v3 = _step_rows(v_cache, v, step, "kv_append")
+    a = KvAppendArgs(step.args, kr, vr, k3, v3)
+    if q is not None:
+        if q_out is None:
+            q_out = _torch().empty_like(q)
+        types = _plain_types()
+        for x in (q, q_out):
+            if x.dim() != 4 or x.shape != q.shape or x.stride(-1) != 1 or types.get(x.dtype) not in (F32, F16) or x.get_device() != dev:
+                raise MI355XError(f"kv_append: queries {x.dtype} {tuple(x.shape)}")
+        if q.shape[:2] != (step.S, step.T) or q.shape[3] != k_cache.D:
+            raise MI355XError(f"kv_append: queries {tuple(q.shape)} of a step of {step.S} x {step.T} tokens and heads of {k_cache.D}")
+        qn, on = q.stride(), q_out.stride()
+        a.q_dev, a.q_nb1, a.q_nb2, a.q_nb3, a.q_type = q.data_ptr(), qn[1], qn[2], qn[0], types[q.dtype]
+        a.qr_dev, a.qr_nb1, a.qr_nb2, a.qr_nb3, a.qr_type = q_out.data_ptr(), on[1], on[2], on[0], types[q_out.dtype]
+        a.H = q.shape[2]
+    if rope is not None:
+        p = rope.positions
+        if rope.freq.get_device() != dev or (p is not None and p.shape != (step.S, step.T)):
+            raise MI355XError("kv_append: the rotation is not this step's")
+        a.freq_dev, a.n_rot, a.neox, a.mscale = rope.freq.data_ptr(), 2 * rope.freq.shape[0], rope.neox, rope.mscale
+        if p is not None:
+            a.pos_dev, a.pos_nb = p.data_ptr(), p.stride(0)
+    check(lib().mi355x_kv_append(a, _kv_err(err, dev, "kv_append"), _launch_stream(dev, "kv_append")), "kv_append")
+    return q_out
+
+
+def kv_keep(step: KvStep, caches, path, n_keep=None, err=None):
+    """The rows of the step's tokens path[s, i] (int32 [S, A], A <= 64, increasing) copied to those of tokens i, for i <
+    n_keep[s] (int32 [S]; None: A each), in each of up to four caches [rows, H, D]: a path of accepted drafts becomes
+    the next rows of its sequence. One launch."""
+    dev, i32 = step.dev, _torch().int32
+    if not 1 <= len(caches) <= 4 or any(c.dev != dev or c._rows is None for c in caches):
+        raise MI355XError("kv_keep: one to four caches [rows, H, D] on the step's device")
+    if path.dtype != i32 or path.dim() != 2 or path.shape[0] != step.S or path.get_device() != dev or (path.shape[1] > 1 and path.stride(1) != 1):
+        raise MI355XError("kv_keep: path is int32 [S, A] on the step's device")
+    if n_keep is not None and (n_keep.dtype != i32 or n_keep.shape != (step.S,) or n_keep.get_device() != dev or (step.S > 1 and n_keep.stride(0) != 1)):
+        raise MI355XError("kv_keep: n_keep is int32 [S] on the step's device")
+    rows = (KvRows * len(caches))(*[KvRows(*c._rows) for c in caches])
+    check(lib().mi355x_kv_keep(step.args, rows, len(caches), path.data_ptr(), path.stride(0), None if n_keep is None else n_keep.data_ptr(),
+                               path.shape[1], _kv_err(err, dev, "kv_keep"), _launch_stream(dev, "kv_keep")), "kv_keep")
+
+
+def _fa_p_args(q, k, v, step, out, scale, softcap, max_kv):
+    types, qs, os = _plain_types(), q.shape, out.shape
+    dev = step.dev
+    if len(qs) != 4 or len(k.shape) != 3 or len(v.shape) != 3 or qs[0] != step.S or qs[2] != step.T or k.shape[-1] != qs[3] or k.shape[:2] != v.shape[:2]:
+        raise MI355XError(f"flash_attn_paged: q {tuple(qs)}, k {k.shape} and v {v.shape} do not fit a step of {step.S} x {step.T} tokens")
+    if os != (step.S, step.T, qs[1], v.shape[-1]):
+        raise MI355XError(f"flash_attn_paged: out {tuple(os)}")
+    qn, on, qt, ot = q.stride(), out.stride(), types.get(q.dtype), types.get(out.dtype)
+    if qn[-1] != 1 or on[-1] != 1 or qt not in (F32, F16) or ot not in (F32, F16):
+        raise MI355XError("flash_attn_paged: q and out are F32 or F16 with contiguous rows")
+    if k.dev != dev or v.dev != dev or q.get_device() != dev or out.get_device() != dev:
+        raise MI355XError("flash_attn_paged: all tensors on one device")
+    kt, kq, kd, rows, k1, k2, HK, D = k._rows
+    vt, vq, vd, _, v1, v2, _, DV = v._rows
+    return FaPArgs(step.args, q.data_ptr(), qn[2], qn[1], qn[0], KvView(kt, kq, kd, k1, k2, 0), KvView(vt, vq, vd, v1, v2, 0), rows,
+                   out.data_ptr(), on[2], on[1], on[0], qt, ot, D, DV, qs[1], HK, scale, softcap, max_kv)
+
+
+def flash_attn_paged_workspace(q, k: KvCache, v: KvCache, step: KvStep, out, nsplit: int = 0, max_kv: int = 0) -> int:
+    """Workspace bytes mi355x_flash_attn_paged needs for these operands (0 for an unsupported op)."""
+    return int(lib().mi355x_flash_attn_paged_workspace(_fa_p_args(q, k, v, step, out, 1.0, 0.0, max_kv), nsplit))
+
+
+def flash_attn_paged(q, k: KvCache, v: KvCache, step: KvStep, scale: float, softcap: float = 0.0, nsplit: int = 0, out=None,
+                     workspace=None, max_kv: int = 0, err=None):
+    """Attention of a step's tokens, q [S, H, T, D] (F32 or F16), over caches in pages k [rows, HK, D] and v [rows, HK, DV]: each
+    token sees the rows its sequence held, itself and the tokens above it. Returns dst [S, T, H, DV], F32 unless `out` is
+    F16; padding is zeros. max_kv: a bound of n_past + n_new that the caller knows (0: what the tables can hold), for
+    the launch's plan alone."""
+    torch = _torch()
+    if out is None:
+        out = torch.empty(q.shape[0], q.shape[2], q.shape[1], v.shape[-1], dtype=torch.float32, device=q.device)
+    a = _fa_p_args(q, k, v, step, out, scale, softcap, max_kv)
+    if workspace is None:
+        need = int(lib().mi355x_flash_attn_paged_workspace(a, nsplit))
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != step.dev:
+        raise MI355XError("flash_attn_paged: the workspace is on another device")
+    check(lib().mi355x_flash_attn_paged(a, nsplit, workspace.data_ptr(), workspace.nbytes, _kv_err(err, step.dev, "flash_attn_paged"),
+                                        _launch_stream(step.dev, "flash_attn_paged")), "flash_attn_paged")
     return out
 
 

@@ -392,6 +392,88 @@ MI355X_API size_t mi355x_flash_attn_q_workspace(const mi355x_fa_q_args * a, int 
 MI355X_API int mi355x_flash_attn_q(const mi355x_fa_q_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
                                    void * stream);
 
+/* ---- a KV cache in pages: append, attention of chains and trees of new tokens, keep ----------- */
+
+/* A step of S sequences over caches in pages. The cache is rows [n_rows][HK][D], page p its rows p * page
+ * up to p * page + page - 1 (rows behind the last whole page belong to none). Sequence s has logical rows j: row
+ * table[s][j / page] * page + j % page of the cache. It holds n_past[s] of them; this step's tokens t < n_new[s] are its
+ * logical rows n_past[s] + t, the others up to T are padding. parent[s][t], if given, makes the tokens a tree:
+ * the number of the token that t follows, before its own, or -1 for one that follows the n_past rows;
+ * without it each follows the one before. All of it is read on the device, when the call runs: a captured call
+ * follows the lengths and tables of its replay. A token whose way up its parents meets any other number counts
+ * as padding. n_past outside [0, n_table * page] counts as a sequence without new tokens, n_new outside [0, T] as
+ * the nearest of the two; logical rows behind the table and rows of pages that the cache does not have are neither
+ * read nor written. Each of these sets *err_dev of the call (a device int32, may be NULL) to 1; table entries that no
+ * row needs are not looked at. */
+typedef struct mi355x_kv_step {
+    const int32_t * table_dev;  int64_t table_nb;    /* [S][n_table], sequence stride in elements */
+    const int32_t * n_past_dev;                      /* [S] */
+    const int32_t * n_new_dev;                       /* [S], or NULL: T */
+    const int32_t * parent_dev; int64_t parent_nb;   /* [S][T], T <= 64, or NULL */
+    int64_t n_table;                                 /* entries a sequence, n_table * page <= 2^29 */
+    int S, T, page;                                  /* page: a multiple of 32; S * T <= 2^22 */
+} mi355x_kv_step;
+
+/* Position rotation and storing of a step's tokens: the keys x of `k`, rotated, and the values x of `v` go to the
+ * rows of their tokens, as mi355x_set_rows stores them (types, bits and plain types as there; x_nb1 and x_nb2 are the
+ * token and head strides, k_nb3 and v_nb3 the sequence strides; n_rows the caches' rows); the queries q [S][T][H][D of k],
+ * rotated, to qr. q_dev NULL: no queries. q and qr are each F32 (0) or F16 (1); qr may be q where types and strides agree
+ * and n_rot is 0 or the pairs are neighbours (neox 0).
+ * Pair i < n_rot / 2 of a head's dims, (2 i, 2 i + 1) or with neox (i, i + n_rot / 2), turns by theta = p * freq_dev[i], p the
+ * position pos_dev[s][t], or, without it, n_past[s] plus the number of tokens above t: c = cos(theta) * mscale and s
+ * likewise are formed in 64 bits and rounded to f32, then a' = a c - b s and b' = a s + b c with every product and sum
+ * rounded to f32. n_rot: a multiple of 8 up to D and 256, or 0. Dims from n_rot on stay as they are.
+ * Where tables share a page and two tokens' rows are one, the last token's (by sequence, then number) stays, whole.
+ * Rows and queries of padding are left as they were. A token without a row in the cache is not stored; its query is
+ * rotated. K and V are different caches. H * D / 32 of each at most 2^16. */
+typedef struct mi355x_kv_append_args {
+    mi355x_kv_step step;
+    mi355x_kv_rows k, v;
+    int64_t k_nb3, v_nb3;
+    const void * q_dev;   int64_t q_nb1, q_nb2, q_nb3;      /* token, head, sequence strides, multiples of 8 */
+    void * qr_dev;        int64_t qr_nb1, qr_nb2, qr_nb3;
+    int q_type, qr_type;
+    int64_t H;
+    const float * freq_dev;
+    const int32_t * pos_dev; int64_t pos_nb;                /* [S][T], sequence stride; or NULL */
+    int n_rot, neox;
+    float mscale;
+} mi355x_kv_append_args;
+MI355X_API int mi355x_kv_append(const mi355x_kv_append_args * a, int32_t * err_dev, void * stream);
+
+/* Attention of a step's tokens over a cache in pages, K and V [n_rows][HK][D] each Q8_0 or Q4_0 (any mix), or both
+ * F16 (values at q_dev, d_dev not read): dst[s][t] = softmax over the keys that t sees of cap(scale * q.k), times v.
+ * Token t of sequence s sees its n_past[s] rows, itself and the tokens above it. Padding, and a token none of whose keys
+ * lies in the cache, are written as zeros. A key that a token does not see adds nothing to it, whatever the cache holds there, NaN
+ * included. Roundings and limits of the values as in mi355x_flash_attn_q.
+ * max_kv: what no n_past + n_new passes, as far as the caller knows (0: n_table * page); it only plans the launch.
+ * H % HK == 0; D and DV multiples of 32 up to 256; S * HK row tiles of 16 (T * H / HK rows) as there. */
+typedef struct mi355x_fa_p_args {
+    mi355x_kv_step step;
+    const void * q_dev;   int64_t q_nb1, q_nb2, q_nb3;         /* token, head, sequence strides */
+    mi355x_kv_view k, v;                                       /* nb1 the row, nb2 the head stride; nb3 is not read */
+    int64_t n_rows;                                            /* rows of K and of V */
+    void * dst_dev;       int64_t dst_nb1, dst_nb2, dst_nb3;   /* head, token, sequence strides */
+    int q_type, dst_type;                                      /* 0 F32 or 1 F16 */
+    int D, DV, H, HK;
+    float scale, softcap;
+    int64_t max_kv;
+} mi355x_fa_p_args;
+/* Workspace bytes of mi355x_flash_attn_paged with `nsplit` KV splits (0 = its own choice); 0 for an op that it does not
+ * take. It follows the sizes and max_kv, not what lies on the device. 256-byte aligned. */
+MI355X_API size_t mi355x_flash_attn_paged_workspace(const mi355x_fa_p_args * a, int nsplit);
+/* Concurrent calls must not share a workspace. Equal inputs give equal bits. */
+MI355X_API int mi355x_flash_attn_paged(const mi355x_fa_p_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
+                                       int32_t * err_dev, void * stream);
+
+/* Accepted tokens kept: for i = 0 .. n_keep[s] - 1 in this order, the row of token path[s][i] is copied to the row of token
+ * i, bit by bit, in each of `n_out` (1..4) caches (the step's n_past then grows by n_keep). The rows' x is not read.
+ * A path is increasing, its numbers below n_new[s]; n_keep NULL: A each. A sequence whose path or numbers are not so, or
+ * whose rows are not all in the cache, is left as it is and sets *err_dev. A <= 64. Pages that a step moves
+ * rows in belong to one sequence, once. */
+MI355X_API int mi355x_kv_keep(const mi355x_kv_step * step, const mi355x_kv_rows * r, int n_out, const int32_t * path_dev,
+                              int64_t path_nb, const int32_t * n_keep_dev, int A, int32_t * err_dev, void * stream);
+
 /* ---- MUL_MAT_ID --------------------------------------------------------------------------- */
 
 /* One expert-GEMM op. Strides in ELEMENTS. */
