@@ -991,11 +991,12 @@ static int fa_p_check(const mi355x_fa_p_args * a, int nsplit, mx::FaPArgs & f) {
     if (!empty && (!a->q_dev || !a->dst_dev)) return MI355X_E_ARG;
     if (a->D <= 0 || a->DV <= 0 || a->D % 32 || a->DV % 32 || !mx::fa_pad_dims(a->D, a->DV, f.D, f.DV)) return MI355X_E_UNSUPPORTED;
     if (2 * a->D < f.D || 2 * a->DV < f.DV) return MI355X_E_UNSUPPORTED;   // the loads of scales
+    const bool f16 = a->k.type == mx::T_F16;
     for (const mi355x_kv_view * w : {&a->k, &a->v}) {
-        if (!kv_type(w->type)) return MI355X_E_UNSUPPORTED;
+        if (f16 ? w->type != mx::T_F16 : !kv_type(w->type)) return MI355X_E_UNSUPPORTED;
         if (w->nb1 < 0 || w->nb2 < 0 || w->nb1 % 32 || w->nb2 % 32 || w->nb1 >= mx::FA_Q_MAX_NB1) return MI355X_E_ARG;
         if ((!empty && !w->q_dev) || !aligned(w->q_dev, 16)) return MI355X_E_ARG;
-        if ((!empty && !w->d_dev) || !aligned(w->d_dev, 8)) return MI355X_E_ARG;
+        if (!f16 && ((!empty && !w->d_dev) || !aligned(w->d_dev, 8))) return MI355X_E_ARG;
     }
     if (a->H <= 0 || a->HK <= 0 || a->H % a->HK || a->max_kv < 0 || nsplit > 64) return MI355X_E_ARG;
     const int64_t tiles = (int64_t)Sn * a->HK * (((int64_t)T * (a->H / a->HK) + 15) / 16);

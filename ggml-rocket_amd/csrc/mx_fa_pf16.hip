@@ -1,0 +1,467 @@
+// SPDX-License-Identifier: MIT
+// Attention of few query rows over an fp16 cache in pages, for gfx950: single tokens, trees of drafts, short prompts.
+//
+//   O[t,h,:] = softmax over the keys that t sees of cap(scale * q[h,t].k[hk,j]), times v[hk,j,:],  hk = h / G, G = H / HK
+//
+// The plan of mx_fa_q.h without its codes: a wave takes 16 NQ query rows of a KV head and 32 keys at a time, S^T = K . Q^T and
+// O^T += V^T . P^T in 16x16x32 MFMAs, so that everything of a row is in the four lanes of its column; K and V come by LDS
+// DMA into buffers of the wave's own and no barrier is in the loop. K's operand is one 16-byte read of LDS (a key's eight
+// dims), V's two transposing reads (ds_read_b64_tr_b16: the lanes i of a group of 16 point at 4 dims of key i / 4, and lane
+// i receives dim i of the four keys).
+// Roundings: Q and P, once each, to fp16; K and V are exact, scores, statistics, sums and O F32.
+//
+// A key that a row does not see has P = 0, and 0 times a V that is no number would still be none. So in the tiles that
+// hold such a key (the last ones of a sequence; all tiles of a block with padding) those of its values that are not finite
+// count as zeros, and the rows that do see the key get a sum of NaN instead.
+
+#include "mx_fa_q.h"
+
+namespace mx {
+
+// NB: tiles of a wave in LDS; NW: waves a block.
+template <int DK, int DV, int NQ, int NB, int NW>
+struct FpCfg {
+    static constexpr int KS = DK / 32, TT = DV / 16;
+    // 16-byte chunks of a row (K: a power of two), DMA instructions a tile
+    static constexpr int KCH = DK <= 64 ? 8 : DK <= 128 ? 16 : 32, VCH = DV / 8, KD = KCH / 2, VD = VCH / 2;
+    static constexpr int K_BYTES = FQ_KEYS * 16 * KCH, STAGE = K_BYTES + FQ_KEYS * 16 * VCH, VRB = 16 * VCH;
+    // Chunk c of K row r lies at c ^ kswz(r), so that the 16 rows of a read lie in 16 different chunks of LDS's 256-byte
+    // window; chunk c of V row r at c ^ 2 vswz(r): the eight 32-byte pieces that 32 lanes read (keys 8 g + 0..3 or 4..7, g two
+    // neighbours) in eight different places of it.
+    __device__ static __forceinline__ int kswz(int r) { return KCH >= 16 ? r & 15 : (r / 2) & 7; }
+    __device__ static __forceinline__ int vswz(int r) { return VCH >= 16 ? (r & 3) | (r >> 1 & 4) : (r >> 1 & 1) | (r >> 2 & 2); }
+    static constexpr int CT = TT * NQ < 8 ? TT * NQ : 8;      // O^T tiles merged at a time
+    static constexpr int LOOP_LDS = NW * NB * STAGE;
+    static constexpr int MERGE_LDS = NW * 16 * NQ * 8 + NW * CT * 1024;
+    static constexpr int LDS = MERGE_LDS > LOOP_LDS ? MERGE_LDS : LOOP_LDS;
+    static_assert(LDS <= FQ_LDS_MAX, "LDS");
+};
+
+// V^T operands of four tiles of 16 dims from addresses a[i] (keys 8 g ..), OFF further, and ROWS4 behind it (keys 8 g + 4 ..):
+// one statement with its wait, as fq_read_tr.
+template <int OFF, int ROWS4>
+__device__ __forceinline__ void fp_read_tr(const uint32_t (&a)[4], fq_v2i (&w)[8]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n"
+                 "ds_read_b64_tr_b16 %1, %8 offset:%13\n"
+                 "ds_read_b64_tr_b16 %2, %9 offset:%12\n"
+                 "ds_read_b64_tr_b16 %3, %9 offset:%13\n"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n"
+                 "ds_read_b64_tr_b16 %5, %10 offset:%13\n"
+                 "ds_read_b64_tr_b16 %6, %11 offset:%12\n"
+                 "ds_read_b64_tr_b16 %7, %11 offset:%13\n"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF), "n"(OFF + ROWS4)
+                 : "memory");
+}
+
+// Bits of the halves of x that are not finite: 0x8000 of each.
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) { return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+
+template <int DK, int DV, int NQ, int NB, int NW>
+__global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) fa_pf16_kernel(FaPArgs a) {
+    using C = FpCfg<DK, DV, NQ, NB, NW>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    asm volatile("" ::"s"(a.q), "s"(a.k.nb3), "s"(a.v.nb2), "s"(a.dst), "s"(a.dst_nb3), "s"(a.T), "s"(a.div_split.mul), "s"(a.softcap), "s"(a.st.table),
+                 "s"(a.st.parent_nb), "s"(a.div_tpp.mul));   // all lines of the arguments at once
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int r = lane % 16, g = lane / 16;
+
+    // block -> (sequence, split, KV head, query rows), as fa_q_kernel
+    int b = xcd_tile(blockIdx.x, gridDim.x), b1 = fq_div(b, a.div_nrt);
+    const int rt = b - b1 * a.nrt;
+    b = b1;
+    b1 = fq_div(b, a.div_hk);
+    const int hk = b - b1 * a.HK, s = fq_div(b1, a.div_split), split = b1 - s * a.nsplit;
+    const StepOf sq = step_of(a.st, s);
+    const int n_past = sq.past, n_new = sq.fresh;
+    if (sq.bad && threadIdx.x == 0 && a.st.err) *a.st.err = 1;
+    const int tok_a = fq_div(rt * 16 * NQ, a.div_g), tok_b = fq_div(min(a.R, (rt + 1) * 16 * NQ) - 1, a.div_g);
+    const int seen = a.st.parent ? n_new : min(n_new, tok_b + 1);
+    const int keys = tok_a < n_new ? min(n_past + seen, a.st.n_table * a.st.page) : 0;
+    const int up = a.st.parent && lane < a.T ? a.st.parent[(int64_t)s * a.st.parent_nb + lane] : -1;
+    const int ntiles = (keys + FQ_KEYS - 1) / FQ_KEYS, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    const int tile0 = split * per, tile1 = min(ntiles, tile0 + per), tile_end = max(ntiles, 1) - 1;
+
+    // Q in the B layout of the Q.K products: lane (row r, dims 8 g + 0..7 of a block of 32); past dk zeros
+    bool ok[NQ];
+    int tok[NQ];
+    int64_t qat[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int row = (rt * NQ + n) * 16 + r;
+        ok[n] = row < a.R;
+        tok[n] = ok[n] ? fq_div(row, a.div_g) : 0;
+        const int head = hk * a.G + (ok[n] ? row - tok[n] * a.G : 0);
+        qat[n] = (int64_t)s * a.q_nb3 + (int64_t)head * a.q_nb2 + (int64_t)tok[n] * a.q_nb1 + 8 * g;
+    }
+    u32x4 qraw[NQ][C::KS][2];   // eight values each: F32, or F16 in the first
+    if (a.q_f16) {
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+#pragma unroll
+            for (int st = 0; st < C::KS; st++) {
+                qraw[n][st][0] = *(const u32x4 *)((const uint16_t *)a.q + qat[n] + (32 * st < a.dk ? 32 * st : 0));
+                qraw[n][st][1] = u32x4{0, 0, 0, 0};
+            }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+#pragma unroll
+            for (int st = 0; st < C::KS; st++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    qraw[n][st][h] = *(const u32x4 *)((const float *)a.q + qat[n] + (32 * st < a.dk ? 32 * st : 0) + 4 * h);
+    }
+
+    const uint16_t * const kq = (const uint16_t *)a.k.q + (int64_t)hk * a.k.nb2;
+    const uint16_t * const vq = (const uint16_t *)a.v.q + (int64_t)hk * a.v.nb2;
+    // this lane's chunk of each DMA instruction: byte offset from the tile's first row; chunks past dk or dv the first ones
+    uint32_t kdma[C::KD], vdma[C::VD];
+#pragma unroll
+    for (int q = 0; q < C::KD; q++) {
+        const int slot = q * WAVE + lane, row = slot / C::KCH, c = (slot % C::KCH) ^ C::kswz(row);
+        const uint32_t key = row % 16 / 4 * 8 + row / 16 * 4 + row % 4;   // K rows lie in the order 16 h + 4 g + e (key 8 g + 4 h + e)
+        kdma[q] = key * 2 * (uint32_t)a.k.nb1 + (c * 8 < a.dk ? 16 * c : 0);
+    }
+#pragma unroll
+    for (int q = 0; q < C::VD; q++) {
+        const int slot = q * WAVE + lane, key = slot / C::VCH, c = (slot % C::VCH) ^ (2 * C::vswz(key));
+        vdma[q] = key * 2 * (uint32_t)a.v.nb1 + (c * 8 < a.dv ? 16 * c : 0);
+    }
+    uint8_t * const wl = smem + wave * NB * C::STAGE;
+    // where this lane reads: chunk 4 i + g of K row r (i: kra ^ 64 i), 4 dims of V row 8 g + r / 4 (tile of 16 dims i: vra ^ 32 i)
+    const uint32_t kra = r * C::KCH * 16 + ((g ^ C::kswz(r)) << 4);
+    const int vrow = 8 * g + r / 4;
+    const uint32_t vra = (uint32_t)(uintptr_t)(fq_lptr_t)wl + C::K_BYTES + vrow * C::VRB + (((r % 4 / 2) ^ (2 * C::vswz(vrow))) << 4) + 8 * (r % 2);
+
+    auto page_of = [&](int t) -> int64_t {   // the row where tile t begins, -1 for a tile of a page that the cache does not have
+        const int p = fq_div(t, a.div_tpp);
+        const int64_t row = page_row(a.st, uniform_i32(a.st.table, (int64_t)s * a.st.table_nb + p));
+        return row < 0 ? -1 : row + FQ_KEYS * (t - p * a.div_tpp.d);
+    };
+    auto dma_k = [&](int64_t row, int buf) {
+        const __amdgpu_buffer_rsrc_t kt = fq_rsrc(kq + max(row, (int64_t)0) * a.k.nb1);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < C::KD; q++) fq_dma16(kt, kdma[q], wl + buf * C::STAGE + q * 1024);
+        asm volatile("" ::: "memory");
+    };
+    auto dma_v = [&](int64_t row, int buf) {
+        const __amdgpu_buffer_rsrc_t vt = fq_rsrc(vq + max(row, (int64_t)0) * a.v.nb1);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < C::VD; q++) fq_dma16(vt, vdma[q], wl + buf * C::STAGE + C::K_BYTES + q * 1024);
+        asm volatile("" ::: "memory");
+    };
+    // The wave's tiles are tile0 + wave + NW k, k < nk; each buffer's next tile is NB further. Waves without a tile read one all
+    // the same, and behind the last the last again: the loads in flight stay what the waits count.
+    const int nk = tile1 - tile0 > wave ? (tile1 - tile0 - wave + NW - 1) / NW : 0;
+    int t = min(tile0 + wave, tile_end);
+    int64_t row_t = page_of(t), row_n = NB == 2 ? page_of(min(t + NW, tile_end)) : 0, row_p = page_of(min(t + NB * NW, tile_end));
+    dma_k(row_t, 0);
+    dma_v(row_t, 0);
+    if constexpr (NB == 2) {
+        dma_k(row_n, 1);
+        dma_v(row_n, 1);
+    }
+
+    // Q, scaled, fp16; a row outside [2^-6, 2^15] divided by a factor that multiplies its scores (fa_q_kernel)
+    half8 qf[NQ][C::KS];
+    float qfac[NQ];
+    bool scaled = false;
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        float amax = 0.0f;
+        auto value = [&](int st, int e) {
+            const float x = a.q_f16 ? h2f_bits((uint16_t)(qraw[n][st][0][e / 2] >> (16 * (e % 2)))) : __uint_as_float(qraw[n][st][e / 4][e % 4]);
+            return ok[n] && 32 * st < a.dk ? x * a.scale : 0.0f;
+        };
+#pragma unroll
+        for (int st = 0; st < C::KS; st++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(value(st, e)));
+        amax = fq_col_max(amax);
+        qfac[n] = (amax > 32768.0f || (amax < 0.015625f && amax > 0.0f)) ? fmaxf(amax / 16.0f, 0x1p-120f) : 1.0f;
+        const float inv = 1.0f / qfac[n];
+#pragma unroll
+        for (int st = 0; st < C::KS; st++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) qf[n][st][e] = (_Float16)(value(st, e) * inv);
+        scaled |= qfac[n] != 1.0f;
+    }
+    scaled = __any(scaled);
+    // row n of this lane sees keys below lim[n] and, of the new tokens', those whose bits are set in anc[n]
+    int lim[NQ], full_to;
+    uint64_t anc[NQ];
+    {
+        const uint64_t node = a.st.parent ? tree_ancestors(up, lane) : 0;
+        if (a.st.parent && lane < n_new && !node && a.st.err) *a.st.err = 1;
+        const int all = n_past + (a.st.parent ? 0 : tok_a + 1);
+        bool none = false;
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            lim[n] = tok[n] < n_new ? n_past : 0;
+            anc[n] = 0;
+            if (a.st.parent) {
+                const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)node, tok[n], WAVE), hi = (uint32_t)__shfl((int)(uint32_t)(node >> 32), tok[n], WAVE);
+                anc[n] = tok[n] < n_new ? (uint64_t)hi << 32 | lo : 0;
+                if (!anc[n]) lim[n] = 0;
+            } else if (tok[n] < n_new) {
+                lim[n] = n_past + tok[n] + 1;
+            }
+            none |= ok[n] && lim[n] < all;
+        }
+        full_to = __any(none) ? 0 : min(keys, all);   // every key below counts for every row
+    }
+
+    float4v o[NQ][C::TT];
+    float m_run[NQ], l_run[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        m_run[n] = -INFINITY;
+        l_run[n] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < C::TT; q++) o[n][q] = float4v{0, 0, 0, 0};
+    }
+    const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
+    const float cap2 = a.softcap != 0.0f ? 2.0f * FQ_LOG2E / a.softcap : 0.0f;
+
+    auto tile = [&](auto buffer) __attribute__((always_inline)) {
+        constexpr int BUF = decltype(buffer)::value;
+        fq_wait_vm<C::VD + (NB - 1) * (C::KD + C::VD)>();   // K has landed
+        const uint8_t * const st = wl + BUF * C::STAGE;
+        float4v sc[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; n++) sc[n][0] = sc[n][1] = float4v{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < C::KS; i++)
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const half8 kf = *(const half8 *)(st + (kra ^ (uint32_t)(64 * i)) + hf * 256 * C::KCH);
+#pragma unroll
+                for (int n = 0; n < NQ; n++) sc[n][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n][i], sc[n][hf], 0, 0, 0);
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        dma_k(row_p, BUF);
+        const bool masked = FQ_KEYS * (t + 1) > full_to || row_t < 0;
+        uint32_t vis[NQ];   // masked: which of this lane's eight keys row n sees
+        u32x4 pf[NQ];       // P, fp16
+        if (masked && row_t < 0 && a.st.err) *a.st.err = 1;
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            if (scaled) {
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[n][hf][e] *= qfac[n];
+            }
+            if (a.softcap != 0.0f) {
+                // cap * tanh(s / cap) = cap - 2 cap / (1 + exp(2 s / cap)): off by some 1e-7 of cap
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        sc[n][hf][e] = fmaf(-2.0f * a.softcap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[n][hf][e] * cap2)), a.softcap);
+            }
+            vis[n] = 0xFFu;
+            if (masked) {
+                const int j = FQ_KEYS * t + 8 * g, c = lim[n] - j, u = j - n_past;
+                vis[n] = c >= 8 ? 0xFFu : c > 0 ? (1u << c) - 1 : 0u;
+                if (u > -8 && u < 64) vis[n] |= (uint32_t)(u >= 0 ? anc[n] >> u : anc[n] << -u) & 0xFFu;
+                if (row_t < 0) vis[n] = 0;
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (!((vis[n] >> (4 * hf + e)) & 1u)) sc[n][hf][e] = -INFINITY;   // a hidden score may be NaN
+            }
+            float mt = -INFINITY;
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mt = fmaxf(mt, sc[n][hf][e]);
+            if (__any(mt > m_run[n] + FQ_LAZY)) {
+                mt = fq_col_max(mt);
+                const float m_new = fmaxf(m_run[n], mt);
+                const float alpha = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m_run[n] - m_new) * FQ_LOG2E);
+                m_run[n] = m_new;
+                l_run[n] *= alpha;
+#pragma unroll
+                for (int q = 0; q < C::TT; q++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[n][q][e] *= alpha;
+            }
+            const float mb = m_run[n] == -INFINITY ? 0.0f : m_run[n] * FQ_LOG2E;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float s0 = sc[n][e / 2][2 * (e % 2)], s1 = sc[n][e / 2][2 * (e % 2) + 1];
+                pf[n][e] = pack2h(__builtin_amdgcn_exp2f(fmaf(s0, FQ_LOG2E, -mb)), __builtin_amdgcn_exp2f(fmaf(s1, FQ_LOG2E, -mb)));
+                l_run[n] = __builtin_amdgcn_fdot2(h2_of(pf[n][e]), one2, l_run[n], false);   // the sum of what is multiplied
+            }
+        }
+        fq_wait_vm<NB * C::KD + (NB - 1) * C::VD>();   // V has landed
+        // ---- O^T += V^T . P^T; shut: all bits of the halves of keys hidden from some row ----
+        auto pv = [&](auto some, const u32x4 & shut, uint32_t & bad) __attribute__((always_inline)) {
+#pragma unroll
+            for (int q = 0; q < C::TT; q += 4) {
+                uint32_t va[4];
+                fq_v2i w[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) va[i] = vra ^ (uint32_t)(32 * (q + i));
+                fp_read_tr<BUF * C::STAGE, 4 * C::VRB>(va, w);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    u32x4 x = {(uint32_t)w[2 * i][0], (uint32_t)w[2 * i][1], (uint32_t)w[2 * i + 1][0], (uint32_t)w[2 * i + 1][1]};
+                    if constexpr (decltype(some)::value) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t nf = not_finite2(x[e]) & shut[e];
+                            x[e] &= ~((nf >> 15) * 0xFFFFu);
+                            bad |= ((nf >> 15 & 1u) | (nf >> 30 & 2u)) << (2 * e);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+                        o[n][q + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, pf[n]), o[n][q + i], 0, 0, 0);
+                }
+            }
+        };
+        uint32_t bad = 0;   // of this lane's keys: shut ones with a value that is not finite
+        if (!masked) {
+            pv(std::false_type{}, u32x4{0, 0, 0, 0}, bad);
+        } else {
+            uint32_t hidden = 0;
+            u32x4 shut = {0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < NQ; n++) hidden |= ok[n] ? ~vis[n] & 0xFFu : 0u;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint64_t rows = __ballot((hidden >> e) & 1u);
+                if ((rows >> (16 * g)) & 0xFFFFu) shut[e / 2] |= 0xFFFFu << (16 * (e % 2));
+            }
+            pv(std::true_type{}, shut, bad);
+            if (__any(bad != 0)) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint64_t dims = __ballot((bad >> e) & 1u);
+                    if ((dims >> (16 * g)) & 0xFFFFu)
+#pragma unroll
+                        for (int n = 0; n < NQ; n++)
+                            if ((vis[n] >> e) & 1u) l_run[n] = NAN;
+                }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        dma_v(row_p, BUF);
+        t += NW;
+        row_t = NB == 2 ? row_n : row_p;
+        row_n = row_p;
+        row_p = page_of(min(t + NB * NW, tile_end));
+    };
+    for (int k = 0; k < nk; k += NB) {
+        tile(std::integral_constant<int, 0>{});
+        if constexpr (NB == 2)
+            if (k + 1 < nk) tile(std::integral_constant<int, 1>{});
+    }
+    fq_wait_vm<0>();   // no DMA may still write what the merge reuses
+
+    // ---- merge the block's waves, as fa_q_kernel ----
+    float * const sml = (float *)smem;                           // [NW][16 NQ][2]: (max, sum)
+    float4v * const so = (float4v *)(smem + NW * 16 * NQ * 8);   // [NW][CT][64]
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        l_run[n] = fq_col_sum(l_run[n]);
+        if (g == 0) {
+            sml[((wave * NQ + n) * 16 + r) * 2] = m_run[n];
+            sml[((wave * NQ + n) * 16 + r) * 2 + 1] = l_run[n];
+        }
+    }
+    __syncthreads();
+    float M[NQ], L[NQ], wgt[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        M[n] = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; w++) M[n] = fmaxf(M[n], sml[((w * NQ + n) * 16 + r) * 2]);
+        L[n] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float mw = sml[((w * NQ + n) * 16 + r) * 2];
+            L[n] += sml[((w * NQ + n) * 16 + r) * 2 + 1] * (mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((mw - M[n]) * FQ_LOG2E));
+        }
+        wgt[n] = m_run[n] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m_run[n] - M[n]) * FQ_LOG2E);
+    }
+    const int64_t unit = ((int64_t)(s * a.HK + hk) * a.nrt + rt) * a.nsplit + split;
+    if (a.nsplit > 1 && wave == 0 && g == 0) {
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            float * ml = a.part_ml + (unit * NQ * 16 + n * 16 + r) * 2;
+            ml[0] = M[n];
+            ml[1] = L[n];
+        }
+    }
+    constexpr int ALL = C::TT * NQ;
+#pragma unroll
+    for (int c0 = 0; c0 < ALL; c0 += C::CT) {
+        if (c0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C::CT; i++) {
+            const int n = (c0 + i) / C::TT, q = (c0 + i) % C::TT;
+            so[(wave * C::CT + i) * WAVE + lane] = o[n][q] * wgt[n];
+        }
+        __syncthreads();
+        for (int i = wave; i < C::CT; i += NW) {
+            float4v v = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const float4v p = so[(w * C::CT + i) * WAVE + lane];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] += p[e];
+            }
+            const int at = c0 + i, n = at / C::TT, q = at % C::TT;
+            if (a.nsplit > 1) {
+                *(float4v *)(a.part_o + ((unit * ALL + at) * WAVE + lane) * 4) = v;
+                continue;
+            }
+            const int row = (rt * NQ + n) * 16 + r;
+            if (row >= a.R) continue;
+            float Ln = L[0];
+#pragma unroll
+            for (int k = 1; k < NQ; k++)
+                if (n == k) Ln = L[k];
+            const float inv = Ln == 0.0f ? 0.0f : 1.0f / Ln;   // no key seen: zeros; a NaN stays
+            const int tk = fq_div(row, a.div_g);
+            const int64_t dst = (int64_t)s * a.dst_nb3 + (int64_t)tk * a.dst_nb2 + (int64_t)(hk * a.G + row - tk * a.G) * a.dst_nb1;
+            fq_store4(a, dst, 16 * q + 4 * g, v, inv);
+        }
+    }
+}
+
+template <int DK, int DV, int NQ, int NB, int NW>
+static hipError_t fp_launch(const FaPArgs & a, hipStream_t st) {
+    using C = FpCfg<DK, DV, NQ, NB, NW>;
+    static bool done = false;
+    if (!done) {
+        const hipError_t e = hipFuncSetAttribute((const void *)fa_pf16_kernel<DK, DV, NQ, NB, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+        if (e != hipSuccess) return e;
+        done = true;
+    }
+    const int64_t units = (int64_t)a.S * a.HK * a.nrt;
+    hipLaunchKernelGGL((fa_pf16_kernel<DK, DV, NQ, NB, NW>), dim3((unsigned)(units * a.nsplit)), dim3(NW * WAVE), C::LDS, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.nsplit == 1) return e;
+    return launch_fa_q_combine(a, DV, NQ, st);
+}
+
+hipError_t launch_fa_p_F16(const FaPArgs & a, hipStream_t st) {
+    if (a.D == 64 && a.DV == 64) return a.nq == 2 ? fp_launch<64, 64, 2, 2, 8>(a, st) : fp_launch<64, 64, 1, 2, 8>(a, st);
+    if (a.nq != 1) return hipErrorInvalidValue;
+    if (a.D == 128 && a.DV == 128) return fp_launch<128, 128, 1, 1, 8>(a, st);
+    if (a.D == 192 && a.DV == 128) return fp_launch<192, 128, 1, 1, 4>(a, st);
+    if (a.D == 256 && a.DV == 256) return fp_launch<256, 256, 1, 1, 4>(a, st);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace mx

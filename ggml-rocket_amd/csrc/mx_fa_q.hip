@@ -87,6 +87,7 @@ hipError_t launch_fa_q(const FaQArgs & a, hipStream_t st) {
 }
 
 hipError_t launch_fa_p(const FaPArgs & a, hipStream_t st) {
+    if (a.k.type == T_F16) return launch_fa_p_F16(a, st);
     if (a.k.type == T_Q8_0) return a.v.type == T_Q8_0 ? launch_fa_p_Q8_0_Q8_0(a, st) : launch_fa_p_Q8_0_Q4_0(a, st);
     return a.v.type == T_Q8_0 ? launch_fa_p_Q4_0_Q8_0(a, st) : launch_fa_p_Q4_0_Q4_0(a, st);
 }

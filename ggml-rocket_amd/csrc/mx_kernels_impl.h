@@ -136,6 +136,7 @@ hipError_t launch_fa_q_Q8_0_Q4_0(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_q_Q4_0_Q8_0(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_q_Q4_0_Q4_0(const FaQArgs & a, hipStream_t st);
 hipError_t launch_fa_p(const FaPArgs & a, hipStream_t st);
+hipError_t launch_fa_p_F16(const FaPArgs & a, hipStream_t st);
 hipError_t launch_fa_p_Q8_0_Q8_0(const FaPArgs & a, hipStream_t st);
 hipError_t launch_fa_p_Q8_0_Q4_0(const FaPArgs & a, hipStream_t st);
 hipError_t launch_fa_p_Q4_0_Q8_0(const FaPArgs & a, hipStream_t st);

@@ -114,7 +114,7 @@ def attend(step_kw=None, k=None, v=None, **kw):
 
 
 ATTEND_REFUSALS = [(dict(D=48), U), (dict(D=0), U), (dict(DV=-32), U), (dict(D=576, DV=512), U), (dict(D=256, DV=96), U), (dict(k=dict(type=mx.Q4_K)), U),
-                   (dict(v=dict(type=mx.BF16)), U), (dict(step_kw=dict(S=1 << 20, T=1, n_table=1), HK=8), U), (dict(step_kw=dict(S=1, T=1 << 20), H=4096, HK=1), U),
+                   (dict(v=dict(type=mx.BF16)), U), (dict(k=dict(type=mx.F16)), U), (dict(v=dict(type=mx.F16)), U), (dict(step_kw=dict(S=1 << 20, T=1, n_table=1), HK=8), U), (dict(step_kw=dict(S=1, T=1 << 20), H=4096, HK=1), U),
                    (dict(q_dev=None), A), (dict(dst_dev=None), A), (dict(q_dev=FAKE + 8), A), (dict(dst_dev=FAKE + 8), A), (dict(k=dict(q_dev=None)), A),
                    (dict(v=dict(d_dev=None)), A), (dict(k=dict(q_dev=FAKE + 8)), A), (dict(v=dict(d_dev=FAKE + 4)), A), (dict(k=dict(nb1=100)), A),
                    (dict(v=dict(nb2=-128)), A), (dict(k=dict(nb1=1 << 24)), A), (dict(H=0), A), (dict(HK=0), A), (dict(HK=3), A), (dict(n_rows=-1), A),

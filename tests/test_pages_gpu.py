@@ -12,6 +12,7 @@ pytestmark = pytest.mark.gpu
 F16, Q4_0, Q8_0 = P.F16, R.Q4_0, R.Q8_0
 NAME = {Q8_0: "q8_0", Q4_0: "q4_0", F16: "f16"}
 MIXES = [(Q8_0, Q8_0), (Q4_0, Q4_0), (Q8_0, Q4_0), (Q4_0, Q8_0)]
+ATTENDED = MIXES + [(F16, F16)]
 
 
 def ids(v):
@@ -96,7 +97,7 @@ APPEND = [  # S, T, tree, past, page, H, HK, D, DV, n_rot, neox, source f16
 ]
 
 
-@pytest.mark.parametrize("kt,vt", MIXES + [(F16, F16), (F16, Q8_0)], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("kt,vt", ATTENDED + [(F16, Q8_0)], ids=lambda t: NAME[t])
 @pytest.mark.parametrize("case", APPEND, ids=lambda c: "S%dT%d%sD%dr%d" % (c[0], c[1], "t" if c[2] else "c", c[7], c[9]))
 def test_append_bits(mx, kt, vt, case):
     """Rows of the real tokens hold the definition's bits, all others keep theirs; so do queries."""
@@ -310,7 +311,7 @@ def check_attend(c, got, scale, softcap=0.0, half=False):
         assert np.isfinite(got[s]).all() and (d <= tol + 1e-30).all(), (s, float((d - tol).max()), np.unravel_index((d - tol).argmax(), d.shape))
 
 
-@pytest.mark.parametrize("kt,vt", MIXES, ids=lambda t: NAME[t])
+@pytest.mark.parametrize("kt,vt", ATTENDED, ids=lambda t: NAME[t])
 @pytest.mark.parametrize("case", ATTEND, ids=lambda c: "S%dT%d%sD%d-%d" % (c[0], c[1], "t" if c[2] else "c", c[7], c[8]))
 def test_attend(mx, kt, vt, case):
     import torch
@@ -323,7 +324,7 @@ def test_attend(mx, kt, vt, case):
     assert int(err) == 0
 
 
-@pytest.mark.parametrize("kt,vt", MIXES, ids=lambda t: NAME[t])
+@pytest.mark.parametrize("kt,vt", ATTENDED, ids=lambda t: NAME[t])
 @pytest.mark.parametrize("nsplit,max_kv", [(1, 0), (2, 0), (7, 0), (64, 0), (0, 2500), (0, 40)])
 def test_attend_splits_softcap_f16(mx, kt, vt, nsplit, max_kv):
     """Every split, plans for less than there is, fp16 queries and results, a soft-cap; the same bits twice."""
@@ -354,7 +355,7 @@ ATTEND_FAULTS = {  # past, new, change of the table
 }
 
 
-@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q4_0)], ids=ids)
+@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q4_0), (F16, F16)], ids=ids)
 @pytest.mark.parametrize("name", ATTEND_FAULTS)
 def test_attend_numbers_out_of_range(mx, mix, name):
     """Keys without a row count for nothing, and the flag is set."""
@@ -374,7 +375,7 @@ def test_attend_numbers_out_of_range(mx, mix, name):
     assert int(err) == 1
 
 
-@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q4_0)], ids=ids)
+@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q4_0), (F16, F16)], ids=ids)
 def test_attend_broken_trees_and_wild_queries(mx, mix):
     """Nodes without a way up are zeros; infinities and NaN in one token's query stay in its rows."""
     import torch
@@ -401,7 +402,7 @@ def test_attend_broken_trees_and_wild_queries(mx, mix):
     assert np.array_equal(again[keep], got[keep]) and np.isnan(again[0, 0, 1]).all()
 
 
-@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q4_0)], ids=ids)
+@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q4_0), (F16, F16)], ids=ids)
 def test_attend_keys_with_nan_scales(mx, mix):
     """A drafted key with a scale that is no number makes exactly the rows of the tokens that see it NaN."""
     T, page, H, HK, D = 12, 32, 2, 1, 128
@@ -411,7 +412,11 @@ def test_attend_keys_with_nan_scales(mx, mix):
     table, pages = tables(rng, past, [T], page)
     for which in range(2):
         caches = [cache_of(mx, t, pages * page, HK, D, rng) for t in mix]
-        caches[which][0].d[P.row(table[0], page, past[0] + 2), 0, 1] = float("inf")
+        c, at = caches[which][0], P.row(table[0], page, past[0] + 2)
+        if c.type == F16:
+            c.q[at, 0, 40] = float("nan")
+        else:
+            c.d[at, 0, 1] = float("inf")
         q = rng.standard_normal((1, T, H, D)).astype(np.float32)
         step = mx.KvStep(i32(table), i32(past), T, page, parents=i32(parents))
         got = cpu(mx.flash_attn_paged(gpu(q).permute(0, 2, 1, 3), caches[0][0], caches[1][0], step, 0.09))
@@ -420,7 +425,7 @@ def test_attend_keys_with_nan_scales(mx, mix):
         assert np.isnan(got[0, sees]).all() and np.isfinite(got[0, ~sees]).all()
 
 
-@pytest.mark.parametrize("kt,vt", [(Q8_0, Q4_0)], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("kt,vt", [(Q8_0, Q4_0), (F16, F16)], ids=lambda t: NAME[t])
 def test_attend_far_rows(mx, kt, vt):
     """Pages past 2^31 bytes and values of the cache."""
     import torch
@@ -436,8 +441,8 @@ def test_attend_far_rows(mx, kt, vt):
     mx.kv_append(first, kc, vc, gpu(k), gpu(v))
     got = mx.get_rows([kc, vc], gpu(at))
     kp, vp = P.planes(k[0], kt), P.planes(v[0], vt)
-    assert np.array_equal(cpu(got[0]), R.values(kp[0], kp[1].view(np.float16), kt).astype(np.float32))
-    assert np.array_equal(cpu(got[1]), R.values(vp[0], vp[1].view(np.float16), vt).astype(np.float32))
+    assert np.array_equal(cpu(got[0]), P.cache_values(kp, kt).astype(np.float32))
+    assert np.array_equal(cpu(got[1]), P.cache_values(vp, vt).astype(np.float32))
     q = rng.standard_normal((1, 1, H, D)).astype(np.float32)
     step = mx.KvStep(i32(pages), i32([n - 1]), 1, page)
     out = cpu(mx.flash_attn_paged(gpu(q).permute(0, 2, 1, 3), kc, vc, step, 0.09))
@@ -568,7 +573,7 @@ class Loop:
         assert np.array_equal(cpu(d["past"]), self.past) and int(d["err"]) == 0
 
 
-@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q8_0)], ids=ids)
+@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q8_0), (F16, F16)], ids=ids)
 def test_loop(mx, mix):
     loop = Loop(mx, *mix, seed=5)
     for _ in range(8):
@@ -577,7 +582,7 @@ def test_loop(mx, mix):
         loop.check()
 
 
-@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q8_0)], ids=ids)
+@pytest.mark.parametrize("mix", [(Q8_0, Q8_0), (Q4_0, Q8_0), (F16, F16)], ids=ids)
 def test_loop_captured(mx, mix):
     """The step captured once follows the lengths, trees and tables of every replay; eager steps in between."""
     import torch
