@@ -807,6 +807,9 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
 // keys, 512 rows 36 / 71; 32 sequences x 256 rows x 1024 187 / 641).
 // Fewer keys than a tile's 32, whose loads the direct form does not bound a lane at a time, are always decoded first: 14 us
 // for one sequence (300 keys 10 us), but 477 us for 32 sequences of 31 keys, one after another, where 32 keys take 9.
+static bool fa_q_few_rows(int64_t R, int64_t HK, int64_t KV, int dims) {
+    return R * dims <= 65536 || HK * ((R + 15) / 16) * ((KV + 31) / 32) <= 64 * (int64_t)device_cus();
+}
 static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (a->KV < mx::FA_Q_MIN_KV || a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
     int D, DV;
@@ -814,8 +817,7 @@ static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (2 * a->D < D || 2 * a->DV < DV) return false;   // its loads of scales
     if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
         if (*e) return atoi(e) != 0;
-    const int64_t R = (int64_t)(a->H / a->HK) * a->T;
-    return R * (D + DV) <= 65536 || a->HK * ((R + 15) / 16) * ((a->KV + 31) / 32) <= 64 * (int64_t)device_cus();
+    return fa_q_few_rows((int64_t)(a->H / a->HK) * a->T, a->HK, a->KV, D + DV);
 }
 struct FaQDirectLayout {
     size_t po, pml, total;
@@ -901,6 +903,7 @@ static int kv_step_lower(const mi355x_kv_step & s, int64_t n_rows, int32_t * err
     a.table = s.table_dev; a.n_past = s.n_past_dev; a.n_new = s.n_new_dev; a.parent = s.parent_dev; a.err = err_dev;
     a.table_nb = s.table_nb; a.parent_nb = s.parent_nb; a.n_table = (int)s.n_table; a.S = s.S; a.T = s.T; a.page = s.page;
     a.n_pages = (int)(n_rows / s.page);
+    a.cap = (int)(s.n_table * s.page);
     a.div_page = mx::fq_div_by(s.page);
     return MI355X_OK;
 }
@@ -981,6 +984,24 @@ MI355X_API int mi355x_kv_keep(const mi355x_kv_step * step, const mi355x_kv_rows 
     return some ? hip_status(mx::launch_kv_keep(a, S(stream))) : MI355X_OK;
 }
 
+// Rows a wave and KV splits over an fp16 cache (mx_fa_pf16.hip; us on 8 KV heads). Two row tiles a wave share the reads of
+// K and V: taken where the blocks that are left still fill the chip (head dim 128, 8000 keys: 256 rows of one sequence 32.6 /
+// 32.6, of four 98 / 76; 2048 rows 152 / 102; 10 sequences x 256 rows of up to 3000 keys 88 / 70, at head dim 64 56 / 48).
+// Keys are split up to one block a compute unit for single row tiles, which the memory bounds (one token on
+// 32768 keys, in 16, 32 and 64 splits 29.2, 28.0, 31.8; 32 tokens on 4096 each whole 56, in two 63), to two where
+// many rows make the work arithmetic (four times 256 rows 100 whole, 84 in two, 76 in four; 2048 102 whole, 126 in two).
+static void fa_p_plan_f16(mx::FaPArgs & f, int nsplit) {
+    const int64_t cus = device_cus(), ntiles = (f.KV + 31) / 32;
+    auto units = [&](int nq) { return (int64_t)f.S * f.HK * ((f.R + 16 * nq - 1) / (16 * nq)); };
+    f.nq = f.D <= 192 && f.R > 16 && units(2) >= cus ? 2 : 1;
+    if (const char * e = getenv("MI355X_FA_Q_ROWS"))
+        if (*e) f.nq = atoi(e) == 32 && f.D <= 192 ? 2 : 1;
+    f.nrt = (f.R + 16 * f.nq - 1) / (16 * f.nq);
+    const int64_t room = (f.R > 16 ? 2 : 1) * cus;
+    f.nsplit = (int)(nsplit > 0 ? nsplit : std::max<int64_t>(1, std::min<int64_t>({64, room / std::max<int64_t>(1, units(f.nq)), ntiles / 4})));
+    f.div_nrt = mx::fq_div_by(f.nrt); f.div_hk = mx::fq_div_by(f.HK); f.div_split = mx::fq_div_by(f.nsplit); f.div_g = mx::fq_div_by(f.G);
+}
+
 static int fa_p_check(const mi355x_fa_p_args * a, int nsplit, mx::FaPArgs & f) {
     memset(&f, 0, sizeof f);
     if (!a) return MI355X_E_ARG;
@@ -1014,21 +1035,62 @@ static int fa_p_check(const mi355x_fa_p_args * a, int nsplit, mx::FaPArgs & f) {
     f.q_nb1 = a->q_nb1; f.q_nb2 = a->q_nb2; f.q_nb3 = a->q_nb3;
     f.dst_nb1 = a->dst_nb1; f.dst_nb2 = a->dst_nb2; f.dst_nb3 = a->dst_nb3;
     f.dk = a->D; f.dv = a->DV;
-    const int64_t cap = a->step.n_table * a->step.page;
-    f.KV = (int)(a->max_kv ? std::min(a->max_kv, cap) : cap);
+    if (a->max_kv) f.st.cap = (int)std::min<int64_t>(a->max_kv, f.st.cap);
+    f.KV = f.st.cap;
     f.T = T; f.S = Sn; f.HK = a->HK; f.G = a->H / a->HK; f.R = T * f.G;
     f.scale = a->scale; f.softcap = a->softcap;
     f.q_f16 = a->q_type == mx::T_F16; f.dst_f16 = a->dst_type == mx::T_F16;
-    fa_q_plan(f, nsplit);
+    if (f16) fa_p_plan_f16(f, nsplit);
+    else fa_q_plan(f, nsplit);
     f.div_tpp = mx::fq_div_by(a->step.page / 32);
     return MI355X_OK;
+}
+
+// Many rows of a chain over a quantized cache: decoded first, a sequence at a time, as mi355x_flash_attn_q (its rule and
+// figures are at fa_q_few_rows). A tree has 64 tokens at most and is never worth it; an fp16 cache needs no decoding.
+static bool fa_p_decodes(const mi355x_fa_p_args * a, const mx::FaPArgs & f) {
+    if (f.k.type == mx::T_F16 || f.st.parent || (size_t)f.KV > mx::fa_max_kv(f.dk, f.dv)) return false;
+    if ((int64_t)f.KV * f.HK * ((f.dk + f.dv) / 32) >= 1 << 29) return false;
+    if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
+        if (*e) return atoi(e) == 0;
+    return !fa_q_few_rows(f.R, f.HK, f.KV, f.D + f.DV);
+}
+
+// The decoded form of sequence s: the op on fp16 K and V [HK][kvp][D] and the mask [T][kvp] that the decoding launch writes.
+static mi355x_fa_args fa_p_lower(const mi355x_fa_p_args * a, const mx::FaPArgs & f, int s, char * k16, char * v16, char * mask) {
+    mi355x_fa_args o;
+    memset(&o, 0, sizeof o);
+    const int64_t kvp = (f.KV + 63) / 64 * 64;
+    o.q_dev = (const float *)((const char *)a->q_dev + s * a->q_nb3 * (f.q_f16 ? 2 : 4)); o.q_nb1 = a->q_nb1; o.q_nb2 = a->q_nb2;
+    o.k_dev = (const uint16_t *)k16; o.k_nb1 = a->D; o.k_nb2 = kvp * a->D;
+    o.v_dev = (const uint16_t *)v16; o.v_nb1 = a->DV; o.v_nb2 = kvp * a->DV;
+    o.mask_dev = (const uint16_t *)mask; o.mask_nb1 = kvp;
+    o.dst_dev = (float *)((char *)a->dst_dev + s * a->dst_nb3 * (f.dst_f16 ? 2 : 4)); o.dst_nb1 = a->dst_nb1; o.dst_nb2 = a->dst_nb2;
+    o.D = a->D; o.DV = a->DV; o.T = a->step.T; o.H = a->H; o.KV = (int)kvp; o.HK = a->HK;
+    o.scale = a->scale; o.softcap = a->softcap;
+    return o;
+}
+struct FaPLayout {
+    size_t k, v, mask, fa, total;
+};
+static FaPLayout fa_p_layout(const mi355x_fa_p_args * a, const mx::FaPArgs & f, int nsplit) {
+    FaPLayout L;
+    const size_t kvp = (size_t)(f.KV + 63) / 64 * 64;
+    L.k = 0;
+    L.v = L.k + align256((size_t)a->HK * kvp * a->D * 2);
+    L.mask = L.v + align256((size_t)a->HK * kvp * a->DV * 2);
+    L.fa = L.mask + align256((size_t)a->step.T * kvp * 2);
+    const mi355x_fa_args one = fa_p_lower(a, f, 0, nullptr, nullptr, nullptr);
+    if (nsplit <= 0) nsplit = fa_plan(&one, 0).nsplit;
+    L.total = L.fa + align256(fa_layout(fa_lower(&one, nsplit)).total);
+    return L;
 }
 
 MI355X_API size_t mi355x_flash_attn_paged_workspace(const mi355x_fa_p_args * a, int nsplit) {
     mx::FaPArgs f;
     if (fa_p_check(a, nsplit, f) != MI355X_OK) return 0;
     if (a->step.T == 0 || a->step.S == 0) return 256;
-    return fa_q_direct_layout(f).total;
+    return fa_p_decodes(a, f) ? fa_p_layout(a, f, nsplit).total : fa_q_direct_layout(f).total;
 }
 
 MI355X_API int mi355x_flash_attn_paged(const mi355x_fa_p_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
@@ -1038,9 +1100,29 @@ MI355X_API int mi355x_flash_attn_paged(const mi355x_fa_p_args * a, int nsplit, v
     if (st != MI355X_OK) return st;
     if (!aligned(err_dev, 4)) return MI355X_E_ARG;
     if (a->step.T == 0 || a->step.S == 0) return MI355X_OK;
+    f.st.err = err_dev;
+    if (fa_p_decodes(a, f)) {
+        const FaPLayout L = fa_p_layout(a, f, nsplit);
+        if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
+        char * ws = (char *)workspace_dev;
+        for (int s = 0; s < a->step.S; s++) {
+            const mi355x_fa_args one = fa_p_lower(a, f, s, ws + L.k, ws + L.v, ws + L.mask);
+            size_t need;
+            const mx::FaArgs g = fa_fused_args(&one, nsplit, f.q_f16, f.dst_f16, ws + L.fa, &need);
+            if (need > workspace_bytes - L.fa) return MI355X_E_NOMEM;
+            mx::KvDecodeArgs d;
+            memset(&d, 0, sizeof d);
+            d.k = f.k; d.v = f.v;
+            d.k16 = (uint16_t *)(ws + L.k); d.v16 = (uint16_t *)(ws + L.v);
+            d.HK = a->HK; d.KV = one.KV; d.D = a->D; d.DV = a->DV;
+            int e = hip_status(mx::launch_kv_decode_paged(d, g, f.st, s, (uint16_t *)(ws + L.mask), S(stream)));
+            if (e == MI355X_OK) e = hip_status(mx::launch_fa(g, false, S(stream)));
+            if (e != MI355X_OK) return e;
+        }
+        return MI355X_OK;
+    }
     const FaQDirectLayout L = fa_q_direct_layout(f);
     if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
-    f.st.err = err_dev;
     f.part_o = (float *)((char *)workspace_dev + L.po);
     f.part_ml = (float *)((char *)workspace_dev + L.pml);
     return hip_status(mx::launch_fa_p(f, S(stream)));

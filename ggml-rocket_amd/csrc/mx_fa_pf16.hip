@@ -18,7 +18,7 @@
 
 namespace mx {
 
-// NB: tiles of a wave in LDS; NW: waves a block.
+// NB: tiles of a wave in LDS; NW: waves a block; WPE: waves a SIMD, whose registers they share.
 template <int DK, int DV, int NQ, int NB, int NW>
 struct FpCfg {
     static constexpr int KS = DK / 32, TT = DV / 16;
@@ -58,8 +58,8 @@ __device__ __forceinline__ void fp_read_tr(const uint32_t (&a)[4], fq_v2i (&w)[8
 // Bits of the halves of x that are not finite: 0x8000 of each.
 __device__ __forceinline__ uint32_t not_finite2(uint32_t x) { return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
 
-template <int DK, int DV, int NQ, int NB, int NW>
-__global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) fa_pf16_kernel(FaPArgs a) {
+template <int DK, int DV, int NQ, int NB, int NW, int WPE>
+__global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) fa_pf16_kernel(FaPArgs a) {
     using C = FpCfg<DK, DV, NQ, NB, NW>;
     extern __shared__ __align__(16) uint8_t smem[];
     asm volatile("" ::"s"(a.q), "s"(a.k.nb3), "s"(a.v.nb2), "s"(a.dst), "s"(a.dst_nb3), "s"(a.T), "s"(a.div_split.mul), "s"(a.softcap), "s"(a.st.table),
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
     if (sq.bad && threadIdx.x == 0 && a.st.err) *a.st.err = 1;
     const int tok_a = fq_div(rt * 16 * NQ, a.div_g), tok_b = fq_div(min(a.R, (rt + 1) * 16 * NQ) - 1, a.div_g);
     const int seen = a.st.parent ? n_new : min(n_new, tok_b + 1);
-    const int keys = tok_a < n_new ? min(n_past + seen, a.st.n_table * a.st.page) : 0;
+    const int keys = tok_a < n_new ? min(n_past + seen, a.st.cap) : 0;
     const int up = a.st.parent && lane < a.T ? a.st.parent[(int64_t)s * a.st.parent_nb + lane] : -1;
     const int ntiles = (keys + FQ_KEYS - 1) / FQ_KEYS, per = (ntiles + a.nsplit - 1) / a.nsplit;
     const int tile0 = split * per, tile1 = min(ntiles, tile0 + per), tile_end = max(ntiles, 1) - 1;
@@ -191,29 +191,9 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
         scaled |= qfac[n] != 1.0f;
     }
     scaled = __any(scaled);
-    // row n of this lane sees keys below lim[n] and, of the new tokens', those whose bits are set in anc[n]
-    int lim[NQ], full_to;
+    int lim[NQ];
     uint64_t anc[NQ];
-    {
-        const uint64_t node = a.st.parent ? tree_ancestors(up, lane) : 0;
-        if (a.st.parent && lane < n_new && !node && a.st.err) *a.st.err = 1;
-        const int all = n_past + (a.st.parent ? 0 : tok_a + 1);
-        bool none = false;
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            lim[n] = tok[n] < n_new ? n_past : 0;
-            anc[n] = 0;
-            if (a.st.parent) {
-                const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)node, tok[n], WAVE), hi = (uint32_t)__shfl((int)(uint32_t)(node >> 32), tok[n], WAVE);
-                anc[n] = tok[n] < n_new ? (uint64_t)hi << 32 | lo : 0;
-                if (!anc[n]) lim[n] = 0;
-            } else if (tok[n] < n_new) {
-                lim[n] = n_past + tok[n] + 1;
-            }
-            none |= ok[n] && lim[n] < all;
-        }
-        full_to = __any(none) ? 0 : min(keys, all);   // every key below counts for every row
-    }
+    const int full_to = fp_sees<NQ>(a, lane, rt, up, n_past, n_new, tok_a, ok, lim, anc);
 
     float4v o[NQ][C::TT];
     float m_run[NQ], l_run[NQ];
@@ -266,10 +246,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
             }
             vis[n] = 0xFFu;
             if (masked) {
-                const int j = FQ_KEYS * t + 8 * g, c = lim[n] - j, u = j - n_past;
-                vis[n] = c >= 8 ? 0xFFu : c > 0 ? (1u << c) - 1 : 0u;
-                if (u > -8 && u < 64) vis[n] |= (uint32_t)(u >= 0 ? anc[n] >> u : anc[n] << -u) & 0xFFu;
-                if (row_t < 0) vis[n] = 0;
+                vis[n] = row_t < 0 ? 0 : fp_visible(FQ_KEYS * t + 8 * g, n_past, lim[n], anc[n]);
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++)
 #pragma unroll
@@ -439,28 +416,27 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
     }
 }
 
-template <int DK, int DV, int NQ, int NB, int NW>
+template <int DK, int DV, int NQ, int NB, int NW, int WPE>
 static hipError_t fp_launch(const FaPArgs & a, hipStream_t st) {
     using C = FpCfg<DK, DV, NQ, NB, NW>;
     static bool done = false;
     if (!done) {
-        const hipError_t e = hipFuncSetAttribute((const void *)fa_pf16_kernel<DK, DV, NQ, NB, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+        const hipError_t e = hipFuncSetAttribute((const void *)fa_pf16_kernel<DK, DV, NQ, NB, NW, WPE>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
         if (e != hipSuccess) return e;
         done = true;
     }
     const int64_t units = (int64_t)a.S * a.HK * a.nrt;
-    hipLaunchKernelGGL((fa_pf16_kernel<DK, DV, NQ, NB, NW>), dim3((unsigned)(units * a.nsplit)), dim3(NW * WAVE), C::LDS, st, a);
+    hipLaunchKernelGGL((fa_pf16_kernel<DK, DV, NQ, NB, NW, WPE>), dim3((unsigned)(units * a.nsplit)), dim3(NW * WAVE), C::LDS, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     return launch_fa_q_combine(a, DV, NQ, st);
 }
 
 hipError_t launch_fa_p_F16(const FaPArgs & a, hipStream_t st) {
-    if (a.D == 64 && a.DV == 64) return a.nq == 2 ? fp_launch<64, 64, 2, 2, 8>(a, st) : fp_launch<64, 64, 1, 2, 8>(a, st);
-    if (a.nq != 1) return hipErrorInvalidValue;
-    if (a.D == 128 && a.DV == 128) return fp_launch<128, 128, 1, 1, 8>(a, st);
-    if (a.D == 192 && a.DV == 128) return fp_launch<192, 128, 1, 1, 4>(a, st);
-    if (a.D == 256 && a.DV == 256) return fp_launch<256, 256, 1, 1, 4>(a, st);
+    if (a.D == 64 && a.DV == 64) return a.nq == 2 ? fp_launch<64, 64, 2, 2, 4, 2>(a, st) : fp_launch<64, 64, 1, 1, 4, 4>(a, st);
+    if (a.D == 128 && a.DV == 128) return a.nq == 2 ? fp_launch<128, 128, 2, 1, 4, 2>(a, st) : fp_launch<128, 128, 1, 1, 4, 2>(a, st);
+    if (a.D == 192 && a.DV == 128) return a.nq == 2 ? fp_launch<192, 128, 2, 1, 4, 1>(a, st) : fp_launch<192, 128, 1, 1, 4, 1>(a, st);
+    if (a.nq == 1 && a.D == 256 && a.DV == 256) return fp_launch<256, 256, 1, 1, 4, 1>(a, st);
     return hipErrorInvalidValue;
 }
 

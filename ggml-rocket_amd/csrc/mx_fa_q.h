@@ -225,6 +225,42 @@ __device__ __forceinline__ void fq_store4(const FaQArgs & a, int64_t dst, int d,
     else *(float4v *)((float *)a.dst + dst + d) = v * inv;
 }
 
+// Pages: row n of this lane (one of rt's 16 NQ) sees keys below lim[n] and, of the new tokens', those whose bits are set in
+// anc[n]. Returns the number of first keys that every row sees; `up`: the parent of tree node `lane`.
+template <int NQ>
+__device__ __forceinline__ int fp_sees(const FaPArgs & a, int lane, int rt, int up, int n_past, int n_new, int tok_a, const bool (&ok)[NQ], int (&lim)[NQ],
+                                       uint64_t (&anc)[NQ]) {
+    const int room = a.st.cap - n_past;   // of new tokens
+    const bool tree = a.st.parent != nullptr;
+    const uint64_t node = tree ? tree_ancestors(up, lane) : 0;
+    if (tree && lane < n_new && !node && a.st.err) *a.st.err = 1;
+    const int all = n_past + (tree ? 0 : min(tok_a + 1, room));
+    bool none = false;
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int tok = ok[n] ? fq_div((rt * NQ + n) * 16 + lane % 16, a.div_g) : 0;
+        lim[n] = tok < n_new ? n_past : 0;
+        anc[n] = 0;
+        if (tree) {
+            const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)node, tok, WAVE), hi = (uint32_t)__shfl((int)(uint32_t)(node >> 32), tok, WAVE);
+            anc[n] = tok < n_new ? (uint64_t)hi << 32 | lo : 0;
+            if (!anc[n]) lim[n] = 0;
+            if (room < KV_TREE_MAX) anc[n] &= ((uint64_t)1 << room) - 1;
+        } else if (tok < n_new) {
+            lim[n] = n_past + min(tok + 1, room);
+        }
+        none |= ok[n] && lim[n] < all;
+    }
+    return __any(none) ? 0 : all;
+}
+// Of keys j .. j + 7 those that a row sees, as bits.
+__device__ __forceinline__ uint32_t fp_visible(int j, int n_past, int lim, uint64_t anc) {
+    const int c = lim - j, u = j - n_past;
+    uint32_t vis = c >= 8 ? 0xFFu : c > 0 ? (1u << c) - 1 : 0u;
+    if (u > -8 && u < KV_TREE_MAX) vis |= (uint32_t)(u >= 0 ? anc >> u : anc << -u) & 0xFFu;
+    return vis;
+}
+
 // A: FaQArgs, or FaPArgs for a cache in pages.
 template <int KT, int VT, int DK, int DV, int NQ, class A>
 __global__ void __launch_bounds__((FqCfg<KT, VT, DK, DV, NQ>::NW * WAVE))
@@ -257,7 +293,7 @@ fa_q_kernel(A a) {
         if (sq.bad && threadIdx.x == 0 && a.st.err) *a.st.err = 1;
         const int tok0 = fq_div(rt * 16 * NQ, a.div_g), tok1 = fq_div(min(a.R, (rt + 1) * 16 * NQ) - 1, a.div_g);
         const int seen = a.st.parent ? n_new : min(n_new, tok1 + 1);
-        keys = tok0 < n_new ? min(n_past + seen, a.st.n_table * a.st.page) : 0;
+        keys = tok0 < n_new ? min(n_past + seen, a.st.cap) : 0;
         if (a.st.parent && lane < a.T) up = a.st.parent[(int64_t)s * a.st.parent_nb + lane];
     }
     const int ntiles = (keys + FQ_KEYS - 1) / FQ_KEYS, per = (ntiles + a.nsplit - 1) / a.nsplit;
@@ -477,30 +513,9 @@ fa_q_kernel(A a) {
         tn = kn >= 0 ? tile0 + wave + NW * kn : t;
         request();
     }
-    // Pages: row n of this lane sees keys below lim[n] and, of the new tokens', those whose bits are set in anc[n]; every key
-    // below full_to counts for every row.
     int lim[NQ], full_to = INT_MAX;
     uint64_t anc[NQ];
-    if constexpr (PG) {
-        const uint64_t node = a.st.parent ? tree_ancestors(up, lane) : 0;
-        if (a.st.parent && lane < n_new && !node && a.st.err) *a.st.err = 1;
-        bool none = false;
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            const int row = (rt * NQ + n) * 16 + r, tok = ok[n] ? fq_div(row, a.div_g) : 0;
-            lim[n] = tok < n_new ? n_past : 0;
-            anc[n] = 0;
-            if (a.st.parent) {
-                const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)node, tok, WAVE), hi = (uint32_t)__shfl((int)(uint32_t)(node >> 32), tok, WAVE);
-                anc[n] = tok < n_new ? (uint64_t)hi << 32 | lo : 0;
-                if (!anc[n]) lim[n] = 0;
-            } else if (tok < n_new) {
-                lim[n] = n_past + tok + 1;
-            }
-            none |= ok[n] && lim[n] < n_past + (a.st.parent ? 0 : tok_a + 1);
-        }
-        full_to = __any(none) ? 0 : min(keys, n_past + (a.st.parent ? 0 : tok_a + 1));
-    }
+    if constexpr (PG) full_to = fp_sees<NQ>(a, lane, rt, up, n_past, n_new, tok_a, ok, lim, anc);
     // a barrier for LDS alone: the first tiles' loads stay in flight
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
@@ -619,11 +634,7 @@ fa_q_kernel(A a) {
                 if constexpr (PG) {
                     if (FQ_KEYS * (t + 1) > full_to || row_t < 0) {
                         if (row_t < 0 && a.st.err) *a.st.err = 1;
-                        // of keys j .. j + 7, those below lim and those whose bits are set
-                        const int j = FQ_KEYS * t + 8 * g, c = lim[n] - j, u = j - n_past;
-                        uint32_t vis = c >= 8 ? 0xFFu : c > 0 ? (1u << c) - 1 : 0u;
-                        if (u > -8 && u < 64) vis |= (uint32_t)(u >= 0 ? anc[n] >> u : anc[n] << -u);
-                        if (row_t < 0) vis = 0;
+                        const uint32_t vis = row_t < 0 ? 0 : fp_visible(FQ_KEYS * t + 8 * g, n_past, lim[n], anc[n]);
 #pragma unroll
                         for (int hf = 0; hf < 2; hf++)
 #pragma unroll

@@ -117,6 +117,7 @@ struct KvStepArgs {
     int32_t * err;             // set to 1 by what the device finds wrong, or null
     int64_t table_nb, parent_nb;
     int n_table, S, T, page, n_pages;   // n_pages: whole pages of the cache
+    int cap;                   // logical rows at most: n_table * page, or what the caller promises not to pass
     FqDiv div_page;
 };
 // The same over a cache in pages of whole 32-key tiles: the keys of sequence s are its first n_past + n_new logical rows
@@ -192,6 +193,9 @@ struct KvKeepArgs {
     int wgs;                   // workgroups a sequence (set by the launcher)
 };
 hipError_t launch_kv_keep(KvKeepArgs a, hipStream_t st);
+// K and V of sequence s of a step without a tree as fp16 (launch_kv_decode), with the mask classes of f and its mask in the
+// mixed tiles; rows behind the sequence's last tile of 64 are left as they were.
+hipError_t launch_kv_decode_paged(const KvDecodeArgs & a, const FaArgs & f, const KvStepArgs & st, int s, uint16_t * mask, hipStream_t stream);
 
 hipError_t launch_get_rows(KvRowsArgs a, hipStream_t st);
 

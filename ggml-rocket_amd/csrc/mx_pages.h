@@ -14,19 +14,18 @@ __device__ __forceinline__ int uniform_i32(const int32_t * p, int64_t i) {
     return ((const_i32_t)(uintptr_t)p)[i];
 }
 
-// What sequence s holds and adds. bad: n_past lies outside the table's rows (nothing is added then), n_new outside [0, T]
-// (held to it), or the new rows pass the table.
+// What sequence s holds and adds. bad: n_past lies outside [0, cap] (nothing is added then), n_new outside [0, T] (held to
+// it), or the new rows pass cap.
 struct StepOf {
     int past, fresh;
     bool bad;
 };
 __device__ __forceinline__ StepOf step_of(const KvStepArgs & a, int s) {
-    const int cap = a.n_table * a.page;
     const int p = uniform_i32(a.n_past, s), n = a.n_new ? uniform_i32(a.n_new, s) : a.T;
     StepOf r;
-    r.past = min(max(p, 0), cap);
+    r.past = min(max(p, 0), a.cap);
     r.fresh = r.past == p ? min(max(n, 0), a.T) : 0;
-    r.bad = r.past != p || r.fresh != n || n > cap - p;
+    r.bad = r.past != p || r.fresh != n || n > a.cap - p;
     return r;
 }
 

@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "mx_common.h"
+#include "mx_fa_prep.h"
 #include "mx_kernels_impl.h"
 #include "mx_kv_rows.h"
 #include "mx_pages.h"
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
         for (int i = s * a.span + t; i < a.st.S * a.span; i += AP_THREADS) {
             const int s2 = fq_div(i, a.div_span), k = i - s2 * a.span;
             const int p0 = a.st.n_past[s2], n2 = a.st.n_new ? min(a.st.n_new[s2], a.st.T) : a.st.T;
-            if (p0 < 0 || p0 >= a.st.n_table * a.st.page) continue;
+            if (p0 < 0 || p0 >= a.st.cap) continue;
             const int pi = fq_div(p0, a.st.div_page) + k, first = pi * a.st.page;
             if (pi >= a.st.n_table || first - p0 >= n2) continue;
             const int e = a.st.table[(int64_t)s2 * a.st.table_nb + pi];
@@ -261,6 +262,79 @@ hipError_t launch_kv_keep(KvKeepArgs a, hipStream_t st) {
     }
     a.wgs = (bpr + AP_THREADS - 1) / AP_THREADS;
     hipLaunchKernelGGL(kv_keep_kernel, dim3((unsigned)(a.st.S * a.wgs), a.n_out), dim3(AP_THREADS), 0, st, a);
+    return hipGetLastError();
+}
+
+// A sequence's rows out of their pages as fp16 for the fused attention (kv_decode_kernel has the values and what becomes of
+// scales that are not finite), and its mask classes: token tq sees the keys below n_past + tq + 1, padding none. Only
+// tiles of which a token sees some keys and not all need a mask; it is written for those alone. Keys of the
+// last tile of 64 behind the sequence's last and those of pages that the cache does not have are zeros.
+__global__ void __launch_bounds__(AP_THREADS) kv_decode_paged_kernel(KvDecodeArgs a, FaArgs f, KvStepArgs st, int s, uint16_t * mask) {
+    const int t = threadIdx.x, l = t % 4;
+    const StepOf sq = step_of(st, s);
+    const int keys = sq.fresh ? min(sq.past + sq.fresh, st.cap) : 0;
+    auto row_of = [&](int j) -> int64_t {
+        const int p = fq_div(j, st.div_page);
+        const int64_t r = p < st.n_table ? page_row(st, st.table[(int64_t)s * st.table_nb + p]) : -1;
+        return r < 0 ? -1 : r + j - p * st.page;
+    };
+    if ((int)blockIdx.x < a.n_prep) {
+        // a wave per (32 tokens, 64 keys): lane l has 32 of the keys for token l / 2
+        if (blockIdx.x == 0 && t < 8) f.kzero[t] = 0;
+        if (blockIdx.x == 0 && t == 0 && sq.bad && st.err) *st.err = 1;
+        const int lane = t % WAVE, ct = (int)blockIdx.x * 4 + t / WAVE, nqt = (f.T + FA_QW - 1) / FA_QW;
+        if (ct >= nqt * f.cls_stride) return;
+        const int qt = ct / f.cls_stride, kt = ct - qt * f.cls_stride;
+        const int tq = qt * FA_QW + lane / 2, jb = kt * FA_BKV + 32 * (lane % 2);
+        int n = tq < sq.fresh ? min(max(min(sq.past + tq + 1, keys) - jb, 0), 32) : 0;
+        if (n > 0 && row_of(jb) < 0) {
+            if (st.err) *st.err = 1;
+            n = 0;
+        }
+        const bool any = __any(n > 0), all = __all(tq >= f.T || n == 32);
+        if (lane == 0) f.cls[ct] = !any ? FA_TILE_SKIP : all ? FA_TILE_FULL : FA_TILE_MIXED;
+        if (!any || all || tq >= f.T) return;
+        u32x4 * m = (u32x4 *)(mask + (int64_t)tq * f.mask_nb1 + jb);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = (8 * i + 2 * e < n ? 0u : 0xFC00u) | (8 * i + 2 * e + 1 < n ? 0u : 0xFC000000u);
+            m[i] = w;
+        }
+        return;
+    }
+    const int kb = a.D / 32, vb = a.DV / 32;
+    const int it = ((int)blockIdx.x - a.n_prep) * AP_BLOCKS + t / 4, kh = fq_div(it, a.div_blocks), b = it - kh * (kb + vb);
+    const int j = fq_div(kh, a.div_hk), h = kh - j * a.HK;
+    if (j >= min(a.KV, (keys + FA_BKV - 1) / FA_BKV * FA_BKV)) return;
+    const bool is_v = b >= kb;
+    const int blk = is_v ? b - kb : b;
+    const int64_t row = j < keys ? row_of(j) : -1;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (row >= 0) {
+        const int64_t at = row * (is_v ? a.v.nb1 : a.k.nb1) + h * (is_v ? a.v.nb2 : a.k.nb2) + 32 * blk;
+        const int type = is_v ? a.v.type : a.k.type;
+        const u32x4 x = kv_codes(type, is_v ? a.v.q : a.k.q, at, l);
+        const uint16_t d = (is_v ? a.v.d : a.k.d)[at / 32];
+        const bool bad = (d & 0x7C00u) == 0x7C00u;
+        bool poison = bad && !is_v;
+        if (!is_v)   // a K block's quad looks at the V blocks blk, blk + kb, ...
+            for (int i = blk; i < vb; i += kb) poison |= (a.v.d[(row * a.v.nb1 + h * a.v.nb2) / 32 + i] & 0x7C00u) == 0x7C00u;
+        const float lim = kv_scale_limit(type);
+        kv_values(type, x, bad ? 0.0f : fmaxf(fminf(h2f_bits(d), lim), -lim), l, v);
+        if (poison) v[0] = NAN;
+    }
+    *(u32x4 *)((is_v ? a.v16 + (h * (int64_t)a.KV + j) * a.DV : a.k16 + (h * (int64_t)a.KV + j) * a.D) + 32 * blk + 8 * l) = kv_pack8(v);
+}
+
+hipError_t launch_kv_decode_paged(const KvDecodeArgs & args, const FaArgs & f, const KvStepArgs & st, int s, uint16_t * mask, hipStream_t stream) {
+    KvDecodeArgs a = args;
+    a.div_blocks = fq_div_by((a.D + a.DV) / 32);
+    a.div_hk = fq_div_by(a.HK);
+    a.n_prep = fa_prep_blocks(f);
+    const int64_t items = (int64_t)a.KV * a.HK * ((a.D + a.DV) / 32);
+    hipLaunchKernelGGL(kv_decode_paged_kernel, dim3((unsigned)(a.n_prep + (items + AP_BLOCKS - 1) / AP_BLOCKS)), dim3(AP_THREADS), 0, stream, a, f, st, s, mask);
     return hipGetLastError();
 }
 

@@ -708,8 +708,8 @@ def flash_attn_paged(q, k: KvCache, v: KvCache, step: KvStep, scale: float, soft
                      workspace=None, max_kv: int = 0, err=None):
     """Attention of a step's tokens, q [S, H, T, D] (F32 or F16), over caches in pages k [rows, HK, D] and v [rows, HK, DV]: each
     token sees the rows its sequence held, itself and the tokens above it. Returns dst [S, T, H, DV], F32 unless `out` is
-    F16; padding is zeros. max_kv: a bound of n_past + n_new that the caller knows (0: what the tables can hold), for
-    the launch's plan alone."""
+    F16; padding is zeros. max_kv: a bound that no n_past + n_new passes (0: what the tables can hold), for which launch and
+    workspace are planned; rows behind it are not read."""
     torch = _torch()
     if out is None:
         out = torch.empty(q.shape[0], q.shape[2], q.shape[1], v.shape[-1], dtype=torch.float32, device=q.device)

@@ -446,8 +446,12 @@ MI355X_API int mi355x_kv_append(const mi355x_kv_append_args * a, int32_t * err_d
  * Token t of sequence s sees its n_past[s] rows, itself and the tokens above it. Padding, and a token none of whose keys
  * lies in the cache, are written as zeros. A key that a token does not see adds nothing to it, whatever the cache holds there, NaN
  * included. Roundings and limits of the values as in mi355x_flash_attn_q.
- * max_kv: what no n_past + n_new passes, as far as the caller knows (0: n_table * page); it only plans the launch.
- * H % HK == 0; D and DV multiples of 32 up to 256; S * HK row tiles of 16 (T * H / HK rows) as there. */
+ * max_kv: a number that no n_past + n_new passes (0: n_table * page). The launch and its workspace are planned for it;
+ * it takes the place of n_table * page in what the step says of numbers out of range.
+ * H % HK == 0; D and DV multiples of 32 up to 256, each at least half of what the kernels are built for (64 / 64, 128 / 128,
+ * 192 / 128, 256 / 256, the smallest that holds both); S * HK row tiles of 16 (T * H / HK rows) as there. Few rows, trees and
+ * fp16 caches are taken from the pages as they are; many rows of a chain over a quantized cache by decoding it to fp16 in
+ * the workspace first, a sequence at a time. MI355X_FA_Q_DIRECT=1|0 and MI355X_FA_Q_ROWS=16|32 pin the choices as there. */
 typedef struct mi355x_fa_p_args {
     mi355x_kv_step step;
     const void * q_dev;   int64_t q_nb1, q_nb2, q_nb3;         /* token, head, sequence strides */

@@ -58,10 +58,11 @@ def cache_values(pl, t):
     return R.held(pl[0], pl[1].view(np.float16), t)
 
 
-def attend(q, kp, vp, kt, vt, table, page, n_pages, n_past, n_new, parents, scale, softcap=0.0):
-    """q [H][T][D] of one sequence, planes of the caches -> (dst [T][H][DV], bound) as kv_oracle.attention."""
+def attend(q, kp, vp, kt, vt, table, page, n_pages, n_past, n_new, parents, scale, softcap=0.0, most=None):
+    """q [H][T][D] of one sequence, planes of the caches -> (dst [T][H][DV], bound) as kv_oracle.attention; most: logical
+    rows that count at most."""
     H, T, D = q.shape
-    cap = len(table) * page
+    cap = min(len(table) * page, most or 1 << 40)
     fresh = max(0, min(T, n_new)) if 0 <= n_past <= cap else 0
     n = min(cap, n_past + fresh) if fresh else 0
     DV = vp[0].shape[-1] * (2 if vt == R.Q4_0 else 1)
