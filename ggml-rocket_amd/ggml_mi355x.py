@@ -177,7 +177,7 @@ def _bind_optional(L):
         L.mi355x_flash_attn_q.argtypes = [pq, i32, vp, sz, vp]
     if hasattr(L, "mi355x_kv_append"):
         pp, ps = ctypes.POINTER(FaPArgs), ctypes.POINTER(KvStepArgs)
-        L.mi355x_kv_append.argtypes = [ctypes.POINTER(KvAppendArgs), vp, vp]
+        L.mi355x_kv_append.argtypes = [vp, vp, vp]
         L.mi355x_flash_attn_paged_workspace.restype = sz
         L.mi355x_flash_attn_paged_workspace.argtypes = [pp, i32]
         L.mi355x_flash_attn_paged.argtypes = [pp, i32, vp, sz, vp, vp]
@@ -575,7 +575,7 @@ class KvStep:
     before, -1: the rows held; T <= 64), a tree. All int32 on one device, read when a call runs, not when the step is
     made: a program keeps the step and changes the tensors' values."""
 
-    __slots__ = ("table", "n_past", "n_new", "parents", "S", "T", "page", "dev", "args")
+    __slots__ = ("table", "n_past", "n_new", "parents", "S", "T", "page", "dev", "args", "_raw")
 
     def __init__(self, table, n_past, T: int, page: int, n_new=None, parents=None):
         self.table, self.n_past, self.n_new, self.parents = table, n_past, n_new, parents
@@ -594,6 +594,7 @@ class KvStep:
         self.args = KvStepArgs(table.data_ptr(), table.stride(0), n_past.data_ptr(), None if n_new is None else n_new.data_ptr(),
                                None if parents is None else parents.data_ptr(), 0 if parents is None else parents.stride(0),
                                table.shape[1], self.S, self.T, self.page)
+        self._raw = bytes(self.args)
 
 
 class Rope:
@@ -601,7 +602,7 @@ class Rope:
     (i, i + len(freq)), turns by position * freq[i] (F32 on the device, radians a position); cosine and sine are
     multiplied by mscale. positions [S, T] int32, or None: n_past[s] plus a token's depth."""
 
-    __slots__ = ("freq", "neox", "mscale", "positions")
+    __slots__ = ("freq", "neox", "mscale", "positions", "dev", "_args")
 
     def __init__(self, freq, neox: bool = False, mscale: float = 1.0, positions=None):
         torch = _torch()
@@ -610,7 +611,10 @@ class Rope:
         if positions is not None and (positions.dtype != torch.int32 or positions.dim() != 2 or positions.get_device() != freq.get_device()
                                       or (positions.shape[-1] > 1 and positions.stride(-1) != 1)):
             raise MI355XError("Rope: positions are int32 [S, T] on freq's device")
-        self.freq, self.neox, self.mscale, self.positions = freq, bool(neox), float(mscale), positions
+        self.freq, self.neox, self.mscale, self.positions, self.dev = freq, bool(neox), float(mscale), positions, freq.get_device()
+        # its part of mi355x_kv_append_args
+        self._args = (freq.data_ptr(), 0 if positions is None else positions.data_ptr(), 0 if positions is None else positions.stride(0),
+                      2 * freq.shape[0], self.neox, self.mscale)
 
 
 def rope_freqs(n_rot: int, base: float = 10000.0, factors=None, device="cuda"):
@@ -622,12 +626,18 @@ def rope_freqs(n_rot: int, base: float = 10000.0, factors=None, device="cuda"):
     return f.float().to(device)
 
 
+# mi355x_kv_append_args behind the step and the two caches' rows: sequence strides, queries, rotation
+_KV_APPEND = struct.Struct("@qqPqqqPqqqiiqPPqiif4x")
+_NO_QUERIES = (0, 0, 0, 0, 0, 0, 0, 0, F32, F32, 0)
+_NO_ROPE = (0, 0, 0, 0, 0, 1.0)
+
+
 def _step_rows(c, x, step, what):
     """mi355x_kv_rows of cache [rows, H, D] and the step's plain rows x [S, T, H, D], with their sequence stride."""
-    t, n = _plain_types().get(x.dtype), x.stride()
-    if c._rows is None or len(c.shape) != 3 or x.shape != (step.S, step.T, *c._tail) or n[-1] != 1 or (t != F32 and t != F16) or x.get_device() != c.dev:
+    t, n, rows = _plain_types().get(x.dtype), x.stride(), c._rows
+    if len(c.shape) != 3 or x.shape != (step.S, step.T, *c._tail) or n[3] != 1 or (t != F32 and t != F16) or x.get_device() != c.dev:
         raise MI355XError(f"{what}: rows {x.dtype} {tuple(x.shape)} do not fit {step.S} x {step.T} rows of a cache {c.shape}")
-    return KvRows(*c._rows, t, x.data_ptr(), n[1], n[2]), n[0]
+    return _KV_ROWS.pack(*rows, t, x.data_ptr(), n[1], n[2]), n[0]
 
 
 def kv_append(step: KvStep, k_cache: KvCache, v_cache: KvCache, k, v, rope: Rope = None, q=None, q_out=None, err=None):
@@ -640,28 +650,24 @@ def kv_append(step: KvStep, k_cache: KvCache, v_cache: KvCache, k, v, rope: Rope
         raise MI355XError("kv_append: the caches are on another device than the step")
     kr, k3 = _step_rows(k_cache, k, step, "kv_append")
     vr, v3 = _step_rows(v_cache, v, step, "kv_append")
-    a = KvAppendArgs(step.args, kr, vr, k3, v3)
+    queries = _NO_QUERIES
     if q is not None:
         if q_out is None:
             q_out = _torch().empty_like(q)
-        types = _plain_types()
-        for x in (q, q_out):
-            if x.dim() != 4 or x.shape != q.shape or x.stride(-1) != 1 or types.get(x.dtype) not in (F32, F16) or x.get_device() != dev:
-                raise MI355XError(f"kv_append: queries {x.dtype} {tuple(x.shape)}")
-        if q.shape[:2] != (step.S, step.T) or q.shape[3] != k_cache.D:
-            raise MI355XError(f"kv_append: queries {tuple(q.shape)} of a step of {step.S} x {step.T} tokens and heads of {k_cache.D}")
-        qn, on = q.stride(), q_out.stride()
-        a.q_dev, a.q_nb1, a.q_nb2, a.q_nb3, a.q_type = q.data_ptr(), qn[1], qn[2], qn[0], types[q.dtype]
-        a.qr_dev, a.qr_nb1, a.qr_nb2, a.qr_nb3, a.qr_type = q_out.data_ptr(), on[1], on[2], on[0], types[q_out.dtype]
-        a.H = q.shape[2]
+        types, shape, qn, on = _plain_types(), q.shape, q.stride(), q_out.stride()
+        qt, ot = types.get(q.dtype), types.get(q_out.dtype)
+        if (len(shape) != 4 or q_out.shape != shape or shape[0] != step.S or shape[1] != step.T or shape[3] != k_cache.D or qn[3] != 1 or on[3] != 1
+                or (qt != F32 and qt != F16) or (ot != F32 and ot != F16) or q.get_device() != dev or q_out.get_device() != dev):
+            raise MI355XError(f"kv_append: queries {q.dtype} {tuple(shape)} -> {q_out.dtype} {tuple(q_out.shape)} of a step of "
+                              f"{step.S} x {step.T} tokens and heads of {k_cache.D}")
+        queries = (q.data_ptr(), qn[1], qn[2], qn[0], q_out.data_ptr(), on[1], on[2], on[0], qt, ot, shape[2])
+    turn = _NO_ROPE
     if rope is not None:
-        p = rope.positions
-        if rope.freq.get_device() != dev or (p is not None and p.shape != (step.S, step.T)):
+        if rope.dev != dev or (rope.positions is not None and rope.positions.shape != (step.S, step.T)):
             raise MI355XError("kv_append: the rotation is not this step's")
-        a.freq_dev, a.n_rot, a.neox, a.mscale = rope.freq.data_ptr(), 2 * rope.freq.shape[0], rope.neox, rope.mscale
-        if p is not None:
-            a.pos_dev, a.pos_nb = p.data_ptr(), p.stride(0)
-    check(lib().mi355x_kv_append(a, _kv_err(err, dev, "kv_append"), _launch_stream(dev, "kv_append")), "kv_append")
+        turn = rope._args
+    check(lib().mi355x_kv_append(step._raw + kr + vr + _KV_APPEND.pack(k3, v3, *queries, *turn), _kv_err(err, dev, "kv_append"),
+                                 _launch_stream(dev, "kv_append")), "kv_append")
     return q_out
 
 
@@ -676,7 +682,7 @@ def kv_keep(step: KvStep, caches, path, n_keep=None, err=None):
         raise MI355XError("kv_keep: path is int32 [S, A] on the step's device")
     if n_keep is not None and (n_keep.dtype != i32 or n_keep.shape != (step.S,) or n_keep.get_device() != dev or (step.S > 1 and n_keep.stride(0) != 1)):
         raise MI355XError("kv_keep: n_keep is int32 [S] on the step's device")
-    rows = (KvRows * len(caches))(*[KvRows(*c._rows) for c in caches])
+    rows = b"".join([_KV_ROWS.pack(*c._rows, F32, 0, 0, 0) for c in caches])
     check(lib().mi355x_kv_keep(step.args, rows, len(caches), path.data_ptr(), path.stride(0), None if n_keep is None else n_keep.data_ptr(),
                                path.shape[1], _kv_err(err, dev, "kv_keep"), _launch_stream(dev, "kv_keep")), "kv_keep")
 

@@ -71,6 +71,15 @@ def test_append_rows(which, bad):
     assert call_append(append(**{which: bad})) == mx.E_ARG
 
 
+def test_append_arguments_as_packed():
+    """The binding packs mi355x_kv_append_args as the struct lies in memory."""
+    a = append(pos_dev=FAKE, pos_nb=3, mscale=0.5)
+    rest = (a.k_nb3, a.v_nb3, a.q_dev, a.q_nb1, a.q_nb2, a.q_nb3, a.qr_dev, a.qr_nb1, a.qr_nb2, a.qr_nb3, a.q_type, a.qr_type, a.H, a.freq_dev, a.pos_dev, a.pos_nb,
+            a.n_rot, a.neox, a.mscale)
+    row = lambda r: mx._KV_ROWS.pack(*[getattr(r, n) or 0 for n, _ in r._fields_])  # noqa: E731
+    assert bytes(a.step) + row(a.k) + row(a.v) + mx._KV_APPEND.pack(*rest) == bytes(a)
+
+
 def test_append_calls():
     assert mx.lib().mi355x_kv_append(None, None, None) == mx.E_ARG
     assert call_append(append(), FAKE + 2) == mx.E_ARG
