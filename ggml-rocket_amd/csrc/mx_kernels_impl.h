@@ -162,9 +162,11 @@ struct KvPlainRows {           // [S][T][H][32 bph], strides in elements
 struct KvAppendRows {          // K, V or Q
     KvPlainRows x;
     int H, bph;                // heads, 32-value blocks a head
-    bool rotate;
-    int items, tok_wg, parts, groups, wg_begin;   // set by the launcher
-    FqDiv div_bph, div_items, div_parts, div_groups;
+    bool rotate, wide;         // wide (set by the launcher): nothing is quantized, a lane takes eight values side by side
+    // set by the launcher: blocks a token; tokens a workgroup, or parts of a token's blocks and the blocks of one; workgroups a
+    // sequence without the parts; the first workgroup; tokens that a workgroup's quads are at, at a time
+    int items, tok_wg, parts, per, groups, wg_begin, down;
+    FqDiv div_bph, div_parts, div_groups, div_across;   // div_across: quads beside each other in a token's row
 };
 struct KvAppendArgs {
     KvStepArgs st;

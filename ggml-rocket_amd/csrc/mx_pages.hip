@@ -25,26 +25,70 @@ namespace mx {
 
 constexpr int AP_THREADS = 256;
 constexpr int AP_BLOCKS = AP_THREADS / 4;   // quads
-constexpr int AP_TOK = 8;                   // tokens a workgroup
+constexpr int AP_TOK = 16;                  // tokens a workgroup
 constexpr int AP_HALF = 128;                // pairs at most (head dim 256)
 
-__device__ __forceinline__ float4v ap_load4(const KvPlainRows & x, int64_t at) {
-    if (!x.f16) return *(const float4v *)((const float *)x.x + at);
-    const half4 v = *(const half4 *)((const uint16_t *)x.x + at);
-    return float4v{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+// A lane's eight values, two runs of four: the first at `at`, the second `apart` values on (wide: 4, one 16-byte piece of F16).
+__device__ __forceinline__ void ap_load8(const KvPlainRows & x, int64_t at, bool wide, u32x4 (&raw)[2]) {
+    if (!x.f16) {
+        const float * p = (const float *)x.x + at;
+        raw[0] = *(const u32x4 *)p;
+        raw[1] = *(const u32x4 *)(p + (wide ? 4 : 16));
+    } else if (wide) {
+        raw[0] = *(const u32x4 *)((const uint16_t *)x.x + at);
+    } else {
+        const uint16_t * p = (const uint16_t *)x.x + at;
+        const u32x2 lo = *(const u32x2 *)p, hi = *(const u32x2 *)(p + 16);
+        raw[0] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
 }
-__device__ __forceinline__ void ap_store4(const KvPlainRows & x, int64_t at, const float * v) {
-    if (x.f16) *(u32x2 *)((uint16_t *)x.x + at) = u32x2{pack2h(v[0], v[1]), pack2h(v[2], v[3])};
-    else *(float4v *)((float *)x.x + at) = float4v{v[0], v[1], v[2], v[3]};
+__device__ __forceinline__ float ap_value(bool f16, const u32x4 (&raw)[2], int e) {
+    return f16 ? h2f_bits((uint16_t)(raw[0][e / 2] >> (16 * (e % 2)))) : __uint_as_float(raw[e / 4][e % 4]);
+}
+
+// Sine and cosine of x, |x| < 2^40, off by some 2^-53: x less a multiple k of pi / 2, whose three parts take 159 bits of it, then
+// the Taylor series up to x^17 and x^18 (|r| <= pi / 4: the next terms are below 1e-19). The library's sincos also
+// takes arguments of any size, with 60 registers, which left room for half as many workgroups.
+__device__ __forceinline__ void ap_sincos(double x, double & sn, double & cn) {
+    const double k = rint(x * 0.6366197723675814);
+    const double r = fma(-k, -1.4973849048591698e-33, fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, x))), z = r * r;
+    double s = 1.0 / 355687428096000.0, c = -1.0 / 6402373705728000.0;   // 17!, 18!
+    s = fma(s, z, -1.0 / 1307674368000.0);
+    c = fma(c, z, 1.0 / 20922789888000.0);
+    s = fma(s, z, 1.0 / 6227020800.0);
+    c = fma(c, z, -1.0 / 87178291200.0);
+    s = fma(s, z, -1.0 / 39916800.0);
+    c = fma(c, z, 1.0 / 479001600.0);
+    s = fma(s, z, 1.0 / 362880.0);
+    c = fma(c, z, -1.0 / 3628800.0);
+    s = fma(s, z, -1.0 / 5040.0);
+    c = fma(c, z, 1.0 / 40320.0);
+    s = fma(s, z, 1.0 / 120.0);
+    c = fma(c, z, -1.0 / 720.0);
+    s = fma(s, z, -1.0 / 6.0);
+    c = fma(c, z, 1.0 / 24.0);
+    c = fma(c, z, -0.5);
+    s = fma(s, z * r, r);
+    c = fma(c, z, 1.0);
+    const int q = (int)(int64_t)k & 3;   // sin(r + q pi / 2)
+    const double a = q & 1 ? c : s, b = q & 1 ? s : c;
+    sn = q & 2 ? -a : a;
+    cn = (q + 1) & 2 ? -b : b;
 }
 
 // A workgroup takes tok_wg tokens of a sequence, one after the other, or one of `parts` of a token's blocks, of K, of V or of
-// Q. A row that a later token (of this sequence or the next ones) has too, because tables share a page where they
-// are written, is left to the last of them, so that it is whole: every workgroup of K and V looks at the pages that
-// the step writes behind its own.
+// Q. A quad stays at its place of the row, block b of head h, and goes from token to token, the next block on its way
+// meanwhile. Where nothing is quantized lane l takes values 8 l .. 8 l + 7 of a block, else 4 l .. and 16 + 4 l ..
+// (kv_quantize). 4091 tokens of 32 + 8 + 8 heads x 128, all F16 (101 MB) 29.6 us, from F32 into Q8_0 (185 MB) 44 us, 4.2 TB/s; a
+// single token 5.3 us, its chain of loads (lengths, table) and the barriers. A wave waits 0.7 of its time, for that chain
+// most of all: with at most eight tokens a workgroup 30.1 and 47 us, with four blocks a thread requested at once 33.
+// A row that a later token (of this sequence or the next ones) has too, because tables share a page where they are
+// written, is left to the last of them, so that it is whole: every workgroup of K and V looks at the pages that the
+// step writes behind its own.
+template <bool NEOX>
 __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
     __shared__ float cs[AP_TOK][AP_HALF][2];
-    __shared__ int64_t at_row[AP_TOK];
+    __shared__ int64_t at_row[AP_TOK];   // element offset of the token's row
     __shared__ int pos[AP_TOK], entry[AP_TOK], off[AP_TOK], dead[AP_TOK];   // dead: 1 its row is not written, 2 nor its query
     const int t = threadIdx.x, l = t % 4;
     int what = 0;
@@ -52,33 +96,72 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
     const KvAppendRows & r = a.r[what];
     const int wg = (int)blockIdx.x - r.wg_begin, grp = fq_div(wg, r.div_parts), part = wg - grp * r.parts;
     const int s = fq_div(grp, r.div_groups), t0 = (grp - s * r.groups) * r.tok_wg;
+    const int end = min(r.items, (part + 1) * r.per);
+    const int rotated = r.rotate ? 2 * a.half : 0;
+    const bool wide = r.wide, x_f16 = r.x.f16;
+    const int run0 = wide ? 8 * l : 4 * l, apart = wide ? 4 : 16;   // this lane's two runs of four values of a block
+    // quad -> (token of the first few, place in the row); places go on by `across`, tokens by `down`
+    const int across = min(r.per, AP_BLOCKS), down = r.down, quad = t / 4;
+    const int tok0 = fq_div(quad, r.div_across), hb0 = part * r.per + quad - tok0 * across;
+    struct At {
+        int hb, tok, j;   // j: this lane's first dim of its head
+        int64_t x, o;     // element offset of its value in the source of token t0, and in a row of the destination
+    };
+    const KvPlainRows & xr = r.x;
+    const int64_t o_nb2 = what == 2 ? a.qr.nb2 : a.o[what].nb2;
+    auto place = [&](int hb, int tok) {
+        const int h = fq_div(hb, r.div_bph), j = 32 * (hb - h * r.bph) + run0;
+        return At{hb, tok, j, (int64_t)s * xr.nb3 + (int64_t)t0 * xr.nb1 + (int64_t)h * xr.nb2 + j, (int64_t)h * o_nb2 + j};
+    };
+    u32x4 v[2], w[2];   // a block's values and those they are paired with
+    auto load = [&](const At & p) {
+        const int64_t at = p.x + p.tok * xr.nb1;
+        ap_load8(xr, at, wide, v);
+        if constexpr (NEOX) {
+            if (wide) {   // half is a multiple of 8
+                if (p.j < rotated) ap_load8(xr, at + (p.j < a.half ? a.half : -a.half), true, w);
+            } else {
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const int j = p.j + 16 * g;
+                    if (j >= rotated) continue;
+                    const int64_t from = at + 16 * g + (j < a.half ? a.half : -a.half);
+                    if (x_f16) {
+                        const u32x2 y = *(const u32x2 *)((const uint16_t *)xr.x + from);
+                        w[0][2 * g] = y[0];
+                        w[0][2 * g + 1] = y[1];
+                    } else {
+                        w[g] = *(const u32x4 *)((const float *)xr.x + from);
+                    }
+                }
+            }
+        }
+    };
+    At p = place(hb0, tok0);
+    // quads left over have nothing to do; padding's sources are there to be read
+    if (tok0 < down && hb0 < end && tok0 < min(r.tok_wg, a.st.T - t0)) load(p);
+
     const StepOf sq = step_of(a.st, s);
     const int toks = min(r.tok_wg, sq.fresh - t0);
     if (sq.bad && t == 0 && t0 == 0 && a.st.err) *a.st.err = 1;
     if (toks <= 0) return;
-    const int per = (r.items + r.parts - 1) / r.parts;
-    const int begin = part * per, end = r.parts > 1 ? min(r.items, begin + per) : toks * r.items;
-    const int rotated = r.rotate ? 2 * a.half : 0;
-
-    auto load = [&](int it, float (&v)[8], float (&w)[8]) {   // a block's values and those they are paired with
-        const int tok = fq_div(it, r.div_items), hb = it - tok * r.items, h = fq_div(hb, r.div_bph), b = hb - h * r.bph;
-        const int64_t at = (int64_t)s * r.x.nb3 + (int64_t)(t0 + tok) * r.x.nb1 + (int64_t)h * r.x.nb2;
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-            const int j = 32 * b + 16 * g + 4 * l;
-            const float4v y = ap_load4(r.x, at + j);
-            float4v z = y;
-            if (a.neox && j < rotated) z = ap_load4(r.x, at + (j < a.half ? j + a.half : j - a.half));
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[4 * g + e] = y[e];
-                w[4 * g + e] = z[e];
-            }
-        }
+    // page k of those that sequence s2 writes, as [first, first + page) of its rows; its entry, or -1 for none
+    struct Later {
+        int s2, first, p0, n2, e;
     };
-    float v[8], w[8];
-    if (begin + t / 4 < end) load(begin + t / 4, v, w);
-
+    auto later = [&](int i) {
+        Later x = {0, 0, 0, 0, -1};
+        if (what == 2 || i >= a.st.S * a.span) return x;
+        x.s2 = fq_div(i, a.div_span);
+        x.p0 = a.st.n_past[x.s2];
+        x.n2 = a.st.n_new ? min(a.st.n_new[x.s2], a.st.T) : a.st.T;
+        if (x.p0 < 0 || x.p0 >= a.st.cap) return x;
+        const int pi = fq_div(x.p0, a.st.div_page) + i - x.s2 * a.span;
+        x.first = pi * a.st.page;
+        if (pi < a.st.n_table && x.first - x.p0 < x.n2) x.e = a.st.table[(int64_t)x.s2 * a.st.table_nb + pi];
+        return x;
+    };
+    Later next = later(s * a.span + t);
     // ---- rows and positions of the tokens ----
     if (t < WAVE) {
         int depth = t0 + t;
@@ -92,7 +175,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
             const int64_t row = page_row(a.st, e);
             entry[t] = e;
             off[t] = j - pi * a.st.page;
-            at_row[t] = row + off[t];
+            at_row[t] = what < 2 ? (row + off[t]) * a.o[what].nb1 : (int64_t)s * a.qr.nb3 + (int64_t)(t0 + t) * a.qr.nb1;
             pos[t] = a.pos ? a.pos[(int64_t)s * a.pos_nb + t0 + t] : sq.past + depth;
             dead[t] = depth < 0 ? 2 : row < 0 ? 1 : 0;
             if (dead[t] && a.st.err) *a.st.err = 1;
@@ -103,90 +186,105 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
     for (int i = t; i < toks * (rotated / 2); i += AP_THREADS) {
         const int tok = fq_div(i, a.div_half), p = i - tok * a.half;
         double sn, c;
-        sincos((double)pos[tok] * (double)a.freq[p], &sn, &c);
+        ap_sincos((double)pos[tok] * (double)a.freq[p], sn, c);
         cs[tok][p][0] = (float)(c * (double)a.mscale);
         cs[tok][p][1] = (float)(sn * (double)a.mscale);
     }
-    if (what < 2) {
-        for (int i = s * a.span + t; i < a.st.S * a.span; i += AP_THREADS) {
-            const int s2 = fq_div(i, a.div_span), k = i - s2 * a.span;
-            const int p0 = a.st.n_past[s2], n2 = a.st.n_new ? min(a.st.n_new[s2], a.st.T) : a.st.T;
-            if (p0 < 0 || p0 >= a.st.cap) continue;
-            const int pi = fq_div(p0, a.st.div_page) + k, first = pi * a.st.page;
-            if (pi >= a.st.n_table || first - p0 >= n2) continue;
-            const int e = a.st.table[(int64_t)s2 * a.st.table_nb + pi];
-            for (int u = 0; u < toks; u++)
-                if (e == entry[u]) {
-                    const int j = first + off[u];   // the row of s2 that this one is
-                    if (j >= p0 && j - p0 < n2 && (s2 > s || j > sq.past + t0 + u)) dead[u] |= 1;
-                }
+    for (int i = s * a.span + t; what < 2 && i < a.st.S * a.span; i += AP_THREADS) {
+        const Later x = next;
+        next = later(i + AP_THREADS);
+        for (int u = 0; u < toks; u++) {
+            const int j = x.first + off[u];   // the row of s2 that token u's is
+            if (x.e >= 0 && x.e == entry[u] && j >= x.p0 && j - x.p0 < x.n2 && (x.s2 > s || j > sq.past + t0 + u)) dead[u] |= 1;
         }
     }
     __syncthreads();
     // ---- blocks ----
-    for (int it = begin + t / 4; it < end; it += AP_BLOCKS) {
-        float v2[8], w2[8];
-        if (it + AP_BLOCKS < end) load(it + AP_BLOCKS, v2, w2);
-        const int tok = fq_div(it, r.div_items), hb = it - tok * r.items, h = fq_div(hb, r.div_bph), b = hb - h * r.bph;
+    if (tok0 >= down || tok0 >= toks) return;
+    while (p.hb < end) {
+        const At c = p;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = ap_value(x_f16, v, e);
+        float z[8];
+        if constexpr (NEOX) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) z[e] = ap_value(x_f16, w, e);
+        }
+        p.tok += down;
+        if (p.tok >= toks) p = place(p.hb + across, tok0);
+        if (p.hb < end) load(p);
 #pragma unroll
         for (int g = 0; g < 2; g++) {
-            const int j = 32 * b + 16 * g + 4 * l;
+            const int j = c.j + g * apart;
             if (j >= rotated) continue;
-            if (a.neox) {
+            if constexpr (NEOX) {
                 const bool second = j >= a.half;
-                const float * c = cs[tok][second ? j - a.half : j];
+                const float * k = cs[c.tok][second ? j - a.half : j];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float p = mul_rn(v[4 * g + e], c[2 * e]), q = mul_rn(w[4 * g + e], c[2 * e + 1]);
-                    v[4 * g + e] = sub_rn(p, second ? -q : q);
+                    const float x = mul_rn(y[4 * g + e], k[2 * e]), q = mul_rn(z[4 * g + e], k[2 * e + 1]);
+                    y[4 * g + e] = sub_rn(x, second ? -q : q);
                 }
             } else {
-                const float * c = cs[tok][j / 2];
+                const float * k = cs[c.tok][j / 2];
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
-                    const float x0 = v[4 * g + e], x1 = v[4 * g + e + 1];
-                    v[4 * g + e] = sub_rn(mul_rn(x0, c[e]), mul_rn(x1, c[e + 1]));
-                    v[4 * g + e + 1] = sub_rn(mul_rn(x0, c[e + 1]), -mul_rn(x1, c[e]));
+                    const float x0 = y[4 * g + e], x1 = y[4 * g + e + 1];
+                    y[4 * g + e] = sub_rn(mul_rn(x0, k[e]), mul_rn(x1, k[e + 1]));
+                    y[4 * g + e + 1] = sub_rn(mul_rn(x0, k[e + 1]), -mul_rn(x1, k[e]));
                 }
             }
         }
+        const int64_t at = at_row[c.tok] + c.o;
         if (what == 2) {
-            if (dead[tok] < 2) {
-                const int64_t at = (int64_t)s * a.qr.nb3 + (int64_t)(t0 + tok) * a.qr.nb1 + (int64_t)h * a.qr.nb2 + 32 * b + 4 * l;
-                ap_store4(a.qr, at, v);
-                ap_store4(a.qr, at + 16, v + 4);
+            if (dead[c.tok] >= 2) continue;
+            if (a.qr.f16) {
+                uint16_t * to = (uint16_t *)a.qr.x + at;
+                const u32x4 q = kv_pack8(y);
+                if (wide) {
+                    *(u32x4 *)to = q;
+                } else {
+                    *(u32x2 *)to = u32x2{q[0], q[1]};
+                    *(u32x2 *)(to + 16) = u32x2{q[2], q[3]};
+                }
+            } else {
+                float * to = (float *)a.qr.x + at;
+                *(float4v *)to = float4v{y[0], y[1], y[2], y[3]};
+                *(float4v *)(to + apart) = float4v{y[4], y[5], y[6], y[7]};
             }
-        } else if (!dead[tok]) {   // the same for the quad
+        } else if (!dead[c.tok]) {   // the same for the quad
             const KvRowsOut & o = a.o[what];
-            kv_quantize(o, at_row[tok] * o.nb1 + (int64_t)h * o.nb2 + 32 * b, l, v);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            v[e] = v2[e];
-            w[e] = w2[e];
+            if (wide) *(u32x4 *)((uint16_t *)o.q + at) = kv_pack8(y);
+            else kv_quantize(o, at - run0, l, y);
         }
     }
 }
 
-// A block a quad while that makes fewer than 2048 workgroups, then more of them: up to eight whole tokens a workgroup.
+// A block a quad while that makes fewer than 2048 workgroups, then more: up to AP_TOK whole tokens a workgroup.
 hipError_t launch_kv_append(KvAppendArgs a, hipStream_t st) {
     int64_t all = 0, wgs = 0;
     for (int k = 0; k < a.n_rows; k++) all += (int64_t)a.st.S * a.st.T * a.r[k].H * a.r[k].bph;
-    const int64_t per = std::max<int64_t>(AP_BLOCKS, all / 2048);
+    const int64_t most = std::max<int64_t>(AP_BLOCKS, all / 2048);
     for (int k = 0; k < a.n_rows; k++) {
         KvAppendRows & r = a.r[k];
         r.items = r.H * r.bph;
-        r.tok_wg = (int)std::min<int64_t>({std::max<int64_t>(1, per / r.items), AP_TOK, a.st.T});
-        r.parts = per >= r.items ? 1 : (int)((r.items + per - 1) / per);
+        r.tok_wg = (int)std::min<int64_t>({std::max<int64_t>(1, most / r.items), AP_TOK, a.st.T});
+        r.parts = most >= r.items ? 1 : (int)((r.items + most - 1) / most);
+        r.per = (r.items + r.parts - 1) / r.parts;
         r.groups = (a.st.T + r.tok_wg - 1) / r.tok_wg;
+        r.down = std::max(1, AP_BLOCKS / r.per);
+        r.wide = (k == 2 || a.o[k].type == T_F16) && (!r.rotate || !a.neox || a.half % 8 == 0);
         r.wg_begin = (int)wgs;
         wgs += (int64_t)a.st.S * r.groups * r.parts;
-        r.div_bph = fq_div_by(r.bph); r.div_items = fq_div_by(r.items); r.div_parts = fq_div_by(r.parts); r.div_groups = fq_div_by(r.groups);
+        r.div_bph = fq_div_by(r.bph); r.div_parts = fq_div_by(r.parts); r.div_groups = fq_div_by(r.groups);
+        r.div_across = fq_div_by(std::min(r.per, AP_BLOCKS));
     }
     a.span = (a.st.T + a.st.page - 2) / a.st.page + 1;
     a.div_half = fq_div_by(std::max(1, a.half));
     a.div_span = fq_div_by(a.span);
-    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)wgs), dim3(AP_THREADS), 0, st, a);
+    if (a.neox) hipLaunchKernelGGL(kv_append_kernel<true>, dim3((unsigned)wgs), dim3(AP_THREADS), 0, st, a);
+    else hipLaunchKernelGGL(kv_append_kernel<false>, dim3((unsigned)wgs), dim3(AP_THREADS), 0, st, a);
     return hipGetLastError();
 }
 

@@ -175,6 +175,27 @@ def test_append_strided_positions_and_f16_queries(mx):
         assert same([p[at] for p in gv], P.planes(xs[s, :n, H + HK:].astype(np.float32), F16))
 
 
+@pytest.mark.parametrize("neox", [False, True])
+def test_append_far_positions(mx, neox):
+    """Angles of any int32 position, to the last bit of the rotated values."""
+    import torch
+    S, T, H, HK, D, page = 1, 600, 2, 1, 64, 64
+    rng = np.random.default_rng(12)
+    table, pages = tables(rng, [0], [T], page)
+    kc, kp = cache_of(mx, F16, pages * page, HK, D, rng)
+    vc, vp = cache_of(mx, Q8_0, pages * page, HK, D, rng)
+    q, k, v = (rng.standard_normal((S, T, h, D)).astype(np.float32) for h in (H, HK, HK))
+    pos = rng.integers(-2 ** 31, 2 ** 31, (S, T)).astype(np.int32)
+    pos[0, :8] = [0, -1, 1, 2 ** 31 - 1, -2 ** 31, 355, 710, 52174]     # 355 and 710: next to multiples of pi
+    freq = np.concatenate([[1.0, 3.75, 0.0, -0.5], 500000.0 ** (-np.arange(28) / 28)]).astype(np.float32)
+    q_out = torch.empty(S, T, H, D, device="cuda")
+    step = mx.KvStep(i32(table), i32([0]), T, page)
+    mx.kv_append(step, kc, vc, gpu(k), gpu(v), rope=mx.Rope(gpu(freq), neox=neox, positions=gpu(pos)), q=gpu(q), q_out=q_out)
+    at = [P.row(table[0], page, t) for t in range(T)]
+    kp[0][at] = P.planes(P.rotate(k[0], pos[0], freq, neox), F16)[0]
+    assert np.array_equal(cpu(q_out)[0], P.rotate(q[0], pos[0], freq, neox)) and same(planes_of(kc), kp)
+
+
 @pytest.mark.parametrize("T,page", [(1, 32), (40, 32), (300, 64)])
 def test_append_rows_that_two_tokens_share(mx, T, page):
     """Tables that share pages: of the tokens with one row the last, by sequence and number, stays whole."""
