@@ -8,7 +8,9 @@
 // DMA into buffers of the wave's own and no barrier is in the loop. K's operand is one 16-byte read of LDS (a key's eight
 // dims), V's two transposing reads (ds_read_b64_tr_b16: the lanes i of a group of 16 point at 4 dims of key i / 4, and lane
 // i receives dim i of the four keys).
-// Roundings: Q and P, once each, to fp16; K and V are exact, scores, statistics, sums and O F32.
+// Roundings: P, once, to fp16. Q is exact: an fp16 one as it is, an F32 one as the sum of two halves, hi + lo, off by 2^-22
+// (a second product in the loop, 8 more MFMAs a tile at head dim 128); its scale multiplies the F32 scores. K and V are exact, scores,
+// statistics, sums and O F32.
 //
 // A key that a row does not see has P = 0, and 0 times a V that is no number would still be none. So in the tiles that
 // hold such a key (the last ones of a sequence; all tiles of a block with padding) those of its values that are not finite
@@ -31,7 +33,8 @@ struct FpCfg {
     __device__ static __forceinline__ int kswz(int r) { return KCH >= 16 ? r & 15 : (r / 2) & 7; }
     __device__ static __forceinline__ int vswz(int r) { return VCH >= 16 ? (r & 3) | (r >> 1 & 4) : (r >> 1 & 1) | (r >> 2 & 2); }
     static constexpr int CT = TT * NQ < 8 ? TT * NQ : 8;      // O^T tiles merged at a time
-    static constexpr int LOOP_LDS = NW * NB * STAGE;
+    static constexpr int Q_LO = NW * NB * STAGE;              // the halves lo of Q: [NQ][KS][64], behind the tiles
+    static constexpr int LOOP_LDS = Q_LO + NQ * KS * 1024;
     static constexpr int MERGE_LDS = NW * 16 * NQ * 8 + NW * CT * 1024;
     static constexpr int LDS = MERGE_LDS > LOOP_LDS ? MERGE_LDS : LOOP_LDS;
     static_assert(LDS <= FQ_LDS_MAX, "LDS");
@@ -58,7 +61,7 @@ __device__ __forceinline__ void fp_read_tr(const uint32_t (&a)[4], fq_v2i (&w)[8
 // Bits of the halves of x that are not finite: 0x8000 of each.
 __device__ __forceinline__ uint32_t not_finite2(uint32_t x) { return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
 
-template <int DK, int DV, int NQ, int NB, int NW, int WPE>
+template <int DK, int DV, int NQ, int NB, int NW, int WPE, bool QF32>
 __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) fa_pf16_kernel(FaPArgs a) {
     using C = FpCfg<DK, DV, NQ, NB, NW>;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -83,7 +86,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
     const int ntiles = (keys + FQ_KEYS - 1) / FQ_KEYS, per = (ntiles + a.nsplit - 1) / a.nsplit;
     const int tile0 = split * per, tile1 = min(ntiles, tile0 + per), tile_end = max(ntiles, 1) - 1;
 
-    // Q in the B layout of the Q.K products: lane (row r, dims 8 g + 0..7 of a block of 32); past dk zeros
+    // Q in the B layout of the Q.K products: lane (row r, dims 8 g + 0..7 of a block of 32); past dk zeros. QF32: F32, two halves
     bool ok[NQ];
     int tok[NQ];
     int64_t qat[NQ];
@@ -96,7 +99,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
         qat[n] = (int64_t)s * a.q_nb3 + (int64_t)head * a.q_nb2 + (int64_t)tok[n] * a.q_nb1 + 8 * g;
     }
     u32x4 qraw[NQ][C::KS][2];   // eight values each: F32, or F16 in the first
-    if (a.q_f16) {
+    if constexpr (!QF32) {
 #pragma unroll
         for (int n = 0; n < NQ; n++)
 #pragma unroll
@@ -166,31 +169,42 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
         dma_v(row_n, 1);
     }
 
-    // Q, scaled, fp16; a row outside [2^-6, 2^15] divided by a factor that multiplies its scores (fa_q_kernel)
+    // Q in halves; a row outside [2^-6, 2^15] divided by a factor that multiplies its scores with the scale (fa_q_kernel)
     half8 qf[NQ][C::KS];
-    float qfac[NQ];
-    bool scaled = false;
+    half8 * const ql = (half8 *)(smem + C::Q_LO);
+    float sfac[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         float amax = 0.0f;
         auto value = [&](int st, int e) {
-            const float x = a.q_f16 ? h2f_bits((uint16_t)(qraw[n][st][0][e / 2] >> (16 * (e % 2)))) : __uint_as_float(qraw[n][st][e / 4][e % 4]);
-            return ok[n] && 32 * st < a.dk ? x * a.scale : 0.0f;
+            const float x = !QF32 ? h2f_bits((uint16_t)(qraw[n][st][0][e / 2] >> (16 * (e % 2)))) : __uint_as_float(qraw[n][st][e / 4][e % 4]);
+            return ok[n] && 32 * st < a.dk ? x : 0.0f;
         };
 #pragma unroll
         for (int st = 0; st < C::KS; st++)
 #pragma unroll
             for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(value(st, e)));
         amax = fq_col_max(amax);
-        qfac[n] = (amax > 32768.0f || (amax < 0.015625f && amax > 0.0f)) ? fmaxf(amax / 16.0f, 0x1p-120f) : 1.0f;
-        const float inv = 1.0f / qfac[n];
+        const float qfac = QF32 && (amax > 32768.0f || (amax < 0.015625f && amax > 0.0f)) ? fmaxf(amax / 16.0f, 0x1p-120f) : 1.0f;
+        const float inv = 1.0f / qfac;
+        sfac[n] = a.scale * qfac;
 #pragma unroll
-        for (int st = 0; st < C::KS; st++)
+        for (int st = 0; st < C::KS; st++) {
+            half8 lo;
 #pragma unroll
-            for (int e = 0; e < 8; e++) qf[n][st][e] = (_Float16)(value(st, e) * inv);
-        scaled |= qfac[n] != 1.0f;
+            for (int e = 0; e < 8; e++) {
+                const float x = value(st, e) * inv;
+                qf[n][st][e] = (_Float16)x;
+                lo[e] = (_Float16)(x - (float)qf[n][st][e]);
+            }
+            if (QF32 && wave == 0) ql[(n * C::KS + st) * WAVE + lane] = lo;
+        }
     }
-    scaled = __any(scaled);
+    // a barrier for LDS alone: the first tiles' loads stay in flight
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     int lim[NQ];
     uint64_t anc[NQ];
     const int full_to = fp_sees<NQ>(a, lane, rt, up, n_past, n_new, tok_a, ok, lim, anc);
@@ -221,6 +235,10 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
                 const half8 kf = *(const half8 *)(st + (kra ^ (uint32_t)(64 * i)) + hf * 256 * C::KCH);
 #pragma unroll
                 for (int n = 0; n < NQ; n++) sc[n][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n][i], sc[n][hf], 0, 0, 0);
+                if constexpr (QF32)
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+                        sc[n][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[(n * C::KS + i) * WAVE + lane], sc[n][hf], 0, 0, 0);
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         dma_k(row_p, BUF);
@@ -230,12 +248,10 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
         if (masked && row_t < 0 && a.st.err) *a.st.err = 1;
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
-            if (scaled) {
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++)
+            for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc[n][hf][e] *= qfac[n];
-            }
+                for (int e = 0; e < 4; e++) sc[n][hf][e] *= sfac[n];
             if (a.softcap != 0.0f) {
                 // cap * tanh(s / cap) = cap - 2 cap / (1 + exp(2 s / cap)): off by some 1e-7 of cap
 #pragma unroll
@@ -416,20 +432,25 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
     }
 }
 
-template <int DK, int DV, int NQ, int NB, int NW, int WPE>
-static hipError_t fp_launch(const FaPArgs & a, hipStream_t st) {
+template <int DK, int DV, int NQ, int NB, int NW, int WPE, bool QF32>
+static hipError_t fp_launch_q(const FaPArgs & a, hipStream_t st) {
     using C = FpCfg<DK, DV, NQ, NB, NW>;
     static bool done = false;
     if (!done) {
-        const hipError_t e = hipFuncSetAttribute((const void *)fa_pf16_kernel<DK, DV, NQ, NB, NW, WPE>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+        const hipError_t e = hipFuncSetAttribute((const void *)fa_pf16_kernel<DK, DV, NQ, NB, NW, WPE, QF32>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
         if (e != hipSuccess) return e;
         done = true;
     }
     const int64_t units = (int64_t)a.S * a.HK * a.nrt;
-    hipLaunchKernelGGL((fa_pf16_kernel<DK, DV, NQ, NB, NW, WPE>), dim3((unsigned)(units * a.nsplit)), dim3(NW * WAVE), C::LDS, st, a);
+    hipLaunchKernelGGL((fa_pf16_kernel<DK, DV, NQ, NB, NW, WPE, QF32>), dim3((unsigned)(units * a.nsplit)), dim3(NW * WAVE), C::LDS, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     return launch_fa_q_combine(a, DV, NQ, st);
+}
+
+template <int DK, int DV, int NQ, int NB, int NW, int WPE>
+static hipError_t fp_launch(const FaPArgs & a, hipStream_t st) {
+    return a.q_f16 ? fp_launch_q<DK, DV, NQ, NB, NW, WPE, false>(a, st) : fp_launch_q<DK, DV, NQ, NB, NW, WPE, true>(a, st);
 }
 
 hipError_t launch_fa_p_F16(const FaPArgs & a, hipStream_t st) {

@@ -73,7 +73,8 @@ constexpr float FQ_LAZY = 8.0f / 1.4426950408889634f;
 constexpr float FQ_LOG2E = 1.4426950408889634f;
 
 // KT, VT: T_Q8_0 or T_Q4_0; DK, DV: the built head dims; NQ: 16-row query tiles a wave.
-template <int KT, int VT, int DK, int DV, int NQ>
+// PG: over a cache in pages.
+template <int KT, int VT, int DK, int DV, int NQ, bool PG>
 struct FqCfg {
     static constexpr int KRB = KT == T_Q8_0 ? DK : DK / 2, VRB = VT == T_Q8_0 ? DV : DV / 2;   // bytes a row
     static constexpr int KS = DK / 32;                        // blocks a K row: Q.K products
@@ -93,7 +94,8 @@ struct FqCfg {
     static_assert(KRB == 16 * KS * KW && VCH * VH == TT, "layout");
     static constexpr int VB = DV / 32, VS = DV / 64, KSC = DK / 64;   // scales a key, and a lane (32 keys, two lanes each)
     static constexpr int KSL = KSC == 3 ? 4 : KSC, VSL = VS;  // and of a lane's load
-    static constexpr int Q_LDS = NQ * (KS * 1024 + 64);       // Q as B operands, then its rows' factors
+    static constexpr int QN = NQ * KS * 64;                   // Q as B operands (pages: twice, halves hi and lo), then its rows' factors
+    static constexpr int Q_LDS = (PG ? 2 : 1) * QN * 16 + NQ * 64;
     static constexpr int SCALE_LDS = KS * FQ_KEYS * 4 + VB * FQ_KEYS * 2;   // a wave's scales: K's F32, V's F16
     static constexpr int WAVE_LDS = SCALE_LDS + 2 * STAGE;
     // registers: O, scores and masks, a block of K and the offsets' product, the rest; the waves a SIMD they
@@ -263,11 +265,11 @@ __device__ __forceinline__ uint32_t fp_visible(int j, int n_past, int lim, uint6
 
 // A: FaQArgs, or FaPArgs for a cache in pages.
 template <int KT, int VT, int DK, int DV, int NQ, class A>
-__global__ void __launch_bounds__((FqCfg<KT, VT, DK, DV, NQ>::NW * WAVE))
-__attribute__((amdgpu_waves_per_eu(FqCfg<KT, VT, DK, DV, NQ>::NW / 4, FqCfg<KT, VT, DK, DV, NQ>::NW / 4)))
+__global__ void __launch_bounds__((FqCfg<KT, VT, DK, DV, NQ, std::is_same<A, FaPArgs>::value>::NW * WAVE))
+__attribute__((amdgpu_waves_per_eu(FqCfg<KT, VT, DK, DV, NQ, std::is_same<A, FaPArgs>::value>::NW / 4, FqCfg<KT, VT, DK, DV, NQ, std::is_same<A, FaPArgs>::value>::NW / 4)))
 fa_q_kernel(A a) {
-    using C = FqCfg<KT, VT, DK, DV, NQ>;
     constexpr bool PG = std::is_same<A, FaPArgs>::value;
+    using C = FqCfg<KT, VT, DK, DV, NQ, PG>;
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int NW = C::NW;
     // The arguments lie in host memory, a round trip of half a microsecond and more a cache line; used
@@ -431,7 +433,7 @@ fa_q_kernel(A a) {
     // Q in the B layout of the Q.K products, scaled, fp16, in LDS: wave n makes the operands of query tile n.
     // Its loads go out before the first tile's, which comes while Q is converted.
     half8 * const lq = (half8 *)smem;                                       // [NQ][KS][64]
-    float * const lqf = (float *)(smem + NQ * C::KS * 1024);                // [NQ][16]: 0 where no row needs a factor
+    float * const lqf = (float *)(smem + C::Q_LDS - NQ * 64);               // [NQ][16]: 0 where no row needs a factor
     // a lane's dims of block st: runs of four at q_dim(st, 0) and q_dim(st, 1); past dk zeros
     auto q_dim = [&](int st, int hlf) { return 32 * st + (KT == T_Q8_0 ? 8 * g + 4 * hlf : 4 * g + 16 * hlf); };
     u32x4 qraw[C::KS][2];   // four values each: F32, or F16 in the first two words
@@ -483,7 +485,7 @@ fa_q_kernel(A a) {
             for (int e = 0; e < 8; e++) {
                 const uint32_t half = qraw[st][e / 4][e % 4 / 2] >> (16 * (e % 2));
                 const float x = a.q_f16 ? h2f_bits((uint16_t)half) : __uint_as_float(qraw[st][e / 4][e % 4]);
-                v[st][e] = qok && q_dim(st, e / 4) < a.dk ? x * a.scale : 0.0f;
+                v[st][e] = qok && q_dim(st, e / 4) < a.dk ? (PG ? x : x * a.scale) : 0.0f;   // pages: K's scales carry it
                 amax = fmaxf(amax, fabsf(v[st][e]));
             }
         amax = fq_col_max(amax);
@@ -494,14 +496,17 @@ fa_q_kernel(A a) {
         const float inv = 1.0f / qfac;
 #pragma unroll
         for (int st = 0; st < C::KS; st++) {
-            half8 qf;
+            half8 qf, lo;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 // slot e of fq_key is value e (Q8_0), or 0, 2, 1, 3 of either half
                 const float x = v[st][KT == T_Q8_0 ? e : (e & 4) | (e & 1) << 1 | (e & 2) >> 1] * inv;
-                qf[e] = (_Float16)(KT == T_Q4_0 && e >= 4 ? x * 0.0625f : x);
+                const float y = KT == T_Q4_0 && e >= 4 ? x * 0.0625f : x;
+                qf[e] = (_Float16)y;
+                lo[e] = (_Float16)(y - (float)qf[e]);
             }
             lq[(wave * C::KS + st) * WAVE + lane] = qf;
+            if constexpr (PG) lq[C::QN + (wave * C::KS + st) * WAVE + lane] = lo;
         }
         if (g == 0) lqf[wave * 16 + r] = __any(qfac != 1.0f) ? qfac : 0.0f;
     }
@@ -548,6 +553,8 @@ fa_q_kernel(A a) {
         vtop[i] = 0;
     }
     const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
+    const bool q_two = PG && !a.q_f16;   // an fp16 Q is its hi
+    const float kscale = PG ? 16777216.0f * a.scale : 16777216.0f;
     const float cap2 = a.softcap != 0.0f ? 2.0f * FQ_LOG2E / a.softcap : 0.0f;
 
     // Tile t in buffer BUF, with its scales and masks in x. Everything of a tile is requested two tiles ahead, each
@@ -567,10 +574,11 @@ fa_q_kernel(A a) {
             // ---- S^T = K . Q^T, each block's product times its scale (and 2^24) ----
 #pragma unroll
             for (int i = 0; i < C::KSC; i++)
-                wk[(half * C::KSC + i) * FQ_KEYS + lane / 2] = fq_scale<KT>((uint16_t)((x.kd >> ksh) >> (16 * i)), NAN) * 16777216.0f;
+                wk[(half * C::KSC + i) * FQ_KEYS + lane / 2] = fq_scale<KT>((uint16_t)((x.kd >> ksh) >> (16 * i)), NAN) * kscale;
             asm volatile("" ::: "memory");   // one wave's LDS operations complete in order
 #pragma unroll
             for (int n = 0; n < NQ; n++) sc[n][0] = sc[n][1] = float4v{0, 0, 0, 0};
+            auto products = [&](auto two) __attribute__((always_inline)) {   // two: Q in halves hi and lo
 #pragma unroll
             for (int i = 0; i < C::KS; i++) {
                 float4v off[NQ];
@@ -580,6 +588,13 @@ fa_q_kernel(A a) {
 #pragma unroll
                 for (int n = 0; n < NQ; n++)
                     off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), qf[n], float4v{0, 0, 0, 0}, 0, 0, 0);
+                half8 ql[NQ];
+                if constexpr (decltype(two)::value)
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) {
+                        ql[n] = lq[C::QN + (n * C::KS + i) * WAVE + lane];
+                        off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), ql[n], off[n], 0, 0, 0);
+                    }
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const float4v d = *(const float4v *)(wk + i * FQ_KEYS + 8 * g + 4 * hf);
@@ -594,12 +609,20 @@ fa_q_kernel(A a) {
                     const half8 kf = fq_key<KT>(kx);
 #pragma unroll
                     for (int n = 0; n < NQ; n++) {
-                        const float4v p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], off[n], 0, 0, 0);
+                        float4v p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], off[n], 0, 0, 0);
+                        if constexpr (decltype(two)::value) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[n], p, 0, 0, 0);
 #pragma unroll
                         for (int e = 0; e < 4; e++) sc[n][hf][e] = fmaf(p[e], d[e], sc[n][hf][e]);
                     }
                 }
                 if (!C::KEEP_OFF) __builtin_amdgcn_sched_barrier(0);   // not every block's operands at once
+            }
+            };
+            if constexpr (PG) {
+                if (q_two) products(std::true_type{});
+                else products(std::false_type{});
+            } else {
+                products(std::false_type{});
             }
         }
         // K's codes have been read: the ones of the tile after the next come in their place (the last ones
@@ -610,7 +633,8 @@ fa_q_kernel(A a) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         dma_k(t2, row2, BUF);
         if constexpr (PG) row_p = page_of(min(t2 + NW, tile_end));
-        u32x4 pf[NQ];   // P, fp16
+        u32x4 pf[NQ];       // P, fp16
+        float px[NQ][8];    // pages: P
         {
             // ---- scale back, cap, mask, softmax ----
             const bool part = kb < FQ_KEYS * t;
@@ -755,6 +779,14 @@ fa_q_kernel(A a) {
                     for (int b = 0; b < C::VB; b++) oc[n][b] *= alpha;
                 }
                 const float mb = m_run[n] == -INFINITY ? 0.0f : m_run[n] * FQ_LOG2E;
+                if constexpr (PG) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        px[n][e] = __builtin_amdgcn_exp2f(fmaf(sc[n][e / 4][e % 4], FQ_LOG2E, -mb));
+                        l_run[n] += px[n][e];
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float s0 = sc[n][e / 2][2 * (e % 2)], s1 = sc[n][e / 2][2 * (e % 2) + 1];
@@ -786,7 +818,12 @@ fa_q_kernel(A a) {
                         for (int n = 0; n < NQ; n++)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                pd[n][e] = u_of(h2_of(pf[n][e]) * h2_of(d[b % 2][e]));
+                                if constexpr (PG) {   // rounded once
+                                    const half2v dd = h2_of(d[b % 2][e]);
+                                    pd[n][e] = u_of(half2v{(_Float16)(px[n][2 * e] * (float)dd[0]), (_Float16)(px[n][2 * e + 1] * (float)dd[1])});
+                                } else {
+                                    pd[n][e] = u_of(h2_of(pf[n][e]) * h2_of(d[b % 2][e]));
+                                }
                                 oc[n][b] = __builtin_amdgcn_fdot2(h2_of(pd[n][e]), one2, oc[n][b], false);
                             }
                     }
@@ -905,7 +942,7 @@ fa_q_kernel(A a) {
 
 template <int KT, int VT, int DK, int DV, int NQ, class A>
 static hipError_t fq_launch(const A & a, hipStream_t st) {
-    using C = FqCfg<KT, VT, DK, DV, NQ>;
+    using C = FqCfg<KT, VT, DK, DV, NQ, std::is_same<A, FaPArgs>::value>;
     static_assert(C::LDS <= 160 * 1024, "LDS");
     static bool done = false;
     if (!done) {
