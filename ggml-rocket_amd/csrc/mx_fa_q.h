@@ -108,6 +108,7 @@ struct FqCfg {
     static_assert(NW >= 4, "LDS");
     // with two waves a SIMD or fewer and one query tile there is room to keep the offsets' products
     static constexpr bool KEEP_OFF = NQ == 1 && NW <= 8;
+    static constexpr bool KEEP_Q = PG && NQ == 1 && NW == 4;  // and with one wave a SIMD Q itself
     static constexpr int CT = TT * NQ < 8 ? TT * NQ : 8;      // O^T tiles merged at a time
     static constexpr int LOOP_LDS = Q_LDS + NW * WAVE_LDS;
     static constexpr int MERGE_LDS = NW * 16 * NQ * 8 + NW * CT * 1024;
@@ -553,6 +554,13 @@ fa_q_kernel(A a) {
         vtop[i] = 0;
     }
     const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
+    half8 kq_hi[C::KEEP_Q ? C::KS : 1], kq_lo[C::KEEP_Q ? C::KS : 1];
+    if constexpr (C::KEEP_Q)
+#pragma unroll
+        for (int i = 0; i < C::KS; i++) {
+            kq_hi[i] = lq[i * WAVE + lane];
+            kq_lo[i] = lq[C::QN + i * WAVE + lane];
+        }
     const bool q_two = PG && !a.q_f16;   // an fp16 Q is its hi
     const float kscale = PG ? 16777216.0f * a.scale : 16777216.0f;
     const float cap2 = a.softcap != 0.0f ? 2.0f * FQ_LOG2E / a.softcap : 0.0f;
@@ -584,7 +592,7 @@ fa_q_kernel(A a) {
                 float4v off[NQ];
                 half8 qf[NQ];
 #pragma unroll
-                for (int n = 0; n < NQ; n++) qf[n] = lq[(n * C::KS + i) * WAVE + lane];
+                for (int n = 0; n < NQ; n++) qf[n] = C::KEEP_Q ? kq_hi[i] : lq[(n * C::KS + i) * WAVE + lane];
 #pragma unroll
                 for (int n = 0; n < NQ; n++)
                     off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), qf[n], float4v{0, 0, 0, 0}, 0, 0, 0);
@@ -592,7 +600,7 @@ fa_q_kernel(A a) {
                 if constexpr (decltype(two)::value)
 #pragma unroll
                     for (int n = 0; n < NQ; n++) {
-                        ql[n] = lq[C::QN + (n * C::KS + i) * WAVE + lane];
+                        ql[n] = C::KEEP_Q ? kq_lo[i] : lq[C::QN + (n * C::KS + i) * WAVE + lane];
                         off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), ql[n], off[n], 0, 0, 0);
                     }
 #pragma unroll
