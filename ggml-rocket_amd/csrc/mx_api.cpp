@@ -807,8 +807,8 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
 // keys, 512 rows 36 / 71; 32 sequences x 256 rows x 1024 187 / 641).
 // Fewer keys than a tile's 32, whose loads the direct form does not bound a lane at a time, are always decoded first: 14 us
 // for one sequence (300 keys 10 us), but 477 us for 32 sequences of 31 keys, one after another, where 32 keys take 9.
-static bool fa_q_few_rows(int64_t R, int64_t HK, int64_t KV, int dims) {
-    return R * dims <= 65536 || HK * ((R + 15) / 16) * ((KV + 31) / 32) <= 64 * (int64_t)device_cus();
+static bool fa_q_few_rows(int64_t R, int64_t HK, int64_t KV, int dims, int64_t most = 65536) {
+    return R * dims <= most || HK * ((R + 15) / 16) * ((KV + 31) / 32) <= 64 * (int64_t)device_cus();
 }
 static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (a->KV < mx::FA_Q_MIN_KV || a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
@@ -1046,14 +1046,17 @@ static int fa_p_check(const mi355x_fa_p_args * a, int nsplit, mx::FaPArgs & f) {
     return MI355X_OK;
 }
 
-// Many rows of a chain over a quantized cache: decoded first, a sequence at a time, as mi355x_flash_attn_q (its rule and
-// figures are at fa_q_few_rows). A tree has 64 tokens at most and is never worth it; an fp16 cache needs no decoding.
+// Many rows of a chain over a quantized cache: decoded first, a sequence at a time, as mi355x_flash_attn_q. The same rule, its
+// line itself on the decoding side: the few-row kernel rounds P and Q less often here and takes a little longer (us direct /
+// decoded, 8-bit, 8 KV heads, F32 Q: head dim 128, 128 rows of 16000 keys 48 / 60, 256 81 / 70, 512 of 4000 46 / 40, of 1000
+// 19 / 27; head dim 64, 512 rows of 16000 72 / 55, of 4000 28 / 31; head dim 256, 128 rows of 16000 117 / 148, 256 213 / 153).
+// A tree has 64 tokens at most and is read as stored; an fp16 cache needs no decoding.
 static bool fa_p_decodes(const mi355x_fa_p_args * a, const mx::FaPArgs & f) {
     if (f.k.type == mx::T_F16 || f.st.parent || (size_t)f.KV > mx::fa_max_kv(f.dk, f.dv)) return false;
     if ((int64_t)f.KV * f.HK * ((f.dk + f.dv) / 32) >= 1 << 29) return false;
     if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
         if (*e) return atoi(e) == 0;
-    return !fa_q_few_rows(f.R, f.HK, f.KV, f.D + f.DV);
+    return !fa_q_few_rows(f.R, f.HK, f.KV, f.D + f.DV, 65535);
 }
 
 // The decoded form of sequence s: the op on fp16 K and V [HK][kvp][D] and the mask [T][kvp] that the decoding launch writes.

@@ -180,7 +180,9 @@ struct KvAppendArgs {
     int half;                  // half the rotated dims
     bool neox;                 // pairs (i, i + half), else (2 i, 2 i + 1)
     float mscale;
-    int span;                  // pages that a sequence's new rows may touch (set by the launcher)
+    // set by the launcher: the launch's tokens of each sequence, first .. first + count - 1 (sources, positions and queries from
+    // there on), and the pages that their rows may touch
+    int first, count, span;
     FqDiv div_half, div_span;
 };
 hipError_t launch_kv_append(KvAppendArgs a, hipStream_t st);

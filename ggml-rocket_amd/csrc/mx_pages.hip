@@ -139,13 +139,13 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
     };
     At p = place(hb0, tok0);
     // quads left over have nothing to do; padding's sources are there to be read
-    if (tok0 < down && hb0 < end && tok0 < min(r.tok_wg, a.st.T - t0)) load(p);
+    if (tok0 < down && hb0 < end && tok0 < min(r.tok_wg, a.count - t0)) load(p);
 
     const StepOf sq = step_of(a.st, s);
-    const int toks = min(r.tok_wg, sq.fresh - t0);
+    const int toks = min(r.tok_wg, min(sq.fresh - a.first, a.count) - t0);
     if (sq.bad && t == 0 && t0 == 0 && a.st.err) *a.st.err = 1;
     if (toks <= 0) return;
-    // page k of those that sequence s2 writes, as [first, first + page) of its rows; its entry, or -1 for none
+    // page k of those that this launch writes for sequence s2, rows [p0, p0 + n2) of it: the page's first row and its entry, or -1 for none
     struct Later {
         int s2, first, p0, n2, e;
     };
@@ -153,9 +153,10 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
         Later x = {0, 0, 0, 0, -1};
         if (what == 2 || i >= a.st.S * a.span) return x;
         x.s2 = fq_div(i, a.div_span);
-        x.p0 = a.st.n_past[x.s2];
-        x.n2 = a.st.n_new ? min(a.st.n_new[x.s2], a.st.T) : a.st.T;
-        if (x.p0 < 0 || x.p0 >= a.st.cap) return x;
+        const int past = a.st.n_past[x.s2];
+        x.n2 = min((a.st.n_new ? min(a.st.n_new[x.s2], a.st.T) : a.st.T) - a.first, a.count);
+        if (past < 0 || past > a.st.cap || x.n2 <= 0) return x;
+        x.p0 = past + a.first;
         const int pi = fq_div(x.p0, a.st.div_page) + i - x.s2 * a.span;
         x.first = pi * a.st.page;
         if (pi < a.st.n_table && x.first - x.p0 < x.n2) x.e = a.st.table[(int64_t)x.s2 * a.st.table_nb + pi];
@@ -164,13 +165,13 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
     Later next = later(s * a.span + t);
     // ---- rows and positions of the tokens ----
     if (t < WAVE) {
-        int depth = t0 + t;
-        if (a.st.parent) {
+        int depth = a.first + t0 + t;
+        if (a.st.parent) {   // at most 64 tokens: first is 0
             const uint64_t anc = tree_ancestors(t < a.st.T ? a.st.parent[(int64_t)s * a.st.parent_nb + t] : -1, t);
             depth = __shfl(__popcll(anc) - 1, t0 + t, WAVE);
         }
         if (t < toks) {
-            const int j = sq.past + t0 + t, pi = fq_div(j, a.st.div_page);
+            const int j = sq.past + a.first + t0 + t, pi = fq_div(j, a.st.div_page);
             const int e = pi < a.st.n_table ? a.st.table[(int64_t)s * a.st.table_nb + pi] : -1;
             const int64_t row = page_row(a.st, e);
             entry[t] = e;
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
         next = later(i + AP_THREADS);
         for (int u = 0; u < toks; u++) {
             const int j = x.first + off[u];   // the row of s2 that token u's is
-            if (x.e >= 0 && x.e == entry[u] && j >= x.p0 && j - x.p0 < x.n2 && (x.s2 > s || j > sq.past + t0 + u)) dead[u] |= 1;
+            if (x.e >= 0 && x.e == entry[u] && j >= x.p0 && j - x.p0 < x.n2 && (x.s2 > s || j > sq.past + a.first + t0 + u)) dead[u] |= 1;
         }
     }
     __syncthreads();
@@ -262,17 +263,17 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
 }
 
 // A block a quad while that makes fewer than 2048 workgroups, then more: up to AP_TOK whole tokens a workgroup.
-hipError_t launch_kv_append(KvAppendArgs a, hipStream_t st) {
+static hipError_t append_launch(KvAppendArgs a, hipStream_t st) {
     int64_t all = 0, wgs = 0;
-    for (int k = 0; k < a.n_rows; k++) all += (int64_t)a.st.S * a.st.T * a.r[k].H * a.r[k].bph;
+    for (int k = 0; k < a.n_rows; k++) all += (int64_t)a.st.S * a.count * a.r[k].H * a.r[k].bph;
     const int64_t most = std::max<int64_t>(AP_BLOCKS, all / 2048);
     for (int k = 0; k < a.n_rows; k++) {
         KvAppendRows & r = a.r[k];
         r.items = r.H * r.bph;
-        r.tok_wg = (int)std::min<int64_t>({std::max<int64_t>(1, most / r.items), AP_TOK, a.st.T});
+        r.tok_wg = (int)std::min<int64_t>({std::max<int64_t>(1, most / r.items), AP_TOK, a.count});
         r.parts = most >= r.items ? 1 : (int)((r.items + most - 1) / most);
         r.per = (r.items + r.parts - 1) / r.parts;
-        r.groups = (a.st.T + r.tok_wg - 1) / r.tok_wg;
+        r.groups = (a.count + r.tok_wg - 1) / r.tok_wg;
         r.down = std::max(1, AP_BLOCKS / r.per);
         r.wide = (k == 2 || a.o[k].type == T_F16) && (!r.rotate || !a.neox || a.half % 8 == 0);
         r.wg_begin = (int)wgs;
@@ -280,12 +281,40 @@ hipError_t launch_kv_append(KvAppendArgs a, hipStream_t st) {
         r.div_bph = fq_div_by(r.bph); r.div_parts = fq_div_by(r.parts); r.div_groups = fq_div_by(r.groups);
         r.div_across = fq_div_by(std::min(r.per, AP_BLOCKS));
     }
-    a.span = (a.st.T + a.st.page - 2) / a.st.page + 1;
     a.div_half = fq_div_by(std::max(1, a.half));
     a.div_span = fq_div_by(a.span);
     if (a.neox) hipLaunchKernelGGL(kv_append_kernel<true>, dim3((unsigned)wgs), dim3(AP_THREADS), 0, st, a);
     else hipLaunchKernelGGL(kv_append_kernel<false>, dim3((unsigned)wgs), dim3(AP_THREADS), 0, st, a);
     return hipGetLastError();
+}
+
+static void advance(KvPlainRows & x, int64_t s, int64_t t) { x.x = (uint8_t *)x.x + (s * x.nb3 + t * x.nb1) * (x.f16 ? 2 : 4); }
+
+// A launch takes AP_TOKENS tokens of a sequence at most, or sequences that write AP_PAGES pages at most, the next ones a next
+// launch, where a row that is named again comes later by itself: what its workgroups look through for later owners grows
+// with the square of a launch.
+constexpr int AP_TOKENS = 1 << 16, AP_PAGES = 2048;
+hipError_t launch_kv_append(KvAppendArgs a, hipStream_t st) {
+    const int S = a.st.S, T = a.st.T, count = std::min(T, AP_TOKENS);
+    a.span = (count + a.st.page - 2) / a.st.page + 1;   // pages that a sequence's rows may touch
+    const int many = count < T ? 1 : std::max(1, AP_PAGES / a.span);
+    for (int s = 0; s < S; s += many)
+        for (int t = 0; t < T; t += count) {
+            KvAppendArgs b = a;
+            b.st.S = std::min(many, S - s);
+            b.first = t;
+            b.count = std::min(count, T - t);
+            b.st.table += s * a.st.table_nb;
+            b.st.n_past += s;
+            if (a.st.n_new) b.st.n_new += s;
+            if (a.st.parent) b.st.parent += s * a.st.parent_nb;
+            if (a.pos) b.pos += s * a.pos_nb + t;
+            for (int k = 0; k < a.n_rows; k++) advance(b.r[k].x, s, t);
+            if (a.n_rows > 2) advance(b.qr, s, t);
+            const hipError_t e = append_launch(b, st);
+            if (e != hipSuccess) return e;
+        }
+    return hipSuccess;
 }
 
 // A thread moves one block of 32 values and its scale, row after row. Source path[i] lies at or behind
@@ -359,8 +388,20 @@ hipError_t launch_kv_keep(KvKeepArgs a, hipStream_t st) {
         bpr = std::max(bpr, a.o[k].div_bpr.d);
     }
     a.wgs = (bpr + AP_THREADS - 1) / AP_THREADS;
-    hipLaunchKernelGGL(kv_keep_kernel, dim3((unsigned)(a.st.S * a.wgs), a.n_out), dim3(AP_THREADS), 0, st, a);
-    return hipGetLastError();
+    const int S = a.st.S, many = std::max(1, (1 << 23) / a.wgs);   // threads of a launch below 2^32
+    for (int s = 0; s < S; s += many) {
+        KvKeepArgs b = a;
+        b.st.S = std::min(many, S - s);
+        b.st.table += s * a.st.table_nb;
+        b.st.n_past += s;
+        if (a.st.n_new) b.st.n_new += s;
+        b.path += s * a.path_nb;
+        if (a.n_keep) b.n_keep += s;
+        hipLaunchKernelGGL(kv_keep_kernel, dim3((unsigned)(b.st.S * a.wgs), a.n_out), dim3(AP_THREADS), 0, st, b);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // A sequence's rows out of their pages as fp16 for the fused attention (kv_decode_kernel has the values and what becomes of

@@ -568,6 +568,13 @@ def flash_attn_q(q, k: KvCache, v: KvCache, mask, scale: float, softcap: float =
 
 # ---- a KV cache in pages --------------------------------------------------------------------
 
+def _set_once(self, name, value):
+    """Of objects that hold their tensors' addresses: another tensor in a field would leave the old address in use."""
+    if hasattr(self, name):
+        raise MI355XError(f"{type(self).__name__}.{name} is fixed: make a new one, or change the tensor's values")
+    object.__setattr__(self, name, value)
+
+
 class KvStep:
     """A step of S sequences over caches in pages (mi355x_kv_step): page p of a cache [rows, HK, D] is its rows
     p * page .. p * page + page - 1; sequence s holds n_past[s] rows, found through the pages table[s] names, and
@@ -596,6 +603,8 @@ class KvStep:
                                table.shape[1], self.S, self.T, self.page)
         self._raw = bytes(self.args)
 
+    __setattr__ = _set_once
+
 
 class Rope:
     """The position rotation of kv_append: pair i of a head's first 2 * len(freq) dims, (2 i, 2 i + 1) or with neox
@@ -615,6 +624,8 @@ class Rope:
         # its part of mi355x_kv_append_args
         self._args = (freq.data_ptr(), 0 if positions is None else positions.data_ptr(), 0 if positions is None else positions.stride(0),
                       2 * freq.shape[0], self.neox, self.mscale)
+
+    __setattr__ = _set_once
 
 
 def rope_freqs(n_rot: int, base: float = 10000.0, factors=None, device="cuda"):
@@ -651,6 +662,8 @@ def kv_append(step: KvStep, k_cache: KvCache, v_cache: KvCache, k, v, rope: Rope
     kr, k3 = _step_rows(k_cache, k, step, "kv_append")
     vr, v3 = _step_rows(v_cache, v, step, "kv_append")
     queries = _NO_QUERIES
+    if q is None and q_out is not None:
+        raise MI355XError("kv_append: q_out without q")
     if q is not None:
         if q_out is None:
             q_out = _torch().empty_like(q)

@@ -422,7 +422,8 @@ typedef struct mi355x_kv_step {
  * Pair i < n_rot / 2 of a head's dims, (2 i, 2 i + 1) or with neox (i, i + n_rot / 2), turns by theta = p * freq_dev[i], p the
  * position pos_dev[s][t], or, without it, n_past[s] plus the number of tokens above t: c = cos(theta) * mscale and s
  * likewise are formed in 64 bits and rounded to f32, then a' = a c - b s and b' = a s + b c with every product and sum
- * rounded to f32. n_rot: a multiple of 8 up to D and 256, or 0. Dims from n_rot on stay as they are.
+ * rounded to f32; |theta| below 2^40. n_rot: a multiple of 8 up to D and 256, or 0. Dims from n_rot on stay as they are.
+ * One launch, or one for every 2^16 tokens of a sequence, or for every so many sequences as may write 2048 pages.
  * Where tables share a page and two tokens' rows are one, the last token's (by sequence, then number) stays, whole.
  * Rows and queries of padding are left as they were. A token without a row in the cache is not stored; its query is
  * rotated. K and V are different caches. H * D / 32 of each at most 2^16. */
@@ -445,7 +446,9 @@ MI355X_API int mi355x_kv_append(const mi355x_kv_append_args * a, int32_t * err_d
  * F16 (values at q_dev, d_dev not read): dst[s][t] = softmax over the keys that t sees of cap(scale * q.k), times v.
  * Token t of sequence s sees its n_past[s] rows, itself and the tokens above it. Padding, and a token none of whose keys
  * lies in the cache, are written as zeros. A key that a token does not see adds nothing to it, whatever the cache holds there, NaN
- * included. Roundings and limits of the values as in mi355x_flash_attn_q.
+ * included. Limits of the values as in mi355x_flash_attn_q; roundings, read from the pages, of the matrix unit's operands to
+ * fp16: P times the scale of V's block (an fp16 cache: P) once, Q only where it is F32 and then by 2^-22 of itself; an output
+ * is 1.7e-4 of its norm from the 64-bit value then, and an fp16 one's own rounding 2.1e-4. Decoded first: as there.
  * max_kv: a number that no n_past + n_new passes (0: n_table * page). The launch and its workspace are planned for it;
  * it takes the place of n_table * page in what the step says of numbers out of range.
  * H % HK == 0; D and DV multiples of 32 up to 256, each at least half of what the kernels are built for (64 / 64, 128 / 128,

@@ -164,6 +164,8 @@ def test_binding_refusals():
         with pytest.raises(mx.MI355XError):
             mx.KvStep(**{**good, **bad})
     st = mx.KvStep(**good)
+    with pytest.raises(mx.MI355XError):
+        st.n_past = i(2)             # the address of the first would stay in use
     for bad in (dict(freq=torch.zeros(6)), dict(freq=torch.zeros(8).double()), dict(freq=torch.zeros(16)[::2]), dict(freq=torch.zeros(8), positions=torch.zeros(2, 3)),
                 dict(freq=torch.zeros(8), positions=i(6))):
         with pytest.raises(mx.MI355XError):
@@ -173,7 +175,7 @@ def test_binding_refusals():
     k, v, q = torch.zeros(2, 3, 2, 64), torch.zeros(2, 3, 2, 32), torch.zeros(2, 3, 4, 64)
     rope = mx.Rope(torch.zeros(32))
     for a, kw in (((kc, vc, k[:, :2], v), {}), ((kc, vc, k, v[..., :16]), {}), ((kc, vc, k.double(), v), {}), ((kc, vc, k, v), dict(q=q[:1])),
-                  ((kc, vc, k, v), dict(q=q[..., :32])), ((kc, vc, k, v), dict(q=q, q_out=q[:, :, :2])), ((kc, vc, k, v), dict(q=q.double())),
+                  ((kc, vc, k, v), dict(q=q[..., :32])), ((kc, vc, k, v), dict(q=q, q_out=q[:, :, :2])), ((kc, vc, k, v), dict(q=q.double())), ((kc, vc, k, v), dict(q_out=q)),
                   ((kc[:, 0], vc, k, v), {}), ((kc, vc, k, v), dict(rope=mx.Rope(torch.zeros(32), positions=i(2, 4)))), ((kc, vc, k, v), dict(rope=rope))):
         with pytest.raises(mx.MI355XError):
             mx.kv_append(st, *a, **kw)

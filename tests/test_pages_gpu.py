@@ -221,6 +221,37 @@ def test_append_rows_that_two_tokens_share(mx, T, page):
     assert same(planes_of(kc), kp) and same(planes_of(vc), vp)
 
 
+@pytest.mark.parametrize("S,T,page", [(2300, 1, 32), (1, 70000, 32), (2, 66000, 96)])
+def test_append_in_several_launches(mx, S, T, page):
+    """More sequences and tokens than a launch takes, and rows shared between those of different launches."""
+    HK, D = 1, 32
+    rng = np.random.default_rng(S + T)
+    past = [int(n) for n in rng.integers(0, 50, S)]
+    new = [T - int(n) for n in rng.integers(0, 2, S)]
+    n_table = (50 + T) // page + 2
+    pages = max(4, S * n_table * 2 // 3)
+    table = rng.integers(0, pages, (S, n_table)).astype(np.int32)
+    kc, kp = cache_of(mx, Q8_0, pages * page, HK, D, rng)
+    vc, vp = cache_of(mx, F16, pages * page, HK, D, rng)
+    q, k, v = (rng.standard_normal((S, T, HK, D)).astype(np.float32) for _ in range(3))
+    freq = np.array([1.0, 0.1, 0.01, 0.001], np.float32)
+    step = mx.KvStep(i32(table), i32(past), T, page, n_new=i32(new))
+    got = cpu(mx.kv_append(step, kc, vc, gpu(k), gpu(v), rope=mx.Rope(gpu(freq)), q=gpu(q)))
+    for s in range(S):
+        n = new[s]
+        if not n:
+            continue
+        j = past[s] + np.arange(n)
+        at = table[s][j // page].astype(np.int64) * page + j % page
+        turned = P.rotate(np.concatenate([k[s, :n], q[s, :n]], 1), j, freq, False)
+        assert np.array_equal(got[s, :n], turned[:, 1:])
+        last = np.unique(at[::-1], return_index=True)     # of the tokens with one row the last
+        for pl, x, ty in ((kp, turned[:, :1], Q8_0), (vp, v[s, :n], F16)):
+            for p, y in zip(pl, P.planes(x, ty)):
+                p[last[0]] = y[::-1][last[1]]
+    assert same(planes_of(kc), kp) and same(planes_of(vc), vp)
+
+
 FAULTS = {   # past, new, what is done to the table; the tokens stored nevertheless
     "past_negative": ([-1, 4], [2, 2], None, {1: [0, 1]}),
     "past_behind": ([97, 4], [1, 2], None, {1: [0, 1]}),
@@ -652,3 +683,68 @@ def test_loop_captured(mx, mix):
         else:
             graph.replay()
         loop.check()
+
+
+@pytest.mark.parametrize("mix", [(Q8_0, Q4_0), (F16, F16)], ids=ids)
+def test_lengths_that_change_inside_a_graph(mx, mix):
+    """Several steps in one graph: each call sees the lengths that the call before it left."""
+    import torch
+    H, HK, D, page, n = 4, 2, 64, 32, 5
+    rng = np.random.default_rng(9)
+    table, pages = tables(rng, [90], [20 * n], page)
+    caches = [cache_of(mx, t, pages * page, HK, D, rng) for t in mix]
+    q, k, v = (rng.standard_normal((n, 1, 1, h, D)).astype(np.float32) for h in (H, HK, HK))
+    dq, dk, dv = gpu(q), gpu(k), gpu(v)
+    past = i32([60])
+    step = mx.KvStep(i32(table), past, 1, page)
+    kc, vc = caches[0][0], caches[1][0]
+    outs = [torch.zeros(1, 1, H, D, device="cuda") for _ in range(n)]
+    ws = torch.empty(mx.flash_attn_paged_workspace(dq[0].permute(0, 2, 1, 3), kc, vc, step, outs[0]), dtype=torch.uint8, device="cuda")
+
+    def calls():
+        for i in range(n):
+            mx.kv_append(step, kc, vc, dk[i], dv[i])
+            mx.flash_attn_paged(dq[i].permute(0, 2, 1, 3), kc, vc, step, 0.125, out=outs[i], workspace=ws)
+            past.add_(1)
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        calls()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        calls()
+    at = 60 + n                                     # the eager steps; capturing runs nothing
+    for _ in range(4):
+        for pl, x, t in ((caches[0][1], k, mix[0]), (caches[1][1], v, mix[1])):
+            pl[:] = planes_of(kc if pl is caches[0][1] else vc)
+        graph.replay()
+        got = [cpu(o) for o in outs]
+        for i in range(n):
+            r = P.row(table[0], page, at + i)
+            for pl, x, t in ((caches[0][1], k, mix[0]), (caches[1][1], v, mix[1])):
+                for p, y in zip(pl, P.planes(x[i, 0], t)):
+                    p[r] = y[0]
+            want, tol = P.attend(q[i, 0].transpose(1, 0, 2).astype(np.float64), caches[0][1], caches[1][1], *mix, table[0], page, pages, at + i, 1, None, 0.125)
+            assert (np.abs(got[i][0] - want) <= tol).all()
+        at += n
+        assert int(past[0]) == at
+
+
+def test_two_streams_at_once(mx):
+    """Calls in flight on two streams, a workspace each, over one cache."""
+    import torch
+    c = attend_case(mx, Q8_0, Q8_0, (4, 6, True, [3000, 2500, 100, 0], 32, 8, 2, 128, 128), seed=2)
+    q = gpu(c["q"]).permute(0, 2, 1, 3)
+    caches = [x[0] for x in c["caches"]]
+    want = cpu(mx.flash_attn_paged(q, *caches, c["step"], 0.09))
+    outs = [torch.zeros(4, 6, 8, 128, device="cuda") for _ in range(2)]
+    need = mx.flash_attn_paged_workspace(q, *caches, c["step"], outs[0])
+    ws = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                mx.flash_attn_paged(q, *caches, c["step"], 0.09, out=outs[i], workspace=ws[i])
+    assert all(np.array_equal(cpu(o), want) for o in outs)
