@@ -51,6 +51,21 @@
 // wave at some 2.5 us each). A block's start until its first data is 3 to 5 us, its end 2.5 us. A tile is the latency
 // of its wave's own chain, not a unit at its limit (32768 Q4_0 keys: VALU instructions 0.23 of a wave's time, waits
 // 0.24, matrix units 0.04 busy).
+//
+// A cache in pages (mi355x_flash_attn_paged; FaPArgs, `PG` below) is read by the same loop. A tile is 32 rows of one page, so its
+// place is one table entry, which comes through the scalar cache a tile ahead: the counts that the waits go by stay
+// as they are. The lengths are read on the device and a unit's keys are split evenly over its blocks, however many there
+// are. Instead of a mask a row has a number of keys that it sees and, of the new tokens, a bit each (fp_sees: the ancestors of
+// its node of the tree, from the parents by doubling, in each wave), looked at in the last tiles alone.
+// Roundings there: P d, from F32, once; Q is exact where it is fp16, its scale in K's F32 scales, and two halves, hi + lo, off
+// by 2^-22, where it is F32 (one more product a block). An output is 1.7e-4 of its norm from 64 bits, 2.7e-4 as fp16, for 2.9e-4
+// and 3.6e-4 with Q rounded and P rounded before d; that takes 1 to 3 % where the memory or latency counts, 12 % with many rows.
+// Measured (this kernel, its merge 4 us more): one token on 1000 Q8_0 keys 11.8 us, 32 sequences of 1 to 4096 keys 54 us (143 MB, 2.6
+// TB/s; the longest ones' chain), a tree of 5 on 131072 Q4_0 keys 80 us (151 MB, 1.9 TB/s), of 16 on 16000 keys of head dim 256 42
+// us. Many keys take 0.92 us a tile and SIMD: some 270 vector instructions and 20 to 28 products, three quarters of what a
+// SIMD can issue in that time. Two tiles side by side through each step (253 registers) took as long, blocks of four waves two
+// a CU 53 us for 40 (32 sequences out of the last-level cache), twelve waves of 168 registers a quarter longer (28 spilled), the
+// offsets as products instead of sums of P d 7 % longer, and parts made alike over all sequences by their lengths 59 us for 53.
 
 #pragma once
 
