@@ -60,12 +60,15 @@
 // Roundings there: P d, from F32, once; Q is exact where it is fp16, its scale in K's F32 scales, and two halves, hi + lo, off
 // by 2^-22, where it is F32 (one more product a block). An output is 1.7e-4 of its norm from 64 bits, 2.7e-4 as fp16, for 2.9e-4
 // and 3.6e-4 with Q rounded and P rounded before d; that takes 1 to 3 % where the memory or latency counts, 12 % with many rows.
-// Measured (this kernel, its merge 4 us more): one token on 1000 Q8_0 keys 11.8 us, 32 sequences of 1 to 4096 keys 54 us (143 MB, 2.6
-// TB/s; the longest ones' chain), a tree of 5 on 131072 Q4_0 keys 80 us (151 MB, 1.9 TB/s), of 16 on 16000 keys of head dim 256 42
-// us. Many keys take 0.92 us a tile and SIMD: some 270 vector instructions and 20 to 28 products, three quarters of what a
-// SIMD can issue in that time. Two tiles side by side through each step (253 registers) took as long, blocks of four waves two
-// a CU 53 us for 40 (32 sequences out of the last-level cache), twelve waves of 168 registers a quarter longer (28 spilled), the
-// offsets as products instead of sums of P d 7 % longer, and parts made alike over all sequences by their lengths 59 us for 53.
+// Measured (this kernel, its merge 4 us more): one token on 1000 Q8_0 keys 11.7 us, 32 sequences of 1 to 4096 keys 56 us (143 MB, 2.6
+// TB/s; the longest ones' chain), a tree of 5 on 131072 Q4_0 keys 77 us (151 MB, 2.0 TB/s), of 16 on 16000 keys of head dim 256 42
+// us. With many keys a wave's tile is 346 vector instructions and 24 products (the tree of 5); with two waves a SIMD vector
+// instructions take 0.60 of its time, instructions of any kind 0.90, waits 0.16 of a wave's. What was taken out of it: the offsets'
+// products are formed once before the loop, P d rounds in one instruction each and a nibble's mask needs no byte moved
+// first (68 of 414 vector instructions and 8 of 32 products; the tree of 5 took 80.8 us with them). What did not help: two tiles side by side through each step (253
+// registers) took as long, blocks of four waves two a CU 53 us for 40 (32 sequences out of the last-level cache), twelve waves of
+// 168 registers a quarter longer (28 spilled), the offsets as products instead of sums of P d 7 % longer, and parts made
+// alike over all sequences by their lengths 59 us for 53.
 
 #pragma once
 
@@ -105,6 +108,8 @@ struct FqCfg {
     __device__ static __forceinline__ int vswz(int row) { return (row * VCH / 16) & (VCH - 1); }
     static constexpr int VH = VT == T_Q4_0 ? 2 : 1;           // nibbles a byte
     static constexpr int VN = 4 / VH;                         // chunks of two of V's blocks, read at a time
+    // pages: a nibble's mask takes the other bytes away, so two of four bytes stay where they are
+    static constexpr bool BY_TWOS = PG && VT == T_Q4_0;
     static constexpr int TT = DV / 16;                        // O^T tiles of 16 dims: chunk * VH + nibble
     static_assert(KRB == 16 * KS * KW && VCH * VH == TT, "layout");
     static constexpr int VB = DV / 32, VS = DV / 64, KSC = DK / 64;   // scales a key, and a lane (32 keys, two lanes each)
@@ -577,6 +582,14 @@ fa_q_kernel(A a) {
             kq_lo[i] = lq[C::QN + i * WAVE + lane];
         }
     const bool q_two = PG && !a.q_f16;   // an fp16 Q is its hi
+    float4v kept_off[PG && C::KEEP_OFF ? C::KS : 1];   // the offsets' products (the compiler leaves them in the loop's two forms)
+    if constexpr (PG && C::KEEP_OFF)
+#pragma unroll
+        for (int i = 0; i < C::KS; i++) {
+            const half8 hi = C::KEEP_Q ? kq_hi[i] : lq[i * WAVE + lane], lo = C::KEEP_Q ? kq_lo[i] : lq[C::QN + i * WAVE + lane];
+            kept_off[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), hi, float4v{0, 0, 0, 0}, 0, 0, 0);
+            if (q_two) kept_off[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), lo, kept_off[i], 0, 0, 0);
+        }
     const float kscale = PG ? 16777216.0f * a.scale : 16777216.0f;
     const float cap2 = a.softcap != 0.0f ? 2.0f * FQ_LOG2E / a.softcap : 0.0f;
 
@@ -610,13 +623,14 @@ fa_q_kernel(A a) {
                 for (int n = 0; n < NQ; n++) qf[n] = C::KEEP_Q ? kq_hi[i] : lq[(n * C::KS + i) * WAVE + lane];
 #pragma unroll
                 for (int n = 0; n < NQ; n++)
-                    off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), qf[n], float4v{0, 0, 0, 0}, 0, 0, 0);
+                    off[n] = PG && C::KEEP_OFF ? kept_off[i] : __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), qf[n], float4v{0, 0, 0, 0}, 0, 0, 0);
                 half8 ql[NQ];
                 if constexpr (decltype(two)::value)
 #pragma unroll
                     for (int n = 0; n < NQ; n++) {
                         ql[n] = C::KEEP_Q ? kq_lo[i] : lq[C::QN + (n * C::KS + i) * WAVE + lane];
-                        off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), ql[n], off[n], 0, 0, 0);
+                        if constexpr (!PG || !C::KEEP_OFF)
+                            off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, koff), ql[n], off[n], 0, 0, 0);
                     }
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
@@ -841,9 +855,10 @@ fa_q_kernel(A a) {
                         for (int n = 0; n < NQ; n++)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                if constexpr (PG) {   // rounded once
-                                    const half2v dd = h2_of(d[b % 2][e]);
-                                    pd[n][e] = u_of(half2v{(_Float16)(px[n][2 * e] * (float)dd[0]), (_Float16)(px[n][2 * e + 1] * (float)dd[1])});
+                                if constexpr (PG) {   // rounded once (with the addition one instruction each, without it 2 1/2)
+                                    const int k0 = C::BY_TWOS ? 4 * (e / 2) + e % 2 : 2 * e, k1 = k0 + (C::BY_TWOS ? 2 : 1);
+                                    pd[n][e] = u_of(half2v{(_Float16)fmaf(px[n][k0], (float)h2_of(d[b % 2][k0 / 2])[k0 % 2], 0.0f),
+                                                           (_Float16)fmaf(px[n][k1], (float)h2_of(d[b % 2][k1 / 2])[k1 % 2], 0.0f)});
                                 } else {
                                     pd[n][e] = u_of(h2_of(pf[n][e]) * h2_of(d[b % 2][e]));
                                 }
@@ -851,9 +866,10 @@ fa_q_kernel(A a) {
                             }
                     }
                     const uint32_t flip = VT == T_Q8_0 ? 0x80808080u : 0u, xl = (uint32_t)w[c][0] ^ flip, xh = (uint32_t)w[c][1] ^ flip;
-                    // bytes of keys (2 e, 2 e + 1), zero-extended
-                    const u32x4 y = {__builtin_amdgcn_perm(0u, xl, 0x0C010C00u), __builtin_amdgcn_perm(0u, xl, 0x0C030C02u),
-                                     __builtin_amdgcn_perm(0u, xh, 0x0C010C00u), __builtin_amdgcn_perm(0u, xh, 0x0C030C02u)};
+                    // bytes of keys (2 e, 2 e + 1), zero-extended, or those of keys (0, 2), (1, 3), (4, 6), (5, 7) in the low ones
+                    const u32x4 y = C::BY_TWOS ? u32x4{xl, xl >> 8, xh, xh >> 8}
+                                               : u32x4{__builtin_amdgcn_perm(0u, xl, 0x0C010C00u), __builtin_amdgcn_perm(0u, xl, 0x0C030C02u),
+                                                       __builtin_amdgcn_perm(0u, xh, 0x0C010C00u), __builtin_amdgcn_perm(0u, xh, 0x0C030C02u)};
 #pragma unroll
                     for (int h = 0; h < C::VH; h++) {
                         const u32x4 u = VT == T_Q8_0 ? y : h ? y & 0x00F000F0u : y & 0x000F000Fu;
