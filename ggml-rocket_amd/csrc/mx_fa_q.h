@@ -59,16 +59,16 @@
 // its node of the tree, from the parents by doubling, in each wave), looked at in the last tiles alone.
 // Roundings there: P d, from F32, once; Q is exact where it is fp16, its scale in K's F32 scales, and two halves, hi + lo, off
 // by 2^-22, where it is F32 (one more product a block). An output is 1.7e-4 of its norm from 64 bits, 2.7e-4 as fp16, for 2.9e-4
-// and 3.6e-4 with Q rounded and P rounded before d; that takes 1 to 3 % where the memory or latency counts, 12 % with many rows.
+// and 3.6e-4 with Q rounded and P rounded before d; an F32 Q takes 0 to 4 % longer than an fp16 one, 6 % with many rows.
 // Measured (this kernel, its merge 4 us more): one token on 1000 Q8_0 keys 11.7 us, 32 sequences of 1 to 4096 keys 56 us (143 MB, 2.6
 // TB/s; the longest ones' chain), a tree of 5 on 131072 Q4_0 keys 77 us (151 MB, 2.0 TB/s), of 16 on 16000 keys of head dim 256 42
 // us. With many keys a wave's tile is 346 vector instructions and 24 products (the tree of 5); with two waves a SIMD vector
 // instructions take 0.60 of its time, instructions of any kind 0.90, waits 0.16 of a wave's. What was taken out of it: the offsets'
 // products are formed once before the loop, P d rounds in one instruction each and a nibble's mask needs no byte moved
-// first (68 of 414 vector instructions and 8 of 32 products; the tree of 5 took 80.8 us with them). What did not help: two tiles side by side through each step (253
-// registers) took as long, blocks of four waves two a CU 53 us for 40 (32 sequences out of the last-level cache), twelve waves of
-// 168 registers a quarter longer (28 spilled), the offsets as products instead of sums of P d 7 % longer, and parts made
-// alike over all sequences by their lengths 59 us for 53.
+// first (68 of 414 vector instructions and 8 of 32 products; the tree of 5 took 80.8 us with them). What did not help: two tiles
+// side by side through each step (253 registers) took as long, blocks of four waves two a CU 53 us for 40 (32 sequences out of the
+// last-level cache), twelve waves of 168 registers a quarter longer (28 spilled), the offsets as products instead of sums of P d
+// 7 % longer, and parts made alike over all sequences by their lengths 59 us for 53.
 
 #pragma once
 
