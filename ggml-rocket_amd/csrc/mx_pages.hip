@@ -162,6 +162,14 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
         if (pi < a.st.n_table && x.first - x.p0 < x.n2) x.e = a.st.table[(int64_t)x.s2 * a.st.table_nb + pi];
         return x;
     };
+    // whether token i of sequence s2 is one of a chain, or has a way up the tree's parents
+    auto stored = [&](int s2, int i) {
+        while (a.st.parent && i >= 0) {
+            const int up = a.st.parent[(int64_t)s2 * a.st.parent_nb + i];
+            i = up < i ? up : -2;
+        }
+        return i >= -1;
+    };
     Later next = later(s * a.span + t);
     // ---- rows and positions of the tokens ----
     if (t < WAVE) {
@@ -196,7 +204,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(KvAppendArgs a) {
         next = later(i + AP_THREADS);
         for (int u = 0; u < toks; u++) {
             const int j = x.first + off[u];   // the row of s2 that token u's is
-            if (x.e >= 0 && x.e == entry[u] && j >= x.p0 && j - x.p0 < x.n2 && (x.s2 > s || j > sq.past + a.first + t0 + u)) dead[u] |= 1;
+            if (x.e >= 0 && x.e == entry[u] && j >= x.p0 && j - x.p0 < x.n2 && (x.s2 > s || j > sq.past + a.first + t0 + u) && stored(x.s2, j - x.p0)) dead[u] |= 1;
         }
     }
     __syncthreads();

@@ -221,6 +221,32 @@ def test_append_rows_that_two_tokens_share(mx, T, page):
     assert same(planes_of(kc), kp) and same(planes_of(vc), vp)
 
 
+def test_append_shared_rows_of_nodes_without_a_way_up(mx):
+    """A node that counts as padding writes no row, so an earlier token's that shares the row stays."""
+    S, T, HK, D, page = 3, 12, 2, 64, 32
+    rng = np.random.default_rng(31)
+    past, new = [20, 20, 17], [12, 12, 9]
+    table = np.array([[0, 1], [0, 1], [0, 2]], np.int32)
+    parents = tree(rng, S, T)
+    parents[1, 3], parents[1, 5], parents[1, 7] = 3, 5, 11
+    parents[2, 1], parents[2, 4] = -5, 4
+    parents[2, 6] = 4                                # below one that has no way up itself
+    kc, kp = cache_of(mx, Q8_0, 3 * page, HK, D, rng)
+    vc, vp = cache_of(mx, F16, 3 * page, HK, D, rng)
+    k, v = (rng.standard_normal((S, T, HK, D)).astype(np.float32) for _ in range(2))
+    err = zeros_i32()
+    mx.kv_append(mx.KvStep(i32(table), i32(past), T, page, n_new=i32(new), parents=i32(parents)), kc, vc, gpu(k), gpu(v), err=err)
+    for s in range(S):
+        for t, w in enumerate(P.ways(parents[s], new[s])):
+            if w is None:
+                continue
+            r = P.row(table[s], page, past[s] + t)
+            for pl, x, ty in ((kp, k, Q8_0), (vp, v, F16)):
+                for p, y in zip(pl, P.planes(x[s, t:t + 1], ty)):
+                    p[r] = y[0]
+    assert same(planes_of(kc), kp) and same(planes_of(vc), vp) and int(err) == 1
+
+
 @pytest.mark.parametrize("S,T,page", [(2300, 1, 32), (1, 70000, 32), (2, 66000, 96)])
 def test_append_in_several_launches(mx, S, T, page):
     """More sequences and tokens than a launch takes, and rows shared between those of different launches."""
