@@ -10,6 +10,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "mx_fa_dims.h"
 #include "mx_kernels_impl.h"
@@ -984,21 +985,50 @@ MI355X_API int mi355x_kv_keep(const mi355x_kv_step * step, const mi355x_kv_rows 
     return some ? hip_status(mx::launch_kv_keep(a, S(stream))) : MI355X_OK;
 }
 
-// Rows a wave and KV splits over an fp16 cache (mx_fa_pf16.hip; us on 8 KV heads). Two row tiles a wave share the reads of
-// K and V: taken where the blocks that are left still fill the chip (head dim 128, 8000 keys: 256 rows of one sequence 32.6 /
-// 32.6, of four 98 / 76; 2048 rows 152 / 102; 10 sequences x 256 rows of up to 3000 keys 88 / 70, at head dim 64 56 / 48).
-// Keys are split up to one block a compute unit for single row tiles, which the memory bounds (one token on
-// 32768 keys, in 16, 32 and 64 splits 29.2, 28.0, 31.8; 32 tokens on 4096 each whole 56, in two 63), to two where
-// many rows make the work arithmetic (four times 256 rows 100 whole, 84 in two, 76 in four; 2048 102 whole, 126 in two).
+// Rows a wave and KV splits over an fp16 cache (mx_fa_pf16.hip): the pair whose estimated time is least. Estimate: a CU holds
+// `slots` blocks; a round of blocks takes a start and end and, for each of a wave's tiles, what a tile's chain takes or, if more, what
+// the blocks beside each other on a CU take of its units; HBM sets a floor; a split adds the merge. The numbers (us) are fitted to
+// some 900 times of 34 shapes a head dim, to 10 to 17 % each; the pair taken is 2 % from the best measured one in the mean (two
+// tiles a wave where that filled the chip, and splits up to it: 14 %). Examples, 8 KV heads, best with one row tile / two:
+// 512 rows of 16000 keys, head dim 64 56 / 42, 128 107 / 74; 64 rows, head dim 128 30 / 26; 256 rows of 1000 and of 4 sequences, head dim
+// 64 12.6 / 15.2, 128 20.6 / 18.5. Not split past one round of blocks: 10 sequences of 3000 keys, 256 rows each, 82 whole and 90 in three.
+struct FpCost {
+    int slots[2];                     // one row tile a wave, two
+    double ends, chain[2], unit[2];   // a block's start and end; a tile's chain; a CU's units, a tile of each block's waves
+    double merge, merge_cu;           // the second launch, and more for each row tile a CU hands it
+};
+static FpCost fp_cost(int D) {
+    return D <= 64    ? FpCost{{4, 3}, 4.2, {0.63, 0.82}, {0.35, 0.53}, 4.4, 0.4}
+           : D <= 128 ? FpCost{{2, 2}, 3.9, {1.05, 1.2}, {0.7, 1.2}, 5.4, 1.0}
+           : D <= 192 ? FpCost{{1, 1}, 4.1, {1.3, 1.8}, {1.3, 1.8}, 5.3, 1.0}
+                      : FpCost{{1, 1}, 6.8, {1.9, 1.9}, {1.9, 1.9}, 5.2, 0.1};
+}
 static void fa_p_plan_f16(mx::FaPArgs & f, int nsplit) {
     const int64_t cus = device_cus(), ntiles = (f.KV + 31) / 32;
-    auto units = [&](int nq) { return (int64_t)f.S * f.HK * ((f.R + 16 * nq - 1) / (16 * nq)); };
-    f.nq = f.D <= 192 && f.R > 16 && units(2) >= cus ? 2 : 1;
+    const FpCost c = fp_cost(f.D);
+    const double hbm = (double)f.S * ntiles * 64 * f.HK * (f.D + f.DV) / 4.6e6 + 4.0;
+    int first = 1, last = f.D <= 192 && f.R > 16 ? 2 : 1;
     if (const char * e = getenv("MI355X_FA_Q_ROWS"))
-        if (*e) f.nq = atoi(e) == 32 && f.D <= 192 ? 2 : 1;
+        if (*e) first = last = atoi(e) == 32 && f.D <= 192 ? 2 : 1;
+    double best = 0.0;
+    f.nsplit = 0;
+    for (int nq = first; nq <= last; nq++) {
+        const int64_t units = (int64_t)f.S * f.HK * ((f.R + 16 * nq - 1) / (16 * nq)), room = c.slots[nq - 1] * cus;
+        const int64_t most = nsplit > 0 ? nsplit : std::max<int64_t>(1, std::min<int64_t>({64, room / units, ntiles / 4}));
+        for (int64_t ns = nsplit > 0 ? nsplit : 1; ns <= most; ns++) {
+            const int64_t blocks = units * ns, chain = ((ntiles + ns - 1) / ns + 3) / 4, rest = blocks % room;
+            auto round = [&](int64_t beside) { return c.ends + chain * std::max(c.chain[nq - 1], beside * c.unit[nq - 1]); };
+            double t = blocks / room * round(c.slots[nq - 1]) + (rest ? round((rest + cus - 1) / cus) : 0.0);
+            t = std::sqrt(std::sqrt(t * t * t * t + hbm * hbm * hbm * hbm));
+            if (ns > 1) t += c.merge + c.merge_cu * nq * blocks / cus;
+            if (!f.nsplit || t < best) {
+                best = t;
+                f.nq = nq;
+                f.nsplit = (int)ns;
+            }
+        }
+    }
     f.nrt = (f.R + 16 * f.nq - 1) / (16 * f.nq);
-    const int64_t room = (f.R > 16 ? 2 : 1) * cus;
-    f.nsplit = (int)(nsplit > 0 ? nsplit : std::max<int64_t>(1, std::min<int64_t>({64, room / std::max<int64_t>(1, units(f.nq)), ntiles / 4})));
     f.div_nrt = mx::fq_div_by(f.nrt); f.div_hk = mx::fq_div_by(f.HK); f.div_split = mx::fq_div_by(f.nsplit); f.div_g = mx::fq_div_by(f.G);
 }
 

@@ -16,7 +16,8 @@
 // sequences of 1 to 4096 keys 67 us (275 MB, 4.1 TB/s). With many rows by a wave's work on a tile and the blocks' starts and
 // ends, some 8 us: 10 sequences x 256 rows of up to 3065 keys at head dim 64 48 us, 2048 rows of 8192 keys 116 us. Small blocks
 // of four waves with one tile each, several a CU, overlap those: for the same single token 31 us with eight waves or two
-// tiles a wave, 28 with these (out of the last-level cache), at head dim 64 22 and 18.6; 2048 rows 163 and, two row tiles a wave, 102.
+// tiles a wave, 28 with these (out of the last-level cache), at head dim 64 22 and 18.6; 2048 rows 163 and, two row tiles a wave, 102;
+// 4 x 2048 rows of 2000 keys at head dim 64 with three blocks a CU 74, with two of two tiles a wave 90, blocks of six waves 131, of twelve 113.
 //
 // A key that a row does not see has P = 0, and 0 times a V that is no number would still be none. So in the tiles that
 // hold such a key (the last ones of a sequence; all tiles of a block with padding) those of its values that are not finite
@@ -26,8 +27,8 @@
 
 namespace mx {
 
-// NB: tiles of a wave in LDS; NW: waves a block; WPE: waves a SIMD, whose registers they share.
-template <int DK, int DV, int NQ, int NB, int NW>
+// NW: waves a block, with a tile each in LDS; WPE: waves a SIMD, whose registers they share.
+template <int DK, int DV, int NQ, int NW>
 struct FpCfg {
     static constexpr int KS = DK / 32, TT = DV / 16;
     // 16-byte chunks of a row (K: a power of two), DMA instructions a tile
@@ -39,16 +40,16 @@ struct FpCfg {
     __device__ static __forceinline__ int kswz(int r) { return KCH >= 16 ? r & 15 : (r / 2) & 7; }
     __device__ static __forceinline__ int vswz(int r) { return VCH >= 16 ? (r & 3) | (r >> 1 & 4) : (r >> 1 & 1) | (r >> 2 & 2); }
     static constexpr int CT = TT * NQ < 8 ? TT * NQ : 8;      // O^T tiles merged at a time
-    static constexpr int Q_LO = NW * NB * STAGE;              // the halves lo of Q: [NQ][KS][64], behind the tiles
+    static constexpr int Q_LO = NW * STAGE;                   // the halves lo of Q: [NQ][KS][64], behind the tiles
     static constexpr int LOOP_LDS = Q_LO + NQ * KS * 1024;
     static constexpr int MERGE_LDS = NW * 16 * NQ * 8 + NW * CT * 1024;
     static constexpr int LDS = MERGE_LDS > LOOP_LDS ? MERGE_LDS : LOOP_LDS;
     static_assert(LDS <= FQ_LDS_MAX, "LDS");
 };
 
-// V^T operands of four tiles of 16 dims from addresses a[i] (keys 8 g ..), OFF further, and ROWS4 behind it (keys 8 g + 4 ..):
+// V^T operands of four tiles of 16 dims from addresses a[i] (keys 8 g ..) and ROWS4 behind them (keys 8 g + 4 ..):
 // one statement with its wait, as fq_read_tr.
-template <int OFF, int ROWS4>
+template <int ROWS4>
 __device__ __forceinline__ void fp_read_tr(const uint32_t (&a)[4], fq_v2i (&w)[8]) {
     asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n"
                  "ds_read_b64_tr_b16 %1, %8 offset:%13\n"
@@ -60,16 +61,16 @@ __device__ __forceinline__ void fp_read_tr(const uint32_t (&a)[4], fq_v2i (&w)[8
                  "ds_read_b64_tr_b16 %7, %11 offset:%13\n"
                  "s_waitcnt lgkmcnt(0)"
                  : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7])
-                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF), "n"(OFF + ROWS4)
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(0), "n"(ROWS4)
                  : "memory");
 }
 
 // Bits of the halves of x that are not finite: 0x8000 of each.
 __device__ __forceinline__ uint32_t not_finite2(uint32_t x) { return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
 
-template <int DK, int DV, int NQ, int NB, int NW, int WPE, bool QF32>
+template <int DK, int DV, int NQ, int NW, int WPE, bool QF32>
 __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) fa_pf16_kernel(FaPArgs a) {
-    using C = FpCfg<DK, DV, NQ, NB, NW>;
+    using C = FpCfg<DK, DV, NQ, NW>;
     extern __shared__ __align__(16) uint8_t smem[];
     asm volatile("" ::"s"(a.q), "s"(a.k.nb3), "s"(a.v.nb2), "s"(a.dst), "s"(a.dst_nb3), "s"(a.T), "s"(a.div_split.mul), "s"(a.softcap), "s"(a.st.table),
                  "s"(a.st.parent_nb), "s"(a.div_tpp.mul));   // all lines of the arguments at once
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
         const int slot = q * WAVE + lane, key = slot / C::VCH, c = (slot % C::VCH) ^ (2 * C::vswz(key));
         vdma[q] = key * 2 * (uint32_t)a.v.nb1 + (c * 8 < a.dv ? 16 * c : 0);
     }
-    uint8_t * const wl = smem + wave * NB * C::STAGE;
+    uint8_t * const wl = smem + wave * C::STAGE;
     // where this lane reads: chunk 4 i + g of K row r (i: kra ^ 64 i), 4 dims of V row 8 g + r / 4 (tile of 16 dims i: vra ^ 32 i)
     const uint32_t kra = r * C::KCH * 16 + ((g ^ C::kswz(r)) << 4);
     const int vrow = 8 * g + r / 4;
@@ -149,31 +150,27 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
         const int64_t row = page_row(a.st, uniform_i32(a.st.table, (int64_t)s * a.st.table_nb + p));
         return row < 0 ? -1 : row + FQ_KEYS * (t - p * a.div_tpp.d);
     };
-    auto dma_k = [&](int64_t row, int buf) {
+    auto dma_k = [&](int64_t row) {
         const __amdgpu_buffer_rsrc_t kt = fq_rsrc(kq + max(row, (int64_t)0) * a.k.nb1);
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int q = 0; q < C::KD; q++) fq_dma16(kt, kdma[q], wl + buf * C::STAGE + q * 1024);
+        for (int q = 0; q < C::KD; q++) fq_dma16(kt, kdma[q], wl + q * 1024);
         asm volatile("" ::: "memory");
     };
-    auto dma_v = [&](int64_t row, int buf) {
+    auto dma_v = [&](int64_t row) {
         const __amdgpu_buffer_rsrc_t vt = fq_rsrc(vq + max(row, (int64_t)0) * a.v.nb1);
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int q = 0; q < C::VD; q++) fq_dma16(vt, vdma[q], wl + buf * C::STAGE + C::K_BYTES + q * 1024);
+        for (int q = 0; q < C::VD; q++) fq_dma16(vt, vdma[q], wl + C::K_BYTES + q * 1024);
         asm volatile("" ::: "memory");
     };
-    // The wave's tiles are tile0 + wave + NW k, k < nk; each buffer's next tile is NB further. Waves without a tile read one all
+    // The wave's tiles are tile0 + wave + NW k, k < nk. Waves without a tile read one all
     // the same, and behind the last the last again: the loads in flight stay what the waits count.
     const int nk = tile1 - tile0 > wave ? (tile1 - tile0 - wave + NW - 1) / NW : 0;
     int t = min(tile0 + wave, tile_end);
-    int64_t row_t = page_of(t), row_n = NB == 2 ? page_of(min(t + NW, tile_end)) : 0, row_p = page_of(min(t + NB * NW, tile_end));
-    dma_k(row_t, 0);
-    dma_v(row_t, 0);
-    if constexpr (NB == 2) {
-        dma_k(row_n, 1);
-        dma_v(row_n, 1);
-    }
+    int64_t row_t = page_of(t), row_n = page_of(min(t + NW, tile_end));
+    dma_k(row_t);
+    dma_v(row_t);
 
     // Q in halves; a row outside [2^-6, 2^15] divided by a factor that multiplies its scores with the scale (fa_q_kernel)
     half8 qf[NQ][C::KS];
@@ -227,10 +224,8 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
     const half2v one2 = {(_Float16)1.0f, (_Float16)1.0f};
     const float cap2 = a.softcap != 0.0f ? 2.0f * FQ_LOG2E / a.softcap : 0.0f;
 
-    auto tile = [&](auto buffer) __attribute__((always_inline)) {
-        constexpr int BUF = decltype(buffer)::value;
-        fq_wait_vm<C::VD + (NB - 1) * (C::KD + C::VD)>();   // K has landed
-        const uint8_t * const st = wl + BUF * C::STAGE;
+    for (int k = 0; k < nk; k++) {
+        fq_wait_vm<C::VD>();   // K has landed
         float4v sc[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; n++) sc[n][0] = sc[n][1] = float4v{0, 0, 0, 0};
@@ -238,7 +233,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
         for (int i = 0; i < C::KS; i++)
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
-                const half8 kf = *(const half8 *)(st + (kra ^ (uint32_t)(64 * i)) + hf * 256 * C::KCH);
+                const half8 kf = *(const half8 *)(wl + (kra ^ (uint32_t)(64 * i)) + hf * 256 * C::KCH);
 #pragma unroll
                 for (int n = 0; n < NQ; n++) sc[n][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n][i], sc[n][hf], 0, 0, 0);
                 if constexpr (QF32)
@@ -247,7 +242,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
                         sc[n][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[(n * C::KS + i) * WAVE + lane], sc[n][hf], 0, 0, 0);
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        dma_k(row_p, BUF);
+        dma_k(row_n);
         const bool masked = FQ_KEYS * (t + 1) > full_to || row_t < 0;
         uint32_t vis[NQ];   // masked: which of this lane's eight keys row n sees
         u32x4 pf[NQ];       // P, fp16
@@ -299,7 +294,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
                 l_run[n] = __builtin_amdgcn_fdot2(h2_of(pf[n][e]), one2, l_run[n], false);   // the sum of what is multiplied
             }
         }
-        fq_wait_vm<NB * C::KD + (NB - 1) * C::VD>();   // V has landed
+        fq_wait_vm<C::KD>();   // V has landed
         // ---- O^T += V^T . P^T; shut: all bits of the halves of keys hidden from some row ----
         auto pv = [&](auto some, const u32x4 & shut, uint32_t & bad) __attribute__((always_inline)) {
 #pragma unroll
@@ -308,7 +303,7 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
                 fq_v2i w[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) va[i] = vra ^ (uint32_t)(32 * (q + i));
-                fp_read_tr<BUF * C::STAGE, 4 * C::VRB>(va, w);
+                fp_read_tr<4 * C::VRB>(va, w);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     u32x4 x = {(uint32_t)w[2 * i][0], (uint32_t)w[2 * i][1], (uint32_t)w[2 * i + 1][0], (uint32_t)w[2 * i + 1][1]};
@@ -352,16 +347,10 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        dma_v(row_p, BUF);
+        dma_v(row_n);
         t += NW;
-        row_t = NB == 2 ? row_n : row_p;
-        row_n = row_p;
-        row_p = page_of(min(t + NB * NW, tile_end));
-    };
-    for (int k = 0; k < nk; k += NB) {
-        tile(std::integral_constant<int, 0>{});
-        if constexpr (NB == 2)
-            if (k + 1 < nk) tile(std::integral_constant<int, 1>{});
+        row_t = row_n;
+        row_n = page_of(min(t + NW, tile_end));
     }
     fq_wait_vm<0>();   // no DMA may still write what the merge reuses
 
@@ -438,29 +427,29 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
     }
 }
 
-template <int DK, int DV, int NQ, int NB, int NW, int WPE, bool QF32>
+template <int DK, int DV, int NQ, int NW, int WPE, bool QF32>
 static hipError_t fp_launch_q(const FaPArgs & a, hipStream_t st) {
-    using C = FpCfg<DK, DV, NQ, NB, NW>;
+    using C = FpCfg<DK, DV, NQ, NW>;
     static bool done[FQ_DEVICES];
-    const hipError_t l = fq_allow_lds((const void *)fa_pf16_kernel<DK, DV, NQ, NB, NW, WPE, QF32>, C::LDS, done);
+    const hipError_t l = fq_allow_lds((const void *)fa_pf16_kernel<DK, DV, NQ, NW, WPE, QF32>, C::LDS, done);
     if (l != hipSuccess) return l;
     const int64_t units = (int64_t)a.S * a.HK * a.nrt;
-    hipLaunchKernelGGL((fa_pf16_kernel<DK, DV, NQ, NB, NW, WPE, QF32>), dim3((unsigned)(units * a.nsplit)), dim3(NW * WAVE), C::LDS, st, a);
+    hipLaunchKernelGGL((fa_pf16_kernel<DK, DV, NQ, NW, WPE, QF32>), dim3((unsigned)(units * a.nsplit)), dim3(NW * WAVE), C::LDS, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     return launch_fa_q_combine(a, DV, NQ, st);
 }
 
-template <int DK, int DV, int NQ, int NB, int NW, int WPE>
+template <int DK, int DV, int NQ, int NW, int WPE>
 static hipError_t fp_launch(const FaPArgs & a, hipStream_t st) {
-    return a.q_f16 ? fp_launch_q<DK, DV, NQ, NB, NW, WPE, false>(a, st) : fp_launch_q<DK, DV, NQ, NB, NW, WPE, true>(a, st);
+    return a.q_f16 ? fp_launch_q<DK, DV, NQ, NW, WPE, false>(a, st) : fp_launch_q<DK, DV, NQ, NW, WPE, true>(a, st);
 }
 
 hipError_t launch_fa_p_F16(const FaPArgs & a, hipStream_t st) {
-    if (a.D == 64 && a.DV == 64) return a.nq == 2 ? fp_launch<64, 64, 2, 2, 4, 2>(a, st) : fp_launch<64, 64, 1, 1, 4, 4>(a, st);
-    if (a.D == 128 && a.DV == 128) return a.nq == 2 ? fp_launch<128, 128, 2, 1, 4, 2>(a, st) : fp_launch<128, 128, 1, 1, 4, 2>(a, st);
-    if (a.D == 192 && a.DV == 128) return a.nq == 2 ? fp_launch<192, 128, 2, 1, 4, 1>(a, st) : fp_launch<192, 128, 1, 1, 4, 1>(a, st);
-    if (a.nq == 1 && a.D == 256 && a.DV == 256) return fp_launch<256, 256, 1, 1, 4, 1>(a, st);
+    if (a.D == 64 && a.DV == 64) return a.nq == 2 ? fp_launch<64, 64, 2, 4, 3>(a, st) : fp_launch<64, 64, 1, 4, 4>(a, st);
+    if (a.D == 128 && a.DV == 128) return a.nq == 2 ? fp_launch<128, 128, 2, 4, 2>(a, st) : fp_launch<128, 128, 1, 4, 2>(a, st);
+    if (a.D == 192 && a.DV == 128) return a.nq == 2 ? fp_launch<192, 128, 2, 4, 1>(a, st) : fp_launch<192, 128, 1, 4, 1>(a, st);
+    if (a.nq == 1 && a.D == 256 && a.DV == 256) return fp_launch<256, 256, 1, 4, 1>(a, st);
     return hipErrorInvalidValue;
 }
 
