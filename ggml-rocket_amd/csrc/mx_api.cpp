@@ -808,9 +808,6 @@ static mx::FaQArgs fa_q_direct(const mi355x_fa_q_args * a, int nsplit) {
 // keys, 512 rows 36 / 71; 32 sequences x 256 rows x 1024 187 / 641).
 // Fewer keys than a tile's 32, whose loads the direct form does not bound a lane at a time, are always decoded first: 14 us
 // for one sequence (300 keys 10 us), but 477 us for 32 sequences of 31 keys, one after another, where 32 keys take 9.
-static bool fa_q_few_rows(int64_t R, int64_t HK, int64_t KV, int dims, int64_t most = 65536) {
-    return R * dims <= most || HK * ((R + 15) / 16) * ((KV + 31) / 32) <= 64 * (int64_t)device_cus();
-}
 static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (a->KV < mx::FA_Q_MIN_KV || a->k.nb1 >= mx::FA_Q_MAX_NB1 || a->v.nb1 >= mx::FA_Q_MAX_NB1) return false;
     int D, DV;
@@ -818,7 +815,8 @@ static bool fa_q_is_direct(const mi355x_fa_q_args * a) {
     if (2 * a->D < D || 2 * a->DV < DV) return false;   // its loads of scales
     if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
         if (*e) return atoi(e) != 0;
-    return fa_q_few_rows((int64_t)(a->H / a->HK) * a->T, a->HK, a->KV, D + DV);
+    const int64_t R = (int64_t)(a->H / a->HK) * a->T;
+    return R * (D + DV) <= 65536 || a->HK * ((R + 15) / 16) * ((a->KV + 31) / 32) <= 64 * (int64_t)device_cus();
 }
 struct FaQDirectLayout {
     size_t po, pml, total;
@@ -1076,17 +1074,33 @@ static int fa_p_check(const mi355x_fa_p_args * a, int nsplit, mx::FaPArgs & f) {
     return MI355X_OK;
 }
 
-// Many rows of a chain over a quantized cache: decoded first, a sequence at a time, as mi355x_flash_attn_q. The same rule, its
-// line itself on the decoding side: the few-row kernel rounds P and Q less often here and takes a little longer (us direct /
-// decoded, 8-bit, 8 KV heads, F32 Q: head dim 128, 128 rows of 16000 keys 48 / 60, 256 81 / 70, 512 of 4000 46 / 40, of 1000
-// 19 / 27; head dim 64, 512 rows of 16000 72 / 55, of 4000 28 / 31; head dim 256, 128 rows of 16000 117 / 148, 256 213 / 153).
+// Many rows of a chain over a quantized cache: decoded first, a sequence at a time, as mi355x_flash_attn_q, where that is estimated
+// to take a tenth less (the direct form rounds less). Direct: a block's start, end and merge, and its waves' tiles, one after
+// another; decoded: launches, the cache's values, the rows' products. The numbers (us) are measured ones of 8 KV heads, 8-bit, F32
+// Q; direct / decoded: head dim 64, 384 rows of 16000 keys 76 / 54, of 4000 26 / 28; 128, 128 rows of 16000 50 / 69, 256 78 / 80, 288
+// 138 / 83, 512 of 4000 43 / 40, of 1000 18 / 26; 192, 192 rows of 16000 144 / 93; 256, 128 115 / 146, 192 208 / 145, 160 of 4000 51 / 74.
 // A tree has 64 tokens at most and is read as stored; an fp16 cache needs no decoding.
+struct FpForms {
+    int waves;                          // a block's
+    double tile, launches, key, row;    // a tile of each; decoded: a sequence, a key of it, and with each row
+};
+static FpForms fp_forms(int D, int nq) {
+    return D <= 64    ? nq == 2 ? FpForms{8, 1.9, 20.0, 1.9e-3, 0.6e-6} : FpForms{12, 1.55, 20.0, 1.9e-3, 0.6e-6}
+           : D <= 128 ? FpForms{8, 2.06, 20.0, 2.4e-3, 5.2e-6}
+           : D <= 192 ? FpForms{4, 2.2, 20.0, 3.3e-3, 6.6e-6}
+                      : FpForms{4, 3.2, 50.0, 5.1e-3, 5.0e-6};
+}
 static bool fa_p_decodes(const mi355x_fa_p_args * a, const mx::FaPArgs & f) {
     if (f.k.type == mx::T_F16 || f.st.parent || (size_t)f.KV > mx::fa_max_kv(f.dk, f.dv)) return false;
     if ((int64_t)f.KV * f.HK * ((f.dk + f.dv) / 32) >= 1 << 29) return false;
     if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
         if (*e) return atoi(e) == 0;
-    return !fa_q_few_rows(f.R, f.HK, f.KV, f.D + f.DV, 65535);
+    const FpForms c = fp_forms(f.D, f.nq);
+    const int64_t cus = device_cus(), blocks = (int64_t)f.S * f.HK * f.nrt * f.nsplit, tiles = (f.KV + 31) / 32;
+    const int64_t chain = ((tiles + f.nsplit - 1) / f.nsplit + c.waves - 1) / c.waves;
+    const double direct = 12.0 + (double)((blocks + cus - 1) / cus) * chain * c.tile;
+    const double decoded = f.S * (c.launches + f.HK / 8.0 * f.KV * (c.key + c.row * f.R));
+    return 1.1 * decoded < direct;
 }
 
 // The decoded form of sequence s: the op on fp16 K and V [HK][kvp][D] and the mask [T][kvp] that the decoding launch writes.
