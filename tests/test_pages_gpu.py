@@ -4,6 +4,7 @@ that a caller should not pass; the three as a decoding loop uses them, eager and
 import numpy as np
 import pytest
 
+import kv_norm
 import kv_oracle as R
 import pages_oracle as P
 
@@ -528,6 +529,31 @@ def test_attend_keys_with_nan_scales(mx, mix):
         sees = np.array([2 in w for w in P.ways(parents[0], T)])
         assert sees.any() and not sees.all()
         assert np.isnan(got[0, sees]).all() and np.isfinite(got[0, ~sees]).all()
+
+
+@pytest.mark.parametrize("vt", [Q8_0, Q4_0], ids=ids)
+@pytest.mark.parametrize("DV", [64, 128, 256])
+@pytest.mark.parametrize("T", [1, 9])
+@pytest.mark.parametrize("ratio", [1e2, 1e4, 1e6])
+def test_attend_blocks_of_a_key_apart(mx, form, vt, DV, T, ratio):
+    """V's blocks of dims whose values are `ratio` apart: each is as good as its own values allow."""
+    H, HK, KV, page, D = 8, 2, 400, 32, 64 if DV < 256 else 256
+    rng = np.random.default_rng(DV + T)
+    table, pages = tables(rng, [KV - T], [T], page)
+    at = np.array([P.row(table[0], page, j) for j in range(KV)])
+    kc, kp = cache_of(mx, Q8_0, pages * page, HK, D, rng)
+    x = rng.standard_normal((pages * page, HK, DV // 32, 32))
+    x *= 8000.0 / np.abs(x).max(-1)[..., None]
+    x[:, :, 1::2] /= ratio
+    vq, vd = R.quantize(x.reshape(-1, HK, DV), vt)
+    q = rng.standard_normal((1, T, H, D)).astype(np.float32)
+    mask = np.where(np.arange(KV) <= KV - T + np.arange(T)[:, None], 0.0, -np.inf)
+    kn, vn = P.cache_values([p[at] for p in kp], Q8_0), R.values(vq, vd, vt)[at]
+    want, limit = kv_norm.attention(q[0].transpose(1, 0, 2), kn.transpose(1, 0, 2), vn.transpose(1, 0, 2), mask, D ** -0.5, vd=vd[at].transpose(1, 0, 2))
+    step = mx.KvStep(i32(table), i32([KV - T]), T, page)
+    for ns in (0, 1, 3):
+        got = cpu(mx.flash_attn_paged(gpu(q).permute(0, 2, 1, 3), kc, mx.KvCache(vt, gpu(vq), gpu(vd)), step, D ** -0.5, nsplit=ns))[0]
+        assert kv_norm.ratio(got, want, limit) <= 1, (ns, kv_norm.ratio(got, want, limit))
 
 
 @pytest.mark.parametrize("kt,vt", [(Q8_0, Q4_0), (F16, F16)], ids=lambda t: NAME[t])
