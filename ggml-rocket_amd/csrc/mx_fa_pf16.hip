@@ -8,8 +8,8 @@
 // DMA into buffers of the wave's own and no barrier is in the loop. K's operand is one 16-byte read of LDS (a key's eight
 // dims), V's two transposing reads (ds_read_b64_tr_b16: the lanes i of a group of 16 point at 4 dims of key i / 4, and lane
 // i receives dim i of the four keys).
-// Roundings: P, once, to fp16. Q is exact: an fp16 one as it is, an F32 one as the sum of two halves, hi + lo, off by 2^-22
-// (a second product in the loop, 8 more MFMAs a tile at head dim 128); its scale multiplies the F32 scores. K and V are exact, scores,
+// Roundings: P, once, to fp16. Q is exact: an fp16 one as it is, an F32 one as the sum of two halves, hi + lo, off by 2^-22 of a value and
+// 2^-39 of its row's largest (a second product in the loop, 8 more MFMAs a tile at head dim 128); its scale multiplies the F32 scores. K and V are exact, scores,
 // statistics, sums and O F32. An output is 1.7e-4 of its norm from 64 bits, as fp16 2.7e-4.
 //
 // Bound by HBM with few rows: one token on 32768 keys of 8 x (128 + 128) 31 us (134 MB, 4.3 TB/s) and 4 for the merge, 32
@@ -172,7 +172,8 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
     dma_k(row_t);
     dma_v(row_t);
 
-    // Q in halves; a row outside [2^-6, 2^15] divided by a factor that multiplies its scores with the scale (fa_q_kernel)
+    // Q in halves; an F32 row times the power of two that brings its largest value to [2^14, 2^15) (at most 2^111), so that its low halves
+    // keep their bits; the scale takes it back
     half8 qf[NQ][C::KS];
     half8 * const ql = (half8 *)(smem + C::Q_LO);
     float sfac[NQ];
@@ -188,8 +189,8 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
 #pragma unroll
             for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(value(st, e)));
         amax = fq_col_max(amax);
-        const float qfac = QF32 && (amax > 32768.0f || (amax < 0.015625f && amax > 0.0f)) ? fmaxf(amax / 16.0f, 0x1p-120f) : 1.0f;
-        const float inv = 1.0f / qfac;
+        const uint32_t e2 = QF32 ? max((int)(__float_as_uint(amax) >> 23) - 14, 16) : 127;
+        const float qfac = __uint_as_float(e2 << 23), inv = __uint_as_float((254u - e2) << 23);
         sfac[n] = a.scale * qfac;
 #pragma unroll
         for (int st = 0; st < C::KS; st++) {

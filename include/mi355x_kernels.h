@@ -447,7 +447,8 @@ MI355X_API int mi355x_kv_append(const mi355x_kv_append_args * a, int32_t * err_d
  * Token t of sequence s sees its n_past[s] rows, itself and the tokens above it. Padding, and a token none of whose keys
  * lies in the cache, are written as zeros. A key that a token does not see adds nothing to it, whatever the cache holds there, NaN
  * included. Limits of the values as in mi355x_flash_attn_q; roundings, read from the pages, of the matrix unit's operands to
- * fp16: P times the scale of V's block (an fp16 cache: P) once, Q only where it is F32 and then by 2^-22 of itself; an output
+ * fp16: P times the scale of V's block (an fp16 cache: P) once, Q only where it is F32 and then by 2^-22 of itself and 2^-27 of its
+ * row's largest value (F16: by 2^-35 of that one, where it is 128 or more and the cache quantized); an output
  * is 1.7e-4 of its norm from the 64-bit value then, and an fp16 one's own rounding 2.1e-4. Decoded first: as there.
  * max_kv: a number that no n_past + n_new passes (0: n_table * page). The launch and its workspace are planned for it;
  * it takes the place of n_table * page in what the step says of numbers out of range.
