@@ -1103,33 +1103,40 @@ static bool fa_p_decodes(const mi355x_fa_p_args * a, const mx::FaPArgs & f) {
     return 1.1 * decoded < direct;
 }
 
-// The decoded form of sequence s: the op on fp16 K and V [HK][kvp][D] and the mask [T][kvp] that the decoding launch writes.
-static mi355x_fa_args fa_p_lower(const mi355x_fa_p_args * a, const mx::FaPArgs & f, int s, char * k16, char * v16, char * mask) {
+// The decoded form of `count` tokens of sequence s, from `first` on: the op on fp16 K and V [HK][kvp][D] and the mask [count][kvp] that the
+// decoding launch writes.
+static mi355x_fa_args fa_p_lower(const mi355x_fa_p_args * a, const mx::FaPArgs & f, int s, int first, int count, char * k16, char * v16, char * mask) {
     mi355x_fa_args o;
     memset(&o, 0, sizeof o);
     const int64_t kvp = (f.KV + 63) / 64 * 64;
-    o.q_dev = (const float *)((const char *)a->q_dev + s * a->q_nb3 * (f.q_f16 ? 2 : 4)); o.q_nb1 = a->q_nb1; o.q_nb2 = a->q_nb2;
+    o.q_dev = (const float *)((const char *)a->q_dev + (s * a->q_nb3 + first * a->q_nb1) * (f.q_f16 ? 2 : 4)); o.q_nb1 = a->q_nb1; o.q_nb2 = a->q_nb2;
     o.k_dev = (const uint16_t *)k16; o.k_nb1 = a->D; o.k_nb2 = kvp * a->D;
     o.v_dev = (const uint16_t *)v16; o.v_nb1 = a->DV; o.v_nb2 = kvp * a->DV;
     o.mask_dev = (const uint16_t *)mask; o.mask_nb1 = kvp;
-    o.dst_dev = (float *)((char *)a->dst_dev + s * a->dst_nb3 * (f.dst_f16 ? 2 : 4)); o.dst_nb1 = a->dst_nb1; o.dst_nb2 = a->dst_nb2;
-    o.D = a->D; o.DV = a->DV; o.T = a->step.T; o.H = a->H; o.KV = (int)kvp; o.HK = a->HK;
+    o.dst_dev = (float *)((char *)a->dst_dev + (s * a->dst_nb3 + first * a->dst_nb2) * (f.dst_f16 ? 2 : 4)); o.dst_nb1 = a->dst_nb1; o.dst_nb2 = a->dst_nb2;
+    o.D = a->D; o.DV = a->DV; o.T = count; o.H = a->H; o.KV = (int)kvp; o.HK = a->HK;
     o.scale = a->scale; o.softcap = a->softcap;
     return o;
 }
+// Only the tiles along the chain's diagonal have a mask that is written and read, but it has a place for every tile. So that
+// long chains over long caches do not take gigabytes for it, tokens go through in pieces whose mask is 2^26 values at most (128 MiB: 512 tokens
+// of 131072 keys), or 32 tokens'; K and V are decoded once. The splits are those of a whole piece. (32 / 8 heads of 128, 4096 tokens of
+// 131072 keys: 656 MiB and 9.9 ms, in one piece 1536 MiB and 9.75 ms; 16384 of 32768 keys 256 MiB for 1152, 7.2 ms either way.)
 struct FaPLayout {
     size_t k, v, mask, fa, total;
+    int piece, nsplit;
 };
 static FaPLayout fa_p_layout(const mi355x_fa_p_args * a, const mx::FaPArgs & f, int nsplit) {
     FaPLayout L;
     const size_t kvp = (size_t)(f.KV + 63) / 64 * 64;
+    L.piece = (int)std::min<int64_t>(a->step.T, std::max<int64_t>(32, (1 << 26) / (int64_t)kvp / 32 * 32));
     L.k = 0;
     L.v = L.k + align256((size_t)a->HK * kvp * a->D * 2);
     L.mask = L.v + align256((size_t)a->HK * kvp * a->DV * 2);
-    L.fa = L.mask + align256((size_t)a->step.T * kvp * 2);
-    const mi355x_fa_args one = fa_p_lower(a, f, 0, nullptr, nullptr, nullptr);
-    if (nsplit <= 0) nsplit = fa_plan(&one, 0).nsplit;
-    L.total = L.fa + align256(fa_layout(fa_lower(&one, nsplit)).total);
+    L.fa = L.mask + align256((size_t)L.piece * kvp * 2);
+    const mi355x_fa_args one = fa_p_lower(a, f, 0, 0, L.piece, nullptr, nullptr, nullptr);
+    L.nsplit = nsplit > 0 ? nsplit : fa_plan(&one, 0).nsplit;
+    L.total = L.fa + align256(fa_layout(fa_lower(&one, L.nsplit)).total);
     return L;
 }
 
@@ -1152,20 +1159,21 @@ MI355X_API int mi355x_flash_attn_paged(const mi355x_fa_p_args * a, int nsplit, v
         const FaPLayout L = fa_p_layout(a, f, nsplit);
         if (!workspace_dev || workspace_bytes < L.total || !aligned(workspace_dev, 256)) return MI355X_E_NOMEM;
         char * ws = (char *)workspace_dev;
-        for (int s = 0; s < a->step.S; s++) {
-            const mi355x_fa_args one = fa_p_lower(a, f, s, ws + L.k, ws + L.v, ws + L.mask);
-            size_t need;
-            const mx::FaArgs g = fa_fused_args(&one, nsplit, f.q_f16, f.dst_f16, ws + L.fa, &need);
-            if (need > workspace_bytes - L.fa) return MI355X_E_NOMEM;
-            mx::KvDecodeArgs d;
-            memset(&d, 0, sizeof d);
-            d.k = f.k; d.v = f.v;
-            d.k16 = (uint16_t *)(ws + L.k); d.v16 = (uint16_t *)(ws + L.v);
-            d.HK = a->HK; d.KV = one.KV; d.D = a->D; d.DV = a->DV;
-            int e = hip_status(mx::launch_kv_decode_paged(d, g, f.st, s, (uint16_t *)(ws + L.mask), S(stream)));
-            if (e == MI355X_OK) e = hip_status(mx::launch_fa(g, false, S(stream)));
-            if (e != MI355X_OK) return e;
-        }
+        for (int s = 0; s < a->step.S; s++)
+            for (int first = 0; first < a->step.T; first += L.piece) {
+                const mi355x_fa_args one = fa_p_lower(a, f, s, first, std::min(L.piece, a->step.T - first), ws + L.k, ws + L.v, ws + L.mask);
+                size_t need;
+                const mx::FaArgs g = fa_fused_args(&one, L.nsplit, f.q_f16, f.dst_f16, ws + L.fa, &need);
+                if (need > workspace_bytes - L.fa) return MI355X_E_NOMEM;
+                mx::KvDecodeArgs d;
+                memset(&d, 0, sizeof d);
+                d.k = f.k; d.v = f.v;
+                d.k16 = (uint16_t *)(ws + L.k); d.v16 = (uint16_t *)(ws + L.v);
+                d.HK = a->HK; d.KV = one.KV; d.D = a->D; d.DV = a->DV;
+                int e = hip_status(mx::launch_kv_decode_paged(d, g, f.st, s, first, (uint16_t *)(ws + L.mask), S(stream)));
+                if (e == MI355X_OK) e = hip_status(mx::launch_fa(g, false, S(stream)));
+                if (e != MI355X_OK) return e;
+            }
         return MI355X_OK;
     }
     const FaQDirectLayout L = fa_q_direct_layout(f);

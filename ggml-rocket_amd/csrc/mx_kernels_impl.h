@@ -198,8 +198,9 @@ struct KvKeepArgs {
 };
 hipError_t launch_kv_keep(KvKeepArgs a, hipStream_t st);
 // K and V of sequence s of a step without a tree as fp16 (launch_kv_decode), with the mask classes of f and its mask in the
-// mixed tiles; rows behind the sequence's last tile of 64 are left as they were.
-hipError_t launch_kv_decode_paged(const KvDecodeArgs & a, const FaArgs & f, const KvStepArgs & st, int s, uint16_t * mask, hipStream_t stream);
+// mixed tiles; rows behind the sequence's last tile of 64 are left as they were. f's tokens are the step's from `first` on; if that is not the
+// first, K and V are there already.
+hipError_t launch_kv_decode_paged(const KvDecodeArgs & a, const FaArgs & f, const KvStepArgs & st, int s, int first, uint16_t * mask, hipStream_t stream);
 
 hipError_t launch_get_rows(KvRowsArgs a, hipStream_t st);
 

@@ -413,10 +413,10 @@ hipError_t launch_kv_keep(KvKeepArgs a, hipStream_t st) {
 }
 
 // A sequence's rows out of their pages as fp16 for the fused attention (kv_decode_kernel has the values and what becomes of
-// scales that are not finite), and its mask classes: token tq sees the keys below n_past + tq + 1, padding none. Only
+// scales that are not finite), and its mask classes: token tq of f, the step's first + tq, sees the keys below n_past + first + tq + 1, padding none. Only
 // tiles of which a token sees some keys and not all need a mask; it is written for those alone. Keys of the
 // last tile of 64 behind the sequence's last and those of pages that the cache does not have are zeros.
-__global__ void __launch_bounds__(AP_THREADS) kv_decode_paged_kernel(KvDecodeArgs a, FaArgs f, KvStepArgs st, int s, uint16_t * mask) {
+__global__ void __launch_bounds__(AP_THREADS) kv_decode_paged_kernel(KvDecodeArgs a, FaArgs f, KvStepArgs st, int s, int first, uint16_t * mask) {
     const int t = threadIdx.x, l = t % 4;
     const StepOf sq = step_of(st, s);
     const int keys = sq.fresh ? min(sq.past + sq.fresh, st.cap) : 0;
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_decode_paged_kernel(KvDecodeArg
         if (ct >= nqt * f.cls_stride) return;
         const int qt = ct / f.cls_stride, kt = ct - qt * f.cls_stride;
         const int tq = qt * FA_QW + lane / 2, jb = kt * FA_BKV + 32 * (lane % 2);
-        int n = tq < sq.fresh ? min(max(min(sq.past + tq + 1, keys) - jb, 0), 32) : 0;
+        int n = first + tq < sq.fresh && tq < f.T ? min(max(min(sq.past + first + tq + 1, keys) - jb, 0), 32) : 0;
         if (n > 0 && row_of(jb) < 0) {
             if (st.err) *st.err = 1;
             n = 0;
@@ -475,13 +475,13 @@ __global__ void __launch_bounds__(AP_THREADS) kv_decode_paged_kernel(KvDecodeArg
     *(u32x4 *)((is_v ? a.v16 + (h * (int64_t)a.KV + j) * a.DV : a.k16 + (h * (int64_t)a.KV + j) * a.D) + 32 * blk + 8 * l) = kv_pack8(v);
 }
 
-hipError_t launch_kv_decode_paged(const KvDecodeArgs & args, const FaArgs & f, const KvStepArgs & st, int s, uint16_t * mask, hipStream_t stream) {
+hipError_t launch_kv_decode_paged(const KvDecodeArgs & args, const FaArgs & f, const KvStepArgs & st, int s, int first, uint16_t * mask, hipStream_t stream) {
     KvDecodeArgs a = args;
     a.div_blocks = fq_div_by((a.D + a.DV) / 32);
     a.div_hk = fq_div_by(a.HK);
     a.n_prep = fa_prep_blocks(f);
-    const int64_t items = (int64_t)a.KV * a.HK * ((a.D + a.DV) / 32);
-    hipLaunchKernelGGL(kv_decode_paged_kernel, dim3((unsigned)(a.n_prep + (items + AP_BLOCKS - 1) / AP_BLOCKS)), dim3(AP_THREADS), 0, stream, a, f, st, s, mask);
+    const int64_t items = first ? 0 : (int64_t)a.KV * a.HK * ((a.D + a.DV) / 32);
+    hipLaunchKernelGGL(kv_decode_paged_kernel, dim3((unsigned)(a.n_prep + (items + AP_BLOCKS - 1) / AP_BLOCKS)), dim3(AP_THREADS), 0, stream, a, f, st, s, first, mask);
     return hipGetLastError();
 }
 

@@ -468,7 +468,8 @@ typedef struct mi355x_fa_p_args {
     int64_t max_kv;
 } mi355x_fa_p_args;
 /* Workspace bytes of mi355x_flash_attn_paged with `nsplit` KV splits (0 = its own choice); 0 for an op that it does not
- * take. It follows the sizes and max_kv, not what lies on the device. 256-byte aligned. */
+ * take. It follows the sizes and max_kv, not what lies on the device: partial results where keys are split, and decoded first one
+ * sequence's K and V, max_kv keys as fp16, and 128 MiB at most (or 64 bytes a key). 256-byte aligned. */
 MI355X_API size_t mi355x_flash_attn_paged_workspace(const mi355x_fa_p_args * a, int nsplit);
 /* Concurrent calls must not share a workspace. Equal inputs give equal bits. */
 MI355X_API int mi355x_flash_attn_paged(const mi355x_fa_p_args * a, int nsplit, void * workspace_dev, size_t workspace_bytes,
