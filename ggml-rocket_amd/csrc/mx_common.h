@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace mx {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -165,6 +167,21 @@ __device__ __forceinline__ int fq_div(int n, const FqDiv & d) {
 __device__ __forceinline__ int xcd_tile(int bid, int nblocks) {
     const int q = nblocks / 8, r = nblocks % 8, x = bid % 8;
     return x * q + min(x, r) + bid / 8;
+}
+
+// Allows a kernel `bytes` of LDS on the current device, once for each of them; any threads may come first.
+struct LdsAllowed {
+    static constexpr int DEVICES = 64;
+    std::atomic<bool> done[DEVICES] = {};
+};
+inline hipError_t allow_lds(const void * kernel, int bytes, LdsAllowed & a) {
+    int dev = 0;
+    const hipError_t d = hipGetDevice(&dev);
+    if (d != hipSuccess) return d;
+    if (dev < LdsAllowed::DEVICES && a.done[dev].load(std::memory_order_relaxed)) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess && dev < LdsAllowed::DEVICES) a.done[dev].store(true, std::memory_order_relaxed);
+    return e;
 }
 
 // Multiplies a wave's MI x NJ accumulator tiles (32x32 MFMA output layout: element e of tile

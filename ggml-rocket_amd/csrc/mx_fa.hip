@@ -899,13 +899,9 @@ hipError_t launch_fa_combine(const FaArgs & a, hipStream_t st) {
 
 template <int DK, int DV, int NT, bool SC>
 static hipError_t fa_launch_main(const FaArgs & a, int nb, hipStream_t st) {
-    static bool done = false;
-    if (!done) {
-        hipError_t e = hipFuncSetAttribute((const void *)fa_kernel<DK, DV, NT, SC>,
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, FA_LDS_MAX - 64);
-        if (e != hipSuccess) return e;
-        done = true;
-    }
+    static LdsAllowed done;
+    const hipError_t e = allow_lds((const void *)fa_kernel<DK, DV, NT, SC>, FA_LDS_MAX - 64, done);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL((fa_kernel<DK, DV, NT, SC>), dim3(nb), dim3(FaCfg<DK, DV, NT>::THREADS), fa_lds_bytes(a), st, a);
     return hipGetLastError();
 }

@@ -431,8 +431,8 @@ __global__ void __launch_bounds__((NW * WAVE)) __attribute__((amdgpu_waves_per_e
 template <int DK, int DV, int NQ, int NW, int WPE, bool QF32>
 static hipError_t fp_launch_q(const FaPArgs & a, hipStream_t st) {
     using C = FpCfg<DK, DV, NQ, NW>;
-    static bool done[FQ_DEVICES];
-    const hipError_t l = fq_allow_lds((const void *)fa_pf16_kernel<DK, DV, NQ, NW, WPE, QF32>, C::LDS, done);
+    static LdsAllowed done;
+    const hipError_t l = allow_lds((const void *)fa_pf16_kernel<DK, DV, NQ, NW, WPE, QF32>, C::LDS, done);
     if (l != hipSuccess) return l;
     const int64_t units = (int64_t)a.S * a.HK * a.nrt;
     hipLaunchKernelGGL((fa_pf16_kernel<DK, DV, NQ, NW, WPE, QF32>), dim3((unsigned)(units * a.nsplit)), dim3(NW * WAVE), C::LDS, st, a);

@@ -993,24 +993,12 @@ fa_q_kernel(A a) {
     }
 }
 
-// Allows a kernel `bytes` of LDS on the current device, once for each of them.
-constexpr int FQ_DEVICES = 64;
-inline hipError_t fq_allow_lds(const void * kernel, int bytes, bool (&done)[FQ_DEVICES]) {
-    int dev = 0;
-    const hipError_t d = hipGetDevice(&dev);
-    if (d != hipSuccess) return d;
-    if (dev < FQ_DEVICES && done[dev]) return hipSuccess;
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == hipSuccess && dev < FQ_DEVICES) done[dev] = true;
-    return e;
-}
-
 template <int KT, int VT, int DK, int DV, int NQ, class A>
 static hipError_t fq_launch(const A & a, hipStream_t st) {
     using C = FqCfg<KT, VT, DK, DV, NQ, std::is_same<A, FaPArgs>::value>;
     static_assert(C::LDS <= 160 * 1024, "LDS");
-    static bool done[FQ_DEVICES];
-    const hipError_t l = fq_allow_lds((const void *)fa_q_kernel<KT, VT, DK, DV, NQ, A>, C::LDS, done);
+    static LdsAllowed done;
+    const hipError_t l = allow_lds((const void *)fa_q_kernel<KT, VT, DK, DV, NQ, A>, C::LDS, done);
     if (l != hipSuccess) return l;
     const int64_t units = (int64_t)a.S * a.HK * a.nrt;
     hipLaunchKernelGGL((fa_q_kernel<KT, VT, DK, DV, NQ, A>), dim3((unsigned)(units * a.nsplit)), dim3(C::NW * WAVE), C::LDS, st, a);
