@@ -446,7 +446,8 @@ MI355X_API int mi355x_kv_append(const mi355x_kv_append_args * a, int32_t * err_d
  * F16 (values at q_dev, d_dev not read): dst[s][t] = softmax over the keys that t sees of cap(scale * q.k), times v.
  * Token t of sequence s sees its n_past[s] rows, itself and the tokens above it. Padding, and a token none of whose keys
  * lies in the cache, are written as zeros. A key that a token does not see adds nothing to it, whatever the cache holds there, NaN
- * included. Limits of the values as in mi355x_flash_attn_q; roundings, read from the pages, of the matrix unit's operands to
+ * included; one that it sees makes it NaN where a block's scale is not finite, and where an F16 V is not, that dim at least not
+ * finite. Limits of the values as in mi355x_flash_attn_q; roundings, read from the pages, of the matrix unit's operands to
  * fp16: P times the scale of V's block (an fp16 cache: P) once, Q only where it is F32 and then by 2^-22 of itself and 2^-27 of its
  * row's largest value (F16: by 2^-35 of that one, where it is 128 or more and the cache quantized); an output
  * is 1.7e-4 of its norm from the 64-bit value then, and an fp16 one's own rounding 2.1e-4. Decoded first: as there.
@@ -455,7 +456,8 @@ MI355X_API int mi355x_kv_append(const mi355x_kv_append_args * a, int32_t * err_d
  * H % HK == 0; D and DV multiples of 32 up to 256, each at least half of what the kernels are built for (64 / 64, 128 / 128,
  * 192 / 128, 256 / 256, the smallest that holds both); S * HK row tiles of 16 (T * H / HK rows) as there. Few rows, trees and
  * fp16 caches are taken from the pages as they are; many rows of a chain over a quantized cache by decoding it to fp16 in
- * the workspace first, a sequence at a time. MI355X_FA_Q_DIRECT=1|0 and MI355X_FA_Q_ROWS=16|32 pin the choices as there. */
+ * the workspace first, a sequence at a time: which of them follows from the sizes and max_kv. MI355X_FA_Q_DIRECT=1|0 and
+ * MI355X_FA_Q_ROWS=16|32 pin the choices as there. */
 typedef struct mi355x_fa_p_args {
     mi355x_kv_step step;
     const void * q_dev;   int64_t q_nb1, q_nb2, q_nb3;         /* token, head, sequence strides */
