@@ -1091,7 +1091,7 @@ static FpForms fp_forms(int D, int nq) {
                       : FpForms{4, 3.2, 50.0, 5.1e-3, 5.0e-6};
 }
 static bool fa_p_decodes(const mi355x_fa_p_args * a, const mx::FaPArgs & f) {
-    if (f.k.type == mx::T_F16 || f.st.parent || (size_t)f.KV > mx::fa_max_kv(f.dk, f.dv)) return false;
+    if (a->from_pages || f.k.type == mx::T_F16 || f.st.parent || (size_t)f.KV > mx::fa_max_kv(f.dk, f.dv)) return false;
     if ((int64_t)f.KV * f.HK * ((f.dk + f.dv) / 32) >= 1 << 29) return false;
     if (const char * e = getenv("MI355X_FA_Q_DIRECT"))
         if (*e) return atoi(e) == 0;

@@ -115,7 +115,7 @@ class FaPArgs(ctypes.Structure):
                 ("q_nb3", ctypes.c_int64), ("k", KvView), ("v", KvView), ("n_rows", ctypes.c_int64), ("dst_dev", ctypes.c_void_p),
                 ("dst_nb1", ctypes.c_int64), ("dst_nb2", ctypes.c_int64), ("dst_nb3", ctypes.c_int64), ("q_type", ctypes.c_int),
                 ("dst_type", ctypes.c_int), ("D", ctypes.c_int), ("DV", ctypes.c_int), ("H", ctypes.c_int), ("HK", ctypes.c_int),
-                ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("max_kv", ctypes.c_int64)]
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("max_kv", ctypes.c_int64), ("from_pages", ctypes.c_int)]
 
 
 def lib():
@@ -700,7 +700,7 @@ def kv_keep(step: KvStep, caches, path, n_keep=None, err=None):
                                path.shape[1], _kv_err(err, dev, "kv_keep"), _launch_stream(dev, "kv_keep")), "kv_keep")
 
 
-def _fa_p_args(q, k, v, step, out, scale, softcap, max_kv):
+def _fa_p_args(q, k, v, step, out, scale, softcap, max_kv, from_pages):
     types, qs, os = _plain_types(), q.shape, out.shape
     dev = step.dev
     if len(qs) != 4 or len(k.shape) != 3 or len(v.shape) != 3 or qs[0] != step.S or qs[2] != step.T or k.shape[-1] != qs[3] or k.shape[:2] != v.shape[:2]:
@@ -715,24 +715,25 @@ def _fa_p_args(q, k, v, step, out, scale, softcap, max_kv):
     kt, kq, kd, rows, k1, k2, HK, D = k._rows
     vt, vq, vd, _, v1, v2, _, DV = v._rows
     return FaPArgs(step.args, q.data_ptr(), qn[2], qn[1], qn[0], KvView(kt, kq, kd, k1, k2, 0), KvView(vt, vq, vd, v1, v2, 0), rows,
-                   out.data_ptr(), on[2], on[1], on[0], qt, ot, D, DV, qs[1], HK, scale, softcap, max_kv)
+                   out.data_ptr(), on[2], on[1], on[0], qt, ot, D, DV, qs[1], HK, scale, softcap, max_kv, bool(from_pages))
 
 
-def flash_attn_paged_workspace(q, k: KvCache, v: KvCache, step: KvStep, out, nsplit: int = 0, max_kv: int = 0) -> int:
+def flash_attn_paged_workspace(q, k: KvCache, v: KvCache, step: KvStep, out, nsplit: int = 0, max_kv: int = 0, from_pages: bool = False) -> int:
     """Workspace bytes mi355x_flash_attn_paged needs for these operands (0 for an unsupported op)."""
-    return int(lib().mi355x_flash_attn_paged_workspace(_fa_p_args(q, k, v, step, out, 1.0, 0.0, max_kv), nsplit))
+    return int(lib().mi355x_flash_attn_paged_workspace(_fa_p_args(q, k, v, step, out, 1.0, 0.0, max_kv, from_pages), nsplit))
 
 
 def flash_attn_paged(q, k: KvCache, v: KvCache, step: KvStep, scale: float, softcap: float = 0.0, nsplit: int = 0, out=None,
-                     workspace=None, max_kv: int = 0, err=None):
+                     workspace=None, max_kv: int = 0, err=None, from_pages: bool = False):
     """Attention of a step's tokens, q [S, H, T, D] (F32 or F16), over caches in pages k [rows, HK, D] and v [rows, HK, DV]: each
     token sees the rows its sequence held, itself and the tokens above it. Returns dst [S, T, H, DV], F32 unless `out` is
     F16; padding is zeros. max_kv: a bound that no n_past + n_new passes (0: what the tables can hold), for which launch and
-    workspace are planned; rows behind it are not read."""
+    workspace are planned; rows behind it are not read. from_pages: a quantized cache is read as it is stored, never decoded to fp16 first, which many
+    rows of a chain may be: less rounding, longer calls."""
     torch = _torch()
     if out is None:
         out = torch.empty(q.shape[0], q.shape[2], q.shape[1], v.shape[-1], dtype=torch.float32, device=q.device)
-    a = _fa_p_args(q, k, v, step, out, scale, softcap, max_kv)
+    a = _fa_p_args(q, k, v, step, out, scale, softcap, max_kv, from_pages)
     if workspace is None:
         need = int(lib().mi355x_flash_attn_paged_workspace(a, nsplit))
         workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)

@@ -456,8 +456,9 @@ MI355X_API int mi355x_kv_append(const mi355x_kv_append_args * a, int32_t * err_d
  * H % HK == 0; D and DV multiples of 32 up to 256, each at least half of what the kernels are built for (64 / 64, 128 / 128,
  * 192 / 128, 256 / 256, the smallest that holds both); S * HK row tiles of 16 (T * H / HK rows) as there. Few rows, trees and
  * fp16 caches are taken from the pages as they are; many rows of a chain over a quantized cache by decoding it to fp16 in
- * the workspace first, a sequence at a time: which of them follows from the sizes and max_kv. MI355X_FA_Q_DIRECT=1|0 and
- * MI355X_FA_Q_ROWS=16|32 pin the choices as there. */
+ * the workspace first, a sequence at a time: which of them follows from the sizes and max_kv, unless from_pages says that
+ * the cache is read as it is (512 tokens of 8192 keys, 32 heads of 128 on 8: 289 us and 2.7e-4 for 107 and 4.7e-4).
+ * MI355X_FA_Q_DIRECT=1|0 and MI355X_FA_Q_ROWS=16|32 pin the choices as there, for calls without from_pages. */
 typedef struct mi355x_fa_p_args {
     mi355x_kv_step step;
     const void * q_dev;   int64_t q_nb1, q_nb2, q_nb3;         /* token, head, sequence strides */
@@ -468,6 +469,7 @@ typedef struct mi355x_fa_p_args {
     int D, DV, H, HK;
     float scale, softcap;
     int64_t max_kv;
+    int from_pages;                                            /* not 0: never decoded first */
 } mi355x_fa_p_args;
 /* Workspace bytes of mi355x_flash_attn_paged with `nsplit` KV splits (0 = its own choice); 0 for an op that it does not
  * take. It follows the sizes and max_kv, not what lies on the device: partial results where keys are split, and decoded first one
